@@ -388,6 +388,91 @@ int ldk_w8a16_matmul_swiglu(const void* x, int64_t ldx, const uint8_t* wq, const
                             void* out, int64_t ldo, int64_t M, int64_t N, int64_t K, void* workspace,
                             int64_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------ paged cache */
+
+/* A cache in pages, for several sequences at once; no counterpart in the reference, whose runner
+ * keeps one static cache per batch row (kernels/e2e/model.py:192-243). Shared by the entries below:
+ *  - dtype LDK_F16 or LDK_BF16 for activations and cache; head_dim 64 or 128; nq % nkv == 0,
+ *    nq <= 4096.
+ *  - k_pages, vt_pages: num_pages pages of page_size positions (a multiple of 32, up to 65536), page
+ *    i at element i * k_page_stride (vt_page_stride), >= nkv * page_size * head_dim and a multiple of
+ *    8. A page holds, per kv head, the tiles of ldk_decode_attention's caches: K tiles
+ *    [page_size/32][2][head_dim/32][16][32] and V^T tiles [page_size/32][head_dim/16][16][32].
+ *  - block_table: int32 [B] rows of ldt >= max_pages ids; position p of sequence b is in page
+ *    block_table[b][p / page_size]. An id outside [0, num_pages) is no page: nothing is written there
+ *    and its positions are not attended to. Positions from max_pages * page_size on do not exist.
+ *  - cu_seqlens: int32 [B + 1], sequence b's new tokens are the rows cu_seqlens[b] ..
+ *    cu_seqlens[b+1] - 1 of the T rows, in rising order; NULL: sequence b has row b (T >= B).
+ *    kv_lens: int32 [B], the positions that sequence b's cache holds with its new tokens, which are
+ *    the last of them: new token i of n is at position kv_lens[b] - n + i. A sequence without new
+ *    tokens, kv_lens of 0 and rows behind the last sequence are allowed: those rows are left as they
+ *    were. All of these are read on the device, so a captured graph takes new lengths and pages.
+ *  - data pointers 16-byte aligned, row strides (elements) multiples of 8. */
+
+/* RoPE on q and k and the cache write of T new tokens: qkv rows [nq * head_dim | nkv * head_dim |
+ * nkv * head_dim] of ldqkv; q_out rows of ldq get the rotated q (q_out may be qkv itself, ldq ==
+ * ldqkv: in place), the pages the rotated k and v. Pair (j, j + head_dim/2) of a head is turned by
+ * r * inv_freq[j], r the token's position or rope_pos[row] (int64, may be NULL), the angle reduced in
+ * 64 bits, the rotation in fp32, one rounding. inv_freq NULL: nothing is rotated. Tokens at
+ * positions without a page write no k and v. Two new tokens of one call may not share a slot.
+ * Replaces the RoPE and the cache's index_copy_ of kernels/e2e/model.py:212-233 for a batch of
+ * ragged sequences. */
+int ldk_paged_append(const void* qkv, int64_t ldqkv, int dtype, const int32_t* cu_seqlens,
+                     const int32_t* kv_lens, const int32_t* block_table, int64_t ldt, int64_t max_pages,
+                     const int64_t* rope_pos, const float* inv_freq, void* k_pages,
+                     int64_t k_page_stride, void* vt_pages, int64_t vt_page_stride, int64_t num_pages,
+                     int64_t page_size, void* q_out, int64_t ldq, int64_t T, int64_t B, int nq, int nkv,
+                     int head_dim, void* stream);
+
+/* Bytes of workspace that ldk_paged_attention (prefix_len 0) and ldk_shared_prefix_attention need for
+ * T rows of B sequences of at most max_q new tokens; negative: -ldk_status. */
+int64_t ldk_paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t max_q, int64_t prefix_len, int nq,
+                                            int nkv, int head_dim);
+
+/* Causal grouped-query softmax attention of the new tokens over the pages (their own k and v
+ * included: append first). The token at position p sees position j <= p of its sequence where
+ * window == 0, j > p - window or j < sinks. q rows of ldq, out rows of ldo; max_q >= every sequence's
+ * number of new tokens (tokens past it are not computed; ignored without cu_seqlens). A token that
+ * sees nothing gives zeros. scale > 0. Scores and softmax in fp32, its numerators rounded to dtype
+ * before they weight V, one rounding at the end. The workspace (16-byte aligned,
+ * ldk_paged_attention_workspace_bytes) holds nothing between calls: calls that may overlap need one
+ * each. Stands beside ldk_decode_attention and ldk_prefill_attention (the reference's
+ * scaled_dot_product_attention over one static cache, kernels/e2e/model.py:236-243). */
+int ldk_paged_attention(const void* q, int64_t ldq, int dtype, const int32_t* cu_seqlens,
+                        const int32_t* kv_lens, const int32_t* block_table, int64_t ldt, int64_t max_pages,
+                        const void* k_pages, int64_t k_page_stride, const void* vt_pages,
+                        int64_t vt_page_stride, int64_t num_pages, int64_t page_size, void* out, int64_t ldo,
+                        int64_t T, int64_t B, int64_t max_q, int nq, int nkv, int head_dim, int64_t window,
+                        int64_t sinks, float scale, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ldk_paged_attention (window 0) for a batch whose sequences share their first prefix_len positions:
+ * those are read through prefix_table (int32, prefix_len / page_size ids) once for the whole batch,
+ * the rest through block_table, whose first prefix_len / page_size ids of each row are not read.
+ * prefix_len a multiple of page_size, at most max_pages * page_size; kv_lens counts the prefix (a
+ * sequence shorter than it sees its part). */
+int ldk_shared_prefix_attention(const void* q, int64_t ldq, int dtype, const int32_t* cu_seqlens,
+                                const int32_t* kv_lens, const int32_t* block_table, int64_t ldt,
+                                int64_t max_pages, const int32_t* prefix_table, int64_t prefix_len,
+                                const void* k_pages, int64_t k_page_stride, const void* vt_pages,
+                                int64_t vt_page_stride, int64_t num_pages, int64_t page_size, void* out,
+                                int64_t ldo, int64_t T, int64_t B, int64_t max_q, int nq, int nkv, int head_dim,
+                                float scale, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* -------------------------------------------------------------------------- log probabilities */
+
+/* Per row of logits [rows, V] (row stride ld, dtype LDK_F16/BF16/F32, any alignment of rows):
+ * logprob = log_softmax(row)[tokens[row]] (NaN for a token outside [0, V)), entropy of the row's
+ * softmax, and for the `top` (0..64, <= V) largest logits in ldk_greedy_step's order (NaN largest, the
+ * lowest index first on ties) their log probabilities top_logprobs [rows, top] and indexes top_ids.
+ * fp32 throughout; a row with +inf or NaN, or of -inf alone, gives NaN. tokens and top_ids int64.
+ * Workspace: ldk_token_logprobs_workspace_bytes (0: may be NULL), nothing held between calls.
+ * No counterpart in the reference, whose runner answers with greedy tokens alone
+ * (kernels/e2e/run.py:69-74). */
+int64_t ldk_token_logprobs_workspace_bytes(int64_t rows, int64_t V, int top);
+int ldk_token_logprobs(const void* logits, int64_t ld, int dtype, const int64_t* tokens, int64_t rows,
+                       int64_t V, int top, float* logprob, float* entropy, float* top_logprobs,
+                       int64_t* top_ids, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------- greedy decode bookkeeping */
 
 /* idx = argmax(logits[0:V]) (torch.argmax order: NaN largest, lowest index on ties), then

@@ -84,6 +84,16 @@ SIGNATURES = {
     "ldk_w4a16_matmul_swiglu": [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp, _i64,
                                 _vp],
     "ldk_w8a16_matmul_swiglu_applies": [_i64, _i64, _i64],
+    "ldk_paged_append": [_vp, _i64, _i32, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64,
+                         _vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp],
+    "ldk_paged_attention_workspace_bytes": [_i64, _i64, _i64, _i64, _i32, _i32, _i32],
+    "ldk_paged_attention": [_vp, _i64, _i32, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _vp,
+                            _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i64, _i64, _f32, _vp, _i64, _vp],
+    "ldk_shared_prefix_attention": [_vp, _i64, _i32, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64,
+                                    _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _f32, _vp, _i64,
+                                    _vp],
+    "ldk_token_logprobs_workspace_bytes": [_i64, _i64, _i32],
+    "ldk_token_logprobs": [_vp, _i64, _i32, _vp, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _vp],
     "ldk_w8a16_matmul_swiglu": [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp],
 }
 
@@ -111,6 +121,8 @@ def load() -> ctypes.CDLL:
                 fn.argtypes = argtypes
                 fn.restype = {"ldk_last_error": ctypes.c_char_p,
                               "ldk_workspace_bytes": ctypes.c_int64,
+                              "ldk_paged_attention_workspace_bytes": ctypes.c_int64,
+                              "ldk_token_logprobs_workspace_bytes": ctypes.c_int64,
                               "ldk_w4a16_row_stats_count": ctypes.c_int64}.get(name, ctypes.c_int)
             _lib = lib
     return _lib
