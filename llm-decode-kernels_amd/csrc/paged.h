@@ -46,7 +46,18 @@ __device__ __forceinline__ float2_t unpack2(uint32_t u) {
 
 constexpr int kChunkPos = 32;          // positions of a chunk
 constexpr int kTileElems = 512;        // elements of a 1 KB tile
-constexpr int64_t kMaxPositions = (int64_t(1) << 31) - 64;  // of one sequence: positions are int
+constexpr int64_t kMaxPositions = int64_t(1) << 25;  // of one sequence
+
+// c / n and c % n of a chunk c < 2^20 by the chunks of a page, 1 <= n <= 2^11: with m = ceil(2^31 / n) =
+// (2^31 + e) / n, e < n, 2 c m / 2^32 = c / n + c e / (n 2^31), and c e < 2^31 keeps its floor.
+struct PageDiv {
+  uint32_t n, m;
+};
+inline PageDiv page_div(int64_t n) { return {(uint32_t)n, (uint32_t)(((int64_t(1) << 31) + n - 1) / n)}; }
+__device__ __forceinline__ void chunk_page(const PageDiv& d, int c, int& page, int& sub) {
+  page = (int)__umulhi(2u * (uint32_t)c, d.m);
+  sub = c - page * (int)d.n;
+}
 
 // The new rows and positions of sequence b.
 struct SeqRows {

@@ -17,6 +17,9 @@
 // meet in LDS. The numerators are rounded to the element type before they weight V (the matrix cores
 // take nothing wider), their sum is taken from the unrounded values.
 //
+// paged_block_kernel: a workgroup takes 64 or 128 rows of one kv head, which share K and V through LDS.
+// For prompts, and for the prefix that a whole batch shares, whose rows are all tokens of the batch.
+//
 // Ranges. The lengths are on the device, so the split is made there: every sequence has its visible
 // chunks (those of the sinks, then those of the window) cut into ranges of `per` chunks, one `per` for
 // the whole batch such that all ranges fit the launch's slots; a ragged batch gets ranges of equal
@@ -25,6 +28,7 @@
 // next launch on the stream, joins them.
 #include <algorithm>
 
+#include "lds_dma.h"
 #include "paged.h"
 
 namespace {
@@ -40,16 +44,26 @@ struct PagedArgs {
   int64_t kps, vps;  // page strides, elements
   void* out;
   int64_t ldo;
-  float* part;    // partials, per (slot, kv head, tile): [16 rows]{m, l} and [16 rows][hd]
+  float* part;    // paged_split_kernel's partials, per (slot, tile, kv head): [16 rows]{m, l} and [16 rows][hd]
+  float* bpart;   // paged_block_kernel's, per (tile, kv head, split): [rows]{m, l} and [rows][hd]
   int32_t* plan;  // [B][2]: first slot and ranges of every sequence
   int T, B, max_q, nq, nkv, gq, nt;  // nt: 16-row tiles of a sequence
-  int pages, cpp, cap;               // cpp: chunks per page; cap: positions a sequence can hold
-  int pchunks;                       // chunks of the shared prefix
+  int pages, cap;                    // cap: positions a sequence can hold
+  PageDiv cpp;                       // chunks per page
+  int pchunks, skip;                 // chunks of the shared prefix; of them, those paged_split_kernel leaves out
   int window, sinks, slots;
+  int btiles, bsplits, bdirect;      // the block kernel's tiles and splits; a lone range writes the output
   float scale;
 };
 
 constexpr int kRows = 16;
+template <int N>
+struct IntC {
+  static constexpr int value = N;
+};
+// Waves of paged_block_kernel that split a block's chunks, by its rows: 8 waves a workgroup.
+template <int BT>
+constexpr int kBlockKG = BT == 128 ? 2 : 4;
 constexpr int kMinRange = 4;     // chunks of a range, at least
 constexpr int kMaxRanges = 128;  // ranges of a sequence
 
@@ -67,6 +81,7 @@ __device__ __forceinline__ Span seq_span(const PagedArgs& a, int b) {
   x.lo = a.window > 0 ? max(0, x.s.pos0 - a.window + 1) / kChunkPos : 0;
   x.lo = min(x.lo, hc);
   x.cs = min((min(a.sinks, a.cap) + kChunkPos - 1) / kChunkPos, x.lo);
+  if (a.skip) x.cs = 0, x.lo = min(a.skip, hc);  // the shared prefix is another kernel's
   x.n = x.cs + hc - x.lo;
   return x;
 }
@@ -192,9 +207,11 @@ __global__ __launch_bounds__(NW * 64) void paged_split_kernel(PagedArgs a) {
     const int c = j < sp.cs ? j : j - sp.cs + sp.lo;
     const int cb = c * kChunkPos;
     if (cb > thi || (cb + kChunkPos <= tlo && cb >= a.sinks)) continue;
-    const int page = c < a.pchunks ? a.ptable[c / a.cpp] : trow[c / a.cpp];
+    int at, sub;
+    chunk_page(a.cpp, c, at, sub);
+    const int page = trow[at];
     if (page < 0 || page >= a.pages) continue;
-    const int64_t in_page = ((int64_t)kvh * a.cpp + c % a.cpp) * (kChunkPos * HD);
+    const int64_t in_page = ((int64_t)kvh * a.cpp.n + sub) * (kChunkPos * HD);
     const auto krs = buffer_rsrc((const T*)a.k + page * a.kps + in_page, chunk_bytes);
     const auto vrs = buffer_rsrc((const T*)a.vt + page * a.vps + in_page, chunk_bytes);
     u32x4 kr[2 * NS], vr[NB];
@@ -287,7 +304,7 @@ __global__ __launch_bounds__(NW * 64) void paged_split_kernel(PagedArgs a) {
       l = __builtin_fmaf(lv[w], f, l);
       v = __builtin_fmaf(ov[w], f, v);
     }
-    if (sl.ranges == 1) {
+    if (sl.ranges == 1 && !a.skip) {
       const int g = tile * kRows + j;
       T* dst = (T*)a.out + (int64_t)(sp.s.row0 + g / a.gq) * a.ldo + (int64_t)(kvh * a.gq + g % a.gq) * HD;
       dst[d] = (T)(l > 0.0f ? v / l : 0.0f);
@@ -301,36 +318,482 @@ __global__ __launch_bounds__(NW * 64) void paged_split_kernel(PagedArgs a) {
   }
 }
 
-// Joins the ranges of one (token, query head): a workgroup per row, wave w the ranges w, w + NW, ...,
-// lane d the dims d and d + 64.
-constexpr int kMergeWaves = 8;
+// ---- blocks of rows that share K and V through LDS
+//
+// A workgroup of CG x KG waves takes 32 CG rows of one kv head: wave (kg, cg) has 32 rows (two MFMA
+// column tiles) over the 32-position chunks kg, kg + KG, ... of the block's range. The waves of a K
+// group share each chunk's K and V tiles through an S-slot LDS ring filled by 16-byte loads to LDS (a
+// tile's lane l reads the 16 bytes lane l wrote: no bank conflicts), so a byte from L2 serves 32 CG
+// rows and a byte from LDS 32. One barrier per chunk; a chunk's V, and with four slots the next
+// chunk's K, leaves LDS before the MFMAs ahead of those that need it. P.V is O^T = V^T P with the row
+// as the column, so a lane's scores, maximum, sum and outputs are the same rows' and the online softmax
+// needs no shuffles beyond the maximum over a tile's positions. Chunks that every row sees whole run
+// without masks. Page ids come through the scalar cache, one chunk ahead of their loads.
+//
+// MODE 0: the rows of one sequence's new tokens over its visible chunks. Sequence b's tiles begin at
+// index cu[b] gq / rows + b (n gq rows need at most one tile more than floor((cu + n) gq / rows) -
+// floor(cu gq / rows)); a workgroup finds its sequence with a binary search. MODE 1: the rows of all
+// tokens over the shared prefix.
+constexpr uint32_t kDead = 0x80000000u;  // buffer offset past every resource: the load returns 0
+constexpr int kAll = 0x7fffffff;
 
-template <typename E, int HD>
-__global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_kernel(PagedArgs a) {
+typedef const __attribute__((address_space(4))) int32_t* ScalarInts;  // read through the scalar cache
+
+struct Block {
+  int b, row0, pos0;     // MODE 0: the sequence, its first row and position
+  int r0, rows;          // the block's first row (of the sequence's, or of the call's) and its number
+  int first, last;       // positions of the first and last row (MODE 0)
+  int cs, lo, n;         // visible chunks
+};
+// The block of tile x (uniform). rows == 0: none.
+template <int MODE>
+__device__ __forceinline__ Block find_block(const PagedArgs& a, int x, int BT) {
+  Block k{};
+  if constexpr (MODE == 1) {
+    k.r0 = x * BT;
+    k.rows = min(BT, a.T * a.gq - k.r0);
+    k.last = kAll;
+    k.n = a.pchunks;
+    return k;
+  }
+  int b = 0;
+  for (int lo = 0, hi = a.B; lo < hi;) {
+    const int mid = (lo + hi) / 2;
+    if ((int64_t)(a.cu ? max(a.cu[mid], 0) : mid) * a.gq / BT + mid <= x)
+      b = mid, lo = mid + 1;
+    else
+      hi = mid;
+  }
+  const SeqRows s = seq_rows(a.cu, a.kv_lens, b, a.T);
+  const int n = min(s.n, a.max_q);
+  k.b = b;
+  k.row0 = s.row0;
+  k.pos0 = s.pos0;
+  k.r0 = (x - (int)(s.row0 * (int64_t)a.gq / BT) - b) * BT;
+  k.rows = k.r0 < 0 ? 0 : max(0, min(BT, n * a.gq - k.r0));
+  if (k.rows <= 0) return k;
+  k.first = k.pos0 + k.r0 / a.gq;
+  k.last = k.pos0 + (k.r0 + k.rows - 1) / a.gq;
+  const int hi = min(k.last, a.cap - 1), hc = hi < 0 ? 0 : hi / kChunkPos + 1;
+  k.lo = min(a.window > 0 ? max(0, k.first - a.window + 1) / kChunkPos : 0, hc);
+  k.cs = min((min(a.sinks, a.cap) + kChunkPos - 1) / kChunkPos, k.lo);
+  k.n = k.cs + hc - k.lo;
+  return k;
+}
+// Chunks of a block's range, a multiple of kg, and its ranges.
+__device__ __forceinline__ int block_range(const PagedArgs& a, int n, int kg) {
+  const int per = (n + a.bsplits - 1) / a.bsplits, least = 2 * kg;
+  return max(least, (per + kg - 1) / kg * kg);
+}
+// The position of row t of the call's (-1: no sequence's), by its sequence.
+__device__ __forceinline__ int row_position(const PagedArgs& a, int t) {
+  int b = t;
+  if (a.cu) {
+    b = -1;
+    for (int lo = 0, hi = a.B; lo < hi;) {  // the last b with cu[b] <= t
+      const int mid = (lo + hi) / 2;
+      if (a.cu[mid] <= t)
+        b = mid, lo = mid + 1;
+      else
+        hi = mid;
+    }
+    if (b < 0) return -1;
+  }
+  const SeqRows s = seq_rows(a.cu, a.kv_lens, b, a.T);
+  return t - s.row0 < min(s.n, a.max_q) ? s.pos0 + t - s.row0 : -1;
+}
+
+template <typename E, int HD, int CG, int KG, int S, int MODE>
+__global__ __launch_bounds__(CG* KG * 64) __attribute__((amdgpu_waves_per_eu(2))) void paged_block_kernel(PagedArgs a) {
+  typedef typename E::T T;
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  constexpr int BT = 32 * CG, NS = HD / 32, NB = HD / 16;
+  constexpr int KB = kChunkPos * HD * 2;  // bytes of a chunk's K (and of its V): NB tiles
+  constexpr int LI = NB / CG;             // K (and V) tiles each wave loads per chunk
+  constexpr bool AHEAD = S >= 4;          // deep enough to read the next chunk's K a step early
+  static_assert(CG * LI == NB && S >= 2, "whole loads per wave, two slots");
+  static_assert(KG * S * 2 * KB >= (KG - 1) * CG * 2 * NB * 64 * 16, "the K groups meet in the ring");
+  __shared__ __align__(16) unsigned char ring[KG * S * 2 * KB];
+  __shared__ float mls[CG * KG][4][64];  // the K groups' m and l per column tile and lane
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kg = wave / CG, cg = wave % CG;
+  const int c16 = lane & 15, kb = lane >> 4;
+  const int kvh = (int)blockIdx.x % a.nkv, tile = a.btiles - 1 - (int)blockIdx.x / a.nkv;  // longest blocks first
+  const int split = (int)blockIdx.y;
+  const Block bk = find_block<MODE>(a, tile, BT);
+  if (bk.rows <= 0) return;
+  const int per = block_range(a, bk.n, KG);
+  const int j0 = split * per;
+  if (split && j0 >= bk.n) return;  // the first range runs with no chunk too: its rows are written
+  const int nsteps = max(0, min(per, bk.n - j0));
+  const int n = (nsteps + KG - 1) / KG;  // steps of a K group (the last ones may be dead)
+
+  // this lane's two rows see the positions above hi - window up to hi, and those below sinks; rows past
+  // the block's are not stored. thi, tlo: last and first of the column tiles (what V is kept of); all_hi,
+  // all_lo: of the block (which chunks every row sees whole)
+  const int window = a.window > 0 ? a.window : kAll;
+  auto row_of = [&](int ct, int ln, int& tok, int& head) __attribute__((always_inline)) {
+    const int r = bk.r0 + min(32 * cg + 16 * ct + (ln & 15), bk.rows - 1);
+    tok = r / a.gq;
+    head = kvh * a.gq + r % a.gq;
+  };
+  int hi[2], thi[2], tlo[2], all_hi, all_lo = 0;
+#pragma unroll
+  for (int ct = 0; ct < 2; ++ct) {
+    int t, h;
+    row_of(ct, lane, t, h);
+    const int p = max(-1, MODE == 1 ? row_position(a, t) : bk.pos0 + t);
+    const int l = max(0, p - window + 1);
+    hi[ct] = p;
+    // over the 16 rows (all four lane groups hold the same 16)
+    int mx = p, mn = l;
+#pragma unroll
+    for (int off = 1; off < 16; off *= 2) {
+      mx = max(mx, __shfl_xor(mx, off));
+      mn = min(mn, __shfl_xor(mn, off));
+    }
+    thi[ct] = __builtin_amdgcn_readfirstlane(mx);
+    tlo[ct] = __builtin_amdgcn_readfirstlane(mn);
+  }
+  if constexpr (MODE == 1) {
+    int mn = kAll;
+    for (int i = lane; i < bk.rows; i += 64) {
+      const int p = row_position(a, (bk.r0 + i) / a.gq);
+      mn = p < 0 ? mn : min(mn, p);  // rows without a position: the merge takes nothing of them
+    }
+#pragma unroll
+    for (int off = 1; off < 64; off *= 2) mn = min(mn, __shfl_xor(mn, off));
+    all_hi = __builtin_amdgcn_readfirstlane(mn);
+  } else {
+    all_hi = bk.first;
+    all_lo = a.window > 0 ? max(0, bk.last - a.window + 1) : 0;
+  }
+  const int whi = max(thi[0], thi[1]), wlo = min(tlo[0], tlo[1]);  // of the wave's rows
+
+  // the block's chunks in order: those that every row sees whole (fl .. fl + nf - 1), the sinks', the others
+  const int fl = max(bk.lo, (all_lo + kChunkPos - 1) / kChunkPos);
+  const int nf = max(0, min(bk.lo + bk.n - bk.cs, (min(all_hi, kAll - 1) + 1) / kChunkPos) - fl);
+  auto chunk_of = [&](int j) __attribute__((always_inline)) {
+    const int i = j0 + j * KG + kg;
+    int d = i - nf - bk.cs + bk.lo < fl ? bk.lo - nf - bk.cs : bk.lo - bk.cs;
+    d = i < nf + bk.cs ? -nf : d;
+    return i + (i < nf ? fl : d);
+  };
+  // Step j of this K group loads from: the chunk's page, its id read through the scalar cache, and its place
+  // in the page. No page (an id outside the pool, a step past the range): zeros are loaded
+  const ScalarInts table = (ScalarInts)(uintptr_t)(MODE == 1 ? a.ptable : a.table + (int64_t)bk.b * a.ldt);
+  int page, sub;
+  auto next_page = [&](int j) __attribute__((always_inline)) {
+    const bool in = j * KG + kg < nsteps;
+    int at;
+    chunk_page(a.cpp, in ? chunk_of(j) : 0, at, sub);
+    page = table[at];  // first used a step later
+  };
+  const uint32_t lane_off = (uint32_t)(c16 * 64 + kb * 16);
+  unsigned char* const kring = ring + kg * S * 2 * KB;
+  unsigned char* const vring = kring + KB;
+  // K or V of the chunk into slot j % S
+  auto usable = [&](int j) __attribute__((always_inline)) { return j * KG + kg < nsteps && (uint32_t)page < (uint32_t)a.pages; };
+  auto load = [&](const void* pool, int64_t stride, unsigned char* slots, int j) __attribute__((always_inline)) {
+    const bool ok = usable(j);
+    const int64_t at = (int64_t)(ok ? page : 0) * stride + (int64_t)(kvh * (int)a.cpp.n + sub) * (kChunkPos * HD);
+    const u32x4 rs = raw_rsrc_uniform((const T*)pool + at, ok ? KB : 0);
+#pragma unroll
+    for (int i = 0; i < LI; ++i)
+      dma_buffer16(rs, lane_off + (uint32_t)((cg * LI + i) * 1024), 0u,
+                   lds_addr(slots + (j % S) * 2 * KB + (cg * LI + i) * 1024));
+  };
+  uint32_t have = 0;  // bit i: whether the step i before the last one loaded has a page
+  int nfull = min((nsteps + KG - 1) / KG, max(0, nf - j0 - kg + KG - 1) / KG);  // unmasked steps: to the first without one
+  auto loaded = [&](int j) __attribute__((always_inline)) {
+    const bool ok = usable(j);
+    have = __builtin_amdgcn_readfirstlane(have << 1 | (ok ? 1u : 0u));
+    nfull = __builtin_amdgcn_readfirstlane(ok ? nfull : min(nfull, j));
+    next_page(j + 1);
+  };
+  next_page(0);
+#pragma unroll
+  for (int j = 0; j < S - 1; ++j) {
+    load(a.k, a.kps, kring, j);
+    load(a.vt, a.vps, vring, j);
+    loaded(j);
+  }
+
+  // this wave's q operands: waited for here, once, so that the compiler has no load of its own left to
+  // wait for inside the loop (its count does not know the loads to LDS)
+  u32x4 q[2][NS];
+#pragma unroll
+  for (int ct = 0; ct < 2; ++ct) {
+    int t, h;
+    row_of(ct, lane, t, h);
+    const T* src = (const T*)a.q + (int64_t)(bk.row0 + t) * a.ldq + (int64_t)h * HD + 8 * kb;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) q[ct][s] = *reinterpret_cast<const u32x4*>(src + 32 * s);
+  }
+#pragma unroll
+  for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+    for (int s = 0; s < NS; ++s) asm volatile("" : "+v"(q[ct][s]));
+
+  const float sc = a.scale * 1.44269504088896341f;
+  float m_run[2] = {-__builtin_inff(), -__builtin_inff()}, l_lane[2] = {0.0f, 0.0f};
+  float4_t o[2][NB];   // O^T[dim 16b + 4kb + r][row c16], unnormalised
+  float4_t acc[2][2];  // [row half hb][column tile]: scores of positions 8kb + 4hb + r
+  u32x4 ph[2];         // numerators: the B operand of P.V
+#pragma unroll
+  for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+    for (int b = 0; b < NB; ++b) o[ct][b] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+
+  u32x4 kt[NB], vv[NB];  // a chunk's K and V, read ahead of the MFMAs before the ones that use them
+  auto tiles = [&](u32x4 (&t)[NB], const unsigned char* src) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i) t[i] = *reinterpret_cast<const u32x4*>(src + i * 1024 + lane * 16);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto scores = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int hb = 0; hb < 2; ++hb)
+#pragma unroll
+      for (int ct = 0; ct < 2; ++ct) acc[hb][ct] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int hb = 0; hb < 2; ++hb)
+#pragma unroll
+        for (int ct = 0; ct < 2; ++ct) acc[hb][ct] = E::mfma(kt[NS * hb + s], q[ct][s], acc[hb][ct]);
+  };
+  auto pv = [&](auto maskedc, int cb0) __attribute__((always_inline)) {
+    uint32_t mk[2][4];
+    if constexpr (decltype(maskedc)::value) {  // zero V that no row of the tile sees (0 x NaN)
+#pragma unroll
+      for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int p0 = cb0 + 8 * kb + 2 * e;
+          mk[ct][e] = (p0 <= thi[ct] && (p0 >= tlo[ct] || p0 < a.sinks) ? 0x0000FFFFu : 0u) |
+                      (p0 + 1 <= thi[ct] && (p0 + 1 >= tlo[ct] || p0 + 1 < a.sinks) ? 0xFFFF0000u : 0u);
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int ct = 0; ct < 2; ++ct) {
+        u32x4 v = vv[b];
+        if constexpr (decltype(maskedc)::value)
+          v = u32x4{v[0] & mk[ct][0], v[1] & mk[ct][1], v[2] & mk[ct][2], v[3] & mk[ct][3]};
+        o[ct][b] = E::mfma(v, ph[ct], o[ct][b]);
+      }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // The rescale is skipped while no row of the tile sees a larger score (its factor is then 1).
+  float nb[2] = {0.0f, 0.0f};  // -m_run * sc, 0 while m_run is -inf
+  auto softmax = [&](auto maskedc, int cb0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int ct = 0; ct < 2; ++ct) {
+      float mc = -__builtin_inff();
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (decltype(maskedc)::value) {
+          const int p = cb0 + 8 * kb + e;
+          if (p > hi[ct] || (p <= hi[ct] - window && p >= a.sinks)) acc[e >> 2][ct][e & 3] = -__builtin_inff();
+        }
+        mc = fmaxf(mc, acc[e >> 2][ct][e & 3]);
+      }
+      mc = max_xor32(max_xor16(mc));
+      if (__any(mc > m_run[ct])) {
+        const float m_new = fmaxf(m_run[ct], mc);
+        // a row that has seen nothing so far keeps m = -inf; its factor is taken against 0
+        nb[ct] = m_new == -__builtin_inff() ? 0.0f : m_new * -sc;
+        const float alpha = __builtin_amdgcn_exp2f(__builtin_fmaf(m_run[ct], sc, nb[ct]));
+        l_lane[ct] *= alpha;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) o[ct][b] *= alpha;
+        m_run[ct] = m_new;
+      }
+      float x[8], ls = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[e >> 2][ct][e & 3], sc, nb[ct]));
+        ls += x[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) ph[ct][e] = pack2<E>(x[2 * e], x[2 * e + 1]);
+      l_lane[ct] += ls;
+    }
+  };
+  auto step = [&](auto maskedc, int j) __attribute__((always_inline)) {
+    // stage j (and with a deep ring j + 1) has landed, and every wave is done with step j - 1, whose
+    // slot takes stage j + S - 1
+    wait_vm<AHEAD ? (S - 3) * 2 * LI : (S - 2) * 2 * LI>();
+    ring_barrier();
+    const int cb0 = chunk_of(j) * kChunkPos;
+    const bool live = !decltype(maskedc)::value || ((have >> (S - 2) & 1) && cb0 <= whi && (cb0 + kChunkPos > wlo || cb0 < a.sinks));
+    if (!AHEAD && live) tiles(kt, kring + (j % S) * 2 * KB);
+    if (live) scores();
+    load(a.k, a.kps, kring, j + S - 1);
+    if (live) {
+      tiles(vv, vring + (j % S) * 2 * KB);
+      softmax(maskedc, cb0);
+    }
+    load(a.vt, a.vps, vring, j + S - 1);
+    loaded(j + S - 1);
+    if (AHEAD) tiles(kt, kring + ((j + 1) % S) * 2 * KB);
+    if (live) pv(maskedc, cb0);
+    __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4));  // lgkmcnt(0): no LDS read is left pending
+  };
+  wait_vm<0>();  // the first stages, with q
+  ring_barrier();
+  if (AHEAD) tiles(kt, kring);
+  int j = 0;
+  for (; j < nfull; ++j) step(IntC<0>(), j);
+  for (; j < n; ++j) step(IntC<1>(), j);
+  wait_vm<0>();
+  __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4));
+  ring_barrier();  // the ring is free: every wave's loads have landed and its reads are done
+
+  // ---- the K groups meet: groups past the first leave m, l and O, lane for lane
+  float l_w[2];
+#pragma unroll
+  for (int ct = 0; ct < 2; ++ct) l_w[ct] = add_xor32(add_xor16(l_lane[ct]));
+  float4_t* const red = reinterpret_cast<float4_t*>(ring);  // [wave - CG][2 NB][64]
+  if (kg > 0) {
+#pragma unroll
+    for (int ct = 0; ct < 2; ++ct) {
+      mls[wave][2 * ct][lane] = m_run[ct];
+      mls[wave][2 * ct + 1][lane] = l_w[ct];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) red[((wave - CG) * 2 * NB + NB * ct + b) * 64 + lane] = o[ct][b];
+    }
+  }
+  lds_barrier();
+  if (kg > 0) return;
+  const bool direct = a.bdirect && bk.n <= per;  // a lone range
+  float* const part = a.bpart + (((int64_t)tile * a.nkv + kvh) * a.bsplits + split) * BT * (2 + HD);
+#pragma unroll
+  for (int ct = 0; ct < 2; ++ct) {
+    float mv[KG], lv[KG], M = m_run[ct];
+    mv[0] = m_run[ct];
+    lv[0] = l_w[ct];
+#pragma unroll
+    for (int g = 1; g < KG; ++g) {
+      mv[g] = mls[cg + g * CG][2 * ct][lane];
+      lv[g] = mls[cg + g * CG][2 * ct + 1][lane];
+      M = fmaxf(M, mv[g]);
+    }
+    float f[KG], l = 0.0f;
+#pragma unroll
+    for (int g = 0; g < KG; ++g) {
+      f[g] = mv[g] != -__builtin_inff() ? __builtin_amdgcn_exp2f((mv[g] - M) * sc) : 0.0f;
+      l = __builtin_fmaf(lv[g], f[g], l);
+    }
+    const int col = 32 * cg + 16 * ct + c16;
+    int t, h, ln = lane;
+    asm volatile("" : "+v"(ln));  // formed again here rather than kept in registers over the loop
+    row_of(ct, ln, t, h);
+    T* dst = (T*)a.out + (int64_t)(bk.row0 + t) * a.ldo + (int64_t)h * HD + 4 * kb;
+    float* pdst = part + 2 * BT + col * HD + 4 * kb;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      float4_t v = o[ct][b] * f[0];
+#pragma unroll
+      for (int g = 1; g < KG; ++g) {
+        const float4_t w = red[((cg + (g - 1) * CG) * 2 * NB + NB * ct + b) * 64 + lane];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = __builtin_fmaf(w[r], f[g], v[r]);
+      }
+      if (col < bk.rows) {
+        if (direct) {
+          T4 y;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) y[r] = (T)(l > 0.0f ? v[r] / l : 0.0f);
+          *reinterpret_cast<T4*>(dst + 16 * b) = y;
+        } else {
+          *reinterpret_cast<float4_t*>(pdst + 16 * b) = v;
+        }
+      }
+    }
+    if (!direct && kb == 0 && col < bk.rows) {
+      part[2 * col] = M;
+      part[2 * col + 1] = l;
+    }
+  }
+}
+
+// ---- joining the ranges of one (token, query head)
+//
+// MW waves per row: wave w takes ranges w, w + MW, ..., lane d the dims d and d + 64; the waves meet in
+// LDS. Rows come from paged_split_kernel's slots, from paged_block_kernel's splits, or (behind a shared
+// prefix) from both; ones whose only range has written the output are left alone.
+template <typename E, int HD, int MW, int BT>
+__global__ __launch_bounds__(MW * 64) void paged_merge_kernel(PagedArgs a) {
   typedef typename E::T T;
   constexpr int ND = HD / 64;
-  __shared__ float ms[kMergeWaves], ls[kMergeWaves], os[kMergeWaves][HD];
-  const int b = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 63;
+  __shared__ float ms[MW], ls[MW], os[MW][HD];
+  const int h = blockIdx.y, lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int first = a.plan[2 * b], n = a.plan[2 * b + 1];
-  if (n <= 1) return;
+  const int t = blockIdx.x, kvh = h / a.gq;
+  int b = t;
+  if (a.cu) {
+    b = -1;
+    for (int lo = 0, hi = a.B; lo < hi;) {
+      const int mid = (lo + hi) / 2;
+      if (a.cu[mid] <= t)
+        b = mid, lo = mid + 1;
+      else
+        hi = mid;
+    }
+    if (b < 0) return;
+  }
   const SeqRows s = seq_rows(a.cu, a.kv_lens, b, a.T);
-  const int tok = blockIdx.x;
+  const int tok = t - s.row0;
   if (tok >= min(s.n, a.max_q)) return;
-  const int kvh = h / a.gq, row = tok * a.gq + h % a.gq, tile = row / kRows, j = row % kRows;
+  const int row = tok * a.gq + h % a.gq;
   const float sc = a.scale * 1.44269504088896341f;
-  const int64_t step = (int64_t)a.nkv * a.nt * part_floats(HD);
-  const float* p0 = a.part + ((int64_t)first * a.nkv * a.nt + tile * a.nkv + kvh) * part_floats(HD);
+  // the two lists: {m, l} and outputs of range i at p + i * step
+  int na = 0, nb = 0, ja = 0, jb = 0;
+  const float *pa = nullptr, *pb = nullptr;
+  int64_t sa = 0;
+  if (a.slots) {
+    na = a.plan[2 * b + 1];
+    if (na <= 1 && !a.skip) return;
+    ja = row % kRows;
+    sa = (int64_t)a.nkv * a.nt * part_floats(HD);
+    pa = a.part + ((int64_t)a.plan[2 * b] * a.nkv * a.nt + row / kRows * a.nkv + kvh) * part_floats(HD);
+  }
+  if (s.pos0 + tok < 0) {
+    na = 0;  // sees nothing: zeros
+  } else if (a.bsplits) {
+    int tile, n;
+    if (a.bdirect) {
+      tile = (int)(s.row0 * (int64_t)a.gq / BT) + b + row / BT;
+      const Block bk = find_block<0>(a, tile, BT);
+      n = bk.n;
+      jb = row % BT;
+    } else {
+      const int r = t * a.gq + h % a.gq;
+      tile = r / BT;
+      n = a.pchunks;
+      jb = r % BT;
+    }
+    const int per = block_range(a, n, kBlockKG<BT>);
+    nb = (n + per - 1) / per;
+    if (a.bdirect && nb <= 1) return;
+    pb = a.bpart + ((int64_t)tile * a.nkv + kvh) * a.bsplits * BT * (2 + HD);
+  }
   float M = -__builtin_inff(), l = 0.0f, o[ND] = {};
-  for (int r = wave; r < n; r += kMergeWaves) {
-    const float* p = p0 + r * step;
+  for (int r = wave; r < na + nb; r += MW) {
+    const bool first = r < na;
+    const float* p = first ? pa + r * sa : pb + (int64_t)(r - na) * BT * (2 + HD);
+    const int j = first ? ja : jb, rows = first ? kRows : BT;
     const float m = p[2 * j], lr = p[2 * j + 1];
     const float mn = fmaxf(M, m);
     const float f0 = M == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((M - mn) * sc);
     const float f1 = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * sc);
     l = l * f0 + lr * f1;
 #pragma unroll
-    for (int i = 0; i < ND; ++i) o[i] = o[i] * f0 + p[2 * kRows + j * HD + lane + 64 * i] * f1;
+    for (int i = 0; i < ND; ++i) o[i] = o[i] * f0 + p[2 * rows + j * HD + lane + 64 * i] * f1;
     M = mn;
   }
   if (lane == 0) {
@@ -340,41 +803,77 @@ __global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_kernel(PagedArgs
 #pragma unroll
   for (int i = 0; i < ND; ++i) os[wave][lane + 64 * i] = o[i];
   __syncthreads();
-  for (int d = threadIdx.x; d < HD; d += kMergeWaves * 64) {
+  for (int d = threadIdx.x; d < HD; d += MW * 64) {
     float MM = -__builtin_inff(), L = 0.0f, v = 0.0f;
-    for (int w = 0; w < kMergeWaves; ++w) MM = fmaxf(MM, ms[w]);
-    for (int w = 0; w < kMergeWaves; ++w) {
+#pragma unroll
+    for (int w = 0; w < MW; ++w) MM = fmaxf(MM, ms[w]);
+#pragma unroll
+    for (int w = 0; w < MW; ++w) {
       const float f = ms[w] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((ms[w] - MM) * sc);
       L += ls[w] * f;
       v += os[w][d] * f;
     }
-    ((T*)a.out)[(int64_t)(s.row0 + tok) * a.ldo + (int64_t)h * HD + d] = (T)(L > 0.0f ? v / L : 0.0f);
+    ((T*)a.out)[(int64_t)t * a.ldo + (int64_t)h * HD + d] = (T)(L > 0.0f ? v / L : 0.0f);
   }
 }
 
 // What a call launches, from its sizes alone.
 struct Plan {
-  int nt, slots;
-  int64_t part_bytes, bytes;  // the partials', and with the plan's after them
+  int nt = 0, slots = 0;                   // paged_split_kernel, slots == 0: not launched
+  int bt = 0, btiles = 0, bsplits = 0;     // paged_block_kernel, bt == 0: not launched
+  int64_t part_bytes = 0, bpart_bytes = 0, bytes = 0;
 };
-Plan make_plan(int64_t B, int64_t max_q, int nq, int nkv, int hd) {
+Plan make_plan(int64_t T, int64_t B, int64_t max_q, int64_t prefix_len, int nq, int nkv, int hd) {
   Plan p;
-  p.nt = (int)((max_q * (nq / nkv) + kRows - 1) / kRows);
-  // about two workgroups per CU beyond one for each sequence
-  const int64_t spare = std::max<int64_t>(1, 512 / ((int64_t)nkv * p.nt));
-  p.slots = (int)(B + spare);
-  p.part_bytes = (int64_t)p.slots * nkv * p.nt * part_floats(hd) * 4;
-  p.bytes = p.part_bytes + B * 8;
+  const int64_t gq = nq / nkv;
+  const bool block = max_q * gq > 2 * kRows;  // rows of a sequence past two tiles: they share K and V in LDS
+  if (prefix_len || !block) {
+    p.nt = (int)((max_q * gq + kRows - 1) / kRows);
+    // about two workgroups per CU beyond one for each sequence
+    const int64_t spare = std::max<int64_t>(1, 512 / ((int64_t)nkv * p.nt));
+    p.slots = (int)(B + spare);
+    p.part_bytes = (int64_t)p.slots * nkv * p.nt * part_floats(hd) * 4;
+  }
+  if (prefix_len || block) {
+    const int64_t rows = T * gq;
+    // 128 rows where they give the CUs a workgroup each, else 64
+    auto tiles = [&](int bt) { return prefix_len ? (rows + bt - 1) / bt : rows / bt + B; };
+    p.bt = nkv * tiles(128) >= 256 || (prefix_len && rows > 64) ? 128 : 64;
+    p.btiles = (int)tiles(p.bt);
+    p.bsplits = (int)std::max<int64_t>(1, std::min<int64_t>(32, 320 / ((int64_t)nkv * p.btiles)));
+    if (prefix_len || p.bsplits > 1) p.bpart_bytes = (int64_t)p.btiles * nkv * p.bsplits * p.bt * (2 + hd) * 4;
+  }
+  p.bytes = p.part_bytes + p.bpart_bytes + B * 8;
   return p;
 }
 
+template <typename E, int HD, int MODE>
+int launch_block(const PagedArgs& a, const Plan& p, hipStream_t s) {
+  const dim3 grid((unsigned)p.btiles * a.nkv, (unsigned)p.bsplits);
+  if (p.bt == 128)
+    paged_block_kernel<E, HD, 4, kBlockKG<128>, 4, MODE><<<grid, 512, 0, s>>>(a);
+  else
+    paged_block_kernel<E, HD, 2, kBlockKG<64>, 2, MODE><<<grid, 512, 0, s>>>(a);
+  return ldk::check_launch("paged_attention block");
+}
+
 template <typename E, int HD>
-int launch(const PagedArgs& a, hipStream_t s) {
+int launch(const PagedArgs& a, const Plan& p, hipStream_t s) {
   (void)hipGetLastError();
-  paged_split_kernel<E, HD, 8><<<(unsigned)a.slots * a.nkv * a.nt, 8 * 64, 0, s>>>(a);
-  const int st = ldk::check_launch("paged_attention");
+  int st = LDK_OK;
+  if (p.bt) st = a.pchunks ? launch_block<E, HD, 1>(a, p, s) : launch_block<E, HD, 0>(a, p, s);
   if (st) return st;
-  paged_merge_kernel<E, HD><<<dim3((unsigned)a.max_q, (unsigned)a.nq, (unsigned)a.B), kMergeWaves * 64, 0, s>>>(a);
+  if (p.slots) {
+    paged_split_kernel<E, HD, 8><<<(unsigned)a.slots * a.nkv * a.nt, 8 * 64, 0, s>>>(a);
+    st = ldk::check_launch("paged_attention split");
+    if (st) return st;
+  }
+  if (!p.slots && p.bsplits == 1) return LDK_OK;
+  const dim3 grid((unsigned)a.T, (unsigned)a.nq);
+  if (p.bt == 128)
+    paged_merge_kernel<E, HD, 8, 128><<<grid, 8 * 64, 0, s>>>(a);
+  else
+    paged_merge_kernel<E, HD, 8, 64><<<grid, 8 * 64, 0, s>>>(a);
   return ldk::check_launch("paged_attention merge");
 }
 
@@ -409,18 +908,29 @@ int run(const char* fn, const void* q, int64_t ldq, int dtype, const int32_t* cu
       ldo % 8 || kps % 8 || vps % 8 || !ldk::aligned(kv_lens, 4) || !ldk::aligned(cu, 4) || !ldk::aligned(table, 4) ||
       !ldk::aligned(ptable, 4) || !ldk::aligned(ws, 16))
     return ldk::fail(LDK_ERR_ALIGN, "%s: q, out, workspace and the pages 16-byte aligned with strides of multiples of 8 elements", fn);
-  const Plan p = make_plan(B, cu ? max_q : 1, nq, nkv, hd);
+  const Plan p = make_plan(cu ? T : B, B, cu ? max_q : 1, prefix_len, nq, nkv, hd);
   if (!ws || ws_bytes < p.bytes)
     return ldk::fail(LDK_ERR_INVALID, "%s: workspace of %lld bytes, this call needs %lld", fn, (long long)ws_bytes, (long long)p.bytes);
-  if ((int64_t)p.slots * nkv * p.nt > INT32_MAX) return ldk::fail(LDK_ERR_UNSUPPORTED, "%s: too many workgroups", fn);
+  if ((int64_t)p.slots * nkv * p.nt > INT32_MAX || (int64_t)p.btiles * nkv > INT32_MAX) return ldk::fail(LDK_ERR_UNSUPPORTED, "%s: too many workgroups", fn);
   const int big = 1 << 30;  // a window or sinks past every position
-  PagedArgs a{q, ldq, cu, kv_lens, table, ptable, ldt, k, vt, kps, vps, out, ldo, (float*)ws,
-              (int32_t*)((char*)ws + p.part_bytes), cu ? (int)T : (int)B, (int)B, cu ? (int)max_q : 1, nq, nkv, nq / nkv, p.nt,
-              (int)num_pages, (int)(page_size / 32), (int)(max_pages * page_size), (int)(prefix_len / 32),
-              (int)std::min<int64_t>(window, big), (int)std::min<int64_t>(sinks, big), p.slots, scale};
+  PagedArgs a{};
+  a.q = q, a.ldq = ldq, a.out = out, a.ldo = ldo;
+  a.cu = cu, a.kv_lens = kv_lens, a.table = table, a.ptable = ptable, a.ldt = ldt;
+  a.k = k, a.vt = vt, a.kps = kps, a.vps = vps;
+  a.part = (float*)ws;
+  a.bpart = (float*)((char*)ws + p.part_bytes);
+  a.plan = (int32_t*)((char*)ws + p.part_bytes + p.bpart_bytes);
+  a.T = cu ? (int)T : (int)B, a.B = (int)B, a.max_q = cu ? (int)max_q : 1;
+  a.nq = nq, a.nkv = nkv, a.gq = nq / nkv, a.nt = p.nt;
+  a.pages = (int)num_pages, a.cpp = page_div(page_size / kChunkPos), a.cap = (int)(max_pages * page_size);
+  a.pchunks = a.skip = (int)(prefix_len / kChunkPos);
+  a.window = (int)std::min<int64_t>(window, big), a.sinks = (int)std::min<int64_t>(sinks, big);
+  a.slots = p.slots;
+  a.btiles = p.btiles, a.bsplits = p.bsplits, a.bdirect = !prefix_len;
+  a.scale = scale;
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == LDK_F16) return hd == 128 ? launch<ldk::F16, 128>(a, s) : launch<ldk::F16, 64>(a, s);
-  return hd == 128 ? launch<ldk::BF16, 128>(a, s) : launch<ldk::BF16, 64>(a, s);
+  if (dtype == LDK_F16) return hd == 128 ? launch<ldk::F16, 128>(a, p, s) : launch<ldk::F16, 64>(a, p, s);
+  return hd == 128 ? launch<ldk::BF16, 128>(a, p, s) : launch<ldk::BF16, 64>(a, p, s);
 }
 
 }  // namespace
@@ -432,7 +942,7 @@ extern "C" int64_t ldk_paged_attention_workspace_bytes(int64_t T, int64_t B, int
     return -ldk::fail(LDK_ERR_INVALID, "paged_attention_workspace_bytes: T=%lld B=%lld max_q=%lld prefix_len=%lld nq=%d nkv=%d head_dim=%d",
                       (long long)T, (long long)B, (long long)max_q, (long long)prefix_len, nq, nkv, head_dim);
   }
-  return make_plan(B, max_q, nq, nkv, head_dim).bytes;
+  return make_plan(T, B, max_q, prefix_len, nq, nkv, head_dim).bytes;
 }
 
 extern "C" int ldk_paged_attention(const void* q, int64_t ldq, int dtype, const int32_t* cu_seqlens,

@@ -43,58 +43,94 @@ def vt_pages_shape(pages: int, n_kv: int, page: int, head_dim: int = 128) -> tup
     return (pages, n_kv, page // CHUNK, head_dim // 16, 16, 32)
 
 
+_CODES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+
+
+# The checks below run on every call of every layer of a step, so they read each property once and test
+# the good case in one expression; what is wrong is found out when something is.
 def _pool(k_pages: torch.Tensor, vt_pages: torch.Tensor, what: str):
     """(pages, n_kv, page, head_dim, k page stride, vt page stride) of a pool, checked."""
     ks, vs = k_pages.shape, vt_pages.shape
     if len(ks) != 7 or len(vs) != 6:
         raise ValueError(f"{what}: k_pages and vt_pages must be k_pages_shape and vt_pages_shape, got "
                          f"{tuple(ks)} and {tuple(vs)}")
-    pages, nkv, cpp, hd = ks[0], ks[1], ks[2], ks[4] * 32
-    page = cpp * CHUNK
-    if (ks[3] != 2 or ks[5] != 16 or ks[6] != 32 or vs[0] != pages or vs[1] != nkv or vs[2] != cpp
-            or vs[3] * 16 != hd or vs[4] != 16 or vs[5] != 32):
+    pages, nkv, cpp, halves, steps, rows, dims = ks
+    if halves != 2 or rows != 16 or dims != 32 or vs != (pages, nkv, cpp, 2 * steps, 16, 32):
         raise ValueError(f"{what}: k_pages and vt_pages must be k_pages_shape and vt_pages_shape of one pool, "
                          f"got {tuple(ks)} and {tuple(vs)}")
-    if k_pages.dtype != vt_pages.dtype:
+    if k_pages.dtype is not vt_pages.dtype:
         raise ValueError(f"{what}: k_pages {k_pages.dtype} and vt_pages {vt_pages.dtype} differ")
-    per = nkv * page * hd
-    kst, vst = (per, per) if pages == 1 else (k_pages.stride(0), vt_pages.stride(0))
+    per = nkv * cpp * steps * (CHUNK * 32)
+    if k_pages.is_contiguous() and vt_pages.is_contiguous():
+        return pages, nkv, cpp * CHUNK, steps * 32, per, per
     for t in (k_pages, vt_pages):
         if not (t.is_contiguous() or (pages and t[0].is_contiguous())):
             raise ValueError(f"{what}: a page's tiles must be contiguous")
-    return pages, nkv, page, hd, kst, vst
+    return (pages, nkv, cpp * CHUNK, steps * 32, k_pages.stride(0) if pages > 1 else per,
+            vt_pages.stride(0) if pages > 1 else per)
 
 
 def _batch(kv_lens: torch.Tensor, block_table: torch.Tensor, cu_seqlens: torch.Tensor | None, rows: int, what: str):
-    """(B, table row stride), of checked lengths, table and row bounds."""
-    B = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
-    if kv_lens.dtype != torch.int32 or B < 0 or (B > 1 and kv_lens.stride(0) != 1):
+    """(B, max_pages, table row stride), of checked lengths, table and row bounds."""
+    if kv_lens.dtype is not torch.int32 or kv_lens.dim() != 1 or not kv_lens.is_contiguous():
         raise ValueError(f"{what}: kv_lens must be a contiguous int32 [B]")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or (
-            block_table.shape[1] > 1 and block_table.stride(1) != 1):
+    B = kv_lens.shape[0]
+    ts = block_table.shape
+    if block_table.dtype is not torch.int32 or len(ts) != 2 or ts[0] != B or not (
+            block_table.is_contiguous() or ts[1] <= 1 or block_table.stride(1) == 1):
         raise ValueError(f"{what}: block_table must be int32 [{B}, max_pages] with contiguous rows")
     if cu_seqlens is None:
         if rows < B:
             raise ValueError(f"{what}: {rows} rows for {B} sequences of one token (cu_seqlens=None)")
-    elif cu_seqlens.dtype != torch.int32 or cu_seqlens.shape != (B + 1,) or cu_seqlens.stride(0) != 1:
+    elif cu_seqlens.dtype is not torch.int32 or cu_seqlens.shape != (B + 1,) or not cu_seqlens.is_contiguous():
         raise ValueError(f"{what}: cu_seqlens must be a contiguous int32 [{B + 1}]")
-    return B, block_table.stride(0) if B > 1 else block_table.shape[1]
+    return B, ts[1], block_table.stride(0) if B > 1 else ts[1]
 
 
-def _heads(t: torch.Tensor, dtype: torch.dtype, hd: int, what: str, name: str) -> None:
-    if t.dim() != 3 or t.shape[2] != hd or t.dtype != dtype:
-        raise ValueError(f"{what}: {name} must be {dtype} [tokens, heads, {hd}], got {t.dtype} {tuple(t.shape)}")
+def _rows3(t: torch.Tensor, rows: int, heads: int, hd: int, dtype: torch.dtype, what: str, name: str) -> int:
+    """The row stride of t [rows, heads, hd] with contiguous heads; 0: its heads are not."""
+    if t.shape != (rows, heads, hd) or t.dtype is not dtype:
+        raise ValueError(f"{what}: {name} must be {dtype} [{rows}, {heads}, {hd}], got {t.dtype} {tuple(t.shape)}")
+    if t.is_contiguous():
+        return heads * hd
+    if t.stride(2) != 1 or (heads > 1 and t.stride(1) != hd):
+        return 0
+    return t.stride(0) if rows > 1 else heads * hd
 
 
-def _check_out(out: torch.Tensor, rows: int, heads: int, hd: int, dtype: torch.dtype, what: str) -> None:
-    _heads(out, dtype, hd, what, "out")
-    if out.shape[0] != rows or out.shape[1] != heads or out.stride(2) != 1 or (heads > 1 and out.stride(1) != hd):
-        raise ValueError(f"{what}: out must be [{rows}, {heads}, {hd}] with contiguous heads, got "
-                         f"{tuple(out.shape)} strides {out.stride()}")
+def _out_stride(out: torch.Tensor, rows: int, heads: int, hd: int, dtype: torch.dtype, what: str) -> int:
+    ldo = _rows3(out, rows, heads, hd, dtype, what, "out")
+    if not ldo:
+        raise ValueError(f"{what}: out must have contiguous heads, got strides {out.stride()}")
+    return ldo
 
 
-def _row_stride(t: torch.Tensor, width: int) -> int:
-    return t.stride(0) if t.shape[0] > 1 else width
+def _device(what: str, first: torch.Tensor, *others: torch.Tensor | None) -> int:
+    """The index of the GPU that all tensors are on."""
+    dev = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            dev = -1
+    if dev < 0:
+        _lib.require_gpu(first, *others, what=what)
+    return dev
+
+
+def _call(entry, dev: int, args: tuple, what: str) -> None:
+    """entry(*args, the device's current stream), with that device current. The callers hold the tensors
+    whose addresses the arguments are."""
+    cur = torch._C._cuda_getDevice()
+    if cur == dev:
+        st = entry(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with _lib.device_guard(torch.device("cuda", dev)):
+            st = entry(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if st:
+        _lib.check(st, what)
+
+
+def _addr(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
 
 
 def paged_append(qkv: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Tensor, k_pages: torch.Tensor,
@@ -110,75 +146,73 @@ def paged_append(qkv: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Te
     what = "paged_append"
     pages, nkv, page, hd, kst, vst = _pool(k_pages, vt_pages, what)
     width = (n_heads + 2 * nkv) * hd
-    if qkv.dim() != 2 or qkv.shape[1] != width or qkv.dtype != k_pages.dtype:
+    dtype = qkv.dtype
+    if qkv.dim() != 2 or qkv.shape[1] != width or dtype is not k_pages.dtype:
         raise ValueError(f"{what}: qkv must be {k_pages.dtype} [tokens, {width}], got {qkv.dtype} {tuple(qkv.shape)}")
     T = qkv.shape[0]
-    B, ldt = _batch(kv_lens, block_table, cu_seqlens, T, what)
-    if inv_freq is not None and (inv_freq.dtype != torch.float32 or inv_freq.shape != (hd // 2,) or inv_freq.stride(0) != 1):
+    B, max_pages, ldt = _batch(kv_lens, block_table, cu_seqlens, T, what)
+    if inv_freq is not None and (inv_freq.dtype is not torch.float32 or inv_freq.shape != (hd // 2,)
+                                 or not inv_freq.is_contiguous()):
         raise ValueError(f"{what}: inv_freq must be a contiguous float32 [{hd // 2}]")
-    if rope_pos is not None and (rope_pos.dtype != torch.int64 or rope_pos.shape != (T,) or (T > 1 and rope_pos.stride(0) != 1)):
+    if rope_pos is not None and (rope_pos.dtype is not torch.int64 or rope_pos.shape != (T,)
+                                 or not rope_pos.is_contiguous()):
         raise ValueError(f"{what}: rope_pos must be a contiguous int64 [{T}]")
-    if out is not None:
-        _check_out(out, T, n_heads, hd, qkv.dtype, what)
-    dev = _lib.require_gpu(qkv, kv_lens, block_table, k_pages, vt_pages, inv_freq, cu_seqlens, rope_pos, out, what=what)
-    q = torch.empty((T, n_heads, hd), dtype=qkv.dtype, device=dev) if out is None else out
+    ldq = n_heads * hd if out is None else _out_stride(out, T, n_heads, hd, dtype, what)
+    dev = _device(what, qkv, kv_lens, block_table, k_pages, vt_pages, inv_freq, cu_seqlens, rope_pos, out)
+    q = torch.empty((T, n_heads, hd), dtype=dtype, device=qkv.device) if out is None else out
     if not T or not B:
         return q
     x = qkv
-    if x.stride(1) != 1 or x.data_ptr() % 16 or _row_stride(x, width) % 8:
+    if not x.is_contiguous() and (x.stride(1) != 1 or (T > 1 and x.stride(0) % 8)):
         x = x.contiguous()
-    with _lib.device_guard(dev):
-        st = _lib.load().ldk_paged_append(
-            _lib.ptr(x), _row_stride(x, width), _lib.dtype_code(x.dtype), _lib.ptr(cu_seqlens), _lib.ptr(kv_lens),
-            _lib.ptr(block_table), ldt, block_table.shape[1], _lib.ptr(rope_pos), _lib.ptr(inv_freq),
-            _lib.ptr(k_pages), kst, _lib.ptr(vt_pages), vst, pages, page, _lib.ptr(q), _row_stride(q, n_heads * hd),
-            T, B, n_heads, nkv, hd, _lib.stream(dev))
-    _lib.check(st, what)
+    if x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+    _call(_lib.load().ldk_paged_append, dev,
+          (x.data_ptr(), x.stride(0) if T > 1 else width, _CODES.get(dtype, -1), _addr(cu_seqlens), kv_lens.data_ptr(),
+           block_table.data_ptr(), ldt, max_pages, _addr(rope_pos), _addr(inv_freq), k_pages.data_ptr(), kst,
+           vt_pages.data_ptr(), vst, pages, page, q.data_ptr(), ldq, T, B, n_heads, nkv, hd), what)
     return q
 
 
 def _attend(what, q, kv_lens, block_table, prefix_table, prefix_len, k_pages, vt_pages, scale, cu_seqlens, max_q, window,
             sinks, out):
     pages, nkv, page, hd, kst, vst = _pool(k_pages, vt_pages, what)
-    _heads(q, k_pages.dtype, hd, what, "q")
-    T, nq = q.shape[0], q.shape[1]
-    B, ldt = _batch(kv_lens, block_table, cu_seqlens, T, what)
-    if prefix_table is not None and (prefix_table.dtype != torch.int32 or prefix_table.dim() != 1
-                                     or prefix_table.shape[0] * page < prefix_len
-                                     or (prefix_table.shape[0] > 1 and prefix_table.stride(0) != 1)):
+    dtype = k_pages.dtype
+    if q.dim() != 3:
+        raise ValueError(f"{what}: q must be {dtype} [tokens, heads, {hd}], got {q.dtype} {tuple(q.shape)}")
+    T, nq, _ = q.shape
+    ldq = _rows3(q, T, nq, hd, dtype, what, "q")
+    B, max_pages, ldt = _batch(kv_lens, block_table, cu_seqlens, T, what)
+    if prefix_table is not None and (prefix_table.dtype is not torch.int32 or prefix_table.dim() != 1
+                                     or prefix_table.shape[0] * page < prefix_len or not prefix_table.is_contiguous()):
         raise ValueError(f"{what}: prefix_table must be a contiguous int32 of at least {prefix_len // page} pages")
-    if out is not None:
-        _check_out(out, T, nq, hd, q.dtype, what)
-    dev = _lib.require_gpu(q, kv_lens, block_table, prefix_table, k_pages, vt_pages, cu_seqlens, out, what=what)
-    o = torch.empty((T, nq, hd), dtype=q.dtype, device=dev) if out is None else out
+    ldo = nq * hd if out is None else _out_stride(out, T, nq, hd, dtype, what)
+    dev = _device(what, q, kv_lens, block_table, prefix_table, k_pages, vt_pages, cu_seqlens, out)
+    o = torch.empty((T, nq, hd), dtype=dtype, device=q.device) if out is None else out
     if not T or not B:
         return o
     x = q
-    if x.stride(2) != 1 or (nq > 1 and x.stride(1) != hd) or x.data_ptr() % 16 or _row_stride(x, 0) % 8:
-        x = x.contiguous()
+    if not ldq or ldq % 8:
+        x, ldq = x.contiguous(), nq * hd
+    if x.data_ptr() % 16:
+        x, ldq = x.clone(memory_format=torch.contiguous_format), nq * hd
     if cu_seqlens is None:
         max_q = 1
     elif max_q is None:
         max_q = T
     lib = _lib.load()
-    with _lib.device_guard(dev):
-        need = lib.ldk_paged_attention_workspace_bytes(T, B, max_q, prefix_len, nq, nkv, hd)
-        if need < 0:
-            _lib.check(-need, what)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        if prefix_table is None:
-            st = lib.ldk_paged_attention(
-                _lib.ptr(x), _row_stride(x, nq * hd), _lib.dtype_code(x.dtype), _lib.ptr(cu_seqlens), _lib.ptr(kv_lens),
-                _lib.ptr(block_table), ldt, block_table.shape[1], _lib.ptr(k_pages), kst, _lib.ptr(vt_pages), vst, pages,
-                page, _lib.ptr(o), _row_stride(o, nq * hd), T, B, max_q, nq, nkv, hd, window, sinks, float(scale),
-                _lib.ptr(ws), need, _lib.stream(dev))
-        else:
-            st = lib.ldk_shared_prefix_attention(
-                _lib.ptr(x), _row_stride(x, nq * hd), _lib.dtype_code(x.dtype), _lib.ptr(cu_seqlens), _lib.ptr(kv_lens),
-                _lib.ptr(block_table), ldt, block_table.shape[1], _lib.ptr(prefix_table), prefix_len, _lib.ptr(k_pages),
-                kst, _lib.ptr(vt_pages), vst, pages, page, _lib.ptr(o), _row_stride(o, nq * hd), T, B, max_q, nq, nkv, hd,
-                float(scale), _lib.ptr(ws), need, _lib.stream(dev))
-    _lib.check(st, what)
+    need = lib.ldk_paged_attention_workspace_bytes(T, B, max_q, prefix_len, nq, nkv, hd)
+    if need < 0:
+        _lib.check(-need, what)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    head = (x.data_ptr(), ldq, _CODES.get(dtype, -1), _addr(cu_seqlens), kv_lens.data_ptr(), block_table.data_ptr(), ldt,
+            max_pages)
+    pool = (k_pages.data_ptr(), kst, vt_pages.data_ptr(), vst, pages, page, o.data_ptr(), ldo, T, B, max_q, nq, nkv, hd)
+    if prefix_table is None:
+        _call(lib.ldk_paged_attention, dev, head + pool + (window, sinks, scale, ws.data_ptr(), need), what)
+    else:
+        _call(lib.ldk_shared_prefix_attention, dev,
+              head + (prefix_table.data_ptr(), prefix_len) + pool + (scale, ws.data_ptr(), need), what)
     return o
 
 

@@ -60,33 +60,38 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     torch.argmax). log_softmax(logits)[tokens], the softmax's entropy and the `top` largest log
     probabilities with their indexes, in fp32. -inf logits (masked words) have probability 0; a row
     that holds +inf or NaN, or nothing but -inf, gives NaN."""
-    V = logits.shape[-1]
-    lead = logits.shape[:-1]
-    if tokens.dtype != torch.int64 or tokens.shape != lead:
+    lead, V = logits.shape[:-1], logits.shape[-1]
+    if tokens.dtype is not torch.int64 or tokens.shape != lead:
         raise ValueError(f"token_logprobs: tokens must be int64 of shape {tuple(lead)}, got "
                          f"{tokens.dtype} {tuple(tokens.shape)}")
     code = _lib.dtype_code(logits.dtype)
-    dev = _lib.require_gpu(logits, tokens, what="token_logprobs")
-    x = logits if logits.dim() == 2 else logits.reshape(-1, V)
-    rows = x.shape[0]
-    if x.stride(1) != 1 or (rows > 1 and x.stride(0) < V):
-        x = x.contiguous()
-    tok = tokens.reshape(-1).contiguous()
-    logprob = torch.empty(lead, dtype=torch.float32, device=dev)
-    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
     if not 0 <= top <= min(MAX_TOP, V):
         raise ValueError(f"token_logprobs: top={top} outside 0..{min(MAX_TOP, V)}")
-    top_lp = torch.empty(lead + (top,), dtype=torch.float32, device=dev)
-    top_ids = torch.empty(lead + (top,), dtype=torch.int64, device=dev)
+    dev = logits.get_device()
+    if dev < 0 or tokens.get_device() != dev:
+        _lib.require_gpu(logits, tokens, what="token_logprobs")
+    x = logits if logits.dim() == 2 else logits.reshape(-1, V)
+    rows = x.shape[0]
+    if not x.is_contiguous() and (x.stride(1) != 1 or (rows > 1 and x.stride(0) < V)):
+        x = x.contiguous()
+    tok = tokens if tokens.is_contiguous() else tokens.contiguous()
+    # the four answers and the workspace of one allocation: [ids | log probabilities | entropies | top | workspace]
+    lib = _lib.load()
+    need = lib.ldk_token_logprobs_workspace_bytes(rows, V, top) if rows else 0
+    if need < 0:
+        _lib.check(-need, "token_logprobs")
+    count = rows * top
+    device = logits.device
+    ids = torch.empty(lead + (top,), dtype=torch.int64, device=device)
+    flat = torch.empty(count + 2 * rows, dtype=torch.float32, device=device)
+    top_lp, logprob, entropy = (flat[:count].view(lead + (top,)), flat[count:count + rows].view(lead),
+                                flat[count + rows:].view(lead))
     if rows:
-        with _lib.device_guard(dev):
-            lib = _lib.load()
-            need = lib.ldk_token_logprobs_workspace_bytes(rows, V, top)
-            if need < 0:
-                _lib.check(-need, "token_logprobs")
-            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-            st = lib.ldk_token_logprobs(_lib.ptr(x), x.stride(0), code, _lib.ptr(tok), rows, V, top,
-                                        _lib.ptr(logprob), _lib.ptr(entropy), _lib.ptr(top_lp), _lib.ptr(top_ids),
-                                        _lib.ptr(ws), need, _lib.stream(dev))
-        _lib.check(st, "token_logprobs")
-    return TokenLogprobs(logprob, entropy, top_lp, top_ids)
+        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        with _lib.device_guard(device):
+            st = lib.ldk_token_logprobs(
+                x.data_ptr(), x.stride(0), code, tok.data_ptr(), rows, V, top, logprob.data_ptr(), entropy.data_ptr(),
+                top_lp.data_ptr(), ids.data_ptr(), None if ws is None else ws.data_ptr(), need, _lib.stream(device))
+        if st:
+            _lib.check(st, "token_logprobs")
+    return TokenLogprobs(logprob, entropy, top_lp, ids)
