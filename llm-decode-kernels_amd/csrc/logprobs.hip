@@ -5,18 +5,19 @@
 //
 // A row is cut into `splits` slices, one workgroup each; a wave takes tiles of 1024 consecutive logits
 // of its slice (16 per lane, the next tile's loads in flight), tiles w, w + 4, ... by wave w.
-//  - Sums: each lane keeps a maximum of its own and rescales its two sums once per tile, so a logit
-//    costs one fma, one exp2, one add and one fma; y = x log2 e - base is in powers of two.
-//    exp(-inf) * -inf would be NaN: a tile whose second sum is NaN is summed again with y clamped.
+//  - Sums: the wave keeps one maximum m, and each lane two sums of 2^y and 2^y y with y = x log2 e -
+//    m log2 e: a logit costs half a maximum, one fma, one exp2, one add and one fma. Only a tile that
+//    raises the maximum rescales them. The maximum's own term is left out of the sums until another
+//    replaces it, so that ln s = log1p(rest) keeps its digits where one token has nearly all the
+//    probability. 2^-inf * -inf would be NaN: a tile whose second sum is NaN is summed again, clamped.
 //  - The largest: each wave keeps candidates (64-bit keys, value then lower index) in its own LDS list
-//    and a threshold below which nothing can be among them: the top-th largest of its 64 lanes'
-//    running maxima (found bit by bit with ballots), which lets through about the logits that are
-//    the largest so far. Tiles come in rising index order, so a later logit equal to the threshold
-//    loses its tie. A list that fills up is cut back to its `top` largest. The lists' entries are
-//    ranked by counting.
-// Rows of several slices leave {base, s, sum, keys} per slice in the workspace, which the next launch
-// joins with one wave per row. What bounds it: the bytes for 32-bit logits; for 16-bit ones the
-// vector instructions come close (one exp2 is four instructions' time).
+//    and a floor that none of the `top` largest can be below. Its first is the top-th largest of its 64
+//    lanes' maxima (found by ballots), which lets through about the logits that are the largest so
+//    far; then the waves share theirs: where each has top/4 lanes at or above what it gives, the least
+//    of the four has `top`. A list that fills up is cut back to its `top` largest. At the end the four
+//    lists' survivors of the highest floor meet, and one wave ranks them by counting.
+// Rows of several slices leave {m, sums, keys} per slice in the workspace, which the next launch
+// joins with one wave per row.
 #include <algorithm>
 
 #include "ldk_common.h"
@@ -28,7 +29,8 @@ constexpr int kPer = 16;             // logits of a lane per tile
 constexpr int kTileLogits = 64 * kPer;
 constexpr int kTopMax = 64;          // a wave's lanes: the threshold is a lane's maximum
 constexpr int kKeep = 128;           // candidates past which a list is cut back
-constexpr int kCap = kKeep + kTileLogits;
+constexpr int kCap = kKeep + 64;     // one more logit of every lane
+constexpr int kCapPer = kCap / 64;
 constexpr int kMergeKeys = 1024;     // keys of a row's slices that the joining wave takes
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
 
@@ -38,7 +40,7 @@ struct LogprobArgs {
   const int64_t* tokens;
   float *logprob, *entropy, *top_lp;
   int64_t* top_ids;
-  float* part;     // [rows][splits][4]: base, s, sum
+  float* part;     // [rows][splits][4]: m, s, y
   uint64_t* keys;  // [rows][splits][top], descending
   int64_t rows;
   int V, top, splits, slice;  // slice: tiles of a slice
@@ -54,60 +56,159 @@ __device__ __forceinline__ float from_order(uint32_t o) {
   return __builtin_bit_cast(float, o == 0xffffffffu ? 0x7fc00000u : o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
 
-// The n-th largest (n in 1..64) of the 64 lanes' values: the largest t with at least n values >= t.
-__device__ __forceinline__ uint32_t nth_largest(uint32_t v, int n) {
+// The float that exactly the numbers of keys above o are larger than (0x7fffffff would be -0: no key).
+__device__ __forceinline__ float float_at(uint32_t o) { return from_order(o == 0x7fffffffu ? 0x7ffffffeu : o); }
+
+// Maximum over the 64 lanes, in every lane (NaN does not count).
+__device__ __forceinline__ float wave_max(float v) {
+  v = fmaxf(v, ldk::row_ror<1>(v));
+  v = fmaxf(v, ldk::row_ror<2>(v));
+  v = fmaxf(v, ldk::row_ror<4>(v));
+  v = fmaxf(v, ldk::row_ror<8>(v));
+  auto p = __builtin_amdgcn_permlane16_swap(ldk::f2u(v), ldk::f2u(v), false, false);
+  v = fmaxf(ldk::u2f(p[0]), ldk::u2f(p[1]));
+  p = __builtin_amdgcn_permlane32_swap(ldk::f2u(v), ldk::f2u(v), false, false);
+  return fmaxf(ldk::u2f(p[0]), ldk::u2f(p[1]));
+}
+
+// The n-th largest of the wave's values, PER of each lane: the largest t with at least n values >= t, two
+// bits a step from the top; with BITS < 32 only its upper bits, the others 0 (a bound below it).
+template <int PER, int BITS>
+__device__ __forceinline__ uint32_t nth_largest(const uint32_t (&v)[PER], int n) {
   uint32_t t = 0;
 #pragma unroll
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t c = t | (1u << bit);
-    if (__popcll(__ballot(v >= c)) >= n) t = c;
+  for (int bit = 30; bit >= 32 - BITS; bit -= 2) {
+    int c[3] = {0, 0, 0};
+#pragma unroll
+    for (int q = 0; q < 3; ++q)
+#pragma unroll
+      for (int i = 0; i < PER; ++i) c[q] += __popcll(__ballot(v[i] >= (t | (uint32_t)(q + 1) << bit)));
+    t |= (c[2] >= n ? 3u : c[1] >= n ? 2u : c[0] >= n ? 1u : 0u) << bit;
   }
   return t;
 }
 
-// Cuts a wave's list of n keys to its `top` largest, in descending order at out[0 ..); absent ones are
-// 0. Keys of one list differ (their indexes do) but for absent zeros, which the position tells apart.
-__device__ __forceinline__ void rank_keys(const uint64_t* list, int n, int top, uint64_t* out, int lane) {
-  for (int i = lane; i < n; i += 64) {
-    const uint64_t key = list[i];
-    int r = 0;
-    for (int j = 0; j < n; ++j) {
-      const uint64_t other = list[j];
-      r += other > key || (other == key && j < i);
-    }
-    if (r < top) out[r] = key;
+// Rank of this lane's key among n keys in LDS (n a multiple of 8, 16-byte aligned): how many are larger,
+// or equal and before position i. Real keys differ (their indexes do); absent ones are 0.
+__device__ __forceinline__ int rank_key(const uint64_t* list, int n, uint64_t key, int i) {
+  typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+  int r = 0;
+#pragma unroll 1
+  for (int j = 0; j < n; j += 8) {
+    u64x2 a[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) a[q] = *reinterpret_cast<const u64x2*>(list + j + 2 * q);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) r += a[q / 2][q % 2] > key || (a[q / 2][q % 2] == key && j + q < i);
   }
-  for (int i = n + lane; i < top; i += 64) out[i] = 0;
+  return r;
 }
 
-// What a row's sums become: the combination of two {base, s, sum} triples over one logits row.
+// Position among the lanes whose bit of mask is set.
+__device__ __forceinline__ int lane_rank(uint64_t mask, int lane) { return __popcll(mask & ((uint64_t(1) << lane) - 1)); }
+
+// Writes the wave's keys, one of each lane that takes part, to list[n ..) and returns the new n.
+__device__ __forceinline__ int append_keys(bool take, uint64_t key, uint64_t* list, int n, int lane) {
+  const uint64_t mask = __ballot(take);
+  if (take) list[n + lane_rank(mask, lane)] = key;
+  return n + __popcll(mask);
+}
+
+// Cuts a wave's list of n <= kCap keys, n > top, to its largest: `top` of them, or up to kKeep / 2 where the
+// last one's value is another's too. Returns their number; *value gets the top-th largest's.
+__device__ __forceinline__ int cut_list(uint64_t* list, int n, int top, uint32_t* value, int lane) {
+  ldk::wave_lds_sync();
+  uint64_t k[kCapPer];
+  uint32_t hi[kCapPer], lo[kCapPer];
+#pragma unroll
+  for (int i = 0; i < kCapPer; ++i) {
+    k[i] = lane + 64 * i < n ? list[lane + 64 * i] : 0;
+    hi[i] = (uint32_t)(k[i] >> 32);
+  }
+  const uint32_t nth = nth_largest<kCapPer, 32>(hi, top);
+  int above = 0, equal = 0;
+#pragma unroll
+  for (int i = 0; i < kCapPer; ++i) {
+    above += __popcll(__ballot(hi[i] > nth));
+    equal += __popcll(__ballot(hi[i] == nth));
+    lo[i] = hi[i] == nth ? (uint32_t)k[i] : 0u;
+  }
+  uint64_t least = (uint64_t)nth << 32;
+  if (above + equal > kKeep / 2) least |= nth_largest<kCapPer, 32>(lo, top - above);  // the lowest indexes of them
+  ldk::wave_lds_sync();
+  n = 0;
+#pragma unroll
+  for (int i = 0; i < kCapPer; ++i) n = append_keys(k[i] >= least, k[i], list, n, lane);
+  ldk::wave_lds_sync();
+  *value = nth;
+  return n;
+}
+
+// The `top` largest of `total` keys (absent ones 0) in descending order: lane r gets the r-th. The loops
+// run as often as there are keys, mostly once or twice: code that runs once waits for its own fetch.
+// list: LDS for total + 8 keys (may be where keys are), sorted: for kTopMax.
+__device__ __forceinline__ uint64_t rank_keys(const uint64_t* keys, int total, int top, uint64_t* list, uint64_t* sorted,
+                                              int lane) {
+  uint32_t most[1] = {0};
+#pragma unroll 1
+  for (int i = lane; i < total; i += 64) most[0] = max(most[0], (uint32_t)(keys[i] >> 32));
+  const uint32_t nth = nth_largest<1, 32>(most, top);
+  int n = 0;
+#pragma unroll 1
+  for (int i = 0; i < total; i += 64) {  // in place: what is written lies before what is read next
+    const uint64_t key = i + lane < total ? keys[i + lane] : 0;
+    ldk::wave_lds_sync();
+    n = append_keys(key != 0 && (uint32_t)(key >> 32) >= nth, key, list, n, lane);
+  }
+  if (lane < 8) list[n + lane] = 0;
+  sorted[lane] = 0;
+  ldk::wave_lds_sync();
+#pragma unroll 1
+  for (int i = lane; i < n; i += 64) {
+    const uint64_t key = list[i];
+    const int r = rank_key(list, (n + 7) & ~7, key, i);
+    if (r < top) sorted[r] = key;
+  }
+  ldk::wave_lds_sync();
+  return lane < top ? sorted[lane] : 0;
+}
+
+// A part of a row: its maximum m, and over its other logits the sums of 2^y and 2^y y, y = x log2 e -
+// m log2 e (as rounded: base_of). m == -inf: nothing but -inf.
 struct Sums {
-  float m, base, s, y;  // maximum, its power-of-two base, sum of 2^(x log2e - base) and of that times its exponent
+  float m, s, y;
 };
 __device__ __forceinline__ float base_of(float m) { return m == -__builtin_inff() ? 0.0f : m * kLog2e; }
-// a's sums taken against another maximum m (not below a's).
+// The maximum's own exponent: what base_of rounded away.
+__device__ __forceinline__ float residue(float m) { return __builtin_fmaf(m, kLog2e, -base_of(m)); }
+// a's sums with its own maximum's term, taken against the maximum m >= a.m.
 __device__ __forceinline__ void rebase(Sums& a, float m) {
-  const float base = base_of(m), d = a.base - base;
-  const float f = a.m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(d);
-  // nothing summed yet, or too far below to matter: 0, and not 0 x inf
-  a.y = f == 0.0f ? a.s * 0.0f : f * __builtin_fmaf(d, a.s, a.y);
+  const float d = base_of(a.m) - base_of(m), f = a.m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(d);
+  if (a.m > -__builtin_inff()) {
+    const float r = residue(a.m), p = __builtin_amdgcn_exp2f(r);
+    a.s += p;
+    a.y = __builtin_fmaf(p, r, a.y);
+  }
+  a.y = f * __builtin_fmaf(d, a.s, a.y);
   a.s *= f;
   a.m = m;
-  a.base = base;
 }
 __device__ __forceinline__ Sums join(Sums a, Sums b) {
-  const float m = fmaxf(a.m, b.m);
-  rebase(a, m);
-  rebase(b, m);
+  if (b.m > a.m) {
+    const Sums t = a;
+    a = b;
+    b = t;
+  }
+  rebase(b, a.m);
   a.s += b.s;
   a.y += b.y;
   return a;
 }
-__device__ __forceinline__ Sums wave_join(Sums a) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1)
-    a = join(a, Sums{__shfl_xor(a.m, off), __shfl_xor(a.base, off), __shfl_xor(a.s, off), __shfl_xor(a.y, off)});
-  return a;
+// Over the lanes: the first that has the largest maximum keeps its term out.
+__device__ __forceinline__ Sums wave_join(Sums a, int lane) {
+  const float m = wave_max(a.m);
+  if (lane != __builtin_ctzll(__ballot(a.m == m) | (uint64_t(1) << 63))) rebase(a, m);
+  return Sums{m, ldk::sum_lanes_strided<1>(a.s), ldk::sum_lanes_strided<1>(a.y)};
 }
 
 template <typename T>
@@ -119,135 +220,194 @@ __device__ __forceinline__ float to_f<float>(float v) { return v; }
 template <>
 __device__ __forceinline__ float to_f<uint16_t>(uint16_t v) { return __builtin_bit_cast(float, (uint32_t)v << 16); }
 
+// The logit of the row's given token (NaN: outside the vocabulary). Read ahead of the row: two dependent loads.
+template <typename T>
+__device__ __forceinline__ float given_logit(const LogprobArgs& a, int64_t row) {
+  const int64_t tok = a.tokens[row];
+  return tok >= 0 && tok < a.V ? to_f<T>(((const T*)a.x)[row * a.ld + tok]) : __builtin_nanf("");
+}
+
 // The answers of one row, from its sums and its sorted keys (lanes 0 .. top - 1 hold one each).
 template <typename T>
-__device__ __forceinline__ void finish(const LogprobArgs& a, int64_t row, const Sums& t, uint64_t key, int lane) {
-  const float log_s = __builtin_amdgcn_logf(t.s);  // powers of two
+__device__ __forceinline__ void finish(const LogprobArgs& a, int64_t row, const Sums& t, float given, uint64_t key, int lane) {
+  // against the maximum itself: without what its base rounded away
+  const float r = residue(t.m), f = __builtin_amdgcn_exp2f(-r);
+  const float rest = t.s * f, y = f * __builtin_fmaf(-r, t.s, t.y);
+  const float log_s = log1pf(rest);
   if (lane == 0) {
-    const int64_t tok = a.tokens[row];
-    float lp = __builtin_nanf("");
-    if (tok >= 0 && tok < a.V) lp = (__builtin_fmaf(to_f<T>(((const T*)a.x)[row * a.ld + tok]), kLog2e, -t.base) - log_s) * kLn2;
-    a.logprob[row] = lp;
-    a.entropy[row] = (log_s - t.y / t.s) * kLn2;
+    a.logprob[row] = (given - t.m) - log_s;
+    a.entropy[row] = log_s - kLn2 * y / (1.0f + rest);
   }
   if (lane < a.top) {
-    a.top_lp[row * a.top + lane] = (__builtin_fmaf(from_order((uint32_t)(key >> 32)), kLog2e, -t.base) - log_s) * kLn2;
+    a.top_lp[row * a.top + lane] = (from_order((uint32_t)(key >> 32)) - t.m) - log_s;
     a.top_ids[row * a.top + lane] = (int64_t)(uint32_t)~(uint32_t)key;
   }
 }
 
 template <typename T, bool TOP>
-__global__ __launch_bounds__(kWaves * 64) void logprobs_kernel(LogprobArgs a) {
+__global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 6 : 5) void logprobs_kernel(LogprobArgs a) {
   constexpr int VEC = 16 / sizeof(T), NV = kPer / VEC;
   typedef T vec_t __attribute__((ext_vector_type(VEC)));
-  __shared__ uint64_t lists[TOP ? kWaves : 1][TOP ? kCap : 1];
-  __shared__ uint64_t best[TOP ? kWaves : 1][kTopMax], sorted[kTopMax];
+  typedef vec_t unaligned_t __attribute__((aligned(sizeof(T))));
+  __shared__ __align__(16) uint64_t lists[TOP ? kWaves : 1][TOP ? kCap : 1], pool[TOP ? kWaves * kCap + 8 : 1];
+  __shared__ uint64_t sorted[kTopMax];
+  __shared__ uint32_t shared_floor[kWaves];  // what each wave gives: top / 4 of its logits are at or above it
+  __shared__ uint32_t floors[kWaves];
+  __shared__ int pooled;
   __shared__ Sums sums[kWaves];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t row = blockIdx.y + (int64_t)blockIdx.z * 65535;
   if (row >= a.rows) return;
   const T* x = (const T*)a.x + row * a.ld;
-  // 16-byte vectors from the address below the row's start on: logit i of vector v is v * VEC + i - head
-  const int head = (int)((uintptr_t)x & 15) / (int)sizeof(T);
-  const int first = (int)blockIdx.x * a.slice, tiles = min(a.slice, (a.V + head + kTileLogits - 1) / kTileLogits - first);
+  // whole vectors from the row's start on (rows of any alignment: the loads take any), then the numbers
+  // that make up none, one per lane, as a tile of their own
+  const int rest = a.V % VEC, whole = a.V - rest, vtiles = (whole + kTileLogits - 1) / kTileLogits;
+  const int first = (int)blockIdx.x * a.slice, tiles = min(a.slice, vtiles + (rest ? 1 : 0) - first);
 
-  // the 16 logits of this lane in tile t: vectors lane + 64 u of it, whole ones as 16-byte loads; -inf past
-  // the row's ends (exp 0 and never among the largest unless the row has fewer numbers)
+  // the row's index of element e of this lane in tile t (of the slice), V or more for none
+  auto place = [&](int t, int e) __attribute__((always_inline)) {
+    if (first + t >= vtiles) return whole + (e ? VEC : lane);
+    return ((first + t) * NV + e / VEC) * 64 * VEC + lane * VEC + e % VEC;
+  };
+  // the vectors of this lane in tile t, a valid one in the place of none: loads under no condition, so that
+  // the wait for a tile's can leave the next tile's in flight
   auto load = [&](int t, vec_t (&v)[NV]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < NV; ++u) {
-      const int i = ((first + t) * NV + u) * 64 * VEC + lane * VEC - head;
-      if (i >= 0 && i + VEC <= a.V) {
-        v[u] = *reinterpret_cast<const vec_t*>(x + i);
-      } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          T none;
-          if constexpr (sizeof(T) == 4)
-            none = -__builtin_inff();
-          else
-            none = __builtin_bit_cast(T, (uint16_t)(__is_same(T, half_t) ? 0xfc00 : 0xff80));
-          v[u][e] = i + e >= 0 && i + e < a.V ? x[i + e] : none;
-        }
-      }
-    }
+    for (int u = 0; u < NV; ++u) v[u] = *reinterpret_cast<const unaligned_t*>(x + min(place(t, u * VEC), whole - VEC));
   };
 
-  Sums s{-__builtin_inff(), 0.0f, 0.0f, 0.0f};
-  uint32_t thr = 0, lmax = 0;  // candidates are above thr; this lane's largest so far
-  int n = 0, next_thr = 0, seen = 0;
+  Sums s{-__builtin_inff(), 0.0f, 0.0f};  // m: of the wave
+  float nb = 0.0f, lmax = -__builtin_inff();  // -base_of(m); this lane's largest so far
+  // Candidates' keys are above floor; `none` is below the key of every number. own: the last value of the
+  // wave's own top so far: later logits that equal it come after it
+  const uint32_t none = order(-__builtin_inff()) - 1;
+  uint32_t own = none;
+  int n = 0, next = 0, seen = 0;
+  uint32_t lodd = 0;  // the largest of tiles whose sum was not a number
+  const int quarter = (a.top + kWaves - 1) / kWaves;
+  if constexpr (TOP) {
+    if (tid < kWaves) shared_floor[tid] = none;
+    if (tid == 0) pooled = 0;
+    __syncthreads();
+  }
+  const float given = a.splits == 1 && wave == 0 ? given_logit<T>(a, row) : 0.0f;
   vec_t cur[NV], nxt[NV];
-  if (wave < tiles) load(wave, cur);
+  if (whole) load(min(wave, vtiles - 1 - first), cur);
   for (int t = wave; t < tiles; t += kWaves) {
-    if (t + kWaves < tiles) load(t + kWaves, nxt);
+    if (whole) load(t + kWaves, nxt);
     float v[kPer];
 #pragma unroll
     for (int u = 0; u < NV; ++u)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) v[u * VEC + e] = to_f<T>(cur[u][e]);
+    if (first + t >= vtiles - 1) {  // the last tiles: -inf for none (exp 0, and not among the largest by its place)
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) v[e] = first + t < vtiles && place(t, e) < whole ? v[e] : -__builtin_inff();
+      if (first + t == vtiles && lane < rest) v[0] = to_f<T>(x[whole + lane]);
+    }
     float tm = v[0];
 #pragma unroll
     for (int e = 1; e < kPer; ++e) tm = fmaxf(tm, v[e]);
-    rebase(s, fmaxf(s.m, tm));
     float ts = 0.0f, ty = 0.0f;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      const float y = __builtin_fmaf(v[e], kLog2e, -s.base), p = __builtin_amdgcn_exp2f(y);
-      ts += p;
-      ty = __builtin_fmaf(p, y, ty);
-    }
-    const bool odd = ty != ty;  // an infinity or a NaN among them
-    if (__any(odd)) {
-      ty = 0.0f;
+    if (__any(tm > s.m)) {  // a new maximum: its first lane leaves one logit that equals it out
+      const float m = wave_max(tm);
+      const bool holds = lane == __builtin_ctzll(__ballot(tm == m));
+      const float d = base_of(s.m) - base_of(m), f = s.m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(d);
+      if (lane == 0 && s.m > -__builtin_inff()) {  // the old maximum's term joins lane 0's sums
+        const float r = residue(s.m), p = __builtin_amdgcn_exp2f(r);
+        s.s += p;
+        s.y = __builtin_fmaf(p, r, s.y);
+      }
+      s.y = f * __builtin_fmaf(d, s.s, s.y);
+      s.s *= f;
+      s.m = m;
+      nb = -base_of(m);
+      bool left = !holds;
 #pragma unroll
       for (int e = 0; e < kPer; ++e) {
-        const float y = __builtin_fmaf(v[e], kLog2e, -s.base), p = __builtin_amdgcn_exp2f(y);
+        const float y = __builtin_fmaf(v[e], kLog2e, nb);
+        const bool out = !left && v[e] == m;
+        const float p = out ? 0.0f : __builtin_amdgcn_exp2f(y);
+        left |= out;
+        ts += p;
         ty = __builtin_fmaf(p, fmaxf(y, -1e30f), ty);
+      }
+      asm volatile("" : "+v"(ts));  // the sum is formed here (left to where the branches join, its terms live on)
+    } else {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const float y = __builtin_fmaf(v[e], kLog2e, nb), p = __builtin_amdgcn_exp2f(y);
+        ts += p;
+        ty = __builtin_fmaf(p, y, ty);
+      }
+      asm volatile("" : "+v"(ts));
+      if (__any(ty != ty)) {  // an infinity or a NaN among them
+        ty = 0.0f;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+          const float y = __builtin_fmaf(v[e], kLog2e, nb), p = __builtin_amdgcn_exp2f(y);
+          ty = __builtin_fmaf(p, fmaxf(y, -1e30f), ty);
+        }
       }
     }
     s.s += ts;
     s.y += ty;
     if constexpr (TOP) {
-      uint32_t tk = order(tm);
-      if (ts != ts) {
+      lmax = fmaxf(lmax, tm);
+      const bool strange = __any(ts != ts);  // a NaN among them, or infinities
+      if (strange && ts != ts) {
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) tk = max(tk, order(v[e]));
+        for (int e = 0; e < kPer; ++e) lodd = max(lodd, order(v[e]));
       }
-      lmax = max(lmax, tk);
-      uint64_t hit = __ballot(tk > thr);
-      if (hit) {
-        uint32_t floor = thr;  // of this tile's candidates: above floor
-        // a new threshold at tiles 0, 1, 3, 7, ... of the wave, and where many lanes hit
-        if (seen >= next_thr || __popcll(hit) > a.top) {
-          const uint32_t nth = nth_largest(lmax, a.top);
-          if (nth > thr) {
-            floor = nth - 1;  // this tile's equals are among the ones that made it
-            thr = nth;
-          }
-          next_thr = 2 * seen + 1;
+      uint32_t floor = own;
+      if (seen == next) {  // tiles 0, 1, 3, 7, ... of the wave
+        const uint32_t mine[1] = {max(order(lmax), lodd)};
+        if (seen == 0) {  // this tile's equals are among the ones that made it
+          own = max(own, nth_largest<1, 20>(mine, a.top));
+          floor = max(floor, own - 1);
         }
-        if (tk > floor) {
+        const uint32_t give = nth_largest<1, 20>(mine, quarter);
+        if (lane == 0 && give > none) *(volatile uint32_t*)&shared_floor[wave] = give;
+        next = 2 * seen + 1;
+      }
+      uint32_t least = 0xffffffffu;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) least = min(least, *(volatile uint32_t*)&shared_floor[w]);
+      floor = max(floor, (uint32_t)__builtin_amdgcn_readfirstlane(least) - 1);
+      floor = max(floor, none);
+      const float floor_f = float_at(floor);
+      const uint64_t hit = __ballot(tm > floor_f || ts != ts);
+      if (hit || floor == none) {
+        // by floats where they order as the keys do: no NaN, above -inf
+        int from = 0;  // the elements from here on go the long way
+        if (!strange && floor > none) {
+          from = kPer;
 #pragma unroll
           for (int e = 0; e < kPer; ++e) {
-            const uint32_t o = order(v[e]);
-            const int i = ((first + t) * NV + e / VEC) * 64 * VEC + lane * VEC + e % VEC - head;
-            const bool take = o > floor && i >= 0 && i < a.V;
-            const uint64_t mask = __ballot(take);
-            if (take) lists[wave][n + __popcll(mask & ((uint64_t(1) << lane) - 1))] = ((uint64_t)o << 32) | (uint32_t)~i;
-            n += __popcll(mask);
+            const uint64_t mask = __ballot(v[e] > floor_f);
+            if (mask && from == kPer) {
+              if (n > kKeep) {
+                from = e;
+              } else {
+                if (v[e] > floor_f) lists[wave][n + lane_rank(mask, lane)] = ((uint64_t)order(v[e]) << 32) | (uint32_t)~place(t, e);
+                n += __popcll(mask);
+              }
+            }
           }
         }
-        // n is the same in every lane that took part: the others take the first hit's
-        n = __builtin_amdgcn_readlane(n, __builtin_ctzll(__ballot(tk > floor) | (uint64_t(1) << 63)));
-        if (n > kKeep) {
-          ldk::wave_lds_sync();
-          rank_keys(lists[wave], n, a.top, best[wave], lane);
-          ldk::wave_lds_sync();
-          if (lane < a.top) lists[wave][lane] = best[wave][lane];
-          n = a.top;
-          ldk::wave_lds_sync();
-          thr = max(thr, (uint32_t)(lists[wave][a.top - 1] >> 32));
+        // the long way: what is left, read again, and the list cut back where it is full
+        if (from < kPer || n > kKeep) {
+          uint32_t value = 0;
+#pragma unroll 1
+          for (int e = from;; ++e) {
+            if (n > kKeep) n = cut_list(lists[wave], n, a.top, &value, lane);
+            if (e >= kPer) break;
+            const int i = place(t, e);
+            const uint32_t o = i < (first + t < vtiles ? whole : a.V) ? order(to_f<T>(x[i])) : 0u;
+            n = append_keys(o > floor, ((uint64_t)o << 32) | (uint32_t)~i, lists[wave], n, lane);
+          }
+          own = max(own, value);
         }
       }
       ++seen;
@@ -256,33 +416,44 @@ __global__ __launch_bounds__(kWaves * 64) void logprobs_kernel(LogprobArgs a) {
     for (int u = 0; u < NV; ++u) cur[u] = nxt[u];
   }
 
-  s = wave_join(s);
+  s.s = ldk::sum_lanes_strided<1>(s.s);
+  s.y = ldk::sum_lanes_strided<1>(s.y);
   if (lane == 0) sums[wave] = s;
+  uint64_t key = 0;
   if constexpr (TOP) {
-    ldk::wave_lds_sync();
-    rank_keys(lists[wave], n, a.top, best[wave], lane);
+    if (seen > 1) {
+      const uint32_t mine[1] = {max(order(lmax), lodd)};
+      own = max(own, nth_largest<1, 20>(mine, a.top));
+    }
+    if (lane == 0) floors[wave] = own;
   }
   __syncthreads();
-  if constexpr (TOP) {
-    if (lane < a.top) {
-      const uint64_t key = best[wave][lane];
-      int r = 0;
-      for (int w = 0; w < kWaves; ++w)
-        for (int j = 0; j < a.top; ++j) {
-          const uint64_t other = best[w][j];
-          r += other > key || (other == key && w * kTopMax + j < wave * kTopMax + lane);
-        }
-      if (r < a.top) sorted[r] = key;
+  if constexpr (TOP) {  // what is at or above every floor, of all four lists
+    uint32_t floor = none, least = 0xffffffffu;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      floor = max(floor, floors[w]);
+      least = min(least, shared_floor[w]);
+    }
+    floor = max(floor, least);
+#pragma unroll 1
+    for (int i = 0; i < n; i += 64) {
+      const uint64_t k1 = i + lane < n ? lists[wave][i + lane] : 0;
+      const bool take = k1 && (uint32_t)(k1 >> 32) >= floor;
+      const int count = __popcll(__ballot(take));
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&pooled, count);
+      append_keys(take, k1, pool, __builtin_amdgcn_readfirstlane(at), lane);
     }
     __syncthreads();
+    if (wave == 0) key = rank_keys(pool, pooled, a.top, pool, sorted, lane);
   }
   if (wave) return;
   Sums all = sums[0];
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) all = join(all, sums[w]);
-  const uint64_t key = TOP && lane < a.top ? sorted[lane] : 0;
   if (a.splits == 1) {
-    finish<T>(a, row, all, key, lane);
+    finish<T>(a, row, all, given, key, lane);
   } else {
     const int64_t at = row * a.splits + blockIdx.x;
     if (lane == 0) {
@@ -298,41 +469,23 @@ __global__ __launch_bounds__(kWaves * 64) void logprobs_kernel(LogprobArgs a) {
 // Joins a row's slices: one wave per row.
 template <typename T>
 __global__ __launch_bounds__(64) void logprobs_join_kernel(LogprobArgs a) {
-  __shared__ uint64_t list[kMergeKeys], sorted[kTopMax];
+  __shared__ __align__(16) uint64_t list[kMergeKeys + 8];
+  __shared__ uint64_t sorted[kTopMax];
   const int lane = threadIdx.x;
   const int64_t row = blockIdx.x;
-  Sums s{-__builtin_inff(), 0.0f, 0.0f, 0.0f};
+  const float given = given_logit<T>(a, row);
+  Sums s{-__builtin_inff(), 0.0f, 0.0f};
   for (int i = lane; i < a.splits; i += 64) {
     const float* p = a.part + (row * a.splits + i) * 4;
-    s = join(s, Sums{p[0], base_of(p[0]), p[1], p[2]});
+    s = join(s, Sums{p[0], p[1], p[2]});
   }
-  s = wave_join(s);
+  s = wave_join(s, lane);
   uint64_t key = 0;
   if (a.top) {
     const int total = a.splits * a.top;
-    constexpr int PER = kMergeKeys / 64;
-    uint64_t k[PER];
-    uint32_t most = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      k[i] = lane + 64 * i < total ? a.keys[row * total + lane + 64 * i] : 0;
-      most = max(most, (uint32_t)(k[i] >> 32));
-    }
-    const uint32_t nth = nth_largest(most, a.top);
-    int n = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const bool take = k[i] && (uint32_t)(k[i] >> 32) >= nth;
-      const uint64_t mask = __ballot(take);
-      if (take) list[n + __popcll(mask & ((uint64_t(1) << lane) - 1))] = k[i];
-      n += __popcll(mask);
-    }
-    ldk::wave_lds_sync();
-    rank_keys(list, n, a.top, sorted, lane);
-    ldk::wave_lds_sync();
-    if (lane < a.top) key = sorted[lane];
+    key = rank_keys(a.keys + row * total, total, a.top, list, sorted, lane);
   }
-  finish<T>(a, row, s, key, lane);
+  finish<T>(a, row, s, given, key, lane);
 }
 
 // Slices of a row: enough workgroups for the CUs, whole tiles for every wave, keys for one joining wave.
@@ -394,8 +547,8 @@ extern "C" int ldk_token_logprobs(const void* logits, int64_t ld, int dtype, con
   LogprobArgs a{logits, ld, tokens, logprob, entropy, top_logprobs, top_ids, (float*)workspace, nullptr, rows, (int)V, top,
                 plan_splits(rows, V, top), 0};
   a.keys = reinterpret_cast<uint64_t*>(a.part + 4 * rows * a.splits);
-  // every row has at most 15 / 2 logits' room before its first vector
-  const int tiles = (int)((V + 7 + kTileLogits - 1) / kTileLogits);
+  const int vec = dtype == LDK_F32 ? 4 : 8;
+  const int tiles = (int)((V / vec * vec + kTileLogits - 1) / kTileLogits + (V % vec ? 1 : 0));
   a.slice = (tiles + a.splits - 1) / a.splits;
   hipStream_t s = (hipStream_t)stream;
   switch (dtype) {
