@@ -61,9 +61,13 @@ template <int N>
 struct IntC {
   static constexpr int value = N;
 };
-// Waves of paged_block_kernel that split a block's chunks, by its rows: 8 waves a workgroup.
+// Of paged_block_kernel, by a block's rows: the waves that split its chunks between them, and LDS slots.
 template <int BT>
-constexpr int kBlockKG = BT == 128 ? 2 : 4;
+constexpr int kBlockKG = BT == 128 ? 1 : 4;
+template <int BT>
+constexpr int kBlockSlots = BT == 128 ? 4 : 2;
+template <int BT>
+constexpr int kBlockThreads = BT / 32 * kBlockKG<BT> * 64;
 constexpr int kMinRange = 4;     // chunks of a range, at least
 constexpr int kMaxRanges = 128;  // ranges of a sequence
 
@@ -723,19 +727,27 @@ __global__ __launch_bounds__(CG* KG * 64) __attribute__((amdgpu_waves_per_eu(2))
 
 // ---- joining the ranges of one (token, query head)
 //
-// MW waves per row: wave w takes ranges w, w + MW, ..., lane d the dims d and d + 64; the waves meet in
-// LDS. Rows come from paged_split_kernel's slots, from paged_block_kernel's splits, or (behind a shared
-// prefix) from both; ones whose only range has written the output are left alone.
-template <typename E, int HD, int MW, int BT>
-__global__ __launch_bounds__(MW * 64) void paged_merge_kernel(PagedArgs a) {
+// Rows come from paged_split_kernel's slots, from paged_block_kernel's splits, or (behind a shared
+// prefix) from both; ones whose only range has written the output are left alone. WR waves of a
+// workgroup per row: wave w takes ranges w, w + WR, ..., lane d the dims HD / 64 d on; where there are
+// several they meet in LDS. One wave per row where there are rows enough for the CUs (attend 509 rows
+// of 16 heads in 2 ranges: 42 us with 8 waves each), 8 for the few rows of a decode step, whose ranges
+// are many.
+constexpr int kMergeWaves = 8;  // of a workgroup
+
+template <typename E, int HD, int WR, int BT>
+__global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_kernel(PagedArgs a) {
   typedef typename E::T T;
   constexpr int ND = HD / 64;
-  __shared__ float ms[MW], ls[MW], os[MW][HD];
-  const int h = blockIdx.y, lane = threadIdx.x & 63;
+  typedef float vec_t __attribute__((ext_vector_type(ND)));
+  __shared__ float ms[kMergeWaves], ls[kMergeWaves], os[kMergeWaves][HD];
+  const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int t = blockIdx.x, kvh = h / a.gq;
+  const int64_t item = (int64_t)blockIdx.x * (kMergeWaves / WR) + wave / WR;  // row of (token, head)
+  const int t = (int)(item / a.nq), h = (int)(item % a.nq), kvh = h / a.gq, w = wave % WR;
   int b = t;
-  if (a.cu) {
+  bool run = t < a.T;
+  if (run && a.cu) {
     b = -1;
     for (int lo = 0, hi = a.B; lo < hi;) {
       const int mid = (lo + hi) / 2;
@@ -744,32 +756,31 @@ __global__ __launch_bounds__(MW * 64) void paged_merge_kernel(PagedArgs a) {
       else
         hi = mid;
     }
-    if (b < 0) return;
+    run = b >= 0;
   }
-  const SeqRows s = seq_rows(a.cu, a.kv_lens, b, a.T);
-  const int tok = t - s.row0;
-  if (tok >= min(s.n, a.max_q)) return;
-  const int row = tok * a.gq + h % a.gq;
+  SeqRows s{};
+  if (run) s = seq_rows(a.cu, a.kv_lens, b, a.T);
+  const int tok = t - s.row0, row = tok * a.gq + h % a.gq;
+  run = run && tok < min(s.n, a.max_q);
   const float sc = a.scale * 1.44269504088896341f;
   // the two lists: {m, l} and outputs of range i at p + i * step
   int na = 0, nb = 0, ja = 0, jb = 0;
   const float *pa = nullptr, *pb = nullptr;
   int64_t sa = 0;
-  if (a.slots) {
+  if (run && a.slots) {
     na = a.plan[2 * b + 1];
-    if (na <= 1 && !a.skip) return;
+    run = na > 1 || a.skip;
     ja = row % kRows;
     sa = (int64_t)a.nkv * a.nt * part_floats(HD);
     pa = a.part + ((int64_t)a.plan[2 * b] * a.nkv * a.nt + row / kRows * a.nkv + kvh) * part_floats(HD);
   }
-  if (s.pos0 + tok < 0) {
+  if (run && s.pos0 + tok < 0) {
     na = 0;  // sees nothing: zeros
-  } else if (a.bsplits) {
+  } else if (run && a.bsplits) {
     int tile, n;
     if (a.bdirect) {
       tile = (int)(s.row0 * (int64_t)a.gq / BT) + b + row / BT;
-      const Block bk = find_block<0>(a, tile, BT);
-      n = bk.n;
+      n = find_block<0>(a, tile, BT).n;
       jb = row % BT;
     } else {
       const int r = t * a.gq + h % a.gq;
@@ -779,42 +790,58 @@ __global__ __launch_bounds__(MW * 64) void paged_merge_kernel(PagedArgs a) {
     }
     const int per = block_range(a, n, kBlockKG<BT>);
     nb = (n + per - 1) / per;
-    if (a.bdirect && nb <= 1) return;
+    run = !a.bdirect || nb > 1;
     pb = a.bpart + ((int64_t)tile * a.nkv + kvh) * a.bsplits * BT * (2 + HD);
   }
-  float M = -__builtin_inff(), l = 0.0f, o[ND] = {};
-  for (int r = wave; r < na + nb; r += MW) {
-    const bool first = r < na;
-    const float* p = first ? pa + r * sa : pb + (int64_t)(r - na) * BT * (2 + HD);
-    const int j = first ? ja : jb, rows = first ? kRows : BT;
-    const float m = p[2 * j], lr = p[2 * j + 1];
-    const float mn = fmaxf(M, m);
-    const float f0 = M == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((M - mn) * sc);
-    const float f1 = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * sc);
-    l = l * f0 + lr * f1;
+  if (WR == 1 && !run) return;
+  float M = -__builtin_inff(), l = 0.0f;
+  vec_t o = vec_t(0.0f);
+  if (run) {
+#pragma unroll 4
+    for (int r = w; r < na + nb; r += WR) {
+      const bool first = r < na;
+      const float* p = first ? pa + r * sa : pb + (int64_t)(r - na) * BT * (2 + HD);
+      const int j = first ? ja : jb, rows = first ? kRows : BT;
+      const float m = p[2 * j], lr = p[2 * j + 1];
+      const vec_t v = *reinterpret_cast<const vec_t*>(p + 2 * rows + j * HD + ND * lane);
+      const float mn = fmaxf(M, m);
+      const float f0 = M == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((M - mn) * sc);
+      const float f1 = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * sc);
+      l = l * f0 + lr * f1;
 #pragma unroll
-    for (int i = 0; i < ND; ++i) o[i] = o[i] * f0 + p[2 * rows + j * HD + lane + 64 * i] * f1;
-    M = mn;
-  }
-  if (lane == 0) {
-    ms[wave] = M;
-    ls[wave] = l;
-  }
-#pragma unroll
-  for (int i = 0; i < ND; ++i) os[wave][lane + 64 * i] = o[i];
-  __syncthreads();
-  for (int d = threadIdx.x; d < HD; d += MW * 64) {
-    float MM = -__builtin_inff(), L = 0.0f, v = 0.0f;
-#pragma unroll
-    for (int w = 0; w < MW; ++w) MM = fmaxf(MM, ms[w]);
-#pragma unroll
-    for (int w = 0; w < MW; ++w) {
-      const float f = ms[w] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((ms[w] - MM) * sc);
-      L += ls[w] * f;
-      v += os[w][d] * f;
+      for (int i = 0; i < ND; ++i) o[i] = __builtin_fmaf(v[i], f1, o[i] * f0);
+      M = mn;
     }
-    ((T*)a.out)[(int64_t)t * a.ldo + (int64_t)h * HD + d] = (T)(L > 0.0f ? v / L : 0.0f);
   }
+  if constexpr (WR > 1) {
+    if (lane == 0) {
+      ms[wave] = M;
+      ls[wave] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < ND; ++i) os[wave][ND * lane + i] = o[i];
+    __syncthreads();
+    if (!run || w) return;
+    float MM = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < WR; ++i) MM = fmaxf(MM, ms[wave + i]);
+    l = 0.0f;
+    o = vec_t(0.0f);
+#pragma unroll
+    for (int i = 0; i < WR; ++i) {
+      const float f = ms[wave + i] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((ms[wave + i] - MM) * sc);
+      l = __builtin_fmaf(ls[wave + i], f, l);
+#pragma unroll
+      for (int q = 0; q < ND; ++q) o[q] = __builtin_fmaf(os[wave + i][ND * lane + q], f, o[q]);
+    }
+  }
+  T* dst = (T*)a.out + (int64_t)t * a.ldo + (int64_t)h * HD + ND * lane;
+#pragma unroll
+  for (int i = 0; i < ND; ++i) o[i] = l > 0.0f ? o[i] / l : 0.0f;
+  if constexpr (ND == 2)
+    *reinterpret_cast<uint32_t*>(dst) = pack2<E>(o[0], o[1]);
+  else
+    dst[0] = (T)o[0];
 }
 
 // What a call launches, from its sizes alone.
@@ -836,11 +863,11 @@ Plan make_plan(int64_t T, int64_t B, int64_t max_q, int64_t prefix_len, int nq, 
   }
   if (prefix_len || block) {
     const int64_t rows = T * gq;
-    // 128 rows where they give the CUs a workgroup each, else 64
+    // 128 rows where the sequences have about as many, else 64; split for two workgroups of 128 (one of 64) per CU
     auto tiles = [&](int bt) { return prefix_len ? (rows + bt - 1) / bt : rows / bt + B; };
-    p.bt = nkv * tiles(128) >= 256 || (prefix_len && rows > 64) ? 128 : 64;
+    p.bt = rows >= 96 * (prefix_len ? 1 : B) ? 128 : 64;
     p.btiles = (int)tiles(p.bt);
-    p.bsplits = (int)std::max<int64_t>(1, std::min<int64_t>(32, 320 / ((int64_t)nkv * p.btiles)));
+    p.bsplits = (int)std::max<int64_t>(1, std::min<int64_t>(32, (p.bt == 128 ? 640 : 320) / ((int64_t)nkv * p.btiles)));
     if (prefix_len || p.bsplits > 1) p.bpart_bytes = (int64_t)p.btiles * nkv * p.bsplits * p.bt * (2 + hd) * 4;
   }
   p.bytes = p.part_bytes + p.bpart_bytes + B * 8;
@@ -851,9 +878,9 @@ template <typename E, int HD, int MODE>
 int launch_block(const PagedArgs& a, const Plan& p, hipStream_t s) {
   const dim3 grid((unsigned)p.btiles * a.nkv, (unsigned)p.bsplits);
   if (p.bt == 128)
-    paged_block_kernel<E, HD, 4, kBlockKG<128>, 4, MODE><<<grid, 512, 0, s>>>(a);
+    paged_block_kernel<E, HD, 4, kBlockKG<128>, kBlockSlots<128>, MODE><<<grid, kBlockThreads<128>, 0, s>>>(a);
   else
-    paged_block_kernel<E, HD, 2, kBlockKG<64>, 2, MODE><<<grid, 512, 0, s>>>(a);
+    paged_block_kernel<E, HD, 2, kBlockKG<64>, kBlockSlots<64>, MODE><<<grid, kBlockThreads<64>, 0, s>>>(a);
   return ldk::check_launch("paged_attention block");
 }
 
@@ -869,11 +896,15 @@ int launch(const PagedArgs& a, const Plan& p, hipStream_t s) {
     if (st) return st;
   }
   if (!p.slots && p.bsplits == 1) return LDK_OK;
-  const dim3 grid((unsigned)a.T, (unsigned)a.nq);
+  const int64_t rows = (int64_t)a.T * a.nq;
+  const bool few = rows < 512;
+  const unsigned grid = (unsigned)(few ? rows : (rows + kMergeWaves - 1) / kMergeWaves);
   if (p.bt == 128)
-    paged_merge_kernel<E, HD, 8, 128><<<grid, 8 * 64, 0, s>>>(a);
+    few ? paged_merge_kernel<E, HD, kMergeWaves, 128><<<grid, kMergeWaves * 64, 0, s>>>(a)
+        : paged_merge_kernel<E, HD, 1, 128><<<grid, kMergeWaves * 64, 0, s>>>(a);
   else
-    paged_merge_kernel<E, HD, 8, 64><<<grid, 8 * 64, 0, s>>>(a);
+    few ? paged_merge_kernel<E, HD, kMergeWaves, 64><<<grid, kMergeWaves * 64, 0, s>>>(a)
+        : paged_merge_kernel<E, HD, 1, 64><<<grid, kMergeWaves * 64, 0, s>>>(a);
   return ldk::check_launch("paged_attention merge");
 }
 
