@@ -51,6 +51,15 @@ __device__ __forceinline__ void dma_buffer16(u32x4 rsrc, uint32_t voffset, uint3
                : "v"(voffset), "s"(rsrc), "s"(lds_base), "s"(soffset)
                : "memory");
 }
+// Two of them 1 KB apart in memory and in LDS (the second's voffset is the first's + 1024).
+__device__ __forceinline__ void dma_buffer16x2(u32x4 rsrc, uint32_t voffset, uint32_t voffset2, uint32_t lds_base) {
+  uint32_t saved;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
+               "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+               : "=&s"(saved)
+               : "v"(voffset), "v"(voffset2), "s"(rsrc), "s"(lds_base)
+               : "memory", "scc");
+}
 // The same with 4 bytes per lane (lane i writes lds_base + 4 i), for rows only 4-byte aligned.
 __device__ __forceinline__ void dma_buffer4(u32x4 rsrc, uint32_t voffset, uint32_t soffset, uint32_t lds_base) {
   uint32_t saved;

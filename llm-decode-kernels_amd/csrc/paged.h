@@ -20,6 +20,7 @@ namespace ldk {
 
 struct F16 {
   typedef half_t T;
+  static constexpr uint32_t kOnes = 0x3C003C00u;  // (1, 1)
   typedef half_t T2 __attribute__((ext_vector_type(2)));
   static __device__ __forceinline__ float4_t mfma(u32x4 a, u32x4 b, float4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
@@ -27,6 +28,7 @@ struct F16 {
 };
 struct BF16 {
   typedef __bf16 T;
+  static constexpr uint32_t kOnes = 0x3F803F80u;
   typedef __bf16 T2 __attribute__((ext_vector_type(2)));
   typedef __bf16 T8 __attribute__((ext_vector_type(8)));
   static __device__ __forceinline__ float4_t mfma(u32x4 a, u32x4 b, float4_t c) {

@@ -15,7 +15,8 @@
 // lanes hold 8 consecutive positions of one row: the softmax numerators go straight into P V as its A
 // operand, V^T tiles being the B operand, with an online maximum and sum in fp32 per wave; the waves
 // meet in LDS. The numerators are rounded to the element type before they weight V (the matrix cores
-// take nothing wider), their sum is taken from the unrounded values.
+// take nothing wider), and their sum is taken of what they were rounded to, so that a row that one
+// position dominates gets that position's v whatever its numerator rounds to.
 //
 // paged_block_kernel: a workgroup takes 64 or 128 rows of one kv head, which share K and V through LDS.
 // For prompts, and for the prefix that a whole batch shares, whose rows are all tokens of the batch.
@@ -167,7 +168,7 @@ template <typename E, int HD, int NW>
 __global__ __launch_bounds__(NW * 64) void paged_split_kernel(PagedArgs a) {
   typedef typename E::T T;
   constexpr int NS = HD / 32, NB = HD / 16;  // K dim steps, V dim blocks
-  __shared__ float mw[NW][kRows], lw[NW][kRows];
+  __shared__ __align__(16) float mw[NW][kRows], lw[NW][kRows];
   __shared__ __align__(16) float ow[NW][kRows][HD];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -199,7 +200,9 @@ __global__ __launch_bounds__(NW * 64) void paged_split_kernel(PagedArgs a) {
     qb[s] = c16 < rows ? *reinterpret_cast<const u32x4*>(qrow + 32 * s + 8 * kb) : u32x4{0, 0, 0, 0};
 
   const float sc = a.scale * 1.44269504088896341f;
-  float m_run = -__builtin_inff(), l_lane = 0.0f;
+  float m_run = -__builtin_inff();
+  float4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};  // of rows 4kb .. 4kb+3's numerators as rounded, by a column of ones
+  const u32x4 ones = {E::kOnes, E::kOnes, E::kOnes, E::kOnes};
   float4_t o[NB];  // O[rows 4kb .. 4kb+3][dim 16b + c16], unnormalised
 #pragma unroll
   for (int b = 0; b < NB; ++b) o[b] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
@@ -242,16 +245,12 @@ __global__ __launch_bounds__(NW * 64) void paged_split_kernel(PagedArgs a) {
     const float base = m_new == -__builtin_inff() ? 0.0f : m_new * sc;
     const float alpha = __builtin_amdgcn_exp2f(__builtin_fmaf(m_run, sc, -base));
     m_run = m_new;
-    float ls = 0.0f, x[8];
+    float x[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], sc, -base));
-      ls += x[e];
-    }
+    for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], sc, -base));
     u32x4 pa;
 #pragma unroll
     for (int e = 0; e < 4; ++e) pa[e] = pack2<E>(x[2 * e], x[2 * e + 1]);
-    l_lane = __builtin_fmaf(l_lane, alpha, ls);
     // V at positions that no row of the tile sees is not this call's data: zero, so that 0 x NaN is not
     if (cb + kChunkPos - 1 > thi || (cb < tlo && cb + kChunkPos > a.sinks)) {
       uint32_t mk[4];
@@ -269,19 +268,18 @@ __global__ __launch_bounds__(NW * 64) void paged_split_kernel(PagedArgs a) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const float al = __shfl(alpha, 4 * kb + r);
+      sum[r] *= al;
 #pragma unroll
       for (int b = 0; b < NB; ++b) o[b][r] *= al;
     }
+    sum = E::mfma(pa, ones, sum);
 #pragma unroll
     for (int b = 0; b < NB; ++b) o[b] = E::mfma(pa, vr[b], o[b]);
   }
 
   // ---- the waves meet
-  const float l_w = add_xor32(add_xor16(l_lane));
-  if (kb == 0) {
-    mw[wave][c16] = m_run;
-    lw[wave][c16] = l_w;
-  }
+  if (kb == 0) mw[wave][c16] = m_run;
+  if (c16 == 0) *reinterpret_cast<float4_t*>(&lw[wave][4 * kb]) = sum;
 #pragma unroll
   for (int r = 0; r < 4; ++r)
     if (4 * kb + r < rows) {
@@ -340,6 +338,7 @@ __global__ __launch_bounds__(NW * 64) void paged_split_kernel(PagedArgs a) {
 // tokens over the shared prefix.
 constexpr uint32_t kDead = 0x80000000u;  // buffer offset past every resource: the load returns 0
 constexpr int kAll = 0x7fffffff;
+constexpr float kLag = 8.0f;
 
 typedef const __attribute__((address_space(4))) int32_t* ScalarInts;  // read through the scalar cache
 
@@ -415,7 +414,7 @@ __global__ __launch_bounds__(CG* KG * 64) __attribute__((amdgpu_waves_per_eu(2))
   constexpr int KB = kChunkPos * HD * 2;  // bytes of a chunk's K (and of its V): NB tiles
   constexpr int LI = NB / CG;             // K (and V) tiles each wave loads per chunk
   constexpr bool AHEAD = S >= 4;          // deep enough to read the next chunk's K a step early
-  static_assert(CG * LI == NB && S >= 2, "whole loads per wave, two slots");
+  static_assert(CG * LI == NB && S >= 2 && (LI == 1 || LI % 2 == 0), "whole loads per wave, two slots");
   static_assert(KG * S * 2 * KB >= (KG - 1) * CG * 2 * NB * 64 * 16, "the K groups meet in the ring");
   __shared__ __align__(16) unsigned char ring[KG * S * 2 * KB];
   __shared__ float mls[CG * KG][4][64];  // the K groups' m and l per column tile and lane
@@ -494,19 +493,25 @@ __global__ __launch_bounds__(CG* KG * 64) __attribute__((amdgpu_waves_per_eu(2))
     chunk_page(a.cpp, in ? chunk_of(j) : 0, at, sub);
     page = table[at];  // first used a step later
   };
-  const uint32_t lane_off = (uint32_t)(c16 * 64 + kb * 16);
+  const uint32_t dma_off = (uint32_t)(c16 * 64 + kb * 16 + cg * LI * 1024);
   unsigned char* const kring = ring + kg * S * 2 * KB;
   unsigned char* const vring = kring + KB;
-  // K or V of the chunk into slot j % S
   auto usable = [&](int j) __attribute__((always_inline)) { return j * KG + kg < nsteps && (uint32_t)page < (uint32_t)a.pages; };
-  auto load = [&](const void* pool, int64_t stride, unsigned char* slots, int j) __attribute__((always_inline)) {
+  // K or V of the chunk into slot j % S
+  const char* const kpool = (const char*)a.k + (int64_t)kvh * a.cpp.n * KB;
+  const char* const vpool = (const char*)a.vt + (int64_t)kvh * a.cpp.n * KB;
+  const uint32_t kstride = (uint32_t)a.kps * 2, vstride = (uint32_t)a.vps * 2;  // bytes: below 2^32
+  auto load = [&](const char* pool, uint32_t stride, unsigned char* slots, int j) __attribute__((always_inline)) {
     const bool ok = usable(j);
-    const int64_t at = (int64_t)(ok ? page : 0) * stride + (int64_t)(kvh * (int)a.cpp.n + sub) * (kChunkPos * HD);
-    const u32x4 rs = raw_rsrc_uniform((const T*)pool + at, ok ? KB : 0);
+    const char* at = pool + (uint64_t)(ok ? (uint32_t)page : 0u) * stride + (uint32_t)sub * (uint32_t)KB;
+    const u32x4 rs = raw_rsrc_uniform(at, ok ? KB : 0);
+    unsigned char* const to = slots + (j % S) * 2 * KB + cg * LI * 1024;
+    if constexpr (LI % 2 == 0) {
 #pragma unroll
-    for (int i = 0; i < LI; ++i)
-      dma_buffer16(rs, lane_off + (uint32_t)((cg * LI + i) * 1024), 0u,
-                   lds_addr(slots + (j % S) * 2 * KB + (cg * LI + i) * 1024));
+      for (int i = 0; i < LI; i += 2) dma_buffer16x2(rs, dma_off + i * 1024, dma_off + (i + 1) * 1024, lds_addr(to + i * 1024));
+    } else {
+      dma_buffer16(rs, dma_off, 0u, lds_addr(to));
+    }
   };
   uint32_t have = 0;  // bit i: whether the step i before the last one loaded has a page
   int nfull = min((nsteps + KG - 1) / KG, max(0, nf - j0 - kg + KG - 1) / KG);  // unmasked steps: to the first without one
@@ -519,8 +524,8 @@ __global__ __launch_bounds__(CG* KG * 64) __attribute__((amdgpu_waves_per_eu(2))
   next_page(0);
 #pragma unroll
   for (int j = 0; j < S - 1; ++j) {
-    load(a.k, a.kps, kring, j);
-    load(a.vt, a.vps, vring, j);
+    load(kpool, kstride, kring, j);
+    load(vpool, vstride, vring, j);
     loaded(j);
   }
 
@@ -541,7 +546,8 @@ __global__ __launch_bounds__(CG* KG * 64) __attribute__((amdgpu_waves_per_eu(2))
     for (int s = 0; s < NS; ++s) asm volatile("" : "+v"(q[ct][s]));
 
   const float sc = a.scale * 1.44269504088896341f;
-  float m_run[2] = {-__builtin_inff(), -__builtin_inff()}, l_lane[2] = {0.0f, 0.0f};
+  float m_run[2] = {-__builtin_inff(), -__builtin_inff()};
+  float4_t sum[2];     // of the numerators as rounded, by a row of ones in the place of V^T: every element is row c16's
   float4_t o[2][NB];   // O^T[dim 16b + 4kb + r][row c16], unnormalised
   float4_t acc[2][2];  // [row half hb][column tile]: scores of positions 8kb + 4hb + r
   u32x4 ph[2];         // numerators: the B operand of P.V
@@ -550,6 +556,9 @@ __global__ __launch_bounds__(CG* KG * 64) __attribute__((amdgpu_waves_per_eu(2))
 #pragma unroll
     for (int b = 0; b < NB; ++b) o[ct][b] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
+#pragma unroll
+  for (int ct = 0; ct < 2; ++ct) sum[ct] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  const u32x4 ones = {E::kOnes, E::kOnes, E::kOnes, E::kOnes};
   u32x4 kt[NB], vv[NB];  // a chunk's K and V, read ahead of the MFMAs before the ones that use them
   auto tiles = [&](u32x4 (&t)[NB], const unsigned char* src) __attribute__((always_inline)) {
 #pragma unroll
@@ -581,6 +590,8 @@ __global__ __launch_bounds__(CG* KG * 64) __attribute__((amdgpu_waves_per_eu(2))
         }
     }
 #pragma unroll
+    for (int ct = 0; ct < 2; ++ct) sum[ct] = E::mfma(ones, ph[ct], sum[ct]);
+#pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int ct = 0; ct < 2; ++ct) {
@@ -591,7 +602,9 @@ __global__ __launch_bounds__(CG* KG * 64) __attribute__((amdgpu_waves_per_eu(2))
       }
     __builtin_amdgcn_sched_barrier(0);
   };
-  // The rescale is skipped while no row of the tile sees a larger score (its factor is then 1).
+  // The maximum that is subtracted may lag the largest score by kLag (in powers of two): the numerators
+  // then reach 2^kLag, far inside every type, and the outputs are rescaled once or twice a block instead of
+  // at most of its chunks (16 rows rarely all keep their maximum over a chunk).
   float nb[2] = {0.0f, 0.0f};  // -m_run * sc, 0 while m_run is -inf
   auto softmax = [&](auto maskedc, int cb0) __attribute__((always_inline)) {
 #pragma unroll
@@ -606,25 +619,21 @@ __global__ __launch_bounds__(CG* KG * 64) __attribute__((amdgpu_waves_per_eu(2))
         mc = fmaxf(mc, acc[e >> 2][ct][e & 3]);
       }
       mc = max_xor32(max_xor16(mc));
-      if (__any(mc > m_run[ct])) {
+      if (__any((mc - m_run[ct]) * sc > kLag)) {
         const float m_new = fmaxf(m_run[ct], mc);
         // a row that has seen nothing so far keeps m = -inf; its factor is taken against 0
         nb[ct] = m_new == -__builtin_inff() ? 0.0f : m_new * -sc;
         const float alpha = __builtin_amdgcn_exp2f(__builtin_fmaf(m_run[ct], sc, nb[ct]));
-        l_lane[ct] *= alpha;
+        sum[ct] *= alpha;
 #pragma unroll
         for (int b = 0; b < NB; ++b) o[ct][b] *= alpha;
         m_run[ct] = m_new;
       }
-      float x[8], ls = 0.0f;
+      float x[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[e >> 2][ct][e & 3], sc, nb[ct]));
-        ls += x[e];
-      }
+      for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[e >> 2][ct][e & 3], sc, nb[ct]));
 #pragma unroll
       for (int e = 0; e < 4; ++e) ph[ct][e] = pack2<E>(x[2 * e], x[2 * e + 1]);
-      l_lane[ct] += ls;
     }
   };
   auto step = [&](auto maskedc, int j) __attribute__((always_inline)) {
@@ -636,12 +645,12 @@ __global__ __launch_bounds__(CG* KG * 64) __attribute__((amdgpu_waves_per_eu(2))
     const bool live = !decltype(maskedc)::value || ((have >> (S - 2) & 1) && cb0 <= whi && (cb0 + kChunkPos > wlo || cb0 < a.sinks));
     if (!AHEAD && live) tiles(kt, kring + (j % S) * 2 * KB);
     if (live) scores();
-    load(a.k, a.kps, kring, j + S - 1);
+    load(kpool, kstride, kring, j + S - 1);
     if (live) {
       tiles(vv, vring + (j % S) * 2 * KB);
       softmax(maskedc, cb0);
     }
-    load(a.vt, a.vps, vring, j + S - 1);
+    load(vpool, vstride, vring, j + S - 1);
     loaded(j + S - 1);
     if (AHEAD) tiles(kt, kring + ((j + 1) % S) * 2 * KB);
     if (live) pv(maskedc, cb0);
@@ -658,9 +667,7 @@ __global__ __launch_bounds__(CG* KG * 64) __attribute__((amdgpu_waves_per_eu(2))
   ring_barrier();  // the ring is free: every wave's loads have landed and its reads are done
 
   // ---- the K groups meet: groups past the first leave m, l and O, lane for lane
-  float l_w[2];
-#pragma unroll
-  for (int ct = 0; ct < 2; ++ct) l_w[ct] = add_xor32(add_xor16(l_lane[ct]));
+  const float l_w[2] = {sum[0][0], sum[1][0]};
   float4_t* const red = reinterpret_cast<float4_t*>(ring);  // [wave - CG][2 NB][64]
   if (kg > 0) {
 #pragma unroll
@@ -932,6 +939,7 @@ int run(const char* fn, const void* q, int64_t ldq, int dtype, const int32_t* cu
   if (window < 0 || sinks < 0) return ldk::fail(LDK_ERR_INVALID, "%s: window=%lld sinks=%lld", fn, (long long)window, (long long)sinks);
   if (!(scale > 1e-20f && scale < 1e20f)) return ldk::fail(LDK_ERR_INVALID, "%s: scale=%g must be positive", fn, (double)scale);
   const int64_t per = (int64_t)nkv * page_size * hd;
+  if (kps > INT32_MAX || vps > INT32_MAX) return ldk::fail(LDK_ERR_UNSUPPORTED, "%s: page strides %lld %lld past 2^31", fn, (long long)kps, (long long)vps);
   if (kps < per || vps < per || ldq < (int64_t)nq * hd || ldo < (int64_t)nq * hd)
     return ldk::fail(LDK_ERR_INVALID, "%s: strides ldq=%lld ldo=%lld pages %lld %lld below what they step over", fn,
                      (long long)ldq, (long long)ldo, (long long)kps, (long long)vps);
