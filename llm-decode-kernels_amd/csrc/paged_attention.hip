@@ -164,18 +164,23 @@ __device__ __forceinline__ float max_xor32(float v) {
 // Floats of one partial: 16 rows of {m, l} and of hd outputs.
 constexpr int part_floats(int hd) { return kRows * (2 + hd); }
 
+// LDS bytes of split_rows: per wave the 16 rows' m, l and outputs.
+constexpr int split_lds(int hd, int nw) { return nw * kRows * (2 + hd) * 4; }
+
+// Workgroup wg of the split: NW waves.
 template <typename E, int HD, int NW>
-__global__ __launch_bounds__(NW * 64) void paged_split_kernel(PagedArgs a) {
+__device__ __forceinline__ void split_rows(const PagedArgs& a, int wg, unsigned char* lds) {
   typedef typename E::T T;
   constexpr int NS = HD / 32, NB = HD / 16;  // K dim steps, V dim blocks
-  __shared__ __align__(16) float mw[NW][kRows], lw[NW][kRows];
-  __shared__ __align__(16) float ow[NW][kRows][HD];
+  float(*const mw)[kRows] = reinterpret_cast<float(*)[kRows]>(lds);
+  float(*const lw)[kRows] = mw + NW;
+  float(*const ow)[kRows][HD] = reinterpret_cast<float(*)[kRows][HD]>(lds + NW * kRows * 8);
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c16 = lane & 15, kb = lane >> 4;
-  const int xy = a.nkv * a.nt, bxy = (int)blockIdx.x % xy;
+  const int xy = a.nkv * a.nt, bxy = wg % xy;
   const int kvh = bxy % a.nkv, tile = bxy / a.nkv;
-  const Slot sl = find_slot(a, (int)blockIdx.x / xy, lane);
+  const Slot sl = find_slot(a, wg / xy, lane);
   if (sl.b < 0) return;
   const Span sp = seq_span(a, sl.b);
   if (kvh == 0 && tile == 0 && sl.split == 0 && tid == 0) {
@@ -287,7 +292,7 @@ __global__ __launch_bounds__(NW * 64) void paged_split_kernel(PagedArgs a) {
       for (int b = 0; b < NB; ++b) ow[wave][4 * kb + r][16 * b + c16] = o[b][r];
     }
   lds_barrier();
-  float* part = a.part + (int64_t)blockIdx.x * part_floats(HD);
+  float* part = a.part + (int64_t)wg * part_floats(HD);
   for (int e = tid; e < rows * HD; e += NW * 64) {
     const int j = e / HD, d = e % HD;
     float mv[NW], lv[NW], ov[NW], M = -__builtin_inff();
@@ -318,6 +323,12 @@ __global__ __launch_bounds__(NW * 64) void paged_split_kernel(PagedArgs a) {
       }
     }
   }
+}
+
+template <typename E, int HD, int NW>
+__global__ __launch_bounds__(NW * 64) void paged_split_kernel(PagedArgs a) {
+  __shared__ __align__(16) unsigned char lds[split_lds(HD, NW)];
+  split_rows<E, HD, NW>(a, (int)blockIdx.x, lds);
 }
 
 // ---- blocks of rows that share K and V through LDS
@@ -406,8 +417,12 @@ __device__ __forceinline__ int row_position(const PagedArgs& a, int t) {
   return t - s.row0 < min(s.n, a.max_q) ? s.pos0 + t - s.row0 : -1;
 }
 
+// LDS bytes of block_rows: the ring, and the K groups' m and l per column tile and lane.
+constexpr int block_lds(int hd, int cg, int kg, int s) { return kg * s * 2 * kChunkPos * hd * 2 + cg * kg * 4 * 64 * 4; }
+
+// Block wg of the launch's tiles x kv heads, range split of it.
 template <typename E, int HD, int CG, int KG, int S, int MODE>
-__global__ __launch_bounds__(CG* KG * 64) __attribute__((amdgpu_waves_per_eu(2))) void paged_block_kernel(PagedArgs a) {
+__device__ __forceinline__ void block_rows(const PagedArgs& a, int wg, int split, unsigned char* lds) {
   typedef typename E::T T;
   typedef T T4 __attribute__((ext_vector_type(4)));
   constexpr int BT = 32 * CG, NS = HD / 32, NB = HD / 16;
@@ -416,14 +431,13 @@ __global__ __launch_bounds__(CG* KG * 64) __attribute__((amdgpu_waves_per_eu(2))
   constexpr bool AHEAD = S >= 4;          // deep enough to read the next chunk's K a step early
   static_assert(CG * LI == NB && S >= 2 && (LI == 1 || LI % 2 == 0), "whole loads per wave, two slots");
   static_assert(KG * S * 2 * KB >= (KG - 1) * CG * 2 * NB * 64 * 16, "the K groups meet in the ring");
-  __shared__ __align__(16) unsigned char ring[KG * S * 2 * KB];
-  __shared__ float mls[CG * KG][4][64];  // the K groups' m and l per column tile and lane
+  unsigned char* const ring = lds;
+  float(*const mls)[4][64] = reinterpret_cast<float(*)[4][64]>(lds + KG * S * 2 * KB);
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kg = wave / CG, cg = wave % CG;
   const int c16 = lane & 15, kb = lane >> 4;
-  const int kvh = (int)blockIdx.x % a.nkv, tile = a.btiles - 1 - (int)blockIdx.x / a.nkv;  // longest blocks first
-  const int split = (int)blockIdx.y;
+  const int kvh = wg % a.nkv, tile = a.btiles - 1 - wg / a.nkv;  // longest blocks first
   const Block bk = find_block<MODE>(a, tile, BT);
   if (bk.rows <= 0) return;
   const int per = block_range(a, bk.n, KG);
@@ -732,6 +746,33 @@ __global__ __launch_bounds__(CG* KG * 64) __attribute__((amdgpu_waves_per_eu(2))
   }
 }
 
+template <typename E, int HD, int BT>
+__global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_eu(2))) void paged_block_kernel(PagedArgs a) {
+  constexpr int CG = BT / 32, KG = kBlockKG<BT>, S = kBlockSlots<BT>;
+  __shared__ __align__(16) unsigned char lds[block_lds(HD, CG, KG, S)];
+  block_rows<E, HD, CG, KG, S, 0>(a, (int)blockIdx.x, (int)blockIdx.y, lds);
+}
+
+// Behind a shared prefix: its blocks, which the matrix cores bound, and the sequences' own positions, which
+// the memory does, in one launch, so that a CU runs some of each. Groups of 8 workgroups (one per XCD)
+// are of one kind, the kinds spread evenly over the launch.
+template <typename E, int HD, int BT>
+__global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_eu(2))) void paged_prefix_kernel(PagedArgs a) {
+  constexpr int CG = BT / 32, KG = kBlockKG<BT>, S = kBlockSlots<BT>, NW = kBlockThreads<BT> / 64;
+  constexpr int kBlockLds = block_lds(HD, CG, KG, S), kSplitLds = split_lds(HD, NW);
+  __shared__ __align__(16) unsigned char lds[kBlockLds > kSplitLds ? kBlockLds : kSplitLds];
+  const int tiles = a.btiles * a.nkv, nblock = tiles * a.bsplits;
+  const int64_t gb = (nblock + 7) / 8, gs = (a.slots * a.nkv * a.nt + 7) / 8, g = blockIdx.x / 8;
+  const int before = (int)(g * gb / (gb + gs));  // block groups before this one
+  if ((g + 1) * gb / (gb + gs) > before) {
+    const int wg = before * 8 + (int)(blockIdx.x % 8);
+    if (wg < nblock) block_rows<E, HD, CG, KG, S, 1>(a, wg % tiles, wg / tiles, lds);
+  } else {
+    const int wg = (int)(g - before) * 8 + (int)(blockIdx.x % 8);
+    if (wg < a.slots * a.nkv * a.nt) split_rows<E, HD, NW>(a, wg, lds);
+  }
+}
+
 // ---- joining the ranges of one (token, query head)
 //
 // Rows come from paged_split_kernel's slots, from paged_block_kernel's splits, or (behind a shared
@@ -881,27 +922,28 @@ Plan make_plan(int64_t T, int64_t B, int64_t max_q, int64_t prefix_len, int nq, 
   return p;
 }
 
-template <typename E, int HD, int MODE>
-int launch_block(const PagedArgs& a, const Plan& p, hipStream_t s) {
-  const dim3 grid((unsigned)p.btiles * a.nkv, (unsigned)p.bsplits);
-  if (p.bt == 128)
-    paged_block_kernel<E, HD, 4, kBlockKG<128>, kBlockSlots<128>, MODE><<<grid, kBlockThreads<128>, 0, s>>>(a);
-  else
-    paged_block_kernel<E, HD, 2, kBlockKG<64>, kBlockSlots<64>, MODE><<<grid, kBlockThreads<64>, 0, s>>>(a);
+template <typename E, int HD, int BT>
+int launch_rows(const PagedArgs& a, const Plan& p, hipStream_t s) {
+  if (a.pchunks) {
+    const int64_t groups = ((int64_t)p.btiles * a.nkv * p.bsplits + 7) / 8 + ((int64_t)p.slots * a.nkv * p.nt + 7) / 8;
+    paged_prefix_kernel<E, HD, BT><<<(unsigned)(8 * groups), kBlockThreads<BT>, 0, s>>>(a);
+  } else {
+    paged_block_kernel<E, HD, BT><<<dim3((unsigned)p.btiles * a.nkv, (unsigned)p.bsplits), kBlockThreads<BT>, 0, s>>>(a);
+  }
   return ldk::check_launch("paged_attention block");
 }
 
 template <typename E, int HD>
 int launch(const PagedArgs& a, const Plan& p, hipStream_t s) {
   (void)hipGetLastError();
-  int st = LDK_OK;
-  if (p.bt) st = a.pchunks ? launch_block<E, HD, 1>(a, p, s) : launch_block<E, HD, 0>(a, p, s);
-  if (st) return st;
-  if (p.slots) {
-    paged_split_kernel<E, HD, 8><<<(unsigned)a.slots * a.nkv * a.nt, 8 * 64, 0, s>>>(a);
+  int st;
+  if (p.bt) {
+    st = p.bt == 128 ? launch_rows<E, HD, 128>(a, p, s) : launch_rows<E, HD, 64>(a, p, s);
+  } else {
+    paged_split_kernel<E, HD, 8><<<(unsigned)p.slots * a.nkv * a.nt, 8 * 64, 0, s>>>(a);
     st = ldk::check_launch("paged_attention split");
-    if (st) return st;
   }
+  if (st) return st;
   if (!p.slots && p.bsplits == 1) return LDK_OK;
   const int64_t rows = (int64_t)a.T * a.nq;
   const bool few = rows < 512;
@@ -950,7 +992,7 @@ int run(const char* fn, const void* q, int64_t ldq, int dtype, const int32_t* cu
   const Plan p = make_plan(cu ? T : B, B, cu ? max_q : 1, prefix_len, nq, nkv, hd);
   if (!ws || ws_bytes < p.bytes)
     return ldk::fail(LDK_ERR_INVALID, "%s: workspace of %lld bytes, this call needs %lld", fn, (long long)ws_bytes, (long long)p.bytes);
-  if ((int64_t)p.slots * nkv * p.nt > INT32_MAX || (int64_t)p.btiles * nkv > INT32_MAX) return ldk::fail(LDK_ERR_UNSUPPORTED, "%s: too many workgroups", fn);
+  if ((int64_t)p.slots * nkv * p.nt + (int64_t)p.btiles * nkv * std::max(1, p.bsplits) > INT32_MAX / 2) return ldk::fail(LDK_ERR_UNSUPPORTED, "%s: too many workgroups", fn);
   const int big = 1 << 30;  // a window or sinks past every position
   PagedArgs a{};
   a.q = q, a.ldq = ldq, a.out = out, a.ldo = ldo;
