@@ -395,11 +395,11 @@ int ldk_w8a16_matmul_swiglu(const void* x, int64_t ldx, const uint8_t* wq, const
  *  - dtype LDK_F16 or LDK_BF16 for activations and cache; head_dim 64 or 128; nq % nkv == 0,
  *    nq <= 4096.
  *  - k_pages, vt_pages: num_pages pages of page_size positions (a multiple of 32, up to 65536), page
- *    i at element i * k_page_stride (vt_page_stride), >= nkv * page_size * head_dim and a multiple of
- *    8. A page holds, per kv head, the tiles of ldk_decode_attention's caches: K tiles
+ *    i at element i * k_page_stride (vt_page_stride),  >= nkv * page_size * head_dim, a multiple of 8
+ *    and below 2^31. A page holds, per kv head, the tiles of ldk_decode_attention's caches: K tiles
  *    [page_size/32][2][head_dim/32][16][32] and V^T tiles [page_size/32][head_dim/16][16][32].
- *  - block_table: int32 [B] rows of ldt >= max_pages ids; position p of sequence b is in page
- *    block_table[b][p / page_size]. An id outside [0, num_pages) is no page: nothing is written there
+ *  - block_table: int32 [B] rows of ldt >= max_pages ids (max_pages * page_size <= 2^25); position p
+ *    of sequence b is in page block_table[b][p / page_size]. An id outside [0, num_pages) is no page: nothing is written there
  *    and its positions are not attended to. Positions from max_pages * page_size on do not exist.
  *  - cu_seqlens: int32 [B + 1], sequence b's new tokens are the rows cu_seqlens[b] ..
  *    cu_seqlens[b+1] - 1 of the T rows, in rising order; NULL: sequence b has row b (T >= B).
@@ -424,9 +424,12 @@ int ldk_paged_append(const void* qkv, int64_t ldqkv, int dtype, const int32_t* c
                      int64_t page_size, void* q_out, int64_t ldq, int64_t T, int64_t B, int nq, int nkv,
                      int head_dim, void* stream);
 
-/* Bytes of workspace that ldk_paged_attention (prefix_len 0) and ldk_shared_prefix_attention need for
- * T rows of B sequences of at most max_q new tokens; negative: -ldk_status. */
-int64_t ldk_paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t max_q, int64_t prefix_len, int nq,
+/* Bytes of workspace that ldk_paged_attention (prefix_len 0) and ldk_shared_prefix_attention (window and
+ * sinks 0) need for T rows of B sequences of at most max_q new tokens (without cu_seqlens: T = B, max_q
+ * = 1) and tables of max_len = max_pages * page_size positions; 0: none, it may be NULL; negative:
+ * -ldk_status. */
+int64_t ldk_paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t max_q, int64_t max_len,
+                                            int64_t window, int64_t sinks, int64_t prefix_len, int nq,
                                             int nkv, int head_dim);
 
 /* Causal grouped-query softmax attention of the new tokens over the pages (their own k and v

@@ -243,6 +243,8 @@ extern "C" int ldk_paged_append(const void* qkv, int64_t ldqkv, int dtype, const
   if (num_pages <= 0 || num_pages > INT32_MAX || max_pages <= 0 || ldt < max_pages || max_pages > ldk::kMaxPositions / page_size)
     return ldk::fail(LDK_ERR_INVALID, "%s: num_pages=%lld max_pages=%lld ldt=%lld", fn, (long long)num_pages, (long long)max_pages, (long long)ldt);
   const int64_t per = (int64_t)nkv * page_size * head_dim;
+  if (k_page_stride > INT32_MAX || vt_page_stride > INT32_MAX)
+    return ldk::fail(LDK_ERR_UNSUPPORTED, "%s: page strides %lld %lld past 2^31", fn, (long long)k_page_stride, (long long)vt_page_stride);
   if (k_page_stride < per || vt_page_stride < per || ldqkv < (int64_t)(nq + 2 * nkv) * head_dim || ldq < (int64_t)nq * head_dim)
     return ldk::fail(LDK_ERR_INVALID, "%s: strides ldqkv=%lld ldq=%lld pages %lld %lld below what they step over", fn,
                      (long long)ldqkv, (long long)ldq, (long long)k_page_stride, (long long)vt_page_stride);

@@ -52,10 +52,12 @@ struct PagedArgs {
   int pages, cap;                    // cap: positions a sequence can hold
   PageDiv cpp;                       // chunks per page
   int pchunks, skip;                 // chunks of the shared prefix; of them, those paged_split_kernel leaves out
-  int window, sinks, slots;
+  int window, sinks, slots, spare;
   int btiles, bsplits, bdirect;      // the block kernel's tiles and splits; a lone range writes the output
   float scale;
 };
+
+typedef const __attribute__((address_space(4))) int32_t* ScalarInts;  // read through the scalar cache
 
 constexpr int kRows = 16;
 template <int N>
@@ -69,6 +71,7 @@ template <int BT>
 constexpr int kBlockSlots = BT == 128 ? 4 : 2;
 template <int BT>
 constexpr int kBlockThreads = BT / 32 * kBlockKG<BT> * 64;
+constexpr int kAll = 0x7fffffff;
 constexpr int kMinRange = 4;     // chunks of a range, at least
 constexpr int kMaxRanges = 128;  // ranges of a sequence
 
@@ -103,26 +106,44 @@ __device__ __forceinline__ int wave_max_i(int v) {
 }
 
 // The sequence and range of a slot: every wave forms it from the lengths of the whole batch. Every
-// sequence has at least one range (its rows have to be written); sum over b of max(1, ceil(n_b / per))
-// <= B + total / per <= slots.
+// sequence has at least one range (its rows have to be written), so sum over b of max(1, ceil(n_b / per))
+// <= B + total / per: with per = total / spare it fits B + spare slots. Where the launch is to be one round
+// of workgroups (spare 0), per is the least for which the sum fits the slots, found by bisection.
 struct Slot {
   int b, split, ranges, first, per;  // b < 0: none
 };
 __device__ __forceinline__ Slot find_slot(const PagedArgs& a, int slot, int lane) {
+  if (!a.plan) return Slot{slot, 0, 1, slot, kAll};  // every sequence in one range
   const int each = (a.B + 63) / 64, b0 = lane * each, b1 = min(b0 + each, a.B);
   int64_t sum = 0;
-  int most = 0;
+  int most = 0, n0 = 0;
   for (int b = b0; b < b1; ++b) {
     const int n = seq_span(a, b).n;
     sum += n;
     most = max(most, n);
+    n0 = n;
   }
   sum = wave_sum64(sum);
   most = wave_max_i(most);
-  const int spare = a.slots - a.B;
-  int64_t per = (sum + spare - 1) / spare;
-  per = max(per, (int64_t)max(kMinRange, (most + kMaxRanges - 1) / kMaxRanges));
-  Slot r{-1, 0, 1, 0, (int)per};
+  const int ways = a.spare ? a.spare : a.slots;
+  int per = (int)max((sum + ways - 1) / ways, (int64_t)max(kMinRange, (most + kMaxRanges - 1) / kMaxRanges));
+  if (!a.spare && a.B > 1) {
+    int hi = max(per, (int)min((int64_t)most, (sum + a.slots - a.B - 1) / (a.slots - a.B)));
+    while (per < hi) {
+      const int mid = (per + hi) / 2;
+      float c = 0.0f;  // exact: below 2^24
+      if (each == 1) {
+        if (b0 < b1) c = (float)max(1, (n0 + mid - 1) / mid);
+      } else {
+        for (int b = b0; b < b1; ++b) c += (float)max(1, (seq_span(a, b).n + mid - 1) / mid);
+      }
+      if (__builtin_amdgcn_readfirstlane((int)sum_lanes_strided<1>(c)) <= a.slots)
+        hi = mid;
+      else
+        per = mid + 1;
+    }
+  }
+  Slot r{-1, 0, 1, 0, per};
   int mine = 0;
   for (int b = b0; b < b1; ++b) mine += max(1, (seq_span(a, b).n + r.per - 1) / r.per);
   int end = mine;  // inclusive scan over the lanes
@@ -183,7 +204,7 @@ __device__ __forceinline__ void split_rows(const PagedArgs& a, int wg, unsigned 
   const Slot sl = find_slot(a, wg / xy, lane);
   if (sl.b < 0) return;
   const Span sp = seq_span(a, sl.b);
-  if (kvh == 0 && tile == 0 && sl.split == 0 && tid == 0) {
+  if (a.plan && kvh == 0 && tile == 0 && sl.split == 0 && tid == 0) {
     a.plan[2 * sl.b] = sl.first;
     a.plan[2 * sl.b + 1] = sl.ranges;
   }
@@ -211,8 +232,8 @@ __device__ __forceinline__ void split_rows(const PagedArgs& a, int wg, unsigned 
   float4_t o[NB];  // O[rows 4kb .. 4kb+3][dim 16b + c16], unnormalised
 #pragma unroll
   for (int b = 0; b < NB; ++b) o[b] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  const int32_t* trow = a.table + (int64_t)sl.b * a.ldt;
-  const int jend = min((sl.split + 1) * sl.per, sp.n);
+  const ScalarInts trow = (ScalarInts)(uintptr_t)(a.table + (int64_t)sl.b * a.ldt);
+  const int jend = (int)min((sl.split + (int64_t)1) * sl.per, (int64_t)sp.n);
   const uint32_t lane_off = (uint32_t)(c16 * 64 + kb * 16);
   const uint32_t chunk_bytes = kChunkPos * HD * 2;
   for (int j = sl.split * sl.per + wave; j < jend; j += NW) {
@@ -348,10 +369,7 @@ __global__ __launch_bounds__(NW * 64) void paged_split_kernel(PagedArgs a) {
 // floor(cu gq / rows)); a workgroup finds its sequence with a binary search. MODE 1: the rows of all
 // tokens over the shared prefix.
 constexpr uint32_t kDead = 0x80000000u;  // buffer offset past every resource: the load returns 0
-constexpr int kAll = 0x7fffffff;
 constexpr float kLag = 8.0f;
-
-typedef const __attribute__((address_space(4))) int32_t* ScalarInts;  // read through the scalar cache
 
 struct Block {
   int b, row0, pos0;     // MODE 0: the sequence, its first row and position
@@ -892,21 +910,42 @@ __global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_kernel(PagedArgs
     dst[0] = (T)o[0];
 }
 
+// Up to this many chunks a sequence is one range, with nothing to merge; and up to kSingleMany where the
+// sequences alone are workgroups for half of the CUs (one streams about 70 GB/s). Graph-timed, one range /
+// ranges and merge, us: 1 sequence of 12/2 heads at 300 positions 8.1 / 10.3, 600 9.7 / 10.4, 1100 13.6 / 10.5;
+// 64 of 28/4 at 1050 29 / 40.
+constexpr int kSingle = 20, kSingleMany = 36;
+
 // What a call launches, from its sizes alone.
 struct Plan {
-  int nt = 0, slots = 0;                   // paged_split_kernel, slots == 0: not launched
+  int nt = 0, slots = 0, spare = 0;        // paged_split_kernel, slots == 0: not launched
   int bt = 0, btiles = 0, bsplits = 0;     // paged_block_kernel, bt == 0: not launched
   int64_t part_bytes = 0, bpart_bytes = 0, bytes = 0;
 };
-Plan make_plan(int64_t T, int64_t B, int64_t max_q, int64_t prefix_len, int nq, int nkv, int hd) {
+// Chunks that a token sees at most, from the positions a table holds and the window.
+int64_t most_chunks(int64_t max_len, int64_t max_q, int64_t window, int64_t sinks) {
+  const int64_t all = (max_len + kChunkPos - 1) / kChunkPos;
+  if (!window) return all;
+  return std::min(all, (window + max_q + kChunkPos - 2) / kChunkPos + 1 + (sinks + kChunkPos - 1) / kChunkPos);
+}
+Plan make_plan(int64_t T, int64_t B, int64_t max_q, int64_t max_len, int64_t window, int64_t sinks, int64_t prefix_len,
+               int nq, int nkv, int hd) {
   Plan p;
   const int64_t gq = nq / nkv;
   const bool block = max_q * gq > 2 * kRows;  // rows of a sequence past two tiles: they share K and V in LDS
   if (prefix_len || !block) {
     p.nt = (int)((max_q * gq + kRows - 1) / kRows);
-    // about two workgroups per CU beyond one for each sequence
-    const int64_t spare = std::max<int64_t>(1, 512 / ((int64_t)nkv * p.nt));
-    p.slots = (int)(B + spare);
+    if (!prefix_len && most_chunks(max_len, max_q, window, sinks) <= (B * nkv * p.nt >= 128 ? kSingleMany : kSingle)) {
+      p.slots = (int)B;
+      return p;
+    }
+    // As many workgroups as run at once (a CU holds one of head_dim 128, two of 64) where that leaves half as
+    // many ranges again as there are sequences. Else a range is at most two thirds of what a CU would
+    // have to read (all of it behind a prefix, whose blocks keep the CUs busy too): with half of it / all, 64
+    // sequences of up to 16000 positions 85 / 92 us against 80, 100 of up to 4000 30 / 26 against 25
+    const int64_t w = (int64_t)nkv * p.nt, round = (hd == 128 ? 256 : 512) / w;
+    p.spare = 2 * round >= 3 * B ? 0 : (int)std::max<int64_t>(1, (prefix_len ? 256 : 384) / w);
+    p.slots = (int)(p.spare ? B + p.spare : round);
     p.part_bytes = (int64_t)p.slots * nkv * p.nt * part_floats(hd) * 4;
   }
   if (prefix_len || block) {
@@ -918,7 +957,7 @@ Plan make_plan(int64_t T, int64_t B, int64_t max_q, int64_t prefix_len, int nq, 
     p.bsplits = (int)std::max<int64_t>(1, std::min<int64_t>(32, (p.bt == 128 ? 640 : 320) / ((int64_t)nkv * p.btiles)));
     if (prefix_len || p.bsplits > 1) p.bpart_bytes = (int64_t)p.btiles * nkv * p.bsplits * p.bt * (2 + hd) * 4;
   }
-  p.bytes = p.part_bytes + p.bpart_bytes + B * 8;
+  p.bytes = p.part_bytes + p.bpart_bytes + (p.part_bytes ? B * 8 : 0);
   return p;
 }
 
@@ -944,7 +983,7 @@ int launch(const PagedArgs& a, const Plan& p, hipStream_t s) {
     st = ldk::check_launch("paged_attention split");
   }
   if (st) return st;
-  if (!p.slots && p.bsplits == 1) return LDK_OK;
+  if (!p.bytes) return LDK_OK;  // no sequence has more than one range
   const int64_t rows = (int64_t)a.T * a.nq;
   const bool few = rows < 512;
   const unsigned grid = (unsigned)(few ? rows : (rows + kMergeWaves - 1) / kMergeWaves);
@@ -989,8 +1028,8 @@ int run(const char* fn, const void* q, int64_t ldq, int dtype, const int32_t* cu
       ldo % 8 || kps % 8 || vps % 8 || !ldk::aligned(kv_lens, 4) || !ldk::aligned(cu, 4) || !ldk::aligned(table, 4) ||
       !ldk::aligned(ptable, 4) || !ldk::aligned(ws, 16))
     return ldk::fail(LDK_ERR_ALIGN, "%s: q, out, workspace and the pages 16-byte aligned with strides of multiples of 8 elements", fn);
-  const Plan p = make_plan(cu ? T : B, B, cu ? max_q : 1, prefix_len, nq, nkv, hd);
-  if (!ws || ws_bytes < p.bytes)
+  const Plan p = make_plan(cu ? T : B, B, cu ? max_q : 1, max_pages * page_size, window, sinks, prefix_len, nq, nkv, hd);
+  if (p.bytes && (!ws || ws_bytes < p.bytes))
     return ldk::fail(LDK_ERR_INVALID, "%s: workspace of %lld bytes, this call needs %lld", fn, (long long)ws_bytes, (long long)p.bytes);
   if ((int64_t)p.slots * nkv * p.nt + (int64_t)p.btiles * nkv * std::max(1, p.bsplits) > INT32_MAX / 2) return ldk::fail(LDK_ERR_UNSUPPORTED, "%s: too many workgroups", fn);
   const int big = 1 << 30;  // a window or sinks past every position
@@ -1000,13 +1039,13 @@ int run(const char* fn, const void* q, int64_t ldq, int dtype, const int32_t* cu
   a.k = k, a.vt = vt, a.kps = kps, a.vps = vps;
   a.part = (float*)ws;
   a.bpart = (float*)((char*)ws + p.part_bytes);
-  a.plan = (int32_t*)((char*)ws + p.part_bytes + p.bpart_bytes);
+  a.plan = p.part_bytes ? (int32_t*)((char*)ws + p.part_bytes + p.bpart_bytes) : nullptr;
   a.T = cu ? (int)T : (int)B, a.B = (int)B, a.max_q = cu ? (int)max_q : 1;
   a.nq = nq, a.nkv = nkv, a.gq = nq / nkv, a.nt = p.nt;
   a.pages = (int)num_pages, a.cpp = page_div(page_size / kChunkPos), a.cap = (int)(max_pages * page_size);
   a.pchunks = a.skip = (int)(prefix_len / kChunkPos);
   a.window = (int)std::min<int64_t>(window, big), a.sinks = (int)std::min<int64_t>(sinks, big);
-  a.slots = p.slots;
+  a.slots = p.slots, a.spare = p.spare;
   a.btiles = p.btiles, a.bsplits = p.bsplits, a.bdirect = !prefix_len;
   a.scale = scale;
   hipStream_t s = (hipStream_t)stream;
@@ -1016,14 +1055,18 @@ int run(const char* fn, const void* q, int64_t ldq, int dtype, const int32_t* cu
 
 }  // namespace
 
-extern "C" int64_t ldk_paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t max_q, int64_t prefix_len, int nq,
-                                                       int nkv, int head_dim) {
-  if (T <= 0 || T > (int64_t(1) << 24) || B <= 0 || B > 65535 || max_q <= 0 || max_q > (int64_t(1) << 24) || prefix_len < 0 || nq <= 0 || nkv <= 0 ||
-      nq % nkv || nq > 4096 || (head_dim != 64 && head_dim != 128)) {
-    return -ldk::fail(LDK_ERR_INVALID, "paged_attention_workspace_bytes: T=%lld B=%lld max_q=%lld prefix_len=%lld nq=%d nkv=%d head_dim=%d",
-                      (long long)T, (long long)B, (long long)max_q, (long long)prefix_len, nq, nkv, head_dim);
+extern "C" int64_t ldk_paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t max_q, int64_t max_len, int64_t window,
+                                                       int64_t sinks, int64_t prefix_len, int nq, int nkv, int head_dim) {
+  if (T <= 0 || T > (int64_t(1) << 24) || B <= 0 || B > 65535 || max_q <= 0 || max_q > (int64_t(1) << 24) || max_len <= 0 ||
+      max_len > ldk::kMaxPositions || window < 0 || sinks < 0 || prefix_len < 0 || nq <= 0 || nkv <= 0 || nq % nkv ||
+      nq > 4096 || (head_dim != 64 && head_dim != 128)) {
+    return -ldk::fail(LDK_ERR_INVALID,
+                      "paged_attention_workspace_bytes: T=%lld B=%lld max_q=%lld max_len=%lld window=%lld sinks=%lld "
+                      "prefix_len=%lld nq=%d nkv=%d head_dim=%d",
+                      (long long)T, (long long)B, (long long)max_q, (long long)max_len, (long long)window, (long long)sinks,
+                      (long long)prefix_len, nq, nkv, head_dim);
   }
-  return make_plan(T, B, max_q, prefix_len, nq, nkv, head_dim).bytes;
+  return make_plan(T, B, max_q, max_len, window, sinks, prefix_len, nq, nkv, head_dim).bytes;
 }
 
 extern "C" int ldk_paged_attention(const void* q, int64_t ldq, int dtype, const int32_t* cu_seqlens,

@@ -86,7 +86,7 @@ SIGNATURES = {
     "ldk_w8a16_matmul_swiglu_applies": [_i64, _i64, _i64],
     "ldk_paged_append": [_vp, _i64, _i32, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _i64,
                          _vp, _i64, _i64, _i64, _i32, _i32, _i32, _vp],
-    "ldk_paged_attention_workspace_bytes": [_i64, _i64, _i64, _i64, _i32, _i32, _i32],
+    "ldk_paged_attention_workspace_bytes": [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32],
     "ldk_paged_attention": [_vp, _i64, _i32, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _vp,
                             _i64, _i64, _i64, _i64, _i32, _i32, _i32, _i64, _i64, _f32, _vp, _i64, _vp],
     "ldk_shared_prefix_attention": [_vp, _i64, _i32, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64,

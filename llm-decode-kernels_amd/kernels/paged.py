@@ -201,18 +201,19 @@ def _attend(what, q, kv_lens, block_table, prefix_table, prefix_len, k_pages, vt
     elif max_q is None:
         max_q = T
     lib = _lib.load()
-    need = lib.ldk_paged_attention_workspace_bytes(T, B, max_q, prefix_len, nq, nkv, hd)
+    need = lib.ldk_paged_attention_workspace_bytes(T if cu_seqlens is not None else B, B, max_q, max_pages * page, window, sinks,
+                                                   prefix_len, nq, nkv, hd)
     if need < 0:
         _lib.check(-need, what)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     head = (x.data_ptr(), ldq, _CODES.get(dtype, -1), _addr(cu_seqlens), kv_lens.data_ptr(), block_table.data_ptr(), ldt,
             max_pages)
     pool = (k_pages.data_ptr(), kst, vt_pages.data_ptr(), vst, pages, page, o.data_ptr(), ldo, T, B, max_q, nq, nkv, hd)
     if prefix_table is None:
-        _call(lib.ldk_paged_attention, dev, head + pool + (window, sinks, scale, ws.data_ptr(), need), what)
+        _call(lib.ldk_paged_attention, dev, head + pool + (window, sinks, scale, _addr(ws), need), what)
     else:
         _call(lib.ldk_shared_prefix_attention, dev,
-              head + (prefix_table.data_ptr(), prefix_len) + pool + (scale, ws.data_ptr(), need), what)
+              head + (prefix_table.data_ptr(), prefix_len) + pool + (scale, _addr(ws), need), what)
     return o
 
 

@@ -50,6 +50,7 @@ def prefix(ptable=P, prefix_len=128, **kw):
         a["nkv"], a["hd"], a["scale"], a["ws"], a["ws_bytes"], None))
 
 
+LONG = dict(max_pages=128, ldt=128)  # tables long enough for a workspace
 COMMON = [(dict(kv=None), _lib.ERR_INVALID), (dict(table=None), _lib.ERR_INVALID), (dict(k=None), _lib.ERR_INVALID),
           (dict(vt=None), _lib.ERR_INVALID), (dict(dtype=_lib.F32), _lib.ERR_INVALID), (dict(hd=96), _lib.ERR_UNSUPPORTED),
           (dict(nq=13), _lib.ERR_INVALID), (dict(nq=0), _lib.ERR_INVALID), (dict(nkv=0), _lib.ERR_INVALID),
@@ -57,7 +58,7 @@ COMMON = [(dict(kv=None), _lib.ERR_INVALID), (dict(table=None), _lib.ERR_INVALID
           (dict(B=5), _lib.ERR_INVALID), (dict(page=48), _lib.ERR_UNSUPPORTED), (dict(page=0), _lib.ERR_UNSUPPORTED),
           (dict(pages=0), _lib.ERR_INVALID), (dict(max_pages=0), _lib.ERR_INVALID), (dict(ldt=7), _lib.ERR_INVALID),
           (dict(max_pages=1 << 26, ldt=1 << 26), _lib.ERR_INVALID), (dict(kps=2 * 64 * 128 - 8), _lib.ERR_INVALID),
-          (dict(vps=0), _lib.ERR_INVALID), (dict(kps=2 * 64 * 128 + 4), _lib.ERR_ALIGN), (dict(k=ODD), _lib.ERR_ALIGN),
+          (dict(vps=0), _lib.ERR_INVALID), (dict(kps=1 << 31), _lib.ERR_UNSUPPORTED), (dict(kps=2 * 64 * 128 + 4), _lib.ERR_ALIGN), (dict(k=ODD), _lib.ERR_ALIGN),
           (dict(vt=ODD), _lib.ERR_ALIGN), (dict(kv=ctypes.c_void_p(4098)), _lib.ERR_ALIGN)]
 
 
@@ -74,7 +75,7 @@ def test_append_refuses(kw, code):
     (dict(q=None), _lib.ERR_INVALID), (dict(out=None), _lib.ERR_INVALID), (dict(max_q=0), _lib.ERR_INVALID),
     (dict(max_q=5), _lib.ERR_INVALID), (dict(window=-1), _lib.ERR_INVALID), (dict(sinks=-1), _lib.ERR_INVALID),
     (dict(scale=0.0), _lib.ERR_INVALID), (dict(scale=-1.0), _lib.ERR_INVALID), (dict(scale=float("nan")), _lib.ERR_INVALID),
-    (dict(ws=None), _lib.ERR_INVALID), (dict(ws_bytes=16), _lib.ERR_INVALID), (dict(ldo=12 * 128 - 8), _lib.ERR_INVALID),
+    (dict(ws=None, **LONG), _lib.ERR_INVALID), (dict(ws_bytes=16, **LONG), _lib.ERR_INVALID), (dict(ldo=12 * 128 - 8), _lib.ERR_INVALID),
     (dict(ldo=12 * 128 + 4), _lib.ERR_ALIGN), (dict(out=ODD), _lib.ERR_ALIGN), (dict(ws=ODD), _lib.ERR_ALIGN)])
 def test_attention_refuses(kw, code):
     st, msg = attend(**kw)
@@ -91,10 +92,11 @@ def test_prefix_refuses(kw, code):
 
 def test_workspace_queries():
     lib = _lib.load()
-    assert lib.ldk_paged_attention_workspace_bytes(4, 4, 1, 0, 12, 2, 128) > 0
-    for bad in ((0, 4, 1, 0, 12, 2, 128), (4, 0, 1, 0, 12, 2, 128), (4, 4, 0, 0, 12, 2, 128), (4, 4, 1, -1, 12, 2, 128),
-                (4, 4, 1, 0, 12, 5, 128), (4, 4, 1, 0, 12, 2, 96)):
-        assert lib.ldk_paged_attention_workspace_bytes(*bad) == -_lib.ERR_INVALID
+    ok = (4, 4, 1, 8192, 0, 0, 0, 12, 2, 128)
+    assert lib.ldk_paged_attention_workspace_bytes(*ok) > 0
+    assert lib.ldk_paged_attention_workspace_bytes(4, 4, 1, 512, 0, 0, 0, 12, 2, 128) == 0
+    for at, bad in ((0, 0), (1, 0), (1, 65536), (2, 0), (3, 0), (3, 1 << 26), (4, -1), (5, -1), (6, -1), (7, 13), (8, 0), (9, 96)):
+        assert lib.ldk_paged_attention_workspace_bytes(*ok[:at], bad, *ok[at + 1:]) == -_lib.ERR_INVALID
     assert lib.ldk_token_logprobs_workspace_bytes(2000, 1000, 5) == 0
     for bad in ((0, 10, 1), (1, 0, 0), (1, 10, 11), (1, 100, 65), (1, 10, -1)):
         assert lib.ldk_token_logprobs_workspace_bytes(*bad) == -_lib.ERR_INVALID
