@@ -68,45 +68,50 @@ __device__ __forceinline__ int vt_at(int c, int r, int d) {
 
 constexpr int kTokThreads = 256;
 
+// Thread i of a token's workgroups (y) takes 8 dims of a q or k head and their partners, or 8 of a v head; its
+// loads go out before the angles, whose length and page loads and trigonometry they then cover.
 template <typename E, int HD>
 __global__ __launch_bounds__(kTokThreads) void append_token_kernel(AppendArgs a) {
   typedef typename E::T T;
-  constexpr int LH = HD / 16;  // lanes per q or k head: 8 dims and their partners each
+  constexpr int LH = HD / 16;  // lanes per q or k head
   constexpr int LV = HD / 8;   // lanes per v head
-  __shared__ float cs[2][HD / 2];
-  const int t = blockIdx.x, tid = threadIdx.x;
-  const SeqRows sr = seq_rows(nullptr, a.kv_lens, t, a.T);
-  const int p = sr.pos0;
-  if (tid < HD / 2 && a.inv_freq) angle(a.rope_pos ? a.rope_pos[t] : (int64_t)p, a.inv_freq[tid], &cs[0][tid], &cs[1][tid]);
+  __shared__ __align__(16) float cs[2][HD / 2];
+  const int t = blockIdx.x, tid = threadIdx.x, i = tid + (int)blockIdx.y * kTokThreads;
+  const int pairs = (a.nq + a.nkv) * LH, j = i - pairs;
+  const bool rot = i < pairs, val = !rot && j < a.nkv * LV;
+  const int h = rot ? i / LH : j / LV, d = (rot ? i % LH : j % LV) * 8;
+  const T* row = (const T*)a.qkv + (int64_t)t * a.ldqkv;
+  u32x4 x0{}, x1{};
+  if (rot) {
+    x0 = *reinterpret_cast<const u32x4*>(row + (int64_t)h * HD + d);
+    x1 = *reinterpret_cast<const u32x4*>(row + (int64_t)h * HD + HD / 2 + d);
+  } else if (val) {
+    x0 = *reinterpret_cast<const u32x4*>(row + (int64_t)(a.nq + a.nkv + h) * HD + d);
+  }
+  const int p = seq_rows(nullptr, a.kv_lens, t, a.T).pos0;
   int64_t page = -1;
   if (p >= 0 && p < a.cap) page = a.table[(int64_t)t * a.ldt + p / (kChunkPos * a.cpp)];
+  if (a.inv_freq) {  // uniform
+    if (tid < HD / 2) angle(a.rope_pos ? a.rope_pos[t] : (int64_t)p, a.inv_freq[tid], &cs[0][tid], &cs[1][tid]);
+    __syncthreads();
+  }
   const bool wr = page >= 0 && page < a.pages;
   const int c = p >= 0 ? p / kChunkPos % a.cpp : 0, r = p & 31;
-  const T* row = (const T*)a.qkv + (int64_t)t * a.ldqkv;
-  const int items = (a.nq + a.nkv) * LH + a.nkv * LV;
-  __syncthreads();
-  for (int i = tid + (int)blockIdx.y * kTokThreads; i < items; i += kTokThreads * (int)gridDim.y) {
-    if (i < (a.nq + a.nkv) * LH) {
-      const int h = i / LH, d = i % LH * 8;
-      u32x4 x0 = *reinterpret_cast<const u32x4*>(row + (int64_t)h * HD + d);
-      u32x4 x1 = *reinterpret_cast<const u32x4*>(row + (int64_t)h * HD + HD / 2 + d);
-      if (a.inv_freq) rotate8<E>(x0, x1, &cs[0][d], &cs[1][d]);
-      if (h < a.nq) {
-        T* q = (T*)a.q + (int64_t)t * a.ldq + (int64_t)h * HD;
-        *reinterpret_cast<u32x4*>(q + d) = x0;
-        *reinterpret_cast<u32x4*>(q + HD / 2 + d) = x1;
-      } else if (wr) {
-        T* k = (T*)a.k + page * a.kps + (int64_t)(h - a.nq) * a.cpp * kChunkPos * HD;
-        *reinterpret_cast<u32x4*>(k + k_at<HD>(c, r, d)) = x0;
-        *reinterpret_cast<u32x4*>(k + k_at<HD>(c, r, HD / 2 + d)) = x1;
-      }
+  if (rot) {
+    if (a.inv_freq) rotate8<E>(x0, x1, &cs[0][d], &cs[1][d]);
+    if (h < a.nq) {
+      T* q = (T*)a.q + (int64_t)t * a.ldq + (int64_t)h * HD;
+      *reinterpret_cast<u32x4*>(q + d) = x0;
+      *reinterpret_cast<u32x4*>(q + HD / 2 + d) = x1;
     } else if (wr) {
-      const int j = i - (a.nq + a.nkv) * LH, h = j / LV, d = j % LV * 8;
-      const u32x4 x = *reinterpret_cast<const u32x4*>(row + (int64_t)(a.nq + a.nkv + h) * HD + d);
-      uint16_t* v = (uint16_t*)a.vt + page * a.vps + (int64_t)h * a.cpp * kChunkPos * HD;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[vt_at<HD>(c, r, d + e)] = (uint16_t)(x[e >> 1] >> (16 * (e & 1)));
+      T* k = (T*)a.k + page * a.kps + (int64_t)(h - a.nq) * a.cpp * kChunkPos * HD;
+      *reinterpret_cast<u32x4*>(k + k_at<HD>(c, r, d)) = x0;
+      *reinterpret_cast<u32x4*>(k + k_at<HD>(c, r, HD / 2 + d)) = x1;
     }
+  } else if (val && wr) {
+    uint16_t* v = (uint16_t*)a.vt + page * a.vps + (int64_t)h * a.cpp * kChunkPos * HD;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[vt_at<HD>(c, r, d + e)] = (uint16_t)(x0[e >> 1] >> (16 * (e & 1)));
   }
 }
 
@@ -212,7 +217,8 @@ template <typename E, int HD>
 int launch(const AppendArgs& a, hipStream_t s) {
   (void)hipGetLastError();
   if (!a.cu) {
-    append_token_kernel<E, HD><<<dim3((unsigned)a.T, 1), kTokThreads, 0, s>>>(a);
+    const int items = (a.nq + a.nkv) * (HD / 16) + a.nkv * (HD / 8);
+    append_token_kernel<E, HD><<<dim3((unsigned)a.T, (unsigned)((items + kTokThreads - 1) / kTokThreads)), kTokThreads, 0, s>>>(a);
   } else {
     const unsigned gx = (unsigned)(a.T / kChunkPos + 2 * a.B);
     const int hb = std::min(a.nq + 2 * a.nkv, std::max(1, 1024 / (int)(a.T / kChunkPos + a.B)));

@@ -188,7 +188,10 @@ def _attend(what, q, kv_lens, block_table, prefix_table, prefix_len, k_pages, vt
         raise ValueError(f"{what}: prefix_table must be a contiguous int32 of at least {prefix_len // page} pages")
     ldo = nq * hd if out is None else _out_stride(out, T, nq, hd, dtype, what)
     dev = _device(what, q, kv_lens, block_table, prefix_table, k_pages, vt_pages, cu_seqlens, out)
-    o = torch.empty((T, nq, hd), dtype=dtype, device=q.device) if out is None else out
+    if out is not None:
+        o = out
+    else:  # (a copy of a contiguous q's form takes the least time)
+        o = torch.empty_like(q) if q.is_contiguous() else torch.empty((T, nq, hd), dtype=dtype, device=q.device)
     if not T or not B:
         return o
     x = q

@@ -75,23 +75,25 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     if not x.is_contiguous() and (x.stride(1) != 1 or (rows > 1 and x.stride(0) < V)):
         x = x.contiguous()
     tok = tokens if tokens.is_contiguous() else tokens.contiguous()
-    # the four answers and the workspace of one allocation: [ids | log probabilities | entropies | top | workspace]
     lib = _lib.load()
     need = lib.ldk_token_logprobs_workspace_bytes(rows, V, top) if rows else 0
     if need < 0:
         _lib.check(-need, "token_logprobs")
-    count = rows * top
     device = logits.device
     ids = torch.empty(lead + (top,), dtype=torch.int64, device=device)
-    flat = torch.empty(count + 2 * rows, dtype=torch.float32, device=device)
-    top_lp, logprob, entropy = (flat[:count].view(lead + (top,)), flat[count:count + rows].view(lead),
-                                flat[count + rows:].view(lead))
+    # the fp32 answers as parts of one allocation
+    top_lp, logprob, entropy = torch.empty(rows * (top + 2), dtype=torch.float32, device=device).split(
+        (rows * top, rows, rows))
+    top_lp = top_lp.view(lead + (top,))
+    if logits.dim() != 2:
+        logprob, entropy = logprob.view(lead), entropy.view(lead)
     if rows:
         ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        p, n = logprob.data_ptr(), 4 * rows  # (an empty top_lp has no address)
         with _lib.device_guard(device):
             st = lib.ldk_token_logprobs(
-                x.data_ptr(), x.stride(0), code, tok.data_ptr(), rows, V, top, logprob.data_ptr(), entropy.data_ptr(),
-                top_lp.data_ptr(), ids.data_ptr(), None if ws is None else ws.data_ptr(), need, _lib.stream(device))
+                x.data_ptr(), x.stride(0), code, tok.data_ptr(), rows, V, top, p, p + n, p - n * top,
+                ids.data_ptr(), None if ws is None else ws.data_ptr(), need, _lib.stream(device))
         if st:
             _lib.check(st, "token_logprobs")
     return TokenLogprobs(logprob, entropy, top_lp, ids)
