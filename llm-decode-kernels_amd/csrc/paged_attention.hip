@@ -638,6 +638,8 @@ __device__ __forceinline__ void block_rows(const PagedArgs& a, int wg, int split
   // then reach 2^kLag, far inside every type, and the outputs are rescaled once or twice a block instead of
   // at most of its chunks (16 rows rarely all keep their maximum over a chunk).
   float nb[2] = {0.0f, 0.0f};  // -m_run * sc, 0 while m_run is -inf
+  const float lag = kLag / sc;
+  float limit[2] = {-__builtin_inff(), -__builtin_inff()};  // m_run + lag
   auto softmax = [&](auto maskedc, int cb0) __attribute__((always_inline)) {
 #pragma unroll
     for (int ct = 0; ct < 2; ++ct) {
@@ -650,8 +652,8 @@ __device__ __forceinline__ void block_rows(const PagedArgs& a, int wg, int split
         }
         mc = fmaxf(mc, acc[e >> 2][ct][e & 3]);
       }
-      mc = max_xor32(max_xor16(mc));
-      if (__any((mc - m_run[ct]) * sc > kLag)) {
+      if (__any(mc > limit[ct])) {  // of any lane: the rows' maxima are only formed here
+        mc = max_xor32(max_xor16(mc));
         const float m_new = fmaxf(m_run[ct], mc);
         // a row that has seen nothing so far keeps m = -inf; its factor is taken against 0
         nb[ct] = m_new == -__builtin_inff() ? 0.0f : m_new * -sc;
@@ -660,6 +662,7 @@ __device__ __forceinline__ void block_rows(const PagedArgs& a, int wg, int split
 #pragma unroll
         for (int b = 0; b < NB; ++b) o[ct][b] *= alpha;
         m_run[ct] = m_new;
+        limit[ct] = m_new + lag;
       }
       float x[8];
 #pragma unroll
