@@ -368,12 +368,12 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 6 : 5) void logprobs_
           floor = max(floor, own - 1);
         }
         const uint32_t give = nth_largest<1, 20>(mine, quarter);
-        if (lane == 0 && give > none) *(volatile uint32_t*)&shared_floor[wave] = give;
+        if (lane == 0 && give > none) __hip_atomic_store(&shared_floor[wave], give, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
         next = 2 * seen + 1;
       }
       uint32_t least = 0xffffffffu;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) least = min(least, *(volatile uint32_t*)&shared_floor[w]);
+      for (int w = 0; w < kWaves; ++w) least = min(least, __hip_atomic_load(&shared_floor[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
       floor = max(floor, (uint32_t)__builtin_amdgcn_readfirstlane(least) - 1);
       floor = max(floor, none);
       const float floor_f = float_at(floor);

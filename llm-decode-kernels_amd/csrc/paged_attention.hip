@@ -51,7 +51,7 @@ struct PagedArgs {
   int T, B, max_q, nq, nkv, gq, nt;  // nt: 16-row tiles of a sequence
   int pages, cap;                    // cap: positions a sequence can hold
   PageDiv cpp;                       // chunks per page
-  int pchunks, skip;                 // chunks of the shared prefix; of them, those paged_split_kernel leaves out
+  int pchunks, skip;                 // chunks of the shared prefix; of them, those that its own blocks take
   int window, sinks, slots, spare;
   int btiles, bsplits, bdirect;      // the block kernel's tiles and splits; a lone range writes the output
   float scale;
@@ -126,7 +126,8 @@ __device__ __forceinline__ Slot find_slot(const PagedArgs& a, int slot, int lane
   sum = wave_sum64(sum);
   most = wave_max_i(most);
   const int ways = a.spare ? a.spare : a.slots;
-  int per = (int)max((sum + ways - 1) / ways, (int64_t)max(kMinRange, (most + kMaxRanges - 1) / kMaxRanges));
+  int per = (int)min((sum + ways - 1) / ways, (int64_t)most);
+  per = max(per, max(kMinRange, (most + kMaxRanges - 1) / kMaxRanges));
   if (!a.spare && a.B > 1) {
     int hi = max(per, (int)min((int64_t)most, (sum + a.slots - a.B - 1) / (a.slots - a.B)));
     while (per < hi) {
@@ -518,12 +519,14 @@ __device__ __forceinline__ void block_rows(const PagedArgs& a, int wg, int split
   // Step j of this K group loads from: the chunk's page, its id read through the scalar cache, and its place
   // in the page. No page (an id outside the pool, a step past the range): zeros are loaded
   const ScalarInts table = (ScalarInts)(uintptr_t)(MODE == 1 ? a.ptable : a.table + (int64_t)bk.b * a.ldt);
+  const ScalarInts ptable = (ScalarInts)(uintptr_t)a.ptable;
   int page, sub;
   auto next_page = [&](int j) __attribute__((always_inline)) {
     const bool in = j * KG + kg < nsteps;
+    const int c = in ? chunk_of(j) : 0;
     int at;
-    chunk_page(a.cpp, in ? chunk_of(j) : 0, at, sub);
-    page = table[at];  // first used a step later
+    chunk_page(a.cpp, c, at, sub);
+    page = (MODE == 0 && c < a.pchunks ? ptable : table)[at];  // first used a step later
   };
   const uint32_t dma_off = (uint32_t)(c16 * 64 + kb * 16 + cg * LI * 1024);
   unsigned char* const kring = ring + kg * S * 2 * KB;
@@ -921,8 +924,9 @@ constexpr int kSingle = 20, kSingleMany = 36;
 
 // What a call launches, from its sizes alone.
 struct Plan {
-  int nt = 0, slots = 0, spare = 0;        // paged_split_kernel, slots == 0: not launched
-  int bt = 0, btiles = 0, bsplits = 0;     // paged_block_kernel, bt == 0: not launched
+  bool apart = false;                               // the shared prefix in blocks of its own
+  int64_t nt = 0, slots = 0, spare = 0;             // paged_split_kernel, slots == 0: not launched
+  int64_t bt = 0, btiles = 0, bsplits = 0;          // paged_block_kernel, bt == 0: not launched
   int64_t part_bytes = 0, bpart_bytes = 0, bytes = 0;
 };
 // Chunks that a token sees at most, from the positions a table holds and the window.
@@ -934,43 +938,52 @@ int64_t most_chunks(int64_t max_len, int64_t max_q, int64_t window, int64_t sink
 Plan make_plan(int64_t T, int64_t B, int64_t max_q, int64_t max_len, int64_t window, int64_t sinks, int64_t prefix_len,
                int nq, int nkv, int hd) {
   Plan p;
-  const int64_t gq = nq / nkv;
-  const bool block = max_q * gq > 2 * kRows;  // rows of a sequence past two tiles: they share K and V in LDS
-  if (prefix_len || !block) {
-    p.nt = (int)((max_q * gq + kRows - 1) / kRows);
+  const int64_t gq = nq / nkv, rows = T * gq;
+  // a sequence's rows past two tiles share K and V in LDS; those that fill a block do so behind a prefix too
+  const bool block = max_q * gq > (prefix_len ? 128 : 2 * kRows);
+  p.apart = prefix_len && !block;
+  if (!block) {
+    p.nt = (max_q * gq + kRows - 1) / kRows;
     if (!prefix_len && most_chunks(max_len, max_q, window, sinks) <= (B * nkv * p.nt >= 128 ? kSingleMany : kSingle)) {
-      p.slots = (int)B;
+      p.slots = B;
       return p;
     }
     // As many workgroups as run at once (a CU holds one of head_dim 128, two of 64) where that leaves half as
     // many ranges again as there are sequences. Else a range is at most two thirds of what a CU would
     // have to read (all of it behind a prefix, whose blocks keep the CUs busy too): with half of it / all, 64
     // sequences of up to 16000 positions 85 / 92 us against 80, 100 of up to 4000 30 / 26 against 25
-    const int64_t w = (int64_t)nkv * p.nt, round = (hd == 128 ? 256 : 512) / w;
-    p.spare = 2 * round >= 3 * B ? 0 : (int)std::max<int64_t>(1, (prefix_len ? 256 : 384) / w);
-    p.slots = (int)(p.spare ? B + p.spare : round);
-    p.part_bytes = (int64_t)p.slots * nkv * p.nt * part_floats(hd) * 4;
+    const int64_t w = nkv * p.nt, round = (hd == 128 ? 256 : 512) / w;
+    p.spare = 2 * round >= 3 * B ? 0 : std::max<int64_t>(1, (prefix_len ? 256 : 384) / w);
+    p.slots = p.spare ? B + p.spare : round;
+    p.part_bytes = p.slots * w * part_floats(hd) * 4;
   }
-  if (prefix_len || block) {
-    const int64_t rows = T * gq;
-    // 128 rows where the sequences have about as many, else 64; split for two workgroups of 128 (one of 64) per CU
-    auto tiles = [&](int bt) { return prefix_len ? (rows + bt - 1) / bt : rows / bt + B; };
-    p.bt = rows >= 96 * (prefix_len ? 1 : B) ? 128 : 64;
-    p.btiles = (int)tiles(p.bt);
-    p.bsplits = (int)std::max<int64_t>(1, std::min<int64_t>(32, (p.bt == 128 ? 640 : 320) / ((int64_t)nkv * p.btiles)));
-    if (prefix_len || p.bsplits > 1) p.bpart_bytes = (int64_t)p.btiles * nkv * p.bsplits * p.bt * (2 + hd) * 4;
+  if (block || p.apart) {
+    // 128 rows where the sequences have about as many, else 64; split for two workgroups of 128 rows a CU (three
+    // of head_dim 64), or one of 64 (a 200-token chunk after 10000 positions, 28/4 heads, with 384 / 512 /
+    // 640 workgroups: 57 / 51 / 61 us)
+    auto tiles = [&](int bt) { return p.apart ? (rows + bt - 1) / bt : rows / bt + B; };
+    p.bt = rows >= 96 * (p.apart ? 1 : B) ? 128 : 64;
+    p.btiles = tiles(p.bt);
+    const int64_t fill = p.bt == 64 ? 320 : hd == 128 ? 512 : 768;
+    p.bsplits = std::max<int64_t>(1, std::min<int64_t>(32, fill / (nkv * p.btiles)));
+    if (p.apart || p.bsplits > 1) p.bpart_bytes = p.btiles * nkv * p.bsplits * p.bt * (2 + hd) * 4;
   }
   p.bytes = p.part_bytes + p.bpart_bytes + (p.part_bytes ? B * 8 : 0);
   return p;
 }
+// A launch holds fewer than 2^32 threads.
+bool launchable(const Plan& p, int64_t T, int nq, int nkv) {
+  const int64_t most = (int64_t(1) << 32) / 512 - 8;
+  return p.slots * nkv * p.nt + p.btiles * nkv * std::max<int64_t>(1, p.bsplits) < most && T * nq < most * 8;
+}
 
 template <typename E, int HD, int BT>
 int launch_rows(const PagedArgs& a, const Plan& p, hipStream_t s) {
-  if (a.pchunks) {
-    const int64_t groups = ((int64_t)p.btiles * a.nkv * p.bsplits + 7) / 8 + ((int64_t)p.slots * a.nkv * p.nt + 7) / 8;
+  if (a.skip) {
+    const int64_t groups = (p.btiles * a.nkv * p.bsplits + 7) / 8 + (p.slots * a.nkv * p.nt + 7) / 8;
     paged_prefix_kernel<E, HD, BT><<<(unsigned)(8 * groups), kBlockThreads<BT>, 0, s>>>(a);
   } else {
-    paged_block_kernel<E, HD, BT><<<dim3((unsigned)p.btiles * a.nkv, (unsigned)p.bsplits), kBlockThreads<BT>, 0, s>>>(a);
+    paged_block_kernel<E, HD, BT><<<dim3((unsigned)(p.btiles * a.nkv), (unsigned)p.bsplits), kBlockThreads<BT>, 0, s>>>(a);
   }
   return ldk::check_launch("paged_attention block");
 }
@@ -982,7 +995,7 @@ int launch(const PagedArgs& a, const Plan& p, hipStream_t s) {
   if (p.bt) {
     st = p.bt == 128 ? launch_rows<E, HD, 128>(a, p, s) : launch_rows<E, HD, 64>(a, p, s);
   } else {
-    paged_split_kernel<E, HD, 8><<<(unsigned)p.slots * a.nkv * a.nt, 8 * 64, 0, s>>>(a);
+    paged_split_kernel<E, HD, 8><<<(unsigned)(p.slots * a.nkv * p.nt), 8 * 64, 0, s>>>(a);
     st = ldk::check_launch("paged_attention split");
   }
   if (st) return st;
@@ -1032,9 +1045,9 @@ int run(const char* fn, const void* q, int64_t ldq, int dtype, const int32_t* cu
       !ldk::aligned(ptable, 4) || !ldk::aligned(ws, 16))
     return ldk::fail(LDK_ERR_ALIGN, "%s: q, out, workspace and the pages 16-byte aligned with strides of multiples of 8 elements", fn);
   const Plan p = make_plan(cu ? T : B, B, cu ? max_q : 1, max_pages * page_size, window, sinks, prefix_len, nq, nkv, hd);
-  if (p.bytes && (!ws || ws_bytes < p.bytes))
+  if (p.bytes > 0 && (!ws || ws_bytes < p.bytes))
     return ldk::fail(LDK_ERR_INVALID, "%s: workspace of %lld bytes, this call needs %lld", fn, (long long)ws_bytes, (long long)p.bytes);
-  if ((int64_t)p.slots * nkv * p.nt + (int64_t)p.btiles * nkv * std::max(1, p.bsplits) > INT32_MAX / 2) return ldk::fail(LDK_ERR_UNSUPPORTED, "%s: too many workgroups", fn);
+  if (!launchable(p, T, nq, nkv)) return ldk::fail(LDK_ERR_UNSUPPORTED, "%s: T=%lld rows of nq=%d heads are too many for a launch", fn, (long long)T, nq);
   const int big = 1 << 30;  // a window or sinks past every position
   PagedArgs a{};
   a.q = q, a.ldq = ldq, a.out = out, a.ldo = ldo;
@@ -1044,12 +1057,12 @@ int run(const char* fn, const void* q, int64_t ldq, int dtype, const int32_t* cu
   a.bpart = (float*)((char*)ws + p.part_bytes);
   a.plan = p.part_bytes ? (int32_t*)((char*)ws + p.part_bytes + p.bpart_bytes) : nullptr;
   a.T = cu ? (int)T : (int)B, a.B = (int)B, a.max_q = cu ? (int)max_q : 1;
-  a.nq = nq, a.nkv = nkv, a.gq = nq / nkv, a.nt = p.nt;
+  a.nq = nq, a.nkv = nkv, a.gq = nq / nkv, a.nt = (int)p.nt;
   a.pages = (int)num_pages, a.cpp = page_div(page_size / kChunkPos), a.cap = (int)(max_pages * page_size);
-  a.pchunks = a.skip = (int)(prefix_len / kChunkPos);
+  a.pchunks = (int)(prefix_len / kChunkPos), a.skip = p.apart ? a.pchunks : 0;
   a.window = (int)std::min<int64_t>(window, big), a.sinks = (int)std::min<int64_t>(sinks, big);
-  a.slots = p.slots, a.spare = p.spare;
-  a.btiles = p.btiles, a.bsplits = p.bsplits, a.bdirect = !prefix_len;
+  a.slots = (int)p.slots, a.spare = (int)p.spare;
+  a.btiles = (int)p.btiles, a.bsplits = (int)p.bsplits, a.bdirect = !p.apart;
   a.scale = scale;
   hipStream_t s = (hipStream_t)stream;
   if (dtype == LDK_F16) return hd == 128 ? launch<ldk::F16, 128>(a, p, s) : launch<ldk::F16, 64>(a, p, s);
