@@ -378,7 +378,24 @@ struct Block {
   int first, last;       // positions of the first and last row (MODE 0)
   int cs, lo, n;         // visible chunks
 };
-// The block of tile x (uniform). rows == 0: none.
+// The block of sequence b's rows from r0 on. rows == 0: none.
+__device__ __forceinline__ Block sequence_block(const PagedArgs& a, int b, const SeqRows& s, int r0, int BT) {
+  Block k{};
+  k.b = b;
+  k.row0 = s.row0;
+  k.pos0 = s.pos0;
+  k.r0 = r0;
+  k.rows = r0 < 0 ? 0 : max(0, min(BT, min(s.n, a.max_q) * a.gq - r0));
+  if (k.rows <= 0) return k;
+  k.first = k.pos0 + k.r0 / a.gq;
+  k.last = k.pos0 + (k.r0 + k.rows - 1) / a.gq;
+  const int hi = min(k.last, a.cap - 1), hc = hi < 0 ? 0 : hi / kChunkPos + 1;
+  k.lo = min(a.window > 0 ? max(0, k.first - a.window + 1) / kChunkPos : 0, hc);
+  k.cs = min((min(a.sinks, a.cap) + kChunkPos - 1) / kChunkPos, k.lo);
+  k.n = k.cs + hc - k.lo;
+  return k;
+}
+// The block of tile x (uniform).
 template <int MODE>
 __device__ __forceinline__ Block find_block(const PagedArgs& a, int x, int BT) {
   Block k{};
@@ -398,25 +415,12 @@ __device__ __forceinline__ Block find_block(const PagedArgs& a, int x, int BT) {
       hi = mid;
   }
   const SeqRows s = seq_rows(a.cu, a.kv_lens, b, a.T);
-  const int n = min(s.n, a.max_q);
-  k.b = b;
-  k.row0 = s.row0;
-  k.pos0 = s.pos0;
-  k.r0 = (x - (int)(s.row0 * (int64_t)a.gq / BT) - b) * BT;
-  k.rows = k.r0 < 0 ? 0 : max(0, min(BT, n * a.gq - k.r0));
-  if (k.rows <= 0) return k;
-  k.first = k.pos0 + k.r0 / a.gq;
-  k.last = k.pos0 + (k.r0 + k.rows - 1) / a.gq;
-  const int hi = min(k.last, a.cap - 1), hc = hi < 0 ? 0 : hi / kChunkPos + 1;
-  k.lo = min(a.window > 0 ? max(0, k.first - a.window + 1) / kChunkPos : 0, hc);
-  k.cs = min((min(a.sinks, a.cap) + kChunkPos - 1) / kChunkPos, k.lo);
-  k.n = k.cs + hc - k.lo;
-  return k;
+  return sequence_block(a, b, s, (x - (int)(s.row0 * (int64_t)a.gq / BT) - b) * BT, BT);
 }
-// Chunks of a block's range, a multiple of kg, and its ranges.
+// Chunks of a block's range, a multiple of kg.
 __device__ __forceinline__ int block_range(const PagedArgs& a, int n, int kg) {
-  const int per = (n + a.bsplits - 1) / a.bsplits, least = 2 * kg;
-  return max(least, (per + kg - 1) / kg * kg);
+  const int per = (n + a.bsplits - 1) / a.bsplits;
+  return max(2 * kg, (per + kg - 1) / kg * kg);
 }
 // The position of row t of the call's (-1: no sequence's), by its sequence.
 __device__ __forceinline__ int row_position(const PagedArgs& a, int t) {
@@ -800,11 +804,10 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
 // ---- joining the ranges of one (token, query head)
 //
 // Rows come from paged_split_kernel's slots, from paged_block_kernel's splits, or (behind a shared
-// prefix) from both; ones whose only range has written the output are left alone. WR waves of a
-// workgroup per row: wave w takes ranges w, w + WR, ..., lane d the dims HD / 64 d on; where there are
-// several they meet in LDS. One wave per row where there are rows enough for the CUs (attend 509 rows
-// of 16 heads in 2 ranges: 42 us with 8 waves each), 8 for the few rows of a decode step, whose ranges
-// are many.
+// prefix) from both; ones whose only range has written the output are left alone. A wave per row, lane d
+// the dims HD / 64 d on (four heads of a token per wave: 128 sequences behind 16384 positions 107 us instead
+// of 97); where rows are few their ranges are many, and WR = 8 waves per row take ranges w, w + 8, ... and
+// meet in LDS.
 constexpr int kMergeWaves = 8;  // of a workgroup
 
 template <typename E, int HD, int WR, int BT>
@@ -815,8 +818,9 @@ __global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_kernel(PagedArgs
   __shared__ float ms[kMergeWaves], ls[kMergeWaves], os[kMergeWaves][HD];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t item = (int64_t)blockIdx.x * (kMergeWaves / WR) + wave / WR;  // row of (token, head)
-  const int t = (int)(item / a.nq), h = (int)(item % a.nq), kvh = h / a.gq, w = wave % WR;
+  const int w = wave % WR;
+  const int64_t item = (int64_t)blockIdx.x * (kMergeWaves / WR) + wave / WR;
+  const int t = (int)(item / a.nq), h = (int)(item % a.nq);
   int b = t;
   bool run = t < a.T;
   if (run && a.cu) {
@@ -832,27 +836,28 @@ __global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_kernel(PagedArgs
   }
   SeqRows s{};
   if (run) s = seq_rows(a.cu, a.kv_lens, b, a.T);
-  const int tok = t - s.row0, row = tok * a.gq + h % a.gq;
+  const int tok = t - s.row0;
   run = run && tok < min(s.n, a.max_q);
-  const float sc = a.scale * 1.44269504088896341f;
-  // the two lists: {m, l} and outputs of range i at p + i * step
-  int na = 0, nb = 0, ja = 0, jb = 0;
-  const float *pa = nullptr, *pb = nullptr;
-  int64_t sa = 0;
+  const bool nothing = s.pos0 + tok < 0;  // zeros
+  int first = 0, na = 0;
   if (run && a.slots) {
-    na = a.plan[2 * b + 1];
-    run = na > 1 || a.skip;
-    ja = row % kRows;
-    sa = (int64_t)a.nkv * a.nt * part_floats(HD);
-    pa = a.part + ((int64_t)a.plan[2 * b] * a.nkv * a.nt + row / kRows * a.nkv + kvh) * part_floats(HD);
+    first = a.plan[2 * b];
+    na = nothing ? 0 : a.plan[2 * b + 1];
+    run = a.skip || a.plan[2 * b + 1] > 1;
   }
-  if (run && s.pos0 + tok < 0) {
-    na = 0;  // sees nothing: zeros
-  } else if (run && a.bsplits) {
+  if (WR == 1 && !run) return;
+  const float sc = a.scale * 1.44269504088896341f;
+  const int kvh = h / a.gq, row = tok * a.gq + h % a.gq;
+  // the two lists: {m, l} and outputs of range i at p + i * step
+  const int64_t sa = (int64_t)a.nkv * a.nt * part_floats(HD);
+  const float* pa = a.part + ((int64_t)first * a.nkv * a.nt + row / kRows * a.nkv + kvh) * part_floats(HD);
+  const float* pb = nullptr;
+  int nb = 0, jb = 0;
+  if (run && a.bsplits && !nothing) {
     int tile, n;
     if (a.bdirect) {
       tile = (int)(s.row0 * (int64_t)a.gq / BT) + b + row / BT;
-      n = find_block<0>(a, tile, BT).n;
+      n = sequence_block(a, b, s, row / BT * BT, BT).n;
       jb = row % BT;
     } else {
       const int r = t * a.gq + h % a.gq;
@@ -871,9 +876,9 @@ __global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_kernel(PagedArgs
   if (run) {
 #pragma unroll 4
     for (int r = w; r < na + nb; r += WR) {
-      const bool first = r < na;
-      const float* p = first ? pa + r * sa : pb + (int64_t)(r - na) * BT * (2 + HD);
-      const int j = first ? ja : jb, rows = first ? kRows : BT;
+      const bool split = r < na;
+      const float* p = split ? pa + r * sa : pb + (int64_t)(r - na) * BT * (2 + HD);
+      const int j = split ? row % kRows : jb, rows = split ? kRows : BT;
       const float m = p[2 * j], lr = p[2 * j + 1];
       const vec_t v = *reinterpret_cast<const vec_t*>(p + 2 * rows + j * HD + ND * lane);
       const float mn = fmaxf(M, m);
@@ -904,7 +909,7 @@ __global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_kernel(PagedArgs
       const float f = ms[wave + i] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((ms[wave + i] - MM) * sc);
       l = __builtin_fmaf(ls[wave + i], f, l);
 #pragma unroll
-      for (int q = 0; q < ND; ++q) o[q] = __builtin_fmaf(os[wave + i][ND * lane + q], f, o[q]);
+      for (int d = 0; d < ND; ++d) o[d] = __builtin_fmaf(os[wave + i][ND * lane + d], f, o[d]);
     }
   }
   T* dst = (T*)a.out + (int64_t)t * a.ldo + (int64_t)h * HD + ND * lane;
@@ -960,12 +965,14 @@ Plan make_plan(int64_t T, int64_t B, int64_t max_q, int64_t max_len, int64_t win
   if (block || p.apart) {
     // 128 rows where the sequences have about as many, else 64; split for two workgroups of 128 rows a CU (three
     // of head_dim 64), or one of 64 (a 200-token chunk after 10000 positions, 28/4 heads, with 384 / 512 /
-    // 640 workgroups: 57 / 51 / 61 us)
+    // 640 workgroups: 57 / 51 / 61 us), unless they are a third as many unsplit: the merge then costs more than
+    // fuller CUs save (2 prompts of 1500, 14/2 heads of 64, in one range / two: 34 / 68 us)
     auto tiles = [&](int bt) { return p.apart ? (rows + bt - 1) / bt : rows / bt + B; };
     p.bt = rows >= 96 * (p.apart ? 1 : B) ? 128 : 64;
     p.btiles = tiles(p.bt);
     const int64_t fill = p.bt == 64 ? 320 : hd == 128 ? 512 : 768;
-    p.bsplits = std::max<int64_t>(1, std::min<int64_t>(32, fill / (nkv * p.btiles)));
+    const int64_t whole = nkv * p.btiles;
+    p.bsplits = !p.apart && 3 * whole >= fill ? 1 : std::max<int64_t>(1, std::min<int64_t>(32, fill / whole));
     if (p.apart || p.bsplits > 1) p.bpart_bytes = p.btiles * nkv * p.bsplits * p.bt * (2 + hd) * 4;
   }
   p.bytes = p.part_bytes + p.bpart_bytes + (p.part_bytes ? B * 8 : 0);
@@ -1000,9 +1007,9 @@ int launch(const PagedArgs& a, const Plan& p, hipStream_t s) {
   }
   if (st) return st;
   if (!p.bytes) return LDK_OK;  // no sequence has more than one range
-  const int64_t rows = (int64_t)a.T * a.nq;
-  const bool few = rows < 512;
-  const unsigned grid = (unsigned)(few ? rows : (rows + kMergeWaves - 1) / kMergeWaves);
+  const bool few = (int64_t)a.T * a.nq < 512;
+  const int64_t waves = (int64_t)a.T * a.nq * (few ? kMergeWaves : 1);
+  const unsigned grid = (unsigned)((waves + kMergeWaves - 1) / kMergeWaves);
   if (p.bt == 128)
     few ? paged_merge_kernel<E, HD, kMergeWaves, 128><<<grid, kMergeWaves * 64, 0, s>>>(a)
         : paged_merge_kernel<E, HD, 1, 128><<<grid, kMergeWaves * 64, 0, s>>>(a);

@@ -247,6 +247,12 @@ def test_attention_many_sequences():
     check_attention(lens, news, 4, 2, 64, 32, F16)
 
 
+@pytest.mark.parametrize("prefix", [0, 64])
+def test_attention_long_contexts_beside_prompts(prefix):
+    """A batch that decodes and prefills at once: one token after many positions beside whole prompts."""
+    check_attention([9000, 300, 17000, 40], [1, 300, 2, 1], 4, 1, 64, 32, F16, prefix=prefix)
+
+
 def test_attention_positions_below_zero():
     """kv_lens below the new tokens' count: the tokens at positions below 0 give zeros."""
     pg = Pages([10, 3], 2, 128, 32, F16)
