@@ -21,6 +21,9 @@ namespace ldk {
 struct F16 {
   typedef half_t T;
   static constexpr uint32_t kOnes = 0x3C003C00u;  // (1, 1)
+  // softmax numerators are held times 2^kShift: a weight of 2^-25 of the largest, where fp16 alone ends,
+  // would be lost, and with it a long context's many small ones beside a large one
+  static constexpr float kShift = 7.0f;
   typedef half_t T2 __attribute__((ext_vector_type(2)));
   static __device__ __forceinline__ float4_t mfma(u32x4 a, u32x4 b, float4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
@@ -29,6 +32,7 @@ struct F16 {
 struct BF16 {
   typedef __bf16 T;
   static constexpr uint32_t kOnes = 0x3F803F80u;
+  static constexpr float kShift = 0.0f;
   typedef __bf16 T2 __attribute__((ext_vector_type(2)));
   typedef __bf16 T8 __attribute__((ext_vector_type(8)));
   static __device__ __forceinline__ float4_t mfma(u32x4 a, u32x4 b, float4_t c) {

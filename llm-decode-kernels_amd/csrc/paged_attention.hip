@@ -15,8 +15,9 @@
 // lanes hold 8 consecutive positions of one row: the softmax numerators go straight into P V as its A
 // operand, V^T tiles being the B operand, with an online maximum and sum in fp32 per wave; the waves
 // meet in LDS. The numerators are rounded to the element type before they weight V (the matrix cores
-// take nothing wider), and their sum is taken of what they were rounded to, so that a row that one
-// position dominates gets that position's v whatever its numerator rounds to.
+// take nothing wider; fp16's are held times 2^7, which keeps weights down to 2^-32), and their sum is
+// taken of what they were rounded to, so that a row that one position dominates gets that position's v
+// whatever its numerator rounds to.
 //
 // paged_block_kernel: a workgroup takes 64 or 128 rows of one kv head, which share K and V through LDS.
 // For prompts, and for the prefix that a whole batch shares, whose rows are all tokens of the batch.
@@ -274,7 +275,7 @@ __device__ __forceinline__ void split_rows(const PagedArgs& a, int wg, unsigned 
     m_run = m_new;
     float x[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], sc, -base));
+    for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], sc, E::kShift - base));
     u32x4 pa;
 #pragma unroll
     for (int e = 0; e < 4; ++e) pa[e] = pack2<E>(x[2 * e], x[2 * e + 1]);
@@ -642,9 +643,9 @@ __device__ __forceinline__ void block_rows(const PagedArgs& a, int wg, int split
     __builtin_amdgcn_sched_barrier(0);
   };
   // The maximum that is subtracted may lag the largest score by kLag (in powers of two): the numerators
-  // then reach 2^kLag, far inside every type, and the outputs are rescaled once or twice a block instead of
+  // then reach 2^(kLag + kShift), inside every type, and the outputs are rescaled once or twice a block instead of
   // at most of its chunks (16 rows rarely all keep their maximum over a chunk).
-  float nb[2] = {0.0f, 0.0f};  // -m_run * sc, 0 while m_run is -inf
+  float nb[2] = {0.0f, 0.0f};  // kShift - m_run * sc, 0 while m_run is -inf
   const float lag = kLag / sc;
   float limit[2] = {-__builtin_inff(), -__builtin_inff()};  // m_run + lag
   auto softmax = [&](auto maskedc, int cb0) __attribute__((always_inline)) {
@@ -663,8 +664,8 @@ __device__ __forceinline__ void block_rows(const PagedArgs& a, int wg, int split
         mc = max_xor32(max_xor16(mc));
         const float m_new = fmaxf(m_run[ct], mc);
         // a row that has seen nothing so far keeps m = -inf; its factor is taken against 0
-        nb[ct] = m_new == -__builtin_inff() ? 0.0f : m_new * -sc;
-        const float alpha = __builtin_amdgcn_exp2f(__builtin_fmaf(m_run[ct], sc, nb[ct]));
+        nb[ct] = m_new == -__builtin_inff() ? 0.0f : __builtin_fmaf(m_new, -sc, E::kShift);
+        const float alpha = __builtin_amdgcn_exp2f(__builtin_fmaf(m_run[ct], sc, nb[ct] - E::kShift));
         sum[ct] *= alpha;
 #pragma unroll
         for (int b = 0; b < NB; ++b) o[ct][b] *= alpha;

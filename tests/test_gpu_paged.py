@@ -2,12 +2,14 @@
 full and over a window with sinks, and attention behind a shared prefix, at the lengths, masks and
 layouts where they can go wrong, and a serving step of all of them together."""
 
+import math
+
 import pytest
 import torch
 
 from _paged import Pages, assert_within, attention64, rows_of
 from kernels import paged
-from kernels.attention import k_from_tiles, v_from_tiles
+from kernels.attention import k_from_tiles, k_to_tiles, v_from_tiles, vt_to_tiles
 from kernels.sample import token_logprobs
 
 pytestmark = pytest.mark.gpu
@@ -337,6 +339,32 @@ def test_attention_large_scores(news):
 
 
 # ---------------------------------------------------------------------------------- shared prefix
+@pytest.mark.parametrize("prefix", [0, 4096])
+@pytest.mark.parametrize("new", [1, 48])
+def test_attention_many_small_weights(new, prefix):
+    """fp16: one position whose weight is 2^25 times that of each of 8191 others, which alone have values.
+    Their numerators e^-17.41 = 2^-25.1 are below the type's least half step; the answer is their sum. Held
+    times 2^7 they are 2^-18.1, off by half of fp16's step of 2^-24 there: by 2^-6.9 of themselves."""
+    L, hd, page = 8192, 64, 64
+    k = torch.zeros(1, 1, L, hd, dtype=F16)
+    v = torch.ones(1, 1, L, hd, dtype=F16)
+    k[0, 0, 5, 0], v[0, 0, 5] = 4.3515625, 0.0
+    k, v = k.view(1, L // page, page, hd).transpose(0, 1), v.view(1, L // page, page, hd).transpose(0, 1)
+    table = torch.arange(L // page, dtype=torch.int32).cuda()[None]
+    q = torch.zeros(new, 4, hd, dtype=F16)
+    q[:, :, 0] = 4.0
+    args = (k_to_tiles(k.contiguous()).cuda(), vt_to_tiles(v.contiguous()).cuda(), 1.0)
+    cu = None if new == 1 else i32([0, new])
+    if prefix:
+        got = paged.shared_prefix_attention(q.cuda(), i32([L]), table, table[0, :prefix // page].clone(), prefix, *args, cu_seqlens=cu)
+    else:
+        got = paged.paged_attention(q.cuda(), i32([L]), table, *args, cu_seqlens=cu)
+    for i in range(new):
+        w = (L - new + i) * math.exp(-4.0 * 4.3515625)
+        ref = w / (1 + w)
+        assert ((got[i].double().cpu() - ref).abs() <= ref * (2.0 ** -6.9 + 2.0 ** -10) + 2.0 ** -25).all(), (i, got[i, 0, 0].item(), ref)
+
+
 @pytest.mark.parametrize("dtype,hd,nq,nkv,page", LAYOUTS)
 @pytest.mark.parametrize("prefix_pages", [1, 7])
 @pytest.mark.parametrize("lens", [[1], [33, 1, 64, 5, 100], [700, 32, 31, 65, 7, 90] * 4])
