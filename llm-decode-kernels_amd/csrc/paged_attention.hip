@@ -337,7 +337,7 @@ __device__ __forceinline__ void split_rows(const PagedArgs& a, int wg, unsigned 
     if (sl.ranges == 1 && !a.skip) {
       const int g = tile * kRows + j;
       T* dst = (T*)a.out + (int64_t)(sp.s.row0 + g / a.gq) * a.ldo + (int64_t)(kvh * a.gq + g % a.gq) * HD;
-      dst[d] = (T)(l > 0.0f ? v / l : 0.0f);
+      dst[d] = (T)(l != 0.0f ? v / l : 0.0f);
     } else {
       part[2 * kRows + e] = v;
       if (d == 0) {
@@ -761,7 +761,7 @@ __device__ __forceinline__ void block_rows(const PagedArgs& a, int wg, int split
         if (direct) {
           T4 y;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) y[r] = (T)(l > 0.0f ? v[r] / l : 0.0f);
+          for (int r = 0; r < 4; ++r) y[r] = (T)(l != 0.0f ? v[r] / l : 0.0f);
           *reinterpret_cast<T4*>(dst + 16 * b) = y;
         } else {
           *reinterpret_cast<float4_t*>(pdst + 16 * b) = v;
@@ -915,7 +915,7 @@ __global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_kernel(PagedArgs
   }
   T* dst = (T*)a.out + (int64_t)t * a.ldo + (int64_t)h * HD + ND * lane;
 #pragma unroll
-  for (int i = 0; i < ND; ++i) o[i] = l > 0.0f ? o[i] / l : 0.0f;
+  for (int i = 0; i < ND; ++i) o[i] = l != 0.0f ? o[i] / l : 0.0f;
   if constexpr (ND == 2)
     *reinterpret_cast<uint32_t*>(dst) = pack2<E>(o[0], o[1]);
   else

@@ -365,6 +365,37 @@ def test_attention_many_small_weights(new, prefix):
         assert ((got[i].double().cpu() - ref).abs() <= ref * (2.0 ** -6.9 + 2.0 ** -10) + 2.0 ** -25).all(), (i, got[i, 0, 0].item(), ref)
 
 
+@pytest.mark.parametrize("dtype,hd", [(F16, 64), (BF16, 128)])
+@pytest.mark.parametrize("prefix", [0, 32])
+@pytest.mark.parametrize("news", [[1, 1, 1], [2, 5, 3], [60, 3, 200]])
+def test_attention_of_nan(news, prefix, dtype, hd):
+    """A NaN in a row of q makes that row's head NaN, one in a k that is seen every row that sees it, and
+    no other row."""
+    lens, nq, nkv, page = [700, 64, 300], 6, 2, 32
+    pg = Pages(lens, nkv, hd, page, dtype)
+    q, cu = q_of(sum(news), nq, hd, dtype), rows_of(news)
+    at = lens[0] - (news[0] + 1) // 2  # seen by half of the first sequence's rows
+    pg.k[0][at, 1, 3] = float("nan")
+    k = k_from_tiles(pg.k_pages.cpu())
+    k[pg.table[0, at // page].item(), 1, at % page, 3] = float("nan")
+    q[cu[1] + news[1] // 2, 0, 5] = float("nan")
+    args = (k_to_tiles(k).cuda(), pg.vt_pages, 0.125)
+    cus = None if max(news) == 1 else i32(cu)
+    if prefix:  # (each sequence alone: the pages differ)
+        got = torch.cat([paged.shared_prefix_attention(q[cu[b]:cu[b + 1]].cuda(), i32([n]), pg.table[b:b + 1], pg.table[b, :1].clone(),
+                                                       prefix, *args, cu_seqlens=cus if cus is None else i32([0, news[b]]))
+                         for b, n in enumerate(lens)])
+    else:
+        got = paged.paged_attention(q.cuda(), i32(lens), pg.table, *args, cu_seqlens=cus, max_q=max(news))
+    got = got.cpu()
+    for b, n in enumerate(lens):
+        ref, bound = attention64(q[cu[b]:cu[b + 1]], pg.k[b], pg.v[b], 0.125, [n - news[b] + i for i in range(news[b])])
+        bad = torch.isnan(ref)
+        mine = got[cu[b]:cu[b + 1]]
+        assert (torch.isnan(mine) == bad).all(), b
+        assert_within(torch.where(bad, 0, mine), torch.where(bad, 0, ref), torch.where(bad, 1, bound))
+
+
 @pytest.mark.parametrize("dtype,hd,nq,nkv,page", LAYOUTS)
 @pytest.mark.parametrize("prefix_pages", [1, 7])
 @pytest.mark.parametrize("lens", [[1], [33, 1, 64, 5, 100], [700, 32, 31, 65, 7, 90] * 4])
