@@ -805,19 +805,22 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
 // ---- joining the ranges of one (token, query head)
 //
 // Rows come from paged_split_kernel's slots, from paged_block_kernel's splits, or (behind a shared
-// prefix) from both; ones whose only range has written the output are left alone. A wave per row, lane d
-// the dims HD / 64 d on (four heads of a token per wave: 128 sequences behind 16384 positions 107 us instead
-// of 97); where rows are few their ranges are many, and WR = 8 waves per row take ranges w, w + 8, ... and
-// meet in LDS.
+// prefix) from both; ones whose only range has written the output are left alone. A wave per row takes
+// 2 or 4 ranges at once, lane d of a range's dims 4d on (one range at once, 509 tokens of 14 heads of 64
+// in 13 ranges each: 77 us for attention and merge instead of 74; four heads of a token per wave: 128
+// sequences behind 16384 positions 107 us instead of 97). Where rows are few, WR = 8 waves per row take
+// ranges w, w + 8, ..., one at once, and meet in LDS (as above: 10.2 us instead of 10.0).
 constexpr int kMergeWaves = 8;  // of a workgroup
 
 template <typename E, int HD, int WR, int BT>
 __global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_kernel(PagedArgs a) {
   typedef typename E::T T;
-  constexpr int ND = HD / 64;
-  typedef float vec_t __attribute__((ext_vector_type(ND)));
-  __shared__ float ms[kMergeWaves], ls[kMergeWaves], os[kMergeWaves][HD];
-  const int lane = threadIdx.x & 63;
+  constexpr int VL = WR == 1 ? 4 : HD / 64, LR = HD / VL, G = 64 / LR;  // dims per lane, lanes per range, ranges at once
+  typedef T out_t __attribute__((ext_vector_type(VL)));
+  typedef float vec_t __attribute__((ext_vector_type(VL)));
+  __shared__ float ms[kMergeWaves], ls[kMergeWaves];
+  __shared__ __align__(16) vec_t os[kMergeWaves][LR];
+  const int lane = threadIdx.x & 63, ld = lane % LR;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int w = wave % WR;
   const int64_t item = (int64_t)blockIdx.x * (kMergeWaves / WR) + wave / WR;
@@ -874,21 +877,33 @@ __global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_kernel(PagedArgs
   if (WR == 1 && !run) return;
   float M = -__builtin_inff(), l = 0.0f;
   vec_t o = vec_t(0.0f);
+  // the factor from maximum m to mn
+  auto factor = [&](float m, float mn) __attribute__((always_inline)) {
+    return m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * sc);
+  };
   if (run) {
 #pragma unroll 4
-    for (int r = w; r < na + nb; r += WR) {
+    for (int r = w * G + lane / LR; r < na + nb; r += WR * G) {
       const bool split = r < na;
       const float* p = split ? pa + r * sa : pb + (int64_t)(r - na) * BT * (2 + HD);
       const int j = split ? row % kRows : jb, rows = split ? kRows : BT;
       const float m = p[2 * j], lr = p[2 * j + 1];
-      const vec_t v = *reinterpret_cast<const vec_t*>(p + 2 * rows + j * HD + ND * lane);
-      const float mn = fmaxf(M, m);
-      const float f0 = M == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((M - mn) * sc);
-      const float f1 = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * sc);
+      const vec_t v = *reinterpret_cast<const vec_t*>(p + 2 * rows + j * HD + VL * ld);
+      const float mn = fmaxf(M, m), f0 = factor(M, mn), f1 = factor(m, mn);
       l = l * f0 + lr * f1;
 #pragma unroll
-      for (int i = 0; i < ND; ++i) o[i] = __builtin_fmaf(v[i], f1, o[i] * f0);
+      for (int i = 0; i < VL; ++i) o[i] = __builtin_fmaf(v[i], f1, o[i] * f0);
       M = mn;
+    }
+  }
+  if constexpr (G > 1) {  // the wave's groups of lanes meet
+    const float mn = max_xor32(G == 4 ? max_xor16(M) : M), f = factor(M, mn);
+    l *= f, o *= f;
+#pragma unroll
+    for (int off = LR; off < 64; off *= 2) {
+      l += __shfl_xor(l, off);
+#pragma unroll
+      for (int i = 0; i < VL; ++i) o[i] += __shfl_xor(o[i], off);
     }
   }
   if constexpr (WR > 1) {
@@ -896,30 +911,27 @@ __global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_kernel(PagedArgs
       ms[wave] = M;
       ls[wave] = l;
     }
-#pragma unroll
-    for (int i = 0; i < ND; ++i) os[wave][ND * lane + i] = o[i];
+    os[wave][ld] = o;
     __syncthreads();
     if (!run || w) return;
-    float MM = -__builtin_inff();
+    float mn = -__builtin_inff();
 #pragma unroll
-    for (int i = 0; i < WR; ++i) MM = fmaxf(MM, ms[wave + i]);
-    l = 0.0f;
-    o = vec_t(0.0f);
+    for (int i = 0; i < WR; ++i) mn = fmaxf(mn, ms[wave + i]);
+    l = 0.0f, o = vec_t(0.0f);
 #pragma unroll
     for (int i = 0; i < WR; ++i) {
-      const float f = ms[wave + i] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((ms[wave + i] - MM) * sc);
-      l = __builtin_fmaf(ls[wave + i], f, l);
+      const float fw = factor(ms[wave + i], mn);
+      l = __builtin_fmaf(ls[wave + i], fw, l);
+      const vec_t v = os[wave + i][ld];
 #pragma unroll
-      for (int d = 0; d < ND; ++d) o[d] = __builtin_fmaf(os[wave + i][ND * lane + d], f, o[d]);
+      for (int d = 0; d < VL; ++d) o[d] = __builtin_fmaf(v[d], fw, o[d]);
     }
   }
-  T* dst = (T*)a.out + (int64_t)t * a.ldo + (int64_t)h * HD + ND * lane;
+  if (lane >= LR) return;
+  out_t y;
 #pragma unroll
-  for (int i = 0; i < ND; ++i) o[i] = l != 0.0f ? o[i] / l : 0.0f;
-  if constexpr (ND == 2)
-    *reinterpret_cast<uint32_t*>(dst) = pack2<E>(o[0], o[1]);
-  else
-    dst[0] = (T)o[0];
+  for (int i = 0; i < VL; ++i) y[i] = (T)(l != 0.0f ? o[i] / l : 0.0f);
+  *reinterpret_cast<out_t*>((T*)a.out + (int64_t)t * a.ldo + (int64_t)h * HD + VL * ld) = y;
 }
 
 // Up to this many chunks a sequence is one range, with nothing to merge; and up to kSingleMany where the
