@@ -399,8 +399,9 @@ int ldk_w8a16_matmul_swiglu(const void* x, int64_t ldx, const uint8_t* wq, const
  *    and below 2^31. A page holds, per kv head, the tiles of ldk_decode_attention's caches: K tiles
  *    [page_size/32][2][head_dim/32][16][32] and V^T tiles [page_size/32][head_dim/16][16][32].
  *  - block_table: int32 [B] rows of ldt >= max_pages ids (max_pages * page_size <= 2^25); position p
- *    of sequence b is in page block_table[b][p / page_size]. An id outside [0, num_pages) is no page: nothing is written there
- *    and its positions are not attended to. Positions from max_pages * page_size on do not exist.
+ *    of sequence b is in page block_table[b][p / page_size]. An id outside [0, num_pages) is no page:
+ *    nothing is written there and its positions are not attended to. Positions from max_pages *
+ *    page_size on do not exist.
  *  - cu_seqlens: int32 [B + 1], sequence b's new tokens are the rows cu_seqlens[b] ..
  *    cu_seqlens[b+1] - 1 of the T rows, in rising order; NULL: sequence b has row b (T >= B).
  *    kv_lens: int32 [B], the positions that sequence b's cache holds with its new tokens, which are
@@ -437,7 +438,11 @@ int64_t ldk_paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t max_q,
  * window == 0, j > p - window or j < sinks. q rows of ldq, out rows of ldo; max_q >= every sequence's
  * number of new tokens (tokens past it are not computed; ignored without cu_seqlens). A token that
  * sees nothing gives zeros. scale > 0. Scores and softmax in fp32, its numerators rounded to dtype
- * before they weight V, one rounding at the end. The workspace (16-byte aligned,
+ * before they weight V (fp16's weights below 2^-32 of a row's largest are lost), one rounding at the
+ * end. A NaN or infinity in v at a position that one token of the call sees may reach tokens that do not
+ * see it (weight 0 x NaN); what no token sees may hold anything, and k may at any position that a token
+ * does not see. A batch that both decodes over long contexts and prefills runs faster as two calls
+ * (max_q chooses one kernel for the call). The workspace (16-byte aligned,
  * ldk_paged_attention_workspace_bytes) holds nothing between calls: calls that may overlap need one
  * each. Stands beside ldk_decode_attention and ldk_prefill_attention (the reference's
  * scaled_dot_product_attention over one static cache, kernels/e2e/model.py:236-243). */

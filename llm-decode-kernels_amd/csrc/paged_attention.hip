@@ -190,7 +190,9 @@ constexpr int part_floats(int hd) { return kRows * (2 + hd); }
 // LDS bytes of split_rows: per wave the 16 rows' m, l and outputs.
 constexpr int split_lds(int hd, int nw) { return nw * kRows * (2 + hd) * 4; }
 
-// Workgroup wg of the split: NW waves.
+// Workgroup wg of the split: NW waves. Memory bounds it where the contexts are long: 64 tokens of 28/4
+// heads over 364 MB 76 us, 4.8 TB/s, the rate of a 2 GiB copy; the latency of finding the ranges and of two
+// launches where they are short (one token behind a window of 1024: 10.0 us with the merge).
 template <typename E, int HD, int NW>
 __device__ __forceinline__ void split_rows(const PagedArgs& a, int wg, unsigned char* lds) {
   typedef typename E::T T;
@@ -365,6 +367,13 @@ __global__ __launch_bounds__(NW * 64) void paged_split_kernel(PagedArgs a) {
 // as the column, so a lane's scores, maximum, sum and outputs are the same rows' and the online softmax
 // needs no shuffles beyond the maximum over a tile's positions. Chunks that every row sees whole run
 // without masks. Page ids come through the scalar cache, one chunk ahead of their loads.
+//
+// Bound by what a SIMD can issue of matrix and softmax instructions between two barriers: 5 windowed
+// prompts of 32/8 heads (124 GFLOP) 173 us, 717 TFLOP/s, 59% of a large matrix product's rate, with the
+// vector unit busy 48% and the matrix unit 35% of a CU's cycles. On those prompts, in us: 1420 with
+// split_rows (16 rows read K and V from L2), 269 with two K groups of 128 rows that met at every
+// barrier, 203 as four waves per workgroup and two workgroups per CU, 178 with the numerators' sum on the
+// matrix unit and the lagging maximum, the rest from forming maxima only where a score passes the limit.
 //
 // MODE 0: the rows of one sequence's new tokens over its visible chunks. Sequence b's tiles begin at
 // index cu[b] gq / rows + b (n gq rows need at most one tile more than floor((cu + n) gq / rows) -
@@ -784,7 +793,8 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
 
 // Behind a shared prefix: its blocks, which the matrix cores bound, and the sequences' own positions, which
 // the memory does, in one launch, so that a CU runs some of each. Groups of 8 workgroups (one per XCD)
-// are of one kind, the kinds spread evenly over the launch.
+// are of one kind, the kinds spread evenly over the launch. 128 sequences of up to 900 positions behind
+// 16384, 32/8 heads (205 MB, 35 GFLOP): 120 us in two launches, 104 in one, 96.5 now with the merge.
 template <typename E, int HD, int BT>
 __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_eu(2))) void paged_prefix_kernel(PagedArgs a) {
   constexpr int CG = BT / 32, KG = kBlockKG<BT>, S = kBlockSlots<BT>, NW = kBlockThreads<BT> / 64;

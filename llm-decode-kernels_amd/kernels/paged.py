@@ -228,7 +228,11 @@ def paged_attention(q: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.T
     hold the tokens' own k and v: the token at position p sees the positions j <= p of its sequence
     with window == 0, j > p - window or j < sinks. max_q: the most new tokens that a sequence has (a
     host number that chooses the launch; rows past it are not computed; None: as many as there are
-    rows). Returns [tokens, n_heads, hd]; a token that sees nothing gives zeros. scale > 0."""
+    rows). Returns [tokens, n_heads, hd]; a token that sees nothing gives zeros. scale > 0.
+
+    k may hold anything at positions that a token does not see, v at those that no token of the call
+    sees (its weights are 0, and 0 x NaN is NaN). max_q chooses one kernel for the call: a batch that
+    decodes over long contexts beside prompts runs faster as two calls."""
     return _attend("paged_attention", q, kv_lens, block_table, None, 0, k_pages, vt_pages, scale, cu_seqlens, max_q,
                    window, sinks, out)
 
