@@ -408,6 +408,7 @@ int ldk_w8a16_matmul_swiglu(const void* x, int64_t ldx, const uint8_t* wq, const
  *    the last of them: new token i of n is at position kv_lens[b] - n + i. A sequence without new
  *    tokens, kv_lens of 0 and rows behind the last sequence are allowed: those rows are left as they
  *    were. All of these are read on the device, so a captured graph takes new lengths and pages.
+ *  - T at most 2^24 rows, B at most 2^20 sequences (65535 for the attention).
  *  - data pointers 16-byte aligned, row strides (elements) multiples of 8. */
 
 /* RoPE on q and k and the cache write of T new tokens: qkv rows [nq * head_dim | nkv * head_dim |
@@ -435,8 +436,8 @@ int64_t ldk_paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t max_q,
 
 /* Causal grouped-query softmax attention of the new tokens over the pages (their own k and v
  * included: append first). The token at position p sees position j <= p of its sequence where
- * window == 0, j > p - window or j < sinks. q rows of ldq, out rows of ldo; max_q >= every sequence's
- * number of new tokens (tokens past it are not computed; ignored without cu_seqlens). A token that
+ * window == 0, j > p - window or j < sinks. q rows of ldq, out rows of ldo; max_q, 1..T, >= every
+ * sequence's number of new tokens (tokens past it are not computed; taken as 1 without cu_seqlens). A token that
  * sees nothing gives zeros. scale > 0. Scores and softmax in fp32, its numerators rounded to dtype
  * before they weight V (fp16's weights below 2^-32 of a row's largest are lost), one rounding at the
  * end. A NaN or infinity in v at a position that one token of the call sees may reach tokens that do not

@@ -25,9 +25,9 @@
 // Ranges. The lengths are on the device, so the split is made there: every sequence has its visible
 // chunks (those of the sinks, then those of the window) cut into ranges of `per` chunks, one `per` for
 // the whole batch such that all ranges fit the launch's slots; a ragged batch gets ranges of equal
-// work. Each wave finds its slot's sequence from the lengths alone. Sequences with more than one
-// range leave {max, sum} and the unnormalised output in the workspace, and paged_merge_kernel, the
-// next launch on the stream, joins them.
+// work. Each wave finds its slot's sequence from the lengths alone, or, of more than 64 sequences, in what
+// paged_plan_kernel found in a launch before. Sequences with more than one range leave {max, sum} and the
+// unnormalised output in the workspace, and paged_merge_kernel, the next launch on the stream, joins them.
 #include <algorithm>
 
 #include "lds_dma.h"
@@ -49,6 +49,7 @@ struct PagedArgs {
   float* part;    // paged_split_kernel's partials, per (slot, tile, kv head): [16 rows]{m, l} and [16 rows][hd]
   float* bpart;   // paged_block_kernel's, per (tile, kv head, split): [rows]{m, l} and [rows][hd]
   int32_t* plan;  // [B][2]: first slot and ranges of every sequence
+  int32_t* map;   // of many sequences: [0] chunks of a range, [1 + slot] its sequence; else null
   int T, B, max_q, nq, nkv, gq, nt;  // nt: 16-row tiles of a sequence
   int pages, cap;                    // cap: positions a sequence can hold
   PageDiv cpp;                       // chunks per page
@@ -113,8 +114,20 @@ __device__ __forceinline__ int wave_max_i(int v) {
 struct Slot {
   int b, split, ranges, first, per;  // b < 0: none
 };
+// Chunks of a range, of `sum` chunks in sequences of at most `most`.
+__device__ __forceinline__ int range_chunks(const PagedArgs& a, int64_t sum, int most) {
+  const int ways = a.spare ? a.spare : a.slots;
+  const int per = (int)min((sum + ways - 1) / ways, (int64_t)most);
+  return max(per, max(kMinRange, (most + kMaxRanges - 1) / kMaxRanges));
+}
 __device__ __forceinline__ Slot find_slot(const PagedArgs& a, int slot, int lane) {
   if (!a.plan) return Slot{slot, 0, 1, slot, kAll};  // every sequence in one range
+  if (a.map) {                                       // paged_plan_kernel has found it
+    const int b = a.map[1 + slot];
+    if (b < 0) return Slot{-1, 0, 1, 0, 0};
+    const int first = a.plan[2 * b];
+    return Slot{b, slot - first, a.plan[2 * b + 1], first, a.map[0]};
+  }
   const int each = (a.B + 63) / 64, b0 = lane * each, b1 = min(b0 + each, a.B);
   int64_t sum = 0;
   int most = 0, n0 = 0;
@@ -126,9 +139,7 @@ __device__ __forceinline__ Slot find_slot(const PagedArgs& a, int slot, int lane
   }
   sum = wave_sum64(sum);
   most = wave_max_i(most);
-  const int ways = a.spare ? a.spare : a.slots;
-  int per = (int)min((sum + ways - 1) / ways, (int64_t)most);
-  per = max(per, max(kMinRange, (most + kMaxRanges - 1) / kMaxRanges));
+  int per = range_chunks(a, sum, most);
   if (!a.spare && a.B > 1) {
     int hi = max(per, (int)min((int64_t)most, (sum + a.slots - a.B - 1) / (a.slots - a.B)));
     while (per < hi) {
@@ -175,6 +186,51 @@ __device__ __forceinline__ Slot find_slot(const PagedArgs& a, int slot, int lane
   return r;
 }
 
+// find_slot for many sequences, once instead of by every wave: one workgroup. spare != 0.
+constexpr int kPlanThreads = 1024;
+__global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedArgs a) {
+  constexpr int NW = kPlanThreads / 64;
+  __shared__ int64_t sums[NW];
+  __shared__ int mosts[NW], totals[NW];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int64_t sum = 0;
+  int most = 0;
+  for (int b = tid; b < a.B; b += kPlanThreads) {
+    const int n = seq_span(a, b).n;
+    sum += n;
+    most = max(most, n);
+  }
+  sum = wave_sum64(sum);
+  most = wave_max_i(most);
+  if (lane == 0) sums[wave] = sum, mosts[wave] = most;
+  __syncthreads();
+  sum = 0, most = 0;
+  for (int w = 0; w < NW; ++w) sum += sums[w], most = max(most, mosts[w]);
+  const int per = range_chunks(a, sum, most);
+  if (tid == 0) a.map[0] = per;
+  int base = 0;
+  for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
+    const int b = b0 + tid, n = b < a.B ? max(1, (seq_span(a, b).n + per - 1) / per) : 0;
+    int end = n;  // inclusive scan over the lanes
+#pragma unroll
+    for (int off = 1; off < 64; off *= 2) {
+      const int v = __shfl_up(end, off);
+      if (lane >= off) end += v;
+    }
+    if (lane == 63) totals[wave] = end;
+    __syncthreads();
+    int first = base + end - n;
+    for (int w = 0; w < NW; ++w) {
+      first += w < wave ? totals[w] : 0;
+      base += totals[w];
+    }
+    if (b < a.B) a.plan[2 * b] = first, a.plan[2 * b + 1] = n;
+    for (int i = first; i < min(first + n, a.slots); ++i) a.map[1 + i] = b;
+    __syncthreads();  // the totals have been read
+  }
+  for (int i = base + tid; i < a.slots; i += kPlanThreads) a.map[1 + i] = -1;
+}
+
 __device__ __forceinline__ float max_xor16(float v) {
   auto p = __builtin_amdgcn_permlane16_swap(f2u(v), f2u(v), false, false);
   return fmaxf(u2f(p[0]), u2f(p[1]));
@@ -208,7 +264,7 @@ __device__ __forceinline__ void split_rows(const PagedArgs& a, int wg, unsigned 
   const Slot sl = find_slot(a, wg / xy, lane);
   if (sl.b < 0) return;
   const Span sp = seq_span(a, sl.b);
-  if (a.plan && kvh == 0 && tile == 0 && sl.split == 0 && tid == 0) {
+  if (a.plan && !a.map && kvh == 0 && tile == 0 && sl.split == 0 && tid == 0) {
     a.plan[2 * sl.b] = sl.first;
     a.plan[2 * sl.b + 1] = sl.ranges;
   }
@@ -794,7 +850,8 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
 // Behind a shared prefix: its blocks, which the matrix cores bound, and the sequences' own positions, which
 // the memory does, in one launch, so that a CU runs some of each. Groups of 8 workgroups (one per XCD)
 // are of one kind, the kinds spread evenly over the launch. 128 sequences of up to 900 positions behind
-// 16384, 32/8 heads (205 MB, 35 GFLOP): 120 us in two launches, 104 in one, 96.5 now with the merge.
+// 16384, 32/8 heads (205 MB, 35 GFLOP): 120 us in two launches, 104 in one, 96 now
+// with the merge.
 template <typename E, int HD, int BT>
 __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_eu(2))) void paged_prefix_kernel(PagedArgs a) {
   constexpr int CG = BT / 32, KG = kBlockKG<BT>, S = kBlockSlots<BT>, NW = kBlockThreads<BT> / 64;
@@ -949,12 +1006,17 @@ __global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_kernel(PagedArgs
 // ranges and merge, us: 1 sequence of 12/2 heads at 300 positions 8.1 / 10.3, 600 9.7 / 10.4, 1100 13.6 / 10.5;
 // 64 of 28/4 at 1050 29 / 40.
 constexpr int kSingle = 20, kSingleMany = 36;
+// More sequences than a wave's lanes have their ranges found by paged_plan_kernel, a launch before: every wave's
+// own search grows with the batch. Graph-timed, own search / launch, us: 28/4 heads, 200 to 1000 positions, 96
+// sequences 37 / 35, 256 72 / 60, 1024 437 / 244, 4096 4119 / 949; 100 to 4000 positions, 96 78 / 79, 512 404 / 370.
+constexpr int kPlanSeqs = 64;
 
 // What a call launches, from its sizes alone.
 struct Plan {
   bool apart = false;                               // the shared prefix in blocks of its own
   int64_t nt = 0, slots = 0, spare = 0;             // paged_split_kernel, slots == 0: not launched
   int64_t bt = 0, btiles = 0, bsplits = 0;          // paged_block_kernel, bt == 0: not launched
+  bool mapped = false;                              // paged_plan_kernel
   int64_t part_bytes = 0, bpart_bytes = 0, bytes = 0;
 };
 // Chunks that a token sees at most, from the positions a table holds and the window.
@@ -983,6 +1045,7 @@ Plan make_plan(int64_t T, int64_t B, int64_t max_q, int64_t max_len, int64_t win
     const int64_t w = nkv * p.nt, round = (hd == 128 ? 256 : 512) / w;
     p.spare = 2 * round >= 3 * B ? 0 : std::max<int64_t>(1, (prefix_len ? 256 : 384) / w);
     p.slots = p.spare ? B + p.spare : round;
+    p.mapped = p.spare && B > kPlanSeqs;
     p.part_bytes = p.slots * w * part_floats(hd) * 4;
   }
   if (block || p.apart) {
@@ -998,7 +1061,7 @@ Plan make_plan(int64_t T, int64_t B, int64_t max_q, int64_t max_len, int64_t win
     p.bsplits = !p.apart && 3 * whole >= fill ? 1 : std::max<int64_t>(1, std::min<int64_t>(32, fill / whole));
     if (p.apart || p.bsplits > 1) p.bpart_bytes = p.btiles * nkv * p.bsplits * p.bt * (2 + hd) * 4;
   }
-  p.bytes = p.part_bytes + p.bpart_bytes + (p.part_bytes ? B * 8 : 0);
+  p.bytes = p.part_bytes + p.bpart_bytes + (p.part_bytes ? B * 8 : 0) + (p.mapped ? (p.slots + 1) * 4 : 0);
   return p;
 }
 // A launch holds fewer than 2^32 threads.
@@ -1022,6 +1085,10 @@ template <typename E, int HD>
 int launch(const PagedArgs& a, const Plan& p, hipStream_t s) {
   (void)hipGetLastError();
   int st;
+  if (p.mapped) {
+    paged_plan_kernel<<<1, kPlanThreads, 0, s>>>(a);
+    if ((st = ldk::check_launch("paged_attention plan"))) return st;
+  }
   if (p.bt) {
     st = p.bt == 128 ? launch_rows<E, HD, 128>(a, p, s) : launch_rows<E, HD, 64>(a, p, s);
   } else {
@@ -1086,6 +1153,7 @@ int run(const char* fn, const void* q, int64_t ldq, int dtype, const int32_t* cu
   a.part = (float*)ws;
   a.bpart = (float*)((char*)ws + p.part_bytes);
   a.plan = p.part_bytes ? (int32_t*)((char*)ws + p.part_bytes + p.bpart_bytes) : nullptr;
+  a.map = p.mapped ? a.plan + 2 * B : nullptr;
   a.T = cu ? (int)T : (int)B, a.B = (int)B, a.max_q = cu ? (int)max_q : 1;
   a.nq = nq, a.nkv = nkv, a.gq = nq / nkv, a.nt = (int)p.nt;
   a.pages = (int)num_pages, a.cpp = page_div(page_size / kChunkPos), a.cap = (int)(max_pages * page_size);

@@ -249,6 +249,16 @@ def test_attention_many_sequences():
     check_attention(lens, news, 4, 2, 64, 32, F16)
 
 
+@pytest.mark.parametrize("prefix", [0, 128])
+@pytest.mark.parametrize("count", [257, 1100])
+def test_attention_ranges_of_very_many_sequences(count, prefix):
+    """Ranges that one workgroup finds for the batch: short sequences, empty ones, and a few of many ranges."""
+    lens = [(37 * i) % 90 for i in range(count)]
+    lens[3] = lens[count // 2] = lens[-1] = 1500
+    check_attention([max(n, 1) for n in lens], [1] * count, 4, 2, 64, 32, F16, cu=False, prefix=prefix)
+    check_attention(lens, [min(n, i % 3) for i, n in enumerate(lens)], 4, 2, 64, 32, BF16, prefix=prefix)
+
+
 @pytest.mark.parametrize("prefix", [0, 64])
 def test_attention_long_contexts_beside_prompts(prefix):
     """A batch that decodes and prefills at once: one token after many positions beside whole prompts."""
