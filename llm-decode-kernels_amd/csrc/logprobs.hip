@@ -10,6 +10,10 @@
 //    raises the maximum rescales them. The maximum's own term is left out of the sums until another
 //    replaces it, so that ln s = log1p(rest) keeps its digits where one token has nearly all the
 //    probability. 2^-inf * -inf would be NaN: a tile whose second sum is NaN is summed again, clamped.
+//    Of a maximum past 2^24 (words masked with a large finite number) m log2 e as rounded is off by whole
+//    powers of two, or infinite. Such a wave sums nothing: next to a slice's larger maximum its logits have no
+//    weight, and a slice whose maximum is far is read again, for y = (x - m) log2 e. (That as a branch of
+//    every tile took 5 to 13% of the time of rows without such logits.)
 //  - The largest: each wave keeps candidates (64-bit keys, value then lower index) in its own LDS list
 //    and a floor that none of the `top` largest can be below. Its first is the top-th largest of its 64
 //    lanes' maxima (found by ballots), which lets through about the logits that are the largest so
@@ -180,18 +184,32 @@ __device__ __forceinline__ uint64_t rank_keys(const uint64_t* keys, int total, i
 }
 
 // A part of a row: its maximum m, and over its other logits the sums of 2^y and 2^y y, y = x log2 e -
-// m log2 e (as rounded: base_of). m == -inf: nothing but -inf.
+// m log2 e (as rounded: base_of). m == -inf: nothing but -inf. Of a far m: y = (x - m) log2 e.
 struct Sums {
   float m, s, y;
 };
+constexpr float kFar = 16777216.0f;    // 2^24, where what base_of rounds away reaches 1
+constexpr float kNoSum = 2.0f * kFar;  // past it a wave sums nothing: between the two it may meet a near maximum
+__device__ __forceinline__ bool is_far(float m) { return fabsf(m) >= kFar && m != -__builtin_inff(); }
 __device__ __forceinline__ float base_of(float m) { return m == -__builtin_inff() ? 0.0f : m * kLog2e; }
-// The maximum's own exponent: what base_of rounded away.
-__device__ __forceinline__ float residue(float m) { return __builtin_fmaf(m, kLog2e, -base_of(m)); }
+__device__ __forceinline__ float rounded_away(float m) { return __builtin_fmaf(m, kLog2e, -base_of(m)); }
+// The maximum's own exponent: what base_of rounded away, 0 of a far one; no number of an infinity.
+template <bool FAR>
+__device__ __forceinline__ float residue(float m) {
+  return FAR && is_far(m) ? m - m : rounded_away(m);
+}
+// From exponents against m to those against top >= m; finite, so that 0 times it is 0.
+template <bool FAR>
+__device__ __forceinline__ float step_to(float m, float top) {
+  if (!FAR || !(is_far(m) || is_far(top))) return base_of(m) - base_of(top);
+  return fmaxf((m - top) * kLog2e - residue<FAR>(m) + residue<FAR>(top), -1e9f);
+}
 // a's sums with its own maximum's term, taken against the maximum m >= a.m.
+template <bool FAR>
 __device__ __forceinline__ void rebase(Sums& a, float m) {
-  const float d = base_of(a.m) - base_of(m), f = a.m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(d);
+  const float d = step_to<FAR>(a.m, m), f = a.m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(d);
   if (a.m > -__builtin_inff()) {
-    const float r = residue(a.m), p = __builtin_amdgcn_exp2f(r);
+    const float r = residue<FAR>(a.m), p = __builtin_amdgcn_exp2f(r);
     a.s += p;
     a.y = __builtin_fmaf(p, r, a.y);
   }
@@ -199,23 +217,36 @@ __device__ __forceinline__ void rebase(Sums& a, float m) {
   a.s *= f;
   a.m = m;
 }
+template <bool FAR>
 __device__ __forceinline__ Sums join(Sums a, Sums b) {
   if (b.m > a.m) {
     const Sums t = a;
     a = b;
     b = t;
   }
-  rebase(b, a.m);
+  rebase<FAR>(b, a.m);
   a.s += b.s;
   a.y += b.y;
   return a;
 }
+// a's sums against its base as those against its maximum itself.
+__device__ __forceinline__ void rebase_to_maximum(Sums& a) {
+  const float r = rounded_away(a.m), f = __builtin_amdgcn_exp2f(-r);
+  a.y = f * __builtin_fmaf(-r, a.s, a.y);
+  a.s *= f;
+}
 // Over the lanes: the first that has the largest maximum keeps its term out.
+template <bool FAR>
 __device__ __forceinline__ Sums wave_join(Sums a, int lane) {
   const float m = wave_max(a.m);
-  if (lane != __builtin_ctzll(__ballot(a.m == m) | (uint64_t(1) << 63))) rebase(a, m);
+  if (lane != __builtin_ctzll(__ballot(a.m == m) | (uint64_t(1) << 63))) rebase<FAR>(a, m);
   return Sums{m, ldk::sum_lanes_strided<1>(a.s), ldk::sum_lanes_strided<1>(a.y)};
 }
+
+template <typename T>
+constexpr bool kCanBeFar = true;
+template <>
+constexpr bool kCanBeFar<half_t> = false;  // 65504 at most
 
 template <typename T>
 __device__ __forceinline__ float to_f(T v);
@@ -237,7 +268,7 @@ __device__ __forceinline__ float given_logit(const LogprobArgs& a, int64_t row) 
 template <typename T>
 __device__ __forceinline__ void finish(const LogprobArgs& a, int64_t row, const Sums& t, float given, uint64_t key, int lane) {
   // against the maximum itself: without what its base rounded away
-  const float r = residue(t.m), f = __builtin_amdgcn_exp2f(-r);
+  const float r = residue<kCanBeFar<T>>(t.m), f = __builtin_amdgcn_exp2f(-r);
   const float rest = t.s * f, y = f * __builtin_fmaf(-r, t.s, t.y);
   const float log_s = log1pf(rest);
   if (lane == 0) {
@@ -250,8 +281,10 @@ __device__ __forceinline__ void finish(const LogprobArgs& a, int64_t row, const 
   }
 }
 
+// Without alternatives 8 waves a SIMD hide the loads best, the most there are: the compiler then keeps to the
+// scalar registers that they leave (1900 rows of 151936 bf16 126 us at 7 waves, 112 at 8).
 template <typename T, bool TOP>
-__global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 6 : 5) void logprobs_kernel(LogprobArgs a) {
+__global__ __launch_bounds__(kWaves * 64, sizeof(T) == 4 ? 5 : TOP ? 6 : 8) void logprobs_kernel(LogprobArgs a) {
   constexpr int VEC = 16 / sizeof(T), NV = kPer / VEC;
   typedef T vec_t __attribute__((ext_vector_type(VEC)));
   typedef vec_t unaligned_t __attribute__((aligned(sizeof(T))));
@@ -261,6 +294,7 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 6 : 5) void logprobs_
   __shared__ uint32_t floors[kWaves];
   __shared__ int pooled;
   __shared__ Sums sums[kWaves];
+  __shared__ Sums far[kWaves];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t row = blockIdx.y + (int64_t)blockIdx.z * 65535;
@@ -283,8 +317,23 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 6 : 5) void logprobs_
     for (int u = 0; u < NV; ++u) v[u] = *reinterpret_cast<const unaligned_t*>(x + min(place(t, u * VEC), whole - VEC));
   };
 
+  // of a far maximum m: how many logits of the wave equal it, and the others' sums
+  auto far_sums = [&](float m) __attribute__((always_inline)) {
+    float equal = 0.0f, s = 0.0f, y = 0.0f;
+    const int begin = min(first * kTileLogits, whole);
+    const int end = first + tiles > vtiles ? a.V : min(whole, (first + tiles) * kTileLogits);
+#pragma unroll 1
+    for (int i = begin + tid; i < end; i += kWaves * 64) {
+      const float v = to_f<T>(x[i]), e = (v - m) * kLog2e, p = v == m ? 0.0f : __builtin_amdgcn_exp2f(e);
+      equal += v == m ? 1.0f : 0.0f;
+      s += p;
+      y = __builtin_fmaf(p, fmaxf(e, -1e30f), y);
+    }
+    return Sums{ldk::sum_lanes_strided<1>(equal), ldk::sum_lanes_strided<1>(s), ldk::sum_lanes_strided<1>(y)};
+  };
+
   Sums s{-__builtin_inff(), 0.0f, 0.0f};  // m: of the wave
-  float nb = 0.0f, lmax = -__builtin_inff();  // -base_of(m); this lane's largest so far
+  float nb = 0.0f, lmax = -__builtin_inff();  // -base_of(m), or -inf for no sums; this lane's largest so far
   // Candidates' keys are above floor; `none` is below the key of every number. own: the last value of the
   // wave's own top so far: later logits that equal it come after it
   const uint32_t none = order(-__builtin_inff()) - 1;
@@ -319,16 +368,18 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 6 : 5) void logprobs_
     if (__any(tm > s.m)) {  // a new maximum: its first lane leaves one logit that equals it out
       const float m = wave_max(tm);
       const bool holds = lane == __builtin_ctzll(__ballot(tm == m));
-      const float d = base_of(s.m) - base_of(m), f = s.m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(d);
-      if (lane == 0 && s.m > -__builtin_inff()) {  // the old maximum's term joins lane 0's sums
-        const float r = residue(s.m), p = __builtin_amdgcn_exp2f(r);
+      // finite, so that 0 times it is 0 (infinite where a product overflows; past 0 only from -inf)
+      const float d = fminf(fmaxf(base_of(s.m) - base_of(m), -1e9f), 0.0f);
+      const float f = s.m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(d);
+      if (lane == 0 && fabsf(s.m) <= kNoSum) {  // the old maximum's term joins lane 0's sums
+        const float r = rounded_away(s.m), p = __builtin_amdgcn_exp2f(r);
         s.s += p;
         s.y = __builtin_fmaf(p, r, s.y);
       }
       s.y = f * __builtin_fmaf(d, s.s, s.y);
       s.s *= f;
       s.m = m;
-      nb = -base_of(m);
+      nb = fabsf(m) <= kNoSum ? -base_of(m) : -__builtin_inff();
       bool left = !holds;
 #pragma unroll
       for (int e = 0; e < kPer; ++e) {
@@ -424,6 +475,7 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 6 : 5) void logprobs_
 
   s.s = ldk::sum_lanes_strided<1>(s.s);
   s.y = ldk::sum_lanes_strided<1>(s.y);
+  if (kCanBeFar<T> && is_far(s.m) && fabsf(s.m) <= kNoSum) rebase_to_maximum(s);
   if (lane == 0) sums[wave] = s;
   uint64_t key = 0;
   if constexpr (TOP) {
@@ -434,6 +486,25 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 6 : 5) void logprobs_
     if (lane == 0) floors[wave] = own;
   }
   __syncthreads();
+  if constexpr (kCanBeFar<T>) {
+    float m = sums[0].m;
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) m = fmaxf(m, sums[w].m);
+    if (is_far(m) && m != __builtin_inff()) {  // of the slice (uniform): its logits are read again
+      const Sums mine = far_sums(m);
+      __syncthreads();  // every wave has read the maxima
+      if (lane == 0) far[wave] = mine;
+      __syncthreads();
+      if (tid == 0) {
+        Sums t{m, -1.0f, 0.0f};
+        for (int w = 0; w < kWaves; ++w) t.s += far[w].m;  // how many equal the maximum
+        for (int w = 0; w < kWaves; ++w) t.s += far[w].s, t.y += far[w].y;
+        sums[0] = t;
+      }
+      if (tid > 0 && tid < kWaves) sums[tid] = Sums{-__builtin_inff(), 0.0f, 0.0f};
+      __syncthreads();
+    }
+  }
   if constexpr (TOP) {  // what is at or above every floor, of all four lists
     uint32_t floor = none, least = 0xffffffffu;
 #pragma unroll
@@ -457,7 +528,7 @@ __global__ __launch_bounds__(kWaves * 64, sizeof(T) == 2 ? 6 : 5) void logprobs_
   if (wave) return;
   Sums all = sums[0];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) all = join(all, sums[w]);
+  for (int w = 1; w < kWaves; ++w) all = join<kCanBeFar<T>>(all, sums[w]);
   if (a.splits == 1) {
     finish<T>(a, row, all, given, key, lane);
   } else {
@@ -483,9 +554,9 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(LogprobArgs a) {
   Sums s{-__builtin_inff(), 0.0f, 0.0f};
   for (int i = lane; i < a.splits; i += 64) {
     const float* p = a.part + (row * a.splits + i) * 4;
-    s = join(s, Sums{p[0], p[1], p[2]});
+    s = join<kCanBeFar<T>>(s, Sums{p[0], p[1], p[2]});
   }
-  s = wave_join(s, lane);
+  s = wave_join<kCanBeFar<T>>(s, lane);
   uint64_t key = 0;
   if (a.top) {
     const int total = a.splits * a.top;

@@ -134,6 +134,74 @@ def test_large_logits():
     check(x + torch.tensor([[3e4], [-3e4], [100.0]], device="cuda"), t, 5)
 
 
+LOWEST = {t: torch.finfo(t).min for t in (torch.float16, torch.bfloat16, torch.float32)}
+
+
+def masked_rows(V, dtype, mask):
+    """Rows whose masked words hold `mask`: the first 1024, the last, all but ten, a tail, all, the first half
+    beside others at the type's lowest value; the given token masked in every second of two passes."""
+    x, t = logits(6, V, dtype, seed=V)
+    i = torch.arange(V, device="cuda")
+    hidden = torch.stack([i < 1024, i == V - 1, i % (V // 10) != 3, i >= 3 * V // 4, i >= 0, i < V // 2])
+    x = torch.where(hidden, torch.tensor(mask, device="cuda", dtype=dtype), x)
+    x[5, V // 2:V // 2 + V // 4] = LOWEST[dtype]
+    return x, t, hidden
+
+
+@pytest.mark.parametrize("dtype,mask", [(torch.float32, -1e5), (torch.float32, -1e9), (torch.float32, -1e10),
+                                        (torch.float32, -2e10), (torch.float32, -1e20), (torch.float32, -1e30),
+                                        (torch.float32, -2.3e38), (torch.float32, LOWEST[torch.float32]),
+                                        (torch.bfloat16, -1e10), (torch.bfloat16, -1e30),
+                                        (torch.bfloat16, LOWEST[torch.bfloat16]), (torch.float16, LOWEST[torch.float16])])
+@pytest.mark.parametrize("V,repeat", [(1025, 1), (5000, 1), (9000, 200), (40000, 1)])
+def test_words_masked_with_finite_numbers(V, repeat, dtype, mask):
+    """A finite mask is a logit like any other: alone in a wave's first tile, in the tile of the last logits,
+    in whole slices, and in a row that holds nothing else (uniform, not NaN)."""
+    x, t, hidden = masked_rows(V, dtype, mask)
+    x, t = x.repeat(repeat, 1), t.repeat(repeat)
+    for top in (0, 5, 64):
+        r = check(x, t, top)
+        assert r.logprob.isfinite().all() and r.entropy.isfinite().all()
+        assert abs(r.entropy[4].item() - math.log(V)) <= 2.0 ** -20 * V / 64
+    check(x, torch.where(hidden.repeat(repeat, 1).any(-1), hidden.repeat(repeat, 1).int().argmax(-1), 0), 1)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("size", [1e5, 1e6, 1e7, 1e10, 1e20, 1e37])
+def test_logits_of_any_size(size, dtype):
+    """Finite logits of both signs, spread as widely as they are large; shifted to either side of 0."""
+    x, t = logits(3, 9000, torch.float32, seed=3)
+    wide = (x * size).to(dtype)
+    check(wide, t, 20)
+    check(wide[:, :1024].contiguous(), t % 1024, 20)
+    if size <= 1e10:  # where a step of the type is left between them
+        check((x + torch.tensor([[size], [-size], [2 * size]], device="cuda")).to(dtype), t, 20)
+
+
+@pytest.mark.parametrize("V", [40, 5000, 40000])
+def test_infinities_beside_finite_masks(V):
+    """+inf and NaN give NaN, -inf beside a finite mask counts as less than it."""
+    x, t = logits(4, V, torch.float32)
+    x[:, V // 2:] = LOWEST[torch.float32]
+    x[0, 3], x[1, 3], x[2, :V // 2] = INF, NAN, -INF
+    x[3] = -INF
+    x[3, V - 1] = LOWEST[torch.float32]
+    r = check(x, torch.tensor([3, 3, V - 1, V - 1], device="cuda"), 5)
+    assert r.logprob[:2].isnan().all() and r.logprob[2].isfinite() and r.logprob[3] == 0
+
+
+def test_far_logits_of_every_slice():
+    """Finite masks in slices that hold whole tiles, the last logits alone, and both; numbers on either side of
+    what a near maximum is, one above the other by little."""
+    for V in (4097, 12289, 16383, 16385, 20487):
+        x = torch.full((4, V), -3e7, device="cuda")
+        x[0, V - 1], x[1, 5], x[2, 1030] = -16777210.0, -16777217.0, 16777218.0
+        x[0, 3], x[0, 9], x[1, 2000], x[2, V - 1] = -16777218.0, -16777212.0, -16777218.0, 16777216.0
+        x[3] += 2 * (torch.arange(V, device="cuda") % 5)
+        for top in (0, 6):
+            check(x, torch.tensor([3, 2000, V - 1, 4], device="cuda"), top)
+
+
 def test_leading_shapes_and_empty():
     x, t = logits(12, 300, torch.float16)
     r = token_logprobs(x.view(3, 4, 300), t.view(3, 4), 2)
