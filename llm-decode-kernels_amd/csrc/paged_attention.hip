@@ -327,13 +327,14 @@ __device__ __forceinline__ void split_rows(const PagedArgs& a, int wg, unsigned 
     }
     mc = max_xor32(max_xor16(mc));
     const float m_new = fmaxf(m_run, mc);
-    // a row that has seen nothing so far keeps m = -inf; its exponents are taken against 0
-    const float base = m_new == -__builtin_inff() ? 0.0f : m_new * sc;
-    const float alpha = __builtin_amdgcn_exp2f(__builtin_fmaf(m_run, sc, -base));
+    // a row that has seen nothing so far keeps m = -inf; its exponents are taken against 0. Differences are
+    // formed before they are scaled: what m sc rounds away would rescale a row at every chunk
+    const float base = m_new == -__builtin_inff() ? 0.0f : m_new;
+    const float alpha = __builtin_amdgcn_exp2f((m_run - base) * sc);
     m_run = m_new;
     float x[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], sc, E::kShift - base));
+    for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e] - base, sc, E::kShift));
     u32x4 pa;
 #pragma unroll
     for (int e = 0; e < 4; ++e) pa[e] = pack2<E>(x[2 * e], x[2 * e + 1]);
@@ -654,7 +655,7 @@ __device__ __forceinline__ void block_rows(const PagedArgs& a, int wg, int split
   float m_run[2] = {-__builtin_inff(), -__builtin_inff()};
   float4_t sum[2];     // of the numerators as rounded, by a row of ones in the place of V^T: every element is row c16's
   float4_t o[2][NB];   // O^T[dim 16b + 4kb + r][row c16], unnormalised
-  float4_t acc[2][2];  // [row half hb][column tile]: scores of positions 8kb + 4hb + r
+  float4_t acc[2][2];  // [row half hb][column tile]: scores of positions 8kb + 4hb + r, less the row's maximum so far
   u32x4 ph[2];         // numerators: the B operand of P.V
 #pragma unroll
   for (int ct = 0; ct < 2; ++ct)
@@ -670,17 +671,15 @@ __device__ __forceinline__ void block_rows(const PagedArgs& a, int wg, int split
     for (int i = 0; i < NB; ++i) t[i] = *reinterpret_cast<const u32x4*>(src + i * 1024 + lane * 16);
     __builtin_amdgcn_sched_barrier(0);
   };
+  // the products are added to -m_run (0 while m_run is -inf), so that a row's exponents need no difference
+  float4_t less[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
   auto scores = [&]() __attribute__((always_inline)) {
-#pragma unroll
-    for (int hb = 0; hb < 2; ++hb)
-#pragma unroll
-      for (int ct = 0; ct < 2; ++ct) acc[hb][ct] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int s = 0; s < NS; ++s)
 #pragma unroll
       for (int hb = 0; hb < 2; ++hb)
 #pragma unroll
-        for (int ct = 0; ct < 2; ++ct) acc[hb][ct] = E::mfma(kt[NS * hb + s], q[ct][s], acc[hb][ct]);
+        for (int ct = 0; ct < 2; ++ct) acc[hb][ct] = E::mfma(kt[NS * hb + s], q[ct][s], s ? acc[hb][ct] : less[ct]);
   };
   auto pv = [&](auto maskedc, int cb0) __attribute__((always_inline)) {
     uint32_t mk[2][4];
@@ -710,9 +709,8 @@ __device__ __forceinline__ void block_rows(const PagedArgs& a, int wg, int split
   // The maximum that is subtracted may lag the largest score by kLag (in powers of two): the numerators
   // then reach 2^(kLag + kShift), inside every type, and the outputs are rescaled once or twice a block instead of
   // at most of its chunks (16 rows rarely all keep their maximum over a chunk).
-  float nb[2] = {0.0f, 0.0f};  // kShift - m_run * sc, 0 while m_run is -inf
   const float lag = kLag / sc;
-  float limit[2] = {-__builtin_inff(), -__builtin_inff()};  // m_run + lag
+  float limit[2] = {-__builtin_inff(), -__builtin_inff()};  // lag, -inf while m_run is
   auto softmax = [&](auto maskedc, int cb0) __attribute__((always_inline)) {
 #pragma unroll
     for (int ct = 0; ct < 2; ++ct) {
@@ -727,19 +725,23 @@ __device__ __forceinline__ void block_rows(const PagedArgs& a, int wg, int split
       }
       if (__any(mc > limit[ct])) {  // of any lane: the rows' maxima are only formed here
         mc = max_xor32(max_xor16(mc));
-        const float m_new = fmaxf(m_run[ct], mc);
-        // a row that has seen nothing so far keeps m = -inf; its factor is taken against 0
-        nb[ct] = m_new == -__builtin_inff() ? 0.0f : __builtin_fmaf(m_new, -sc, E::kShift);
-        const float alpha = __builtin_amdgcn_exp2f(__builtin_fmaf(m_run[ct], sc, nb[ct] - E::kShift));
+        // a row that has seen nothing so far keeps m = -inf; its scores are less 0. One that keeps its
+        // maximum keeps its sums to the bit
+        const float old = less[ct][0], m_new = fmaxf(m_run[ct], mc - old);
+        const float now = m_new == -__builtin_inff() ? 0.0f : -m_new, more = old - now;
+        const float alpha = m_run[ct] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(-more * sc);
         sum[ct] *= alpha;
 #pragma unroll
         for (int b = 0; b < NB; ++b) o[ct][b] *= alpha;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e >> 2][ct][e & 3] -= more;
         m_run[ct] = m_new;
-        limit[ct] = m_new + lag;
+        less[ct] = float4_t{now, now, now, now};
+        limit[ct] = m_new == -__builtin_inff() ? m_new : lag;
       }
       float x[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[e >> 2][ct][e & 3], sc, nb[ct]));
+      for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[e >> 2][ct][e & 3], sc, E::kShift));
 #pragma unroll
       for (int e = 0; e < 4; ++e) ph[ct][e] = pack2<E>(x[2 * e], x[2 * e + 1]);
     }

@@ -348,6 +348,92 @@ def test_attention_large_scores(news):
     assert_within(got, ref, bound)
 
 
+def _one_pool(k, v, page):
+    """Pages of one sequence's k, v [L, 1, hd] in order, and their table."""
+    L, _, hd = k.shape
+    k, v = (t.view(L // page, page, 1, hd).transpose(1, 2).contiguous() for t in (k, v))
+    return k_to_tiles(k).cuda(), vt_to_tiles(v).cuda(), torch.arange(L // page, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("dtype,hd", [(F16, 128), (BF16, 64)])
+def test_attention_of_equal_scores_far_from_zero(dtype, hd):
+    """131072 positions of one score, 840, the first half of value 1 and the others of 0: every weight is the
+    same, whatever the maximum's product with scale log2 e loses in rounding (here 2^-14 of an exponent, at each
+    of a wave's 512 chunks). The result is a half: the fp32 sums of 512 chunks and 8 waves, each to half a step of
+    2^-24 per term, and one rounding, of which a half of the type's step is 2^-1 eps / 2."""
+    B, L, page = 170, 131072, 64
+    k, v = torch.zeros(L, 1, hd, dtype=dtype), torch.zeros(L, 1, hd, dtype=dtype)
+    k[:, 0, 0], v[:L // 2] = 112.0, 1.0
+    k, v, table = _one_pool(k, v, page)
+    q = torch.zeros(B, 1, hd, dtype=dtype, device="cuda")
+    q[:, 0, 0] = 62.5  # 7000 exactly
+    got = paged.paged_attention(q, i32([L] * B), table.expand(B, -1).contiguous(), k, v, 0.12)
+    assert ((got.double() - 0.5).abs() <= torch.finfo(dtype).eps / 4 + (2 * 512 + 64) * 2.0 ** -24).all(), got.double().sub(0.5).abs().max()
+
+
+@pytest.mark.parametrize("dtype,hd", [(F16, 128), (BF16, 64)])
+@pytest.mark.parametrize("prefix", [False, True])
+def test_attention_rows_beside_a_rising_one(prefix, dtype, hd):
+    """Two heads whose rows share the matrix cores' tiles: of head 0 every score is 840, of head 1 they rise by
+    more than 8 powers of two per chunk, so that its rows are rescaled at each of 511 chunks. Head 0's sums must
+    not change with them. Bounds as above; head 1 sees the last chunk's positions with equal weights."""
+    B, new, L, page, scale = 86, 64, 16384, 64, 0.12
+    if prefix:
+        B, new = 64, 1
+    k, v = torch.zeros(L, 1, hd, dtype=dtype), torch.zeros(L, 1, hd, dtype=dtype)
+    k[:, 0, 0], v[:L // 2] = 112.0, 1.0
+    rise = torch.arange(L) // 32 % 256  # (twice from 0 on: bf16 holds whole numbers to 256)
+    k[:, 0, 1], k[:, 0, 2] = rise.to(dtype), (torch.arange(L) // 8192 * 256).to(dtype)
+    k, v, table = _one_pool(k, v, page)
+    q = torch.zeros(B * new, 2, hd, dtype=dtype, device="cuda")
+    q[:, 0, 0] = 62.5
+    q[:, 1, 1], q[:, 1, 2] = 60.0, 60.0  # 60 * 0.12 * log2 e = 10.4 per chunk
+    tables = table.expand(B, -1).contiguous()
+    if prefix:
+        kv = i32([L] * B)
+        got = paged.shared_prefix_attention(q, kv, tables, table, L, k, v, scale)
+        at = torch.full((B,), L - 1, device="cuda")
+    else:
+        kv = i32([L] * B)
+        got = paged.paged_attention(q, kv, tables, k, v, scale, cu_seqlens=i32([b * new for b in range(B + 1)]), max_q=new)
+        at = torch.arange(B * new, device="cuda") % new + L - new
+    want = (L / 2 / (at + 1).double())[:, None]
+    assert ((got[:, 0].double() - want).abs() <= torch.finfo(dtype).eps / 2 * want + (2 * 512 + 64) * 2.0 ** -24).all(), \
+        (got[:, 0].double() - want).abs().max()
+    assert (got[:, 1] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("power", [10, 25, 40])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("hd,new,prefix", [(128, 1, 0), (64, 1, 128), (128, 1, 256), (64, 40, 0), (128, 100, 0), (128, 100, 64)])
+def test_attention_of_scores_of_any_size(hd, new, prefix, sign, power, dtype):
+    """Scores of 50 sizes, 2^power times 0.12 or half of that apart: what has the largest has all the weight, in
+    equal parts, also where the scores' products with log2 e are rounded by whole powers of two."""
+    L, page = 1600, 64
+    g = torch.Generator().manual_seed(power + new)
+    order = torch.randperm(L, generator=g) % 50
+    steps = order + 1 if sign > 0 else order - 50
+    k, v = torch.zeros(L, 1, hd, dtype=dtype), torch.randn(L, 1, hd, generator=g).to(dtype)
+    k[:, 0, 0] = (steps * 2.0 ** (min(power, 25) - 15)).to(dtype)  # exact, below fp16's largest
+    scale = 0.12 * 2.0 ** (power - min(power, 25))
+    kk, vv, table = _one_pool(k, v, page)
+    q = torch.zeros(new, 2, hd, dtype=dtype)
+    q[:, 0, 0], q[:, 1, 0] = 2.0 ** 15, 2.0 ** 14
+    kw = dict(cu_seqlens=None if new == 1 else i32([0, new]))
+    if prefix:
+        got = paged.shared_prefix_attention(q.cuda(), i32([L]), table[None], table[:prefix // page].clone(), prefix, kk, vv, scale, **kw)
+    else:
+        got = paged.paged_attention(q.cuda(), i32([L]), table[None], kk, vv, scale, **kw)
+    half = torch.finfo(dtype).eps / 2
+    for i in range(new):
+        seen = steps[:L - new + i + 1]
+        best = v[:len(seen), 0][seen == seen.max()].double()
+        # equal weights (the others' are below e^-61): their fp32 sum, one rounding
+        bound = half * best.mean(0).abs() + (len(best) + 64) * 2.0 ** -23 * best.abs().mean(0) + 2.0 ** -25
+        assert_within(got[i], best.mean(0).expand(2, -1), bound.expand(2, -1), f"token {i}")
+
+
 # ---------------------------------------------------------------------------------- shared prefix
 @pytest.mark.parametrize("prefix", [0, 4096])
 @pytest.mark.parametrize("new", [1, 48])
