@@ -233,6 +233,25 @@ def test_attention_window(dtype, hd, nq, nkv, page, window, sinks):
     check_attention([10, 300, 97, 640], [10, 70, 97, 5], nq, nkv, hd, page, dtype, window, sinks)
 
 
+@pytest.mark.parametrize("window,sinks", [(1024, 0), (1024, 4), (1500, 40), (2000, 100)])
+@pytest.mark.parametrize("dtype,hd,nq,nkv,page", LAYOUTS[:3])
+def test_attention_window_over_ranges(dtype, hd, nq, nkv, page, window, sinks):
+    """Windows whose chunks, with those of the sinks a gap before them, are cut into several ranges that a
+    merge joins: one token per sequence, and a few; short sequences beside them."""
+    lens = [6000, 300, 3100, 1, 4500]
+    check_attention(lens, [1] * 5, nq, nkv, hd, page, dtype, window, sinks, cu=False)
+    check_attention(lens, [3, 2, 1, 1, 2], nq, nkv, hd, page, dtype, window, sinks)
+
+
+@pytest.mark.parametrize("window,sinks", [(2000, 40), (1300, 5)])
+def test_attention_window_over_ranges_of_many_sequences(window, sinks):
+    """The same where the ranges are found in a launch of their own."""
+    lens = [(37 * i) % 90 + 1 for i in range(100)]
+    lens[3], lens[50], lens[99] = 5000, 3300, 2500
+    check_attention(lens, [1] * 100, 4, 2, 128, 32, F16, window, sinks, cu=False)
+    check_attention(lens, [min(n, 1 + i % 3) for i, n in enumerate(lens)], 8, 2, 128, 32, BF16, window, sinks)
+
+
 @pytest.mark.parametrize("new", [200, 600])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (150, 3), (40, 100)])
 @pytest.mark.parametrize("dtype,hd,nq,nkv,page", [(F16, 128, 4, 2, 64), (BF16, 64, 3, 1, 32)])
