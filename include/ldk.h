@@ -405,9 +405,12 @@ int ldk_w8a16_matmul_swiglu(const void* x, int64_t ldx, const uint8_t* wq, const
  *  - cu_seqlens: int32 [B + 1], sequence b's new tokens are the rows cu_seqlens[b] ..
  *    cu_seqlens[b+1] - 1 of the T rows, in rising order; NULL: sequence b has row b (T >= B).
  *    kv_lens: int32 [B], the positions that sequence b's cache holds with its new tokens, which are
- *    the last of them: new token i of n is at position kv_lens[b] - n + i. A sequence without new
- *    tokens, kv_lens of 0 and rows behind the last sequence are allowed: those rows are left as they
- *    were. All of these are read on the device, so a captured graph takes new lengths and pages.
+ *    the last of them: new token i of n is at position kv_lens[b] - n + i. Sequences without new
+ *    tokens and rows behind the last sequence are allowed: those rows are left as they were. So is
+ *    kv_lens below the new tokens' number (0 of a padded sequence): its rows are at positions below
+ *    0, where ldk_paged_append turns their q by the negative position (or rope_pos) and writes no k
+ *    and v, and the attention gives zeros. All of these are read on the device, so a captured graph
+ *    takes new lengths and pages.
  *  - T at most 2^24 rows, B at most 2^20 sequences (65535 for the attention).
  *  - data pointers 16-byte aligned, row strides (elements) multiples of 8. */
 
