@@ -436,7 +436,6 @@ __global__ __launch_bounds__(NW * 64) void paged_split_kernel(PagedArgs a) {
 // index cu[b] gq / rows + b (n gq rows need at most one tile more than floor((cu + n) gq / rows) -
 // floor(cu gq / rows)); a workgroup finds its sequence with a binary search. MODE 1: the rows of all
 // tokens over the shared prefix.
-constexpr uint32_t kDead = 0x80000000u;  // buffer offset past every resource: the load returns 0
 constexpr float kLag = 8.0f;
 
 struct Block {
