@@ -32,10 +32,6 @@ import torch
 
 own = False
 
-PKG = Path(__file__).resolve().parent.parent / "llm-decode-kernels_amd"
-if str(PKG) not in sys.path:
-    sys.path.insert(0, str(PKG))
-
 THETA = 1_000_000.0
 INF = float("inf")
 DTYPES = {"fp16": torch.float16, "bf16": torch.bfloat16, "fp32": torch.float32}
@@ -255,6 +251,9 @@ def run(s: Bag):
 
 
 def _framework(s: Bag):
+    pkg = str(Path(__file__).resolve().parent.parent / "llm-decode-kernels_amd")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
     if s.kind == "logprobs":
         from kernels.sample import token_logprobs
 
