@@ -458,8 +458,10 @@ int ldk_paged_attention(const void* q, int64_t ldq, int dtype, const int32_t* cu
                         int64_t sinks, float scale, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ldk_paged_attention (window 0) for a batch whose sequences share their first prefix_len positions:
- * those are read through prefix_table (int32, prefix_len / page_size ids) once for the whole batch,
- * the rest through block_table, whose first prefix_len / page_size ids of each row are not read.
+ * those are read through prefix_table (int32, prefix_len / page_size ids), the rest through
+ * block_table, whose first prefix_len / page_size ids of each row are not read. The prefix is read
+ * once for the whole batch where max_q * nq / nkv <= 128; past that every sequence's rows read it for
+ * themselves, at the cost of ldk_paged_attention.
  * prefix_len a multiple of page_size, at most max_pages * page_size; kv_lens counts the prefix (a
  * sequence shorter than it sees its part). */
 int ldk_shared_prefix_attention(const void* q, int64_t ldq, int dtype, const int32_t* cu_seqlens,

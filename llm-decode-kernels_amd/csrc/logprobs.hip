@@ -24,8 +24,8 @@
 // joins with one wave per row.
 //
 // Bound by the vector instructions, close behind by memory: 1900 rows of 151936 bf16 (577 MB) with 20
-// alternatives 142-150 us, 3.9-4.1 TB/s, the vector unit busy 69%; without alternatives 109 us, 5.3 TB/s.
-// 77 rows of 50257 fp32 (15.5 MB, 20 alternatives) 22.8 us and one row of 151936 14.3: two launches, each a
+// alternatives 150 us, 3.8 TB/s, the vector unit busy 69%; without alternatives 113 us, 5.1 TB/s.
+// 77 rows of 50257 fp32 (15.5 MB, 20 alternatives) 23.6 us and one row of 151936 fp16 14.0: two launches, each a
 // load's latency, the ballots of the first floor, and the ranking of the keys. Per lane maxima and a
 // threshold per wave instead of the shared floors took 275 us on the first.
 #include <algorithm>

@@ -425,9 +425,9 @@ __global__ __launch_bounds__(NW * 64) void paged_split_kernel(PagedArgs a) {
 // needs no shuffles beyond the maximum over a tile's positions. Chunks that every row sees whole run
 // without masks. Page ids come through the scalar cache, one chunk ahead of their loads.
 //
-// Bound by what a SIMD can issue of matrix and softmax instructions between two barriers: 5 windowed
-// prompts of 32/8 heads (124 GFLOP) 173 us, 717 TFLOP/s, 59% of a large matrix product's rate, with the
-// vector unit busy 48% and the matrix unit 35% of a CU's cycles. On those prompts, in us: 1420 with
+// Bound by the order of a wave's own work, scores, softmax and P.V of a chunk one after the other between two
+// barriers: 5 windowed prompts of 32/8 heads (124 GFLOP) 169 us, 734 TFLOP/s, 61% of a large matrix product's
+// rate, with the vector unit busy 48% and the matrix unit 35% of a CU's cycles. On those prompts, in us: 1420 with
 // split_rows (16 rows read K and V from L2), 269 with two K groups of 128 rows that met at every
 // barrier, 203 as four waves per workgroup and two workgroups per CU, 178 with the numerators' sum on the
 // matrix unit and the lagging maximum, the rest from forming maxima only where a score passes the limit.
@@ -851,7 +851,7 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
 // Behind a shared prefix: its blocks, which the matrix cores bound, and the sequences' own positions, which
 // the memory does, in one launch, so that a CU runs some of each. Groups of 8 workgroups (one per XCD)
 // are of one kind, the kinds spread evenly over the launch. 128 sequences of up to 900 positions behind
-// 16384, 32/8 heads (205 MB, 35 GFLOP): 120 us in two launches, 104 in one, 96 now
+// 16384, 32/8 heads (205 MB, 35 GFLOP): 120 us in two launches, 104 in one, 95 now
 // with the merge.
 template <typename E, int HD, int BT>
 __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_eu(2))) void paged_prefix_kernel(PagedArgs a) {
@@ -874,7 +874,7 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
 //
 // Rows come from paged_split_kernel's slots, from paged_block_kernel's splits, or (behind a shared
 // prefix) from both; ones whose only range has written the output are left alone. A wave per row takes
-// 2 or 4 ranges at once, lane d of a range's dims 4d on (one range at once, 509 tokens of 14 heads of 64
+// 2 or 4 ranges at once, lane d of a range's dims 4d on (one range at once, 509 tokens of 14/2 heads of 64
 // in 13 ranges each: 77 us for attention and merge instead of 74; four heads of a token per wave: 128
 // sequences behind 16384 positions 107 us instead of 97). Where rows are few, WR = 8 waves per row take
 // ranges w, w + 8, ..., one at once, and meet in LDS (as above: 10.2 us instead of 10.0).
@@ -1030,7 +1030,9 @@ Plan make_plan(int64_t T, int64_t B, int64_t max_q, int64_t max_len, int64_t win
                int nq, int nkv, int hd) {
   Plan p;
   const int64_t gq = nq / nkv, rows = T * gq;
-  // a sequence's rows past two tiles share K and V in LDS; those that fill a block do so behind a prefix too
+  // a sequence's rows past two tiles share K and V in LDS; those that fill a block do so behind a prefix too, and
+  // with them every other sequence's of the call (127 tokens and a chunk of 64 behind 16384, 32/8 heads: 828 us; 128
+  // tokens 111)
   const bool block = max_q * gq > (prefix_len ? 128 : 2 * kRows);
   p.apart = prefix_len && !block;
   if (!block) {
@@ -1051,9 +1053,12 @@ Plan make_plan(int64_t T, int64_t B, int64_t max_q, int64_t max_len, int64_t win
   }
   if (block || p.apart) {
     // 128 rows where the sequences have about as many, else 64; split for two workgroups of 128 rows a CU (three
-    // of head_dim 64), or one of 64 (a 200-token chunk after 10000 positions, 28/4 heads, with 384 / 512 /
-    // 640 workgroups: 57 / 51 / 61 us), unless they are a third as many unsplit: the merge then costs more than
-    // fuller CUs save (2 prompts of 1500, 14/2 heads of 64, in one range / two: 34 / 68 us)
+    // of head_dim 64), or one of 64. With 384 / 512 / 640 workgroups of 128 rows, us: 200 tokens after 10000
+    // positions, 28/4 heads, 56 / 51 / 60, 300 after 6000, 32/8, 65 / 54 / 62; with 512 / 768 / 896 of head_dim 64: 509
+    // after 20000, 16/16, 75 / 71 / 84. With 192 / 320 / 448 of 64 rows: 4 times 10 after 5000, 32/8, 29 / 26 / 36, 50
+    // after 8000, 16/16 of 64, 18 / 17 / 24. With 2 kv heads, where 32 ranges are the limit, all alike. Not split
+    // where they are a third as many unsplit: the merge then costs more than fuller CUs save (2 prompts of
+    // 1500, 14/2 heads of 64, in one range / two: 34 / 68 us)
     auto tiles = [&](int bt) { return p.apart ? (rows + bt - 1) / bt : rows / bt + B; };
     p.bt = rows >= 96 * (p.apart ? 1 : B) ? 128 : 64;
     p.btiles = tiles(p.bt);

@@ -2,7 +2,7 @@
 tokens' q and k and writes k and v into the pages (`ldk_paged_append`), `paged_attention` attends over
 them, in full or over a sliding window with a few first positions that stay visible
 (`ldk_paged_attention`), and `shared_prefix_attention` does so for a batch whose sequences begin with
-the same pages, reading those once (`ldk_shared_prefix_attention`).
+the same pages, which it reads once for tokens that are few (`ldk_shared_prefix_attention`).
 
 They are the batch's counterparts of kernels.attention, whose `decode_attention` and
 `prefill_attention` serve one sequence over one static cache (the attention block of the reference's
@@ -141,8 +141,9 @@ def paged_append(qkv: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Te
     [hd/2], or None for no rotation; rope_pos int64 [tokens]: positions to turn q and k by instead of
     their cache positions. Writes the rotated k and v at their positions' pages and returns the
     rotated q [tokens, n_heads, hd], into `out` where given (which may be qkv's own q columns).
-    Angles are reduced in 64 bits, the rotation is fp32, rounded once. Two tokens of one call may not
-    share a position of a page."""
+    Angles are reduced in 64 bits, the rotation is fp32, rounded once. A token at a position without a page
+    (below 0, where kv_lens is below the new tokens' number, too) has its q turned and writes no k and v.
+    Two tokens of one call may not share a position of a page."""
     what = "paged_append"
     pages, nkv, page, hd, kst, vst = _pool(k_pages, vt_pages, what)
     width = (n_heads + 2 * nkv) * hd
@@ -242,9 +243,11 @@ def shared_prefix_attention(q: torch.Tensor, kv_lens: torch.Tensor, block_table:
                             vt_pages: torch.Tensor, scale: float, cu_seqlens: torch.Tensor | None = None,
                             max_q: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """paged_attention (no window) for a batch whose sequences share their first prefix_len positions,
-    whole pages: those are read through prefix_table (int32 [>= prefix_len / page]) once for all
-    sequences instead of once for each, the rest through block_table, whose entries before them are not
-    read. kv_lens counts the prefix; a sequence shorter than it sees its part of it."""
+    whole pages: those are read through prefix_table (int32 [>= prefix_len / page]), the rest through
+    block_table, whose entries before them are not read. The prefix is read once for all sequences where
+    max_q * n_heads / n_kv <= 128, else by each sequence's rows for themselves, as paged_attention does: a
+    batch of single tokens beside a prompt runs faster as two calls. kv_lens counts the prefix; a sequence
+    shorter than it sees its part of it."""
     if prefix_len <= 0:
         raise ValueError(f"shared_prefix_attention: prefix_len={prefix_len} must be positive (paged_attention "
                          "serves a batch without a prefix)")
