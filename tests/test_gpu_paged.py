@@ -511,6 +511,34 @@ def test_attention_of_nan(news, prefix, dtype, hd):
         assert_within(torch.where(bad, 0, mine), torch.where(bad, 0, ref), torch.where(bad, 1, bound))
 
 
+@pytest.mark.parametrize("dtype,hd", [(F16, 64), (BF16, 128)])
+@pytest.mark.parametrize("news", [[1, 1], [60, 200]])
+def test_attention_of_infinite_scores(news, dtype, hd):
+    """An infinity in a k makes the rows whose q gives it +inf NaN, as the formula's inf - inf is, and has no
+    weight in the rows that it gives -inf, the other positions' results unchanged."""
+    lens, nq, nkv, page = [700, 300], 6, 2, 32
+    pg = Pages(lens, nkv, hd, page, dtype)
+    q, cu = q_of(sum(news), nq, hd, dtype), rows_of(news)
+    k = k_from_tiles(pg.k_pages.cpu())
+    at = [333, 299]
+    for b, j in enumerate(at):
+        k[pg.table[b, j // page].item(), 1, j % page, 3] = float("inf")
+    got = paged.paged_attention(q.cuda(), i32(lens), pg.table, k_to_tiles(k).cuda(), pg.vt_pages, 0.125,
+                                cu_seqlens=None if max(news) == 1 else i32(cu), max_q=max(news)).cpu()
+    for b, n in enumerate(lens):
+        mine, rows = got[cu[b]:cu[b + 1]], q[cu[b]:cu[b + 1]]
+        where = [n - news[b] + i for i in range(news[b])]
+        hit = torch.zeros(rows.shape[:2], dtype=torch.bool)
+        hit[:, 3:] = torch.tensor([p >= at[b] for p in where])[:, None]
+        nan = hit & (rows[:, :, 3] > 0)
+        assert (mine.isnan() == nan[:, :, None]).all(), b
+        without = torch.ones(n, dtype=torch.bool)
+        without[at[b]] = False
+        for present, choose in ((None, ~hit), (without, hit & ~nan)):
+            ref, bound = attention64(rows, pg.k[b], pg.v[b], 0.125, where, present=present)
+            assert_within(mine[choose], ref[choose], bound[choose], f"sequence {b}")
+
+
 @pytest.mark.parametrize("dtype,hd,nq,nkv,page", LAYOUTS)
 @pytest.mark.parametrize("prefix_pages", [1, 7])
 @pytest.mark.parametrize("lens", [[1], [33, 1, 64, 5, 100], [700, 32, 31, 65, 7, 90] * 4])
