@@ -472,6 +472,51 @@ int ldk_shared_prefix_attention(const void* q, int64_t ldq, int dtype, const int
                                 int64_t ldo, int64_t T, int64_t B, int64_t max_q, int nq, int nkv, int head_dim,
                                 float scale, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------- paged cache in 4 bits */
+
+/* The paged cache with k and v in 4 bits; no counterpart in the reference. Tables, lengths, row bounds, limits and
+ * alignments as above; what is new:
+ *  - kv_pages holds k and v: num_pages pages, page i at element (16 bits) i * page_stride, >= nkv *
+ *    (page_size / 32) * words, a multiple of 8 and below 2^31; words = 16 head_dim + 128 head_dim / group, group 32, 64
+ *    or 128 (at most head_dim). A page holds [kv head][page_size/32] blocks of 32 positions, each a block of codes and of
+ *    steps and offsets of dtype (csrc/paged_int4.h has the bytes).
+ *  - Position by position, kv head by kv head and group by group, value = z + (code - 8) step, code 0..15. Of the
+ *    group's values x, which have dtype: step = rnd((max/2 - min/2) / 7.5), z = rnd((min/2 + max/2) + step/2), code =
+ *    clamp(rint((x - z) / step) + 8, 0, 15), in fp32, rnd to dtype; step 0: code 8. A group with a NaN or an
+ *    infinity gets step 0 and z NaN. */
+
+/* ldk_paged_append into 4-bit pages. q is rotated as there; k in 64 bits, angles included, then rounded to fp32, to
+ * dtype, and quantised; v is quantised as it comes. Two new tokens of one call may not share a slot. */
+int ldk_paged_append_int4(const void* qkv, int64_t ldqkv, int dtype, const int32_t* cu_seqlens,
+                          const int32_t* kv_lens, const int32_t* block_table, int64_t ldt, int64_t max_pages,
+                          const int64_t* rope_pos, const float* inv_freq, void* kv_pages, int64_t page_stride,
+                          int64_t num_pages, int64_t page_size, void* q_out, int64_t ldq, int64_t T, int64_t B,
+                          int nq, int nkv, int head_dim, int group, void* stream);
+
+/* The values back: rows cu_seqlens[b] .. cu_seqlens[b+1] - 1 of k_out (rows of ld_k elements, [nkv * head_dim]) and v_out
+ * get the last of sequence b's kv_lens[b] positions (cu_seqlens NULL: row b its last position), rounded once to dtype;
+ * zeros at positions below 0 or without a page. Rows behind the last sequence are left as they were. */
+int ldk_paged_read_int4(int dtype, const int32_t* cu_seqlens, const int32_t* kv_lens, const int32_t* block_table,
+                        int64_t ldt, int64_t max_pages, const void* kv_pages, int64_t page_stride,
+                        int64_t num_pages, int64_t page_size, void* k_out, int64_t ld_k, void* v_out, int64_t ld_v,
+                        int64_t T, int64_t B, int nkv, int head_dim, int group, void* stream);
+
+/* Bytes of workspace that ldk_paged_attention_int4 needs, as ldk_paged_attention_workspace_bytes. */
+int64_t ldk_paged_attention_int4_workspace_bytes(int64_t T, int64_t B, int64_t max_q, int64_t max_len,
+                                                 int64_t window, int64_t sinks, int nq, int nkv, int head_dim);
+
+/* ldk_paged_attention over the values that 4-bit pages hold: masks, max_q, workspace and limits as there. Scores,
+ * softmax and sums in fp32 from the codes as they are; the weights times v's steps are rounded to fp16 (with 11
+ * bits down to 2^-25 of the largest weight times the row's largest step, with fewer to 2^-35), one rounding at the
+ * end. An element of bf16 q below 2^-38 of its row's largest counts as 0; a row of q with an infinity or a NaN gives NaN.
+ * What a token does not see may hold anything. */
+int ldk_paged_attention_int4(const void* q, int64_t ldq, int dtype, const int32_t* cu_seqlens,
+                             const int32_t* kv_lens, const int32_t* block_table, int64_t ldt, int64_t max_pages,
+                             const void* kv_pages, int64_t page_stride, int64_t num_pages, int64_t page_size,
+                             void* out, int64_t ldo, int64_t T, int64_t B, int64_t max_q, int nq, int nkv,
+                             int head_dim, int group, int64_t window, int64_t sinks, float scale, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+
 /* -------------------------------------------------------------------------- log probabilities */
 
 /* Per row of logits [rows, V] (row stride ld, dtype LDK_F16/BF16/F32, any alignment of rows):

@@ -28,163 +28,12 @@
 // work. Each wave finds its slot's sequence from the lengths alone, or, of more than 64 sequences, in what
 // paged_plan_kernel found in a launch before. Sequences with more than one range leave {max, sum} and the
 // unnormalised output in the workspace, and paged_merge_kernel, the next launch on the stream, joins them.
-#include <algorithm>
-
 #include "lds_dma.h"
-#include "paged.h"
+#include "paged_attention.h"
 
 namespace {
 
 using namespace ldk;
-
-struct PagedArgs {
-  const void* q;
-  int64_t ldq;
-  const int32_t *cu, *kv_lens, *table, *ptable;  // ptable: the shared prefix's pages
-  int64_t ldt;
-  const void *k, *vt;
-  int64_t kps, vps;  // page strides, elements
-  void* out;
-  int64_t ldo;
-  float* part;    // paged_split_kernel's partials, per (slot, tile, kv head): [16 rows]{m, l} and [16 rows][hd]
-  float* bpart;   // paged_block_kernel's, per (tile, kv head, split): [rows]{m, l} and [rows][hd]
-  int32_t* plan;  // [B][2]: first slot and ranges of every sequence
-  int32_t* map;   // of many sequences: [0] chunks of a range, [1 + slot] its sequence; else null
-  int T, B, max_q, nq, nkv, gq, nt;  // nt: 16-row tiles of a sequence
-  int pages, cap;                    // cap: positions a sequence can hold
-  PageDiv cpp;                       // chunks per page
-  int pchunks, skip;                 // chunks of the shared prefix; of them, those that its own blocks take
-  int window, sinks, slots, spare;
-  int btiles, bsplits, bdirect;      // the block kernel's tiles and splits; a lone range writes the output
-  float scale;
-};
-
-typedef const __attribute__((address_space(4))) int32_t* ScalarInts;  // read through the scalar cache
-
-constexpr int kRows = 16;
-template <int N>
-struct IntC {
-  static constexpr int value = N;
-};
-// Of paged_block_kernel, by a block's rows: the waves that split its chunks between them, and LDS slots.
-template <int BT>
-constexpr int kBlockKG = BT == 128 ? 1 : 4;
-template <int BT>
-constexpr int kBlockSlots = BT == 128 ? 4 : 2;
-template <int BT>
-constexpr int kBlockThreads = BT / 32 * kBlockKG<BT> * 64;
-constexpr int kAll = 0x7fffffff;
-constexpr int kMinRange = 4;     // chunks of a range, at least
-constexpr int kMaxRanges = 128;  // ranges of a sequence
-
-// The visible chunks of a sequence's new tokens: cs chunks from 0 (the sinks), then those from lo on.
-struct Span {
-  SeqRows s;
-  int cs, lo, n;
-};
-__device__ __forceinline__ Span seq_span(const PagedArgs& a, int b) {
-  Span x;
-  x.s = seq_rows(a.cu, a.kv_lens, b, a.T);
-  x.s.n = min(x.s.n, a.max_q);
-  const int hi = min(x.s.pos0 + x.s.n - 1, a.cap - 1);  // the last position that a row sees
-  const int hc = hi < 0 || x.s.n <= 0 ? 0 : hi / kChunkPos + 1;
-  x.lo = a.window > 0 ? max(0, x.s.pos0 - a.window + 1) / kChunkPos : 0;
-  x.lo = min(x.lo, hc);
-  x.cs = min((min(a.sinks, a.cap) + kChunkPos - 1) / kChunkPos, x.lo);
-  if (a.skip) x.cs = 0, x.lo = min(a.skip, hc);  // the shared prefix is another kernel's
-  x.n = x.cs + hc - x.lo;
-  return x;
-}
-
-__device__ __forceinline__ int64_t wave_sum64(int64_t v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor((long long)v, off);
-  return v;
-}
-__device__ __forceinline__ int wave_max_i(int v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = max(v, __shfl_xor(v, off));
-  return v;
-}
-
-// The sequence and range of a slot: every wave forms it from the lengths of the whole batch. Every
-// sequence has at least one range (its rows have to be written), so sum over b of max(1, ceil(n_b / per))
-// <= B + total / per: with per = total / spare it fits B + spare slots. Where the launch is to be one round
-// of workgroups (spare 0), per is the least for which the sum fits the slots, found by bisection.
-struct Slot {
-  int b, split, ranges, first, per;  // b < 0: none
-};
-// Chunks of a range, of `sum` chunks in sequences of at most `most`.
-__device__ __forceinline__ int range_chunks(const PagedArgs& a, int64_t sum, int most) {
-  const int ways = a.spare ? a.spare : a.slots;
-  const int per = (int)min((sum + ways - 1) / ways, (int64_t)most);
-  return max(per, max(kMinRange, (most + kMaxRanges - 1) / kMaxRanges));
-}
-__device__ __forceinline__ Slot find_slot(const PagedArgs& a, int slot, int lane) {
-  if (!a.plan) return Slot{slot, 0, 1, slot, kAll};  // every sequence in one range
-  if (a.map) {                                       // paged_plan_kernel has found it
-    const int b = a.map[1 + slot];
-    if (b < 0) return Slot{-1, 0, 1, 0, 0};
-    const int first = a.plan[2 * b];
-    return Slot{b, slot - first, a.plan[2 * b + 1], first, a.map[0]};
-  }
-  const int each = (a.B + 63) / 64, b0 = lane * each, b1 = min(b0 + each, a.B);
-  int64_t sum = 0;
-  int most = 0, n0 = 0;
-  for (int b = b0; b < b1; ++b) {
-    const int n = seq_span(a, b).n;
-    sum += n;
-    most = max(most, n);
-    n0 = n;
-  }
-  sum = wave_sum64(sum);
-  most = wave_max_i(most);
-  int per = range_chunks(a, sum, most);
-  if (!a.spare && a.B > 1) {
-    int hi = max(per, (int)min((int64_t)most, (sum + a.slots - a.B - 1) / (a.slots - a.B)));
-    while (per < hi) {
-      const int mid = (per + hi) / 2;
-      float c = 0.0f;  // exact: below 2^24
-      if (each == 1) {
-        if (b0 < b1) c = (float)max(1, (n0 + mid - 1) / mid);
-      } else {
-        for (int b = b0; b < b1; ++b) c += (float)max(1, (seq_span(a, b).n + mid - 1) / mid);
-      }
-      if (__builtin_amdgcn_readfirstlane((int)sum_lanes_strided<1>(c)) <= a.slots)
-        hi = mid;
-      else
-        per = mid + 1;
-    }
-  }
-  Slot r{-1, 0, 1, 0, per};
-  int mine = 0;
-  for (int b = b0; b < b1; ++b) mine += max(1, (seq_span(a, b).n + r.per - 1) / r.per);
-  int end = mine;  // inclusive scan over the lanes
-#pragma unroll
-  for (int off = 1; off < 64; off *= 2) {
-    const int v = __shfl_up(end, off);
-    if (lane >= off) end += v;
-  }
-  int at = end - mine;
-  const uint64_t has = __ballot(slot >= at && slot < end);
-  if (!has) return r;
-  for (int b = b0; b < b1; ++b) {
-    const int n = max(1, (seq_span(a, b).n + r.per - 1) / r.per);
-    if (slot >= at && slot < at + n) {
-      r.b = b;
-      r.split = slot - at;
-      r.ranges = n;
-      r.first = at;
-    }
-    at += n;
-  }
-  const int src = __builtin_ctzll(has);
-  r.b = __builtin_amdgcn_readlane(r.b, src);
-  r.split = __builtin_amdgcn_readlane(r.split, src);
-  r.ranges = __builtin_amdgcn_readlane(r.ranges, src);
-  r.first = __builtin_amdgcn_readlane(r.first, src);
-  return r;
-}
 
 // find_slot for many sequences, once instead of by every wave: one workgroup. spare != 0.
 constexpr int kPlanThreads = 1024;
@@ -230,18 +79,6 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedArgs a) {
   }
   for (int i = base + tid; i < a.slots; i += kPlanThreads) a.map[1 + i] = -1;
 }
-
-__device__ __forceinline__ float max_xor16(float v) {
-  auto p = __builtin_amdgcn_permlane16_swap(f2u(v), f2u(v), false, false);
-  return fmaxf(u2f(p[0]), u2f(p[1]));
-}
-__device__ __forceinline__ float max_xor32(float v) {
-  auto p = __builtin_amdgcn_permlane32_swap(f2u(v), f2u(v), false, false);
-  return fmaxf(u2f(p[0]), u2f(p[1]));
-}
-
-// Floats of one partial: 16 rows of {m, l} and of hd outputs.
-constexpr int part_floats(int hd) { return kRows * (2 + hd); }
 
 // LDS bytes of split_rows: per wave the 16 rows' m, l and outputs.
 constexpr int split_lds(int hd, int nw) { return nw * kRows * (2 + hd) * 4; }
@@ -437,74 +274,6 @@ __global__ __launch_bounds__(NW * 64) void paged_split_kernel(PagedArgs a) {
 // floor(cu gq / rows)); a workgroup finds its sequence with a binary search. MODE 1: the rows of all
 // tokens over the shared prefix.
 constexpr float kLag = 8.0f;
-
-struct Block {
-  int b, row0, pos0;     // MODE 0: the sequence, its first row and position
-  int r0, rows;          // the block's first row (of the sequence's, or of the call's) and its number
-  int first, last;       // positions of the first and last row (MODE 0)
-  int cs, lo, n;         // visible chunks
-};
-// The block of sequence b's rows from r0 on. rows == 0: none.
-__device__ __forceinline__ Block sequence_block(const PagedArgs& a, int b, const SeqRows& s, int r0, int BT) {
-  Block k{};
-  k.b = b;
-  k.row0 = s.row0;
-  k.pos0 = s.pos0;
-  k.r0 = r0;
-  k.rows = r0 < 0 ? 0 : max(0, min(BT, min(s.n, a.max_q) * a.gq - r0));
-  if (k.rows <= 0) return k;
-  k.first = k.pos0 + k.r0 / a.gq;
-  k.last = k.pos0 + (k.r0 + k.rows - 1) / a.gq;
-  const int hi = min(k.last, a.cap - 1), hc = hi < 0 ? 0 : hi / kChunkPos + 1;
-  k.lo = min(a.window > 0 ? max(0, k.first - a.window + 1) / kChunkPos : 0, hc);
-  k.cs = min((min(a.sinks, a.cap) + kChunkPos - 1) / kChunkPos, k.lo);
-  k.n = k.cs + hc - k.lo;
-  return k;
-}
-// The block of tile x (uniform).
-template <int MODE>
-__device__ __forceinline__ Block find_block(const PagedArgs& a, int x, int BT) {
-  Block k{};
-  if constexpr (MODE == 1) {
-    k.r0 = x * BT;
-    k.rows = min(BT, a.T * a.gq - k.r0);
-    k.last = kAll;
-    k.n = a.pchunks;
-    return k;
-  }
-  int b = 0;
-  for (int lo = 0, hi = a.B; lo < hi;) {
-    const int mid = (lo + hi) / 2;
-    if ((int64_t)(a.cu ? max(a.cu[mid], 0) : mid) * a.gq / BT + mid <= x)
-      b = mid, lo = mid + 1;
-    else
-      hi = mid;
-  }
-  const SeqRows s = seq_rows(a.cu, a.kv_lens, b, a.T);
-  return sequence_block(a, b, s, (x - (int)(s.row0 * (int64_t)a.gq / BT) - b) * BT, BT);
-}
-// Chunks of a block's range, a multiple of kg.
-__device__ __forceinline__ int block_range(const PagedArgs& a, int n, int kg) {
-  const int per = (n + a.bsplits - 1) / a.bsplits;
-  return max(2 * kg, (per + kg - 1) / kg * kg);
-}
-// The position of row t of the call's (-1: no sequence's), by its sequence.
-__device__ __forceinline__ int row_position(const PagedArgs& a, int t) {
-  int b = t;
-  if (a.cu) {
-    b = -1;
-    for (int lo = 0, hi = a.B; lo < hi;) {  // the last b with cu[b] <= t
-      const int mid = (lo + hi) / 2;
-      if (a.cu[mid] <= t)
-        b = mid, lo = mid + 1;
-      else
-        hi = mid;
-    }
-    if (b < 0) return -1;
-  }
-  const SeqRows s = seq_rows(a.cu, a.kv_lens, b, a.T);
-  return t - s.row0 < min(s.n, a.max_q) ? s.pos0 + t - s.row0 : -1;
-}
 
 // LDS bytes of block_rows: the ring, and the K groups' m and l per column tile and lane.
 constexpr int block_lds(int hd, int cg, int kg, int s) { return kg * s * 2 * kChunkPos * hd * 2 + cg * kg * 4 * 64 * 4; }
@@ -1012,20 +781,6 @@ constexpr int kSingle = 20, kSingleMany = 36;
 // sequences 37 / 35, 256 72 / 60, 1024 437 / 244, 4096 4119 / 949; 100 to 4000 positions, 96 78 / 79, 512 404 / 370.
 constexpr int kPlanSeqs = 64;
 
-// What a call launches, from its sizes alone.
-struct Plan {
-  bool apart = false;                               // the shared prefix in blocks of its own
-  int64_t nt = 0, slots = 0, spare = 0;             // paged_split_kernel, slots == 0: not launched
-  int64_t bt = 0, btiles = 0, bsplits = 0;          // paged_block_kernel, bt == 0: not launched
-  bool mapped = false;                              // paged_plan_kernel
-  int64_t part_bytes = 0, bpart_bytes = 0, bytes = 0;
-};
-// Chunks that a token sees at most, from the positions a table holds and the window.
-int64_t most_chunks(int64_t max_len, int64_t max_q, int64_t window, int64_t sinks) {
-  const int64_t all = (max_len + kChunkPos - 1) / kChunkPos;
-  if (!window) return all;
-  return std::min(all, (window + max_q + kChunkPos - 2) / kChunkPos + 1 + (sinks + kChunkPos - 1) / kChunkPos);
-}
 Plan make_plan(int64_t T, int64_t B, int64_t max_q, int64_t max_len, int64_t window, int64_t sinks, int64_t prefix_len,
                int nq, int nkv, int hd) {
   Plan p;
@@ -1067,13 +822,8 @@ Plan make_plan(int64_t T, int64_t B, int64_t max_q, int64_t max_len, int64_t win
     p.bsplits = !p.apart && 3 * whole >= fill ? 1 : std::max<int64_t>(1, std::min<int64_t>(32, fill / whole));
     if (p.apart || p.bsplits > 1) p.bpart_bytes = p.btiles * nkv * p.bsplits * p.bt * (2 + hd) * 4;
   }
-  p.bytes = p.part_bytes + p.bpart_bytes + (p.part_bytes ? B * 8 : 0) + (p.mapped ? (p.slots + 1) * 4 : 0);
+  p.bytes = workspace_bytes(p, B);
   return p;
-}
-// A launch holds fewer than 2^32 threads.
-bool launchable(const Plan& p, int64_t T, int nq, int nkv) {
-  const int64_t most = (int64_t(1) << 32) / 512 - 8;
-  return p.slots * nkv * p.nt + p.btiles * nkv * std::max<int64_t>(1, p.bsplits) < most && T * nq < most * 8;
 }
 
 template <typename E, int HD, int BT>
@@ -1088,25 +838,26 @@ int launch_rows(const PagedArgs& a, const Plan& p, hipStream_t s) {
 }
 
 template <typename E, int HD>
-int launch(const PagedArgs& a, const Plan& p, hipStream_t s) {
+int launch(const PagedArgs& a, const Plan& p, int dtype, hipStream_t s) {
   (void)hipGetLastError();
   int st;
-  if (p.mapped) {
-    paged_plan_kernel<<<1, kPlanThreads, 0, s>>>(a);
-    if ((st = ldk::check_launch("paged_attention plan"))) return st;
-  }
+  if (p.mapped && (st = paged_find_ranges(a, s))) return st;
   if (p.bt) {
     st = p.bt == 128 ? launch_rows<E, HD, 128>(a, p, s) : launch_rows<E, HD, 64>(a, p, s);
   } else {
     paged_split_kernel<E, HD, 8><<<(unsigned)(p.slots * a.nkv * p.nt), 8 * 64, 0, s>>>(a);
     st = ldk::check_launch("paged_attention split");
   }
-  if (st) return st;
-  if (!p.bytes) return LDK_OK;  // no sequence has more than one range
+  if (st || !p.bytes) return st;  // no bytes: no sequence has more than one range
+  return paged_join(a, dtype, HD, p.bt, s);
+}
+
+template <typename E, int HD>
+int join(const PagedArgs& a, int64_t bt, hipStream_t s) {
   const bool few = (int64_t)a.T * a.nq < 512;
   const int64_t waves = (int64_t)a.T * a.nq * (few ? kMergeWaves : 1);
   const unsigned grid = (unsigned)((waves + kMergeWaves - 1) / kMergeWaves);
-  if (p.bt == 128)
+  if (bt == 128)
     few ? paged_merge_kernel<E, HD, kMergeWaves, 128><<<grid, kMergeWaves * 64, 0, s>>>(a)
         : paged_merge_kernel<E, HD, 1, 128><<<grid, kMergeWaves * 64, 0, s>>>(a);
   else
@@ -1156,10 +907,7 @@ int run(const char* fn, const void* q, int64_t ldq, int dtype, const int32_t* cu
   a.q = q, a.ldq = ldq, a.out = out, a.ldo = ldo;
   a.cu = cu, a.kv_lens = kv_lens, a.table = table, a.ptable = ptable, a.ldt = ldt;
   a.k = k, a.vt = vt, a.kps = kps, a.vps = vps;
-  a.part = (float*)ws;
-  a.bpart = (float*)((char*)ws + p.part_bytes);
-  a.plan = p.part_bytes ? (int32_t*)((char*)ws + p.part_bytes + p.bpart_bytes) : nullptr;
-  a.map = p.mapped ? a.plan + 2 * B : nullptr;
+  lay_out(a, p, ws, B);
   a.T = cu ? (int)T : (int)B, a.B = (int)B, a.max_q = cu ? (int)max_q : 1;
   a.nq = nq, a.nkv = nkv, a.gq = nq / nkv, a.nt = (int)p.nt;
   a.pages = (int)num_pages, a.cpp = page_div(page_size / kChunkPos), a.cap = (int)(max_pages * page_size);
@@ -1169,11 +917,25 @@ int run(const char* fn, const void* q, int64_t ldq, int dtype, const int32_t* cu
   a.btiles = (int)p.btiles, a.bsplits = (int)p.bsplits, a.bdirect = !p.apart;
   a.scale = scale;
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == LDK_F16) return hd == 128 ? launch<ldk::F16, 128>(a, p, s) : launch<ldk::F16, 64>(a, p, s);
-  return hd == 128 ? launch<ldk::BF16, 128>(a, p, s) : launch<ldk::BF16, 64>(a, p, s);
+  if (dtype == LDK_F16) return hd == 128 ? launch<ldk::F16, 128>(a, p, dtype, s) : launch<ldk::F16, 64>(a, p, dtype, s);
+  return hd == 128 ? launch<ldk::BF16, 128>(a, p, dtype, s) : launch<ldk::BF16, 64>(a, p, dtype, s);
 }
 
 }  // namespace
+
+namespace ldk {
+
+int paged_find_ranges(const PagedArgs& a, hipStream_t s) {
+  paged_plan_kernel<<<1, kPlanThreads, 0, s>>>(a);
+  return check_launch("paged_attention plan");
+}
+
+int paged_join(const PagedArgs& a, int dtype, int hd, int64_t bt, hipStream_t s) {
+  if (dtype == LDK_F16) return hd == 128 ? join<F16, 128>(a, bt, s) : join<F16, 64>(a, bt, s);
+  return hd == 128 ? join<BF16, 128>(a, bt, s) : join<BF16, 64>(a, bt, s);
+}
+
+}  // namespace ldk
 
 extern "C" int64_t ldk_paged_attention_workspace_bytes(int64_t T, int64_t B, int64_t max_q, int64_t max_len, int64_t window,
                                                        int64_t sinks, int64_t prefix_len, int nq, int nkv, int head_dim) {

@@ -1,0 +1,413 @@
+// Grouped-query attention of new tokens over a paged cache held in 4 bits (paged_int4.h), causal, in full or over a
+// sliding window whose first positions stay visible. Ranges, tiles of 16 rows and the join are
+// paged_attention.hip's (paged_attention.h).
+//
+// With k = z + (c - 8) step and v likewise, per group g of dims:
+//   q.k_j = sum_g step_jg sum_d q_d (c_jd - 8) + z_jg U_g,   U_g = sum of q_d over the group,
+//   out_d = [sum_j (w_j step_jg) (c_jd - 8) + sum_j w_j z_jg] / sum_j w_j,   w_j = exp(scale q.k_j - max).
+// The matrix cores take c - 8, a whole number that fp16 holds exactly; what depends on the position, its step and
+// offset, is applied outside in fp32, one fused multiply per score and group. So nothing of K is rounded, and of V
+// only the weight w_j step_jg, to fp16, for bf16 too: its 11 bits are the closer, and the units below keep its range.
+//
+// Units. A row of bf16 q is scaled by the power of two that brings its largest element below 2^14: fp16 keeps its bits down
+// to 2^-30 of the largest, and elements below 2^-38 are lost. Weights are held times 2^11 over a power of two that
+// follows the row's largest step so far (kept like the maximum): fp16 keeps weights down to 2^-35 of it, whatever the
+// size of V is.
+#include "paged_attention.h"
+#include "paged_int4.h"
+
+namespace {
+
+using namespace ldk;
+
+// A power of two from its exponent, -126 .. 127.
+__device__ __forceinline__ float pow2i(int e) { return u2f((uint32_t)(e + 127) << 23); }
+
+// 8 params of the type as fp32.
+template <typename E>
+__device__ __forceinline__ void params8(const u32x4& v, float* f) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2_t a = unpack2<E>(v[i]);
+    f[2 * i] = a[0], f[2 * i + 1] = a[1];
+  }
+}
+// Two words of codes less 8 as fp16, the low four bits' (the even step's or block's) and the high four bits' operands.
+// 1024 + c and 1024 + 16 c have the code in fp16's last bits.
+struct Codes {
+  u32x4 low, high;
+};
+__device__ __forceinline__ Codes codes_less8(uint32_t a, uint32_t b) {
+  const half2_t less = {(half_t)-1032.0f, (half_t)-1032.0f}, by = {(half_t)0.0625f, (half_t)0.0625f}, less72 = {(half_t)-72.0f, (half_t)-72.0f};
+  const uint32_t w[4] = {a, a >> 8, b, b >> 8};
+  Codes r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    r.low[i] = h22u(u2h2((w[i] & kLow4) | 0x64006400u) + less);
+    r.high[i] = h22u(__builtin_elementwise_fma(u2h2((w[i] & kHigh4) | 0x64006400u), by, less72));
+  }
+  return r;
+}
+
+constexpr float kLag4 = 3.0f;  // powers of two that a row's maximum may lag
+constexpr int kUnit4 = 11;     // weights times 2^kUnit4: 2^(kLag4 + kUnit4 + 1) is inside fp16
+
+constexpr int kPad = 4;  // floats after a row of outputs in LDS: 16 rows' float4 in different banks
+constexpr int split4_lds(int hd, int nw) { return nw * kRows * (2 + hd + kPad) * 4; }
+
+// A workgroup takes 16 rows of one kv head (paged_attention.hip) over a range of chunks, chunk w, w + NW, ... by wave w.
+// Both products have the row as the matrix cores' column, so that a lane's scores, weights, sums and outputs are
+// one row's.
+template <typename E, int HD, int NG, int NW>
+__global__ __launch_bounds__(NW * 64) void paged_split4_kernel(PagedArgs a) {
+  typedef typename E::T T;
+  typedef Int4Block<HD, NG> L;
+  constexpr int NS = HD / 32, NB = HD / 16, NP = HD / 64;  // K dim steps, V dim blocks, pairs of steps
+  constexpr int NL = HD / 64;                              // 16-byte loads per lane of K's codes, and of V's
+  __shared__ __align__(16) unsigned char lds[split4_lds(HD, NW)];
+  float(*const mw)[kRows] = reinterpret_cast<float(*)[kRows]>(lds);
+  float(*const lw)[kRows] = mw + NW;
+  float(*const ow)[kRows][HD + kPad] = reinterpret_cast<float(*)[kRows][HD + kPad]>(lds + NW * kRows * 8);
+  const int tid = threadIdx.x, lane = tid & 63, wg = (int)blockIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c16 = lane & 15, kb = lane >> 4;
+  const int xy = a.nkv * a.nt, bxy = wg % xy;
+  const int kvh = bxy % a.nkv, tile = bxy / a.nkv;
+  const Slot sl = find_slot(a, wg / xy, lane);
+  if (sl.b < 0) return;
+  const Span sp = seq_span(a, sl.b);
+  if (a.plan && !a.map && kvh == 0 && tile == 0 && sl.split == 0 && tid == 0) {
+    a.plan[2 * sl.b] = sl.first;
+    a.plan[2 * sl.b + 1] = sl.ranges;
+  }
+  const int rows = min(kRows, sp.s.n * a.gq - tile * kRows);  // this tile's
+  if (rows <= 0) return;
+  // this lane's row and the positions that it sees: lo..hi and below sinks
+  const int row = tile * kRows + c16, tok = row / a.gq;
+  const int p = sp.s.pos0 + tok;
+  const int hi = c16 < rows ? min(p, a.cap - 1) : -1;
+  const int lo = a.window > 0 ? max(0, p - a.window + 1) : 0;
+  // of the tile's rows: the last position and the first that one of them sees past the sinks, and that all see
+  const int pt0 = sp.s.pos0 + tile * kRows / a.gq, pt1 = sp.s.pos0 + (tile * kRows + rows - 1) / a.gq;
+  const int thi = min(pt1, a.cap - 1), tlo = a.window > 0 ? max(0, pt0 - a.window + 1) : 0;
+  const int alo = a.window > 0 ? max(0, pt1 - a.window + 1) : 0;
+
+  // ---- row c16's q at dims 8kb + 32s .. + 7, as the B operands: 2^qs q in fp16
+  const T* qrow = (const T*)a.q + (int64_t)(sp.s.row0 + tok) * a.ldq + (int64_t)(kvh * a.gq + row % a.gq) * HD;
+  u32x4 qb[NS];
+  float us[NG];  // U_g in the same units
+  int qs = 0;
+#pragma unroll
+  for (int s = 0; s < NS; ++s)
+    qb[s] = c16 < rows ? *reinterpret_cast<const u32x4*>(qrow + 32 * s + 8 * kb) : u32x4{0, 0, 0, 0};
+  if constexpr (E::kOnes == BF16::kOnes) {
+    float amax = 0.0f;
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2_t f = unpack2<E>(qb[s][i]);
+        amax = fmaxf(amax, fmaxf(__builtin_fabsf(f[0]), __builtin_fabsf(f[1])));
+      }
+    amax = max_xor32(max_xor16(amax));
+    qs = 13 - max(-100, min(127, (int)(f2u(amax) >> 23) - 127));  // amax < 2^(14 - qs)
+    const float by = pow2i(qs);
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2_t f = unpack2<E>(qb[s][i]);
+        qb[s][i] = pack2<F16>(f[0] * by, f[1] * by);
+      }
+  }
+#pragma unroll
+  for (int g = 0; g < NG; ++g) us[g] = 0.0f;
+#pragma unroll
+  for (int s = 0; s < NS; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2_t h = unpack2<F16>(qb[s][i]);
+      us[s * NG / NS] += h[0] + h[1];
+    }
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    us[g] = add_xor32(add_xor16(us[g]));
+    if (!(__builtin_fabsf(us[g]) < __builtin_inff())) us[g] = __builtin_nanf("");  // a row with an infinity: no score
+  }
+  // scores are formed as 2^qs q.k; their exponents' factor, finite and, as -inf 0 is NaN, not 0
+  const float f1 = fmaxf(0x1p-126f, fminf(a.scale * 1.44269504088896341f * pow2i(-qs), 0x1p126f));
+
+  // The maximum that is subtracted may lag the largest score by kLag4; it and the unit of the weights move where a lane
+  // finds more, and with them what is summed so far. Scores start from -m (0 while m is -inf), so that differences
+  // are formed before they are scaled: what m f1 rounds away would rescale a row at every chunk.
+  float m_run = -__builtin_inff(), less = 0.0f, limit = -__builtin_inff(), l = 0.0f;
+  int ve = -100;                 // 2^ve: the row's largest step's power of two
+  float ms[NG];                  // sum of w z
+  float4_t o[NB];                // O^T[dim 16b + 4kb + r][row c16]; l, ms and o in units of 2^(kUnit4 - ve)
+#pragma unroll
+  for (int g = 0; g < NG; ++g) ms[g] = 0.0f;
+#pragma unroll
+  for (int b = 0; b < NB; ++b) o[b] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  const ScalarInts trow = (ScalarInts)(uintptr_t)(a.table + (int64_t)sl.b * a.ldt);
+  const int jend = (int)min((sl.split + (int64_t)1) * sl.per, (int64_t)sp.n);
+  for (int j = sl.split * sl.per + wave; j < jend; j += NW) {
+    const int c = j < sp.cs ? j : j - sp.cs + sp.lo;
+    const int cb = c * kChunkPos;
+    if (cb > thi || (cb + kChunkPos <= tlo && cb >= a.sinks)) continue;
+    int at, sub;
+    chunk_page(a.cpp, c, at, sub);
+    const int page = trow[at];
+    if (page < 0 || page >= a.pages) continue;
+    const auto rs = buffer_rsrc((const T*)a.k + page * a.kps + ((int64_t)kvh * a.cpp.n + sub) * L::kWords, L::kBytes);
+    u32x4 kc[NL], vc[NL], kp[NG][2], vp[NG][2];
+#pragma unroll
+    for (int t = 0; t < NL; ++t) kc[t] = buffer_load16(rs, (uint32_t)(t * 1024 + lane * 16));
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) kp[g][i] = buffer_load16(rs, (uint32_t)(L::kParams + g * 128 + kb * 32 + i * 16));
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) vp[g][i] = buffer_load16(rs, (uint32_t)(L::kVParams + g * 128 + kb * 32 + i * 16));
+#pragma unroll
+    for (int t = 0; t < NL; ++t) vc[t] = buffer_load16(rs, (uint32_t)(L::kV + t * 1024 + lane * 16));
+
+    // ---- scores of positions 8kb + e, less the row's maximum so far
+    float sv[8];
+    {
+      float4_t acc[2][NG];
+#pragma unroll
+      for (int n = 0; n < NP; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const Codes c = HD == 128 ? codes_less8(kc[h % NL][2 * n], kc[h % NL][2 * n + 1]) : codes_less8(kc[0][2 * h], kc[0][2 * h + 1]);
+#pragma unroll
+          for (int odd = 0; odd < 2; ++odd) {
+            const int s = 2 * n + odd, g = s * NG / NS;
+            const float4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
+            acc[h][g] = F16::mfma(odd ? c.high : c.low, qb[s], s % (NS / NG) ? acc[h][g] : zero);
+          }
+        }
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        float st[8], z[8];
+        params8<E>(kp[g][0], st);
+        params8<E>(kp[g][1], z);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sv[e] = __builtin_fmaf(st[e], acc[e >> 2][g][e & 3], __builtin_fmaf(z[e], us[g], g ? sv[e] : less));
+      }
+    }
+    float vst[NG][8], vz[NG][8];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      params8<E>(vp[g][0], vst[g]);
+      params8<E>(vp[g][1], vz[g]);
+    }
+    // a chunk that not every row sees whole: what a row does not see has no score, and steps and offsets of 0 (they may
+    // be anything, and 0 x NaN is NaN)
+    if (cb + kChunkPos - 1 > pt0 || (cb < alo && cb + kChunkPos > a.sinks)) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int pj = cb + 8 * kb + e;
+        const bool seen = pj <= hi && (pj >= lo || pj < a.sinks);
+        sv[e] = seen ? sv[e] : -__builtin_inff();
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          vst[g][e] = seen ? vst[g][e] : 0.0f;
+          vz[g][e] = seen ? vz[g][e] : 0.0f;
+        }
+      }
+    }
+    float mc = sv[0], sm = vst[0][0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) mc = fmaxf(mc, sv[e]);
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sm = fmaxf(sm, vst[g][e]);
+    if (__any(mc > limit || sm >= pow2i(ve + 1))) {
+      mc = max_xor32(max_xor16(mc));
+      sm = max_xor32(max_xor16(sm));
+      const float old = less, m_new = fmaxf(m_run, mc - old);
+      const float now = m_new == -__builtin_inff() ? 0.0f : -m_new, more = old - now;
+      const int vn = min(126, max(ve, (int)(f2u(sm) >> 23) - 127));
+      const float al = (m_run == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(-more * f1)) * pow2i(max(ve - vn, -126));
+      l *= al;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) ms[g] *= al;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) o[b] *= al;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sv[e] -= more;
+      m_run = m_new;
+      less = now;
+      limit = m_new == -__builtin_inff() ? m_new : kLag4 / f1;
+      ve = vn;
+    }
+    const float unit = (float)(kUnit4 - ve);
+    float w[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[e], f1, unit));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) l += w[e];
+    u32x4 pw[NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ms[g] = __builtin_fmaf(w[e], vz[g][e], ms[g]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) pw[g][e] = pack2<F16>(w[2 * e] * vst[g][2 * e], w[2 * e + 1] * vst[g][2 * e + 1]);
+    }
+#pragma unroll
+    for (int t = 0; t < NB / 2; ++t) {  // pairs of blocks
+      const Codes c = codes_less8(vc[t / 2][2 * (t % 2)], vc[t / 2][2 * (t % 2) + 1]);
+      o[2 * t] = F16::mfma(c.low, pw[2 * t * NG / NB], o[2 * t]);
+      o[2 * t + 1] = F16::mfma(c.high, pw[2 * t * NG / NB], o[2 * t + 1]);
+    }
+  }
+
+  // ---- the waves meet, maxima in q.k's own units
+  l = add_xor32(add_xor16(l));
+#pragma unroll
+  for (int g = 0; g < NG; ++g) ms[g] = add_xor32(add_xor16(ms[g]));
+  const float one = pow2i(ve - kUnit4);
+  if (kb == 0) {
+    mw[wave][c16] = m_run * pow2i(-qs);
+    lw[wave][c16] = l * one;
+  }
+  if (c16 < rows) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      float4_t v;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = (o[b][r] + ms[b * NG / NB]) * one;
+      *reinterpret_cast<float4_t*>(&ow[wave][c16][16 * b + 4 * kb]) = v;
+    }
+  }
+  lds_barrier();
+  const float sc = a.scale * 1.44269504088896341f;
+  float* part = a.part + (int64_t)wg * part_floats(HD);
+  for (int e = tid; e < rows * HD; e += NW * 64) {
+    const int j = e / HD, d = e % HD;
+    float mv[NW], lv[NW], ov[NW], M = -__builtin_inff();
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      mv[w] = mw[w][j];
+      lv[w] = lw[w][j];
+      ov[w] = ow[w][j][d];
+    }
+#pragma unroll
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, mv[w]);
+    float ls = 0.0f, v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float f = mv[w] != -__builtin_inff() ? __builtin_amdgcn_exp2f((mv[w] - M) * sc) : 0.0f;
+      ls = __builtin_fmaf(lv[w], f, ls);
+      v = __builtin_fmaf(ov[w], f, v);
+    }
+    if (sl.ranges == 1) {
+      const int g = tile * kRows + j;
+      T* dst = (T*)a.out + (int64_t)(sp.s.row0 + g / a.gq) * a.ldo + (int64_t)(kvh * a.gq + g % a.gq) * HD;
+      dst[d] = (T)(ls != 0.0f ? v / ls : 0.0f);
+    } else {
+      part[2 * kRows + e] = v;
+      if (d == 0) {
+        part[2 * j] = M;
+        part[2 * j + 1] = ls;
+      }
+    }
+  }
+}
+
+constexpr int kWaves = 8;       // of a workgroup
+constexpr int kSingle4 = 20;    // chunks up to which a sequence is one range
+constexpr int kPlanSeqs4 = 64;  // more sequences have their ranges found in a launch before
+
+Plan make_plan4(int64_t T, int64_t B, int64_t max_q, int64_t max_len, int64_t window, int64_t sinks, int nq, int nkv, int hd) {
+  Plan p;
+  (void)T;
+  p.nt = (max_q * (nq / nkv) + kRows - 1) / kRows;
+  if (most_chunks(max_len, max_q, window, sinks) <= kSingle4) {
+    p.slots = B;
+    return p;
+  }
+  const int64_t w = nkv * p.nt, round = (hd == 128 ? 256 : 512) / w;
+  p.spare = 2 * round >= 3 * B ? 0 : std::max<int64_t>(1, 384 / w);
+  p.slots = p.spare ? B + p.spare : round;
+  p.mapped = p.spare && B > kPlanSeqs4;
+  p.part_bytes = p.slots * w * part_floats(hd) * 4;
+  p.bytes = workspace_bytes(p, B);
+  return p;
+}
+
+template <typename E, int HD, int NG>
+int launch(const PagedArgs& a, const Plan& p, int dtype, hipStream_t s) {
+  (void)hipGetLastError();
+  int st;
+  if (p.mapped && (st = ldk::paged_find_ranges(a, s))) return st;
+  paged_split4_kernel<E, HD, NG, kWaves><<<(unsigned)(p.slots * a.nkv * p.nt), kWaves * 64, 0, s>>>(a);
+  if ((st = ldk::check_launch("paged_attention_int4")) || !p.bytes) return st;
+  return ldk::paged_join(a, dtype, HD, p.bt, s);
+}
+template <typename E>
+int launch(const PagedArgs& a, const Plan& p, int dtype, int hd, int group, hipStream_t s) {
+  if (hd == 64) return group == 32 ? launch<E, 64, 2>(a, p, dtype, s) : launch<E, 64, 1>(a, p, dtype, s);
+  return group == 32 ? launch<E, 128, 4>(a, p, dtype, s) : group == 64 ? launch<E, 128, 2>(a, p, dtype, s) : launch<E, 128, 1>(a, p, dtype, s);
+}
+
+}  // namespace
+
+extern "C" int64_t ldk_paged_attention_int4_workspace_bytes(int64_t T, int64_t B, int64_t max_q, int64_t max_len, int64_t window,
+                                                            int64_t sinks, int nq, int nkv, int head_dim) {
+  if (T <= 0 || T > (int64_t(1) << 24) || B <= 0 || B > 65535 || max_q <= 0 || max_q > (int64_t(1) << 24) || max_len <= 0 ||
+      max_len > ldk::kMaxPositions || window < 0 || sinks < 0 || nq <= 0 || nkv <= 0 || nq % nkv || nq > 4096 ||
+      (head_dim != 64 && head_dim != 128)) {
+    return -ldk::fail(LDK_ERR_INVALID,
+                      "paged_attention_int4_workspace_bytes: T=%lld B=%lld max_q=%lld max_len=%lld window=%lld sinks=%lld nq=%d "
+                      "nkv=%d head_dim=%d",
+                      (long long)T, (long long)B, (long long)max_q, (long long)max_len, (long long)window, (long long)sinks, nq,
+                      nkv, head_dim);
+  }
+  return make_plan4(T, B, max_q, max_len, window, sinks, nq, nkv, head_dim).bytes;
+}
+
+extern "C" int ldk_paged_attention_int4(const void* q, int64_t ldq, int dtype, const int32_t* cu_seqlens, const int32_t* kv_lens,
+                                        const int32_t* block_table, int64_t ldt, int64_t max_pages, const void* kv_pages,
+                                        int64_t page_stride, int64_t num_pages, int64_t page_size, void* out, int64_t ldo,
+                                        int64_t T, int64_t B, int64_t max_q, int nq, int nkv, int head_dim, int group,
+                                        int64_t window, int64_t sinks, float scale, void* workspace, int64_t workspace_bytes,
+                                        void* stream) {
+  static const char* fn = "paged_attention_int4";
+  if (!q || !kv_lens || !block_table || !kv_pages || !out) return ldk::fail(LDK_ERR_INVALID, "%s: null pointer", fn);
+  int st = ldk::check_int4_pool(fn, dtype, nkv, head_dim, group, page_stride, num_pages, page_size, ldt, max_pages);
+  if (st || (st = ldk::check_int4_batch(fn, T, B, 65535, cu_seqlens))) return st;
+  if (nq <= 0 || nq % nkv || nq > 4096)
+    return ldk::fail(LDK_ERR_INVALID, "%s: nq=%d must be a positive multiple of nkv=%d (at most 4096)", fn, nq, nkv);
+  if (max_q <= 0 || max_q > T) return ldk::fail(LDK_ERR_INVALID, "%s: max_q=%lld outside 1..%lld", fn, (long long)max_q, (long long)T);
+  if (window < 0 || sinks < 0) return ldk::fail(LDK_ERR_INVALID, "%s: window=%lld sinks=%lld", fn, (long long)window, (long long)sinks);
+  if (!(scale > 1e-20f && scale < 1e20f)) return ldk::fail(LDK_ERR_INVALID, "%s: scale=%g must be positive", fn, (double)scale);
+  if (ldq < (int64_t)nq * head_dim || ldo < (int64_t)nq * head_dim)
+    return ldk::fail(LDK_ERR_INVALID, "%s: strides ldq=%lld ldo=%lld below what they step over", fn, (long long)ldq, (long long)ldo);
+  if (!ldk::aligned(q, 16) || !ldk::aligned(out, 16) || !ldk::aligned(kv_pages, 16) || ldq % 8 || ldo % 8 || page_stride % 8 ||
+      !ldk::aligned(kv_lens, 4) || !ldk::aligned(cu_seqlens, 4) || !ldk::aligned(block_table, 4) || !ldk::aligned(workspace, 16))
+    return ldk::fail(LDK_ERR_ALIGN, "%s: q, out, workspace and the pages 16-byte aligned with strides of multiples of 8 elements", fn);
+  const Plan p = make_plan4(cu_seqlens ? T : B, B, cu_seqlens ? max_q : 1, max_pages * page_size, window, sinks, nq, nkv, head_dim);
+  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes))
+    return ldk::fail(LDK_ERR_INVALID, "%s: workspace of %lld bytes, this call needs %lld", fn, (long long)workspace_bytes, (long long)p.bytes);
+  if (!launchable(p, T, nq, nkv)) return ldk::fail(LDK_ERR_UNSUPPORTED, "%s: T=%lld rows of nq=%d heads are too many for a launch", fn, (long long)T, nq);
+  const int big = 1 << 30;  // a window or sinks past every position
+  PagedArgs a{};
+  a.q = q, a.ldq = ldq, a.out = out, a.ldo = ldo;
+  a.cu = cu_seqlens, a.kv_lens = kv_lens, a.table = block_table, a.ldt = ldt;
+  a.k = kv_pages, a.kps = page_stride;
+  lay_out(a, p, workspace, B);
+  a.T = cu_seqlens ? (int)T : (int)B, a.B = (int)B, a.max_q = cu_seqlens ? (int)max_q : 1;
+  a.nq = nq, a.nkv = nkv, a.gq = nq / nkv, a.nt = (int)p.nt;
+  a.pages = (int)num_pages, a.cpp = page_div(page_size / kChunkPos), a.cap = (int)(max_pages * page_size);
+  a.window = (int)std::min<int64_t>(window, big), a.sinks = (int)std::min<int64_t>(sinks, big);
+  a.slots = (int)p.slots, a.spare = (int)p.spare;
+  a.scale = scale;
+  hipStream_t s = (hipStream_t)stream;
+  return dtype == LDK_F16 ? launch<ldk::F16>(a, p, dtype, head_dim, group, s) : launch<ldk::BF16>(a, p, dtype, head_dim, group, s);
+}
