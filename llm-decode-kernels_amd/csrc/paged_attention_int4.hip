@@ -52,6 +52,52 @@ __device__ __forceinline__ Codes codes_less8(uint32_t a, uint32_t b) {
 constexpr float kLag4 = 3.0f;  // powers of two that a row's maximum may lag
 constexpr int kUnit4 = 11;     // weights times 2^kUnit4: 2^(kLag4 + kUnit4 + 1) is inside fp16
 
+// A row of q as the matrix cores' operands, 2^qs q in fp16: lane c16 + 16 kb has row c16's dims 8kb + 32s .. + 7, raw in
+// qb; us: the row's sums over the groups in the same units. Returns qs.
+template <typename E, int NS, int NG>
+__device__ __forceinline__ int scale_q(u32x4* qb, float* us) {
+  int qs = 0;
+  if constexpr (E::kOnes == BF16::kOnes) {
+    float amax = 0.0f;
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2_t f = unpack2<E>(qb[s][i]);
+        amax = fmaxf(amax, fmaxf(__builtin_fabsf(f[0]), __builtin_fabsf(f[1])));
+      }
+    amax = max_xor32(max_xor16(amax));
+    qs = 13 - max(-100, min(127, (int)(f2u(amax) >> 23) - 127));  // amax < 2^(14 - qs)
+    const float by = pow2i(qs);
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2_t f = unpack2<E>(qb[s][i]);
+        qb[s][i] = pack2<F16>(f[0] * by, f[1] * by);
+      }
+  }
+#pragma unroll
+  for (int g = 0; g < NG; ++g) us[g] = 0.0f;
+#pragma unroll
+  for (int s = 0; s < NS; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2_t h = unpack2<F16>(qb[s][i]);
+      us[s * NG / NS] += h[0] + h[1];
+    }
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    us[g] = add_xor32(add_xor16(us[g]));
+    if (!(__builtin_fabsf(us[g]) < __builtin_inff())) us[g] = __builtin_nanf("");  // a row with an infinity: no score
+  }
+  return qs;
+}
+// The exponents' factor of scores formed as 2^qs q.k: finite and, as -inf 0 is NaN, not 0.
+__device__ __forceinline__ float score_factor(float scale, int qs) {
+  return fmaxf(0x1p-126f, fminf(scale * 1.44269504088896341f * pow2i(-qs), 0x1p126f));
+}
+
 constexpr int kPad = 4;  // floats after a row of outputs in LDS: 16 rows' float4 in different banks
 constexpr int split4_lds(int hd, int nw) { return nw * kRows * (2 + hd + kPad) * 4; }
 
@@ -92,50 +138,14 @@ __global__ __launch_bounds__(NW * 64) void paged_split4_kernel(PagedArgs a) {
   const int thi = min(pt1, a.cap - 1), tlo = a.window > 0 ? max(0, pt0 - a.window + 1) : 0;
   const int alo = a.window > 0 ? max(0, pt1 - a.window + 1) : 0;
 
-  // ---- row c16's q at dims 8kb + 32s .. + 7, as the B operands: 2^qs q in fp16
   const T* qrow = (const T*)a.q + (int64_t)(sp.s.row0 + tok) * a.ldq + (int64_t)(kvh * a.gq + row % a.gq) * HD;
   u32x4 qb[NS];
-  float us[NG];  // U_g in the same units
-  int qs = 0;
+  float us[NG];
 #pragma unroll
   for (int s = 0; s < NS; ++s)
     qb[s] = c16 < rows ? *reinterpret_cast<const u32x4*>(qrow + 32 * s + 8 * kb) : u32x4{0, 0, 0, 0};
-  if constexpr (E::kOnes == BF16::kOnes) {
-    float amax = 0.0f;
-#pragma unroll
-    for (int s = 0; s < NS; ++s)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2_t f = unpack2<E>(qb[s][i]);
-        amax = fmaxf(amax, fmaxf(__builtin_fabsf(f[0]), __builtin_fabsf(f[1])));
-      }
-    amax = max_xor32(max_xor16(amax));
-    qs = 13 - max(-100, min(127, (int)(f2u(amax) >> 23) - 127));  // amax < 2^(14 - qs)
-    const float by = pow2i(qs);
-#pragma unroll
-    for (int s = 0; s < NS; ++s)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2_t f = unpack2<E>(qb[s][i]);
-        qb[s][i] = pack2<F16>(f[0] * by, f[1] * by);
-      }
-  }
-#pragma unroll
-  for (int g = 0; g < NG; ++g) us[g] = 0.0f;
-#pragma unroll
-  for (int s = 0; s < NS; ++s)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2_t h = unpack2<F16>(qb[s][i]);
-      us[s * NG / NS] += h[0] + h[1];
-    }
-#pragma unroll
-  for (int g = 0; g < NG; ++g) {
-    us[g] = add_xor32(add_xor16(us[g]));
-    if (!(__builtin_fabsf(us[g]) < __builtin_inff())) us[g] = __builtin_nanf("");  // a row with an infinity: no score
-  }
-  // scores are formed as 2^qs q.k; their exponents' factor, finite and, as -inf 0 is NaN, not 0
-  const float f1 = fmaxf(0x1p-126f, fminf(a.scale * 1.44269504088896341f * pow2i(-qs), 0x1p126f));
+  const int qs = scale_q<E, NS, NG>(qb, us);
+  const float f1 = score_factor(a.scale, qs);
 
   // The maximum that is subtracted may lag the largest score by kLag4; it and the unit of the weights move where a lane
   // finds more, and with them what is summed so far. Scores start from -m (0 while m is -inf), so that differences
@@ -320,14 +330,413 @@ __global__ __launch_bounds__(NW * 64) void paged_split4_kernel(PagedArgs a) {
   }
 }
 
+// ---- blocks of rows that share K and V through LDS
+//
+// As paged_attention.hip's: CG x KG waves take 32 CG rows of one kv head, wave (kg, cg) 32 rows (two column tiles) over the
+// chunks kg, kg + KG, ... of the block's range. The waves of a K group unpack each chunk once for all of its
+// rows, a step ahead of its use: each wave its part of the codes, into whole tiles of c - 8 in one of two LDS slots, and of
+// the steps and offsets, as fp32. What a wave unpacks it has loaded two steps before. One barrier per chunk: behind it
+// the chunk's slot is written, and the other slot, whose readers are done, is free for the next one.
+
+// LDS bytes: of a K group two slots of tiles, steps and offsets; the K groups' m and l per column tile and lane.
+constexpr int slot4_bytes(int hd, int ng) { return hd / 8 * 1024 + 512 * ng; }
+constexpr int block4_lds(int hd, int ng, int cg, int kg) { return kg * 2 * slot4_bytes(hd, ng) + (kg > 1 ? cg * kg * 4 * 64 * 4 : 0); }
+
+template <typename E, int HD, int NG, int BT>
+__global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_eu(2))) void paged_block4_kernel(PagedArgs a) {
+  typedef typename E::T T;
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  typedef Int4Block<HD, NG> L;
+  constexpr int CG = BT / 32, KG = kBlockKG<BT>, NS = HD / 32, NB = HD / 16, NP = HD / 64;
+  constexpr int NU = 4 / CG;                                  // of a chunk's four quarters of codes, a wave's
+  constexpr int NT = 2 * NP;                                  // tiles of a quarter
+  constexpr int PW = (64 * NG + CG * 64 - 1) / (CG * 64);     // words of steps and offsets per thread
+  constexpr int kSlot = slot4_bytes(HD, NG);
+  static_assert(KG == 1 || KG * 2 * kSlot >= (KG - 1) * CG * 2 * NB * 64 * 16, "the K groups meet in the slots");
+  __shared__ __align__(16) unsigned char lds[block4_lds(HD, NG, CG, KG)];
+  const int tid = threadIdx.x, lane = tid & 63, wg = (int)blockIdx.x, split = (int)blockIdx.y;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kg = wave / CG, cg = wave % CG;
+  const int c16 = lane & 15, kb = lane >> 4;
+  const int kvh = wg % a.nkv, tile = a.btiles - 1 - wg / a.nkv;  // longest blocks first
+  const Block bk = find_block<0>(a, tile, BT);
+  if (bk.rows <= 0) return;
+  const int per = block_range(a, bk.n, KG);
+  const int j0 = split * per;
+  if (split && j0 >= bk.n) return;  // the first range runs with no chunk too: its rows are written
+  const int nsteps = max(0, min(per, bk.n - j0));
+  const int n = (nsteps + KG - 1) / KG;  // steps of a K group (the last ones may be dead)
+
+  // this lane's two rows see the positions above hi - window up to hi, and those below sinks; rows past
+  // the block's are not stored. whi, wlo: the last and the first past the sinks that a row of the wave sees
+  const int window = a.window > 0 ? a.window : kAll;
+  auto row_of = [&](int ct, int ln, int& tok, int& head) __attribute__((always_inline)) {
+    const int r = bk.r0 + min(32 * cg + 16 * ct + (ln & 15), bk.rows - 1);
+    tok = r / a.gq;
+    head = kvh * a.gq + r % a.gq;
+  };
+  int hi[2], whi = -1, wlo = kAll;
+#pragma unroll
+  for (int ct = 0; ct < 2; ++ct) {
+    int t, h;
+    row_of(ct, lane, t, h);
+    hi[ct] = max(-1, bk.pos0 + t);
+    whi = max(whi, hi[ct]);
+    wlo = min(wlo, max(0, hi[ct] - window + 1));
+  }
+#pragma unroll
+  for (int off = 1; off < 16; off *= 2) {
+    whi = max(whi, __shfl_xor(whi, off));
+    wlo = min(wlo, __shfl_xor(wlo, off));
+  }
+  whi = __builtin_amdgcn_readfirstlane(whi);
+  wlo = __builtin_amdgcn_readfirstlane(wlo);
+  // of the block: positions that every row sees, all_lo .. first, and that one sees, any_lo .. last
+  const int all_lo = a.window > 0 ? max(0, bk.last - a.window + 1) : 0;
+  const int any_lo = a.window > 0 ? max(0, bk.first - a.window + 1) : 0;
+
+  // the block's chunks in order: those that every row sees whole (fl .. fl + nf - 1), the sinks', the others
+  const int fl = max(bk.lo, (all_lo + kChunkPos - 1) / kChunkPos);
+  const int nf = max(0, min(bk.lo + bk.n - bk.cs, (min(bk.first, kAll - 1) + 1) / kChunkPos) - fl);
+  auto chunk_of = [&](int j) __attribute__((always_inline)) {
+    const int i = j0 + j * KG + kg;
+    int d = i - nf - bk.cs + bk.lo < fl ? bk.lo - nf - bk.cs : bk.lo - bk.cs;
+    d = i < nf + bk.cs ? -nf : d;
+    return i + (i < nf ? fl : d);
+  };
+  // the page of a step that is to be loaded next, its id read through the scalar cache a step ahead
+  const ScalarInts table = (ScalarInts)(uintptr_t)(a.table + (int64_t)bk.b * a.ldt);
+  int page, sub;
+  auto next_page = [&](int j) __attribute__((always_inline)) {
+    const int c = j * KG + kg < nsteps ? chunk_of(j) : 0;
+    int at;
+    chunk_page(a.cpp, c, at, sub);
+    page = table[at];
+  };
+  uint32_t have = 0;  // bit i: whether the step i before the last one loaded has a page
+  int nfull = min(n, max(0, nf - j0 - kg + KG - 1) / KG);  // unmasked steps: to the first without a page
+  struct Raw {
+    u32x4 codes[NU];
+    uint32_t params[PW];
+  };
+  const int gt = cg * 64 + lane;  // of the K group's threads
+  // A chunk's bytes that this thread unpacks; no page (an id outside the pool, a step past the range): zeros
+  auto load = [&](int j) __attribute__((always_inline)) {
+    const bool ok = j * KG + kg < nsteps && (uint32_t)page < (uint32_t)a.pages;
+    const auto rs = buffer_rsrc((const T*)a.k + (ok ? page * a.kps : 0) + ((int64_t)kvh * a.cpp.n + (ok ? sub : 0)) * L::kWords, ok ? L::kBytes : 0);
+    Raw r;
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      const int u = cg + CG * i;
+      if constexpr (HD == 128) {
+        r.codes[i] = buffer_load16(rs, (uint32_t)(u * 1024 + lane * 16));
+      } else {
+        const auto v = __builtin_amdgcn_raw_buffer_load_b64(rs, (uint32_t)((u >> 1) * 1024 + lane * 16 + (u & 1) * 8), 0, 0);
+        r.codes[i] = u32x4{v[0], v[1], 0, 0};
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < PW; ++i) {
+      const int w = gt + i * CG * 64;
+      r.params[i] = __builtin_amdgcn_raw_buffer_load_b32(rs, (uint32_t)(w < 64 * NG ? L::kParams + w * 4 : L::kBytes), 0, 0);
+    }
+    have = __builtin_amdgcn_readfirstlane(have << 1 | (ok ? 1u : 0u));
+    nfull = __builtin_amdgcn_readfirstlane(ok ? nfull : min(nfull, j));
+    next_page(j + 1);
+    return r;
+  };
+  unsigned char* const slots = lds + kg * 2 * kSlot;
+  auto unpack = [&](const Raw& r, int j) __attribute__((always_inline)) {
+    unsigned char* const to = slots + (j & 1) * kSlot;
+#pragma unroll
+    for (int i = 0; i < NU; ++i)
+#pragma unroll
+      for (int t = 0; t < NP; ++t) {
+        const Codes c = codes_less8(r.codes[i][2 * t], r.codes[i][2 * t + 1]);
+        unsigned char* const at = to + ((cg + CG * i) * NT + 2 * t) * 1024 + lane * 16;
+        *reinterpret_cast<u32x4*>(at) = c.low;
+        *reinterpret_cast<u32x4*>(at + 1024) = c.high;
+      }
+    // word w of the params: of k or v, group, position / 8, step or offset, a pair of positions. What no row of the block
+    // sees may be anything: zero
+    float* const par = reinterpret_cast<float*>(to + HD / 8 * 1024);
+    const int cb = chunk_of(j) * kChunkPos;
+#pragma unroll
+    for (int i = 0; i < PW; ++i) {
+      const int w = gt + i * CG * 64;
+      const int pos = (w >> 3 & 3) * 8 + (w & 3) * 2, kind = (w >> 2 & 1) + (w >= 32 * NG ? 2 : 0), g = w / 32 % NG;
+      float2_t f = unpack2<E>(r.params[i]);
+      const int p0 = cb + pos;
+      if (!(p0 <= bk.last && (p0 >= any_lo || p0 < a.sinks))) f[0] = 0.0f;
+      if (!(p0 + 1 <= bk.last && (p0 + 1 >= any_lo || p0 + 1 < a.sinks))) f[1] = 0.0f;
+      if (w < 64 * NG) *reinterpret_cast<float2_t*>(par + (kind * NG + g) * 32 + pos) = f;
+    }
+  };
+  next_page(0);
+  {
+    const Raw r0 = load(0);
+    unpack(r0, 0);
+  }
+  Raw r1 = load(1), r2 = load(2);
+
+  // this wave's q operands
+  u32x4 q[2][NS];
+  float us[2][NG], f1[2];
+  int qs[2];
+#pragma unroll
+  for (int ct = 0; ct < 2; ++ct) {
+    int t, h;
+    row_of(ct, lane, t, h);
+    const T* src = (const T*)a.q + (int64_t)(bk.row0 + t) * a.ldq + (int64_t)h * HD + 8 * kb;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) q[ct][s] = *reinterpret_cast<const u32x4*>(src + 32 * s);
+    qs[ct] = scale_q<E, NS, NG>(q[ct], us[ct]);
+    f1[ct] = score_factor(a.scale, qs[ct]);
+  }
+  float m_run[2], less[2], limit[2], l[2], ms[2][NG];
+  int ve = -100;      // 2^ve: the power of two of the largest step of v that a row of the block has seen
+  float4_t o[2][NB];  // O^T[dim 16b + 4kb + r][row c16], unnormalised; l, ms and o in units of 2^(kUnit4 - ve)
+#pragma unroll
+  for (int ct = 0; ct < 2; ++ct) {
+    m_run[ct] = limit[ct] = -__builtin_inff();
+    less[ct] = l[ct] = 0.0f;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) ms[ct][g] = 0.0f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) o[ct][b] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  auto step = [&](auto maskedc, int j) __attribute__((always_inline)) {
+    constexpr bool kMasked = decltype(maskedc)::value;
+    lds_barrier();
+    const unsigned char* const from = slots + (j & 1) * kSlot;
+    const float* const par = reinterpret_cast<const float*>(from + HD / 8 * 1024);
+    const int cb = chunk_of(j) * kChunkPos;
+    const bool live = !kMasked || ((have >> 2 & 1) && cb <= whi && (cb + kChunkPos > wlo || cb < a.sinks));
+    float sv[2][8];
+    auto params = [&](int kind, int g, float* f) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float4_t v = *reinterpret_cast<const float4_t*>(par + (kind * NG + g) * 32 + 8 * kb + 4 * i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[4 * i + e] = v[e];
+      }
+    };
+    if (live) {
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        float4_t acc[2][2];
+#pragma unroll
+        for (int s = g * NS / NG; s < (g + 1) * NS / NG; ++s)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const u32x4 k = *reinterpret_cast<const u32x4*>(from + (h * NS + s) * 1024 + lane * 16);
+#pragma unroll
+            for (int ct = 0; ct < 2; ++ct) {
+              const float4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
+              acc[h][ct] = F16::mfma(k, q[ct][s], s % (NS / NG) ? acc[h][ct] : zero);
+            }
+          }
+        float st[8], z[8];
+        params(0, g, st);
+        params(1, g, z);
+#pragma unroll
+        for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            sv[ct][e] = __builtin_fmaf(st[e], acc[e >> 2][ct][e & 3], __builtin_fmaf(z[e], us[ct][g], g ? sv[ct][e] : less[ct]));
+      }
+    }
+    unpack(r1, j + 1);
+    r1 = r2;
+    r2 = load(j + 3);
+    if (live) {
+      float sm = 0.0f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        float st[8];
+        params(2, g, st);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sm = fmaxf(sm, st[e]);
+      }
+      if (NG == 4) asm volatile("" : : : "memory");  // read again below rather than kept: 256 registers do not hold them
+      bool more_any = sm >= pow2i(ve + 1);
+      bool seen[2][8];
+#pragma unroll
+      for (int ct = 0; ct < 2; ++ct) {
+        float mc = -__builtin_inff();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if constexpr (kMasked) {
+            const int p = cb + 8 * kb + e;
+            seen[ct][e] = p <= hi[ct] && (p > hi[ct] - window || p < a.sinks);
+            sv[ct][e] = seen[ct][e] ? sv[ct][e] : -__builtin_inff();
+          }
+          mc = fmaxf(mc, sv[ct][e]);
+        }
+        more_any = more_any || mc > limit[ct];
+      }
+      if (__any(more_any)) {
+        sm = max_xor32(max_xor16(sm));
+        const int vn = min(126, max(ve, (int)(f2u(sm) >> 23) - 127));
+        const float by = pow2i(max(ve - vn, -126));
+        ve = vn;
+#pragma unroll
+        for (int ct = 0; ct < 2; ++ct) {
+          float mc = sv[ct][0];
+#pragma unroll
+          for (int e = 1; e < 8; ++e) mc = fmaxf(mc, sv[ct][e]);
+          mc = max_xor32(max_xor16(mc));
+          const float old = less[ct], m_new = fmaxf(m_run[ct], mc - old);
+          const float now = m_new == -__builtin_inff() ? 0.0f : -m_new, more = old - now;
+          const float al = (m_run[ct] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(-more * f1[ct])) * by;
+          l[ct] *= al;
+#pragma unroll
+          for (int g = 0; g < NG; ++g) ms[ct][g] *= al;
+#pragma unroll
+          for (int b = 0; b < NB; ++b) o[ct][b] *= al;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sv[ct][e] -= more;
+          m_run[ct] = m_new;
+          less[ct] = now;
+          limit[ct] = m_new == -__builtin_inff() ? m_new : kLag4 / f1[ct];
+        }
+      }
+      const float unit = (float)(kUnit4 - ve);
+#pragma unroll
+      for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          sv[ct][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[ct][e], f1[ct], unit));
+          l[ct] += sv[ct][e];
+        }
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        float st[8], z[8];
+        params(2, g, st);
+        params(3, g, z);
+        u32x4 pw[2];
+#pragma unroll
+        for (int ct = 0; ct < 2; ++ct) {
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            // what this row does not see and another does may be NaN
+            const bool on = !kMasked || seen[ct][e];
+            ms[ct][g] = __builtin_fmaf(sv[ct][e], on ? z[e] : 0.0f, ms[ct][g]);
+            x[e] = sv[ct][e] * (on ? st[e] : 0.0f);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) pw[ct][e] = pack2<F16>(x[2 * e], x[2 * e + 1]);
+        }
+#pragma unroll
+        for (int b = g * NB / NG; b < (g + 1) * NB / NG; ++b) {
+          const u32x4 v = *reinterpret_cast<const u32x4*>(from + (2 * NS + b) * 1024 + lane * 16);
+#pragma unroll
+          for (int ct = 0; ct < 2; ++ct) o[ct][b] = F16::mfma(v, pw[ct], o[ct][b]);
+        }
+      }
+    }
+  };
+  int j = 0;
+  for (; j < nfull; ++j) step(IntC<0>(), j);
+  for (; j < n; ++j) step(IntC<1>(), j);
+
+  // ---- what the rows have, in q.k's and v's own units; groups past the first leave it to the first, lane for lane
+#pragma unroll
+  for (int ct = 0; ct < 2; ++ct) {
+    const float one = pow2i(ve - kUnit4);
+    l[ct] = add_xor32(add_xor16(l[ct])) * one;
+    m_run[ct] *= pow2i(-qs[ct]);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) ms[ct][g] = add_xor32(add_xor16(ms[ct][g]));
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[ct][b][r] = (o[ct][b][r] + ms[ct][b * NG / NB]) * one;
+  }
+  float4_t* const red = reinterpret_cast<float4_t*>(lds);  // [wave - CG][2 NB][64]
+  float(*const mls)[4][64] = reinterpret_cast<float(*)[4][64]>(lds + KG * 2 * kSlot);
+  if constexpr (KG > 1) {
+    lds_barrier();  // the slots have been read
+    if (kg > 0) {
+#pragma unroll
+      for (int ct = 0; ct < 2; ++ct) {
+        mls[wave][2 * ct][lane] = m_run[ct];
+        mls[wave][2 * ct + 1][lane] = l[ct];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) red[((wave - CG) * 2 * NB + NB * ct + b) * 64 + lane] = o[ct][b];
+      }
+    }
+    lds_barrier();
+    if (kg > 0) return;
+  }
+  const float sc = a.scale * 1.44269504088896341f;
+  const bool direct = bk.n <= per;  // a lone range
+  float* const part = a.bpart + (((int64_t)tile * a.nkv + kvh) * a.bsplits + split) * BT * (2 + HD);
+#pragma unroll
+  for (int ct = 0; ct < 2; ++ct) {
+    float mv[KG], f[KG], M = m_run[ct], ls = 0.0f;
+    mv[0] = m_run[ct];
+#pragma unroll
+    for (int g = 1; g < KG; ++g) {
+      mv[g] = mls[cg + g * CG][2 * ct][lane];
+      M = fmaxf(M, mv[g]);
+    }
+#pragma unroll
+    for (int g = 0; g < KG; ++g) {
+      f[g] = mv[g] != -__builtin_inff() ? __builtin_amdgcn_exp2f((mv[g] - M) * sc) : 0.0f;
+      ls = __builtin_fmaf(g ? mls[cg + g * CG][2 * ct + 1][lane] : l[ct], f[g], ls);
+    }
+    const int col = 32 * cg + 16 * ct + c16;
+    int t, h;
+    row_of(ct, lane, t, h);
+    T* dst = (T*)a.out + (int64_t)(bk.row0 + t) * a.ldo + (int64_t)h * HD + 4 * kb;
+    float* pdst = part + 2 * BT + col * HD + 4 * kb;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      float4_t v = o[ct][b] * f[0];
+#pragma unroll
+      for (int g = 1; g < KG; ++g) {
+        const float4_t w = red[((cg + (g - 1) * CG) * 2 * NB + NB * ct + b) * 64 + lane];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = __builtin_fmaf(w[r], f[g], v[r]);
+      }
+      if (col < bk.rows) {
+        if (direct) {
+          T4 y;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) y[r] = (T)(ls != 0.0f ? v[r] / ls : 0.0f);
+          *reinterpret_cast<T4*>(dst + 16 * b) = y;
+        } else {
+          *reinterpret_cast<float4_t*>(pdst + 16 * b) = v;
+        }
+      }
+    }
+    if (!direct && kb == 0 && col < bk.rows) {
+      part[2 * col] = M;
+      part[2 * col + 1] = ls;
+    }
+  }
+}
+
 constexpr int kWaves = 8;       // of a workgroup
 constexpr int kSingle4 = 20;    // chunks up to which a sequence is one range
 constexpr int kPlanSeqs4 = 64;  // more sequences have their ranges found in a launch before
 
 Plan make_plan4(int64_t T, int64_t B, int64_t max_q, int64_t max_len, int64_t window, int64_t sinks, int nq, int nkv, int hd) {
   Plan p;
-  (void)T;
-  p.nt = (max_q * (nq / nkv) + kRows - 1) / kRows;
+  const int64_t gq = nq / nkv, rows = T * gq;
+  if (max_q * gq > 2 * kRows) {  // blocks of rows
+    p.bt = rows >= 96 * B ? 128 : 64;
+    p.btiles = rows / p.bt + B;
+    const int64_t fill = p.bt == 64 ? 320 : hd == 128 ? 512 : 768, whole = nkv * p.btiles;
+    p.bsplits = 3 * whole >= fill ? 1 : std::max<int64_t>(1, std::min<int64_t>(32, fill / whole));
+    if (p.bsplits > 1) p.bpart_bytes = p.btiles * nkv * p.bsplits * p.bt * (2 + hd) * 4;
+    p.bytes = workspace_bytes(p, B);
+    return p;
+  }
+  p.nt = (max_q * gq + kRows - 1) / kRows;
   if (most_chunks(max_len, max_q, window, sinks) <= kSingle4) {
     p.slots = B;
     return p;
@@ -346,7 +755,13 @@ int launch(const PagedArgs& a, const Plan& p, int dtype, hipStream_t s) {
   (void)hipGetLastError();
   int st;
   if (p.mapped && (st = ldk::paged_find_ranges(a, s))) return st;
-  paged_split4_kernel<E, HD, NG, kWaves><<<(unsigned)(p.slots * a.nkv * p.nt), kWaves * 64, 0, s>>>(a);
+  const dim3 blocks((unsigned)(p.btiles * a.nkv), (unsigned)p.bsplits);
+  if (p.bt == 128)
+    paged_block4_kernel<E, HD, NG, 128><<<blocks, kBlockThreads<128>, 0, s>>>(a);
+  else if (p.bt)
+    paged_block4_kernel<E, HD, NG, 64><<<blocks, kBlockThreads<64>, 0, s>>>(a);
+  else
+    paged_split4_kernel<E, HD, NG, kWaves><<<(unsigned)(p.slots * a.nkv * p.nt), kWaves * 64, 0, s>>>(a);
   if ((st = ldk::check_launch("paged_attention_int4")) || !p.bytes) return st;
   return ldk::paged_join(a, dtype, HD, p.bt, s);
 }
@@ -407,6 +822,7 @@ extern "C" int ldk_paged_attention_int4(const void* q, int64_t ldq, int dtype, c
   a.pages = (int)num_pages, a.cpp = page_div(page_size / kChunkPos), a.cap = (int)(max_pages * page_size);
   a.window = (int)std::min<int64_t>(window, big), a.sinks = (int)std::min<int64_t>(sinks, big);
   a.slots = (int)p.slots, a.spare = (int)p.spare;
+  a.btiles = (int)p.btiles, a.bsplits = (int)p.bsplits, a.bdirect = 1;
   a.scale = scale;
   hipStream_t s = (hipStream_t)stream;
   return dtype == LDK_F16 ? launch<ldk::F16>(a, p, dtype, head_dim, group, s) : launch<ldk::BF16>(a, p, dtype, head_dim, group, s);
