@@ -32,22 +32,43 @@ __device__ __forceinline__ void params8(const u32x4& v, float* f) {
     f[2 * i] = a[0], f[2 * i + 1] = a[1];
   }
 }
+// The largest of 8 params that are not negative, whose bits order as they do.
+template <typename E>
+__device__ __forceinline__ float largest8(const u32x4& v) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  auto h = [](uint32_t w) { return __builtin_bit_cast(u16x2, w); };  // (by value: a cast of v[i] itself is of v[0])
+  const u16x2 m = __builtin_elementwise_max(__builtin_elementwise_max(h(v[0]), h(v[1])), __builtin_elementwise_max(h(v[2]), h(v[3])));
+  const uint16_t t = __builtin_elementwise_max(m[0], m[1]);
+  return (float)__builtin_bit_cast(typename E::T, t);
+}
+// The largest of three, NaN aside (the compiler's own would first make a number of what it does not know to be one).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
 // Two words of codes less 8 as fp16, the low four bits' (the even step's or block's) and the high four bits' operands.
-// 1024 + c and 1024 + 16 c have the code in fp16's last bits.
+// 1024 + c and 1024 + 16 c have the code in fp16's last bits. The masks are in registers, so that each is one
+// instruction with its or.
 struct Codes {
   u32x4 low, high;
 };
-__device__ __forceinline__ Codes codes_less8(uint32_t a, uint32_t b) {
-  const half2_t less = {(half_t)-1032.0f, (half_t)-1032.0f}, by = {(half_t)0.0625f, (half_t)0.0625f}, less72 = {(half_t)-72.0f, (half_t)-72.0f};
-  const uint32_t w[4] = {a, a >> 8, b, b >> 8};
-  Codes r;
+struct Unpack {
+  uint32_t low, high, magic;
+  __device__ __forceinline__ Unpack() : low(sgpr_const<kLow4>()), high(sgpr_const<kHigh4>()), magic(vgpr_const<0x64006400u>()) {}
+  __device__ __forceinline__ Codes operator()(uint32_t a, uint32_t b) const {
+    const half2_t less = {(half_t)-1032.0f, (half_t)-1032.0f}, by = {(half_t)0.0625f, (half_t)0.0625f}, less72 = {(half_t)-72.0f, (half_t)-72.0f};
+    const uint32_t w[4] = {a, a >> 8, b, b >> 8};
+    Codes r;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    r.low[i] = h22u(u2h2((w[i] & kLow4) | 0x64006400u) + less);
-    r.high[i] = h22u(__builtin_elementwise_fma(u2h2((w[i] & kHigh4) | 0x64006400u), by, less72));
+    for (int i = 0; i < 4; ++i) {
+      r.low[i] = h22u(u2h2((w[i] & low) | magic) + less);
+      r.high[i] = h22u(__builtin_elementwise_fma(u2h2((w[i] & high) | magic), by, less72));
+    }
+    return r;
   }
-  return r;
-}
+};
 
 constexpr float kLag4 = 3.0f;  // powers of two that a row's maximum may lag
 constexpr int kUnit4 = 11;     // weights times 2^kUnit4: 2^(kLag4 + kUnit4 + 1) is inside fp16
@@ -119,9 +140,26 @@ __global__ __launch_bounds__(NW * 64) void paged_split4_kernel(PagedArgs a) {
   const int c16 = lane & 15, kb = lane >> 4;
   const int xy = a.nkv * a.nt, bxy = wg % xy;
   const int kvh = bxy % a.nkv, tile = bxy / a.nkv;
-  const Slot sl = find_slot(a, wg / xy, lane);
-  if (sl.b < 0) return;
-  const Span sp = seq_span(a, sl.b);
+  Slot sl{wg / xy, 0, 1, wg / xy, kAll};  // without a plan every sequence is one range
+  if (a.plan) {                           // found by one wave for all
+    int* const found = reinterpret_cast<int*>(lds);
+    if (wave == 0) {
+      sl = find_slot(a, wg / xy, lane);
+      if (lane == 0) found[0] = sl.b, found[1] = sl.split, found[2] = sl.ranges, found[3] = sl.first, found[4] = sl.per;
+    }
+    lds_barrier();
+    auto uniform = [&](int i) { return __builtin_amdgcn_readfirstlane(found[i]); };
+    sl = Slot{uniform(0), uniform(1), uniform(2), uniform(3), uniform(4)};
+    lds_barrier();  // read before the waves' results go there
+    if (sl.b < 0) return;
+  }
+  Span sp = seq_span(a, sl.b);  // one sequence's for the whole workgroup: scalars, and with them what is formed of them
+  sp.s.row0 = __builtin_amdgcn_readfirstlane(sp.s.row0);
+  sp.s.n = __builtin_amdgcn_readfirstlane(sp.s.n);
+  sp.s.pos0 = __builtin_amdgcn_readfirstlane(sp.s.pos0);
+  sp.cs = __builtin_amdgcn_readfirstlane(sp.cs);
+  sp.lo = __builtin_amdgcn_readfirstlane(sp.lo);
+  sp.n = __builtin_amdgcn_readfirstlane(sp.n);
   if (a.plan && !a.map && kvh == 0 && tile == 0 && sl.split == 0 && tid == 0) {
     a.plan[2 * sl.b] = sl.first;
     a.plan[2 * sl.b + 1] = sl.ranges;
@@ -158,6 +196,7 @@ __global__ __launch_bounds__(NW * 64) void paged_split4_kernel(PagedArgs a) {
   for (int g = 0; g < NG; ++g) ms[g] = 0.0f;
 #pragma unroll
   for (int b = 0; b < NB; ++b) o[b] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  const Unpack unpacked;
   const ScalarInts trow = (ScalarInts)(uintptr_t)(a.table + (int64_t)sl.b * a.ldt);
   const int jend = (int)min((sl.split + (int64_t)1) * sl.per, (int64_t)sp.n);
   for (int j = sl.split * sl.per + wave; j < jend; j += NW) {
@@ -191,7 +230,7 @@ __global__ __launch_bounds__(NW * 64) void paged_split4_kernel(PagedArgs a) {
       for (int n = 0; n < NP; ++n)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const Codes c = HD == 128 ? codes_less8(kc[h % NL][2 * n], kc[h % NL][2 * n + 1]) : codes_less8(kc[0][2 * h], kc[0][2 * h + 1]);
+          const Codes c = HD == 128 ? unpacked(kc[h % NL][2 * n], kc[h % NL][2 * n + 1]) : unpacked(kc[0][2 * h], kc[0][2 * h + 1]);
 #pragma unroll
           for (int odd = 0; odd < 2; ++odd) {
             const int s = 2 * n + odd, g = s * NG / NS;
@@ -208,34 +247,24 @@ __global__ __launch_bounds__(NW * 64) void paged_split4_kernel(PagedArgs a) {
         for (int e = 0; e < 8; ++e) sv[e] = __builtin_fmaf(st[e], acc[e >> 2][g][e & 3], __builtin_fmaf(z[e], us[g], g ? sv[e] : less));
       }
     }
-    float vst[NG][8], vz[NG][8];
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      params8<E>(vp[g][0], vst[g]);
-      params8<E>(vp[g][1], vz[g]);
-    }
     // a chunk that not every row sees whole: what a row does not see has no score, and steps and offsets of 0 (they may
     // be anything, and 0 x NaN is NaN)
     if (cb + kChunkPos - 1 > pt0 || (cb < alo && cb + kChunkPos > a.sinks)) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int pj = cb + 8 * kb + e;
-        const bool seen = pj <= hi && (pj >= lo || pj < a.sinks);
-        sv[e] = seen ? sv[e] : -__builtin_inff();
+      for (int i = 0; i < 4; ++i) {
+        const int p0 = cb + 8 * kb + 2 * i;
+        const bool on0 = p0 <= hi && (p0 >= lo || p0 < a.sinks), on1 = p0 + 1 <= hi && (p0 + 1 >= lo || p0 + 1 < a.sinks);
+        sv[2 * i] = on0 ? sv[2 * i] : -__builtin_inff();
+        sv[2 * i + 1] = on1 ? sv[2 * i + 1] : -__builtin_inff();
+        const uint32_t mk = (on0 ? 0x0000FFFFu : 0u) | (on1 ? 0xFFFF0000u : 0u);
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          vst[g][e] = seen ? vst[g][e] : 0.0f;
-          vz[g][e] = seen ? vz[g][e] : 0.0f;
-        }
+        for (int g = 0; g < NG; ++g) vp[g][0][i] &= mk, vp[g][1][i] &= mk;
       }
     }
-    float mc = sv[0], sm = vst[0][0];
+    float sm = largest8<E>(vp[0][0]);
 #pragma unroll
-    for (int e = 1; e < 8; ++e) mc = fmaxf(mc, sv[e]);
-#pragma unroll
-    for (int g = 0; g < NG; ++g)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sm = fmaxf(sm, vst[g][e]);
+    for (int g = 1; g < NG; ++g) sm = fmaxf(sm, largest8<E>(vp[g][0]));
+    float mc = max3(max3(max3(sv[0], sv[1], sv[2]), sv[3], sv[4]), max3(sv[5], sv[6], sv[7]), sv[7]);
     if (__any(mc > limit || sm >= pow2i(ve + 1))) {
       mc = max_xor32(max_xor16(mc));
       sm = max_xor32(max_xor16(sm));
@@ -264,14 +293,17 @@ __global__ __launch_bounds__(NW * 64) void paged_split4_kernel(PagedArgs a) {
     u32x4 pw[NG];
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
+      float st[8], z[8];
+      params8<E>(vp[g][0], st);
+      params8<E>(vp[g][1], z);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ms[g] = __builtin_fmaf(w[e], vz[g][e], ms[g]);
+      for (int e = 0; e < 8; ++e) ms[g] = __builtin_fmaf(w[e], z[e], ms[g]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) pw[g][e] = pack2<F16>(w[2 * e] * vst[g][2 * e], w[2 * e + 1] * vst[g][2 * e + 1]);
+      for (int e = 0; e < 4; ++e) pw[g][e] = pack2<F16>(w[2 * e] * st[2 * e], w[2 * e + 1] * st[2 * e + 1]);
     }
 #pragma unroll
     for (int t = 0; t < NB / 2; ++t) {  // pairs of blocks
-      const Codes c = codes_less8(vc[t / 2][2 * (t % 2)], vc[t / 2][2 * (t % 2) + 1]);
+      const Codes c = unpacked(vc[t / 2][2 * (t % 2)], vc[t / 2][2 * (t % 2) + 1]);
       o[2 * t] = F16::mfma(c.low, pw[2 * t * NG / NB], o[2 * t]);
       o[2 * t + 1] = F16::mfma(c.high, pw[2 * t * NG / NB], o[2 * t + 1]);
     }
@@ -446,13 +478,14 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
     return r;
   };
   unsigned char* const slots = lds + kg * 2 * kSlot;
+  const Unpack unpacked;
   auto unpack = [&](const Raw& r, int j) __attribute__((always_inline)) {
     unsigned char* const to = slots + (j & 1) * kSlot;
 #pragma unroll
     for (int i = 0; i < NU; ++i)
 #pragma unroll
       for (int t = 0; t < NP; ++t) {
-        const Codes c = codes_less8(r.codes[i][2 * t], r.codes[i][2 * t + 1]);
+        const Codes c = unpacked(r.codes[i][2 * t], r.codes[i][2 * t + 1]);
         unsigned char* const at = to + ((cg + CG * i) * NT + 2 * t) * 1024 + lane * 16;
         *reinterpret_cast<u32x4*>(at) = c.low;
         *reinterpret_cast<u32x4*>(at + 1024) = c.high;
@@ -545,6 +578,7 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             sv[ct][e] = __builtin_fmaf(st[e], acc[e >> 2][ct][e & 3], __builtin_fmaf(z[e], us[ct][g], g ? sv[ct][e] : less[ct]));
+        if constexpr (NG == 4) __builtin_amdgcn_sched_barrier(0);  // one group's reads at a time: 256 registers hold no more
       }
     }
     unpack(r1, j + 1);
@@ -559,7 +593,7 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
 #pragma unroll
         for (int e = 0; e < 8; ++e) sm = fmaxf(sm, st[e]);
       }
-      if (NG == 4) asm volatile("" : : : "memory");  // read again below rather than kept: 256 registers do not hold them
+      if constexpr (NG == 4) asm volatile("" : : : "memory");  // read again below rather than kept
       bool more_any = sm >= pow2i(ve + 1);
       bool seen[2][8];
 #pragma unroll
@@ -635,6 +669,7 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
 #pragma unroll
           for (int ct = 0; ct < 2; ++ct) o[ct][b] = F16::mfma(v, pw[ct], o[ct][b]);
         }
+        if constexpr (NG == 4) __builtin_amdgcn_sched_barrier(0);
       }
     }
   };
