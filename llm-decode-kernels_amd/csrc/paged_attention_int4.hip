@@ -119,40 +119,114 @@ __device__ __forceinline__ float score_factor(float scale, int qs) {
   return fmaxf(0x1p-126f, fminf(scale * 1.44269504088896341f * pow2i(-qs), 0x1p126f));
 }
 
+// ---- few rows
+//
+// A workgroup takes up to 16 rows of one kv head over a range of chunks. Both products have the row as the matrix
+// cores' column, so that a lane's scores, weights, sums and outputs are one row's. Of a tile of R = 16 / C rows (a token's few
+// query heads) the 16 columns take C chunks at once: q stands in the columns of one chunk (zeros in the others) when
+// that chunk's K is the operand, so that the scores of all of them fill one accumulator, and the weights of one chunk's
+// columns when its V is. What is done per score is then done once for C chunks on full lanes, and each column
+// is a partial result over positions of its own; they meet at the end. A wave's loads are a group of chunks ahead.
+//
+// The vector unit bounds it next to memory: 9 instructions per word of 8 codes, some 110 per group of columns.
+// Waves of a SIMD that the registers are to leave room for.
+template <int HD, int NG, int C>
+constexpr int kSplitOcc = HD == 64 ? (NG == 1 && C < 4 ? 4 : 3) : NG == 4 ? 2 : 3;
 constexpr int kPad = 4;  // floats after a row of outputs in LDS: 16 rows' float4 in different banks
-constexpr int split4_lds(int hd, int nw) { return nw * kRows * (2 + hd + kPad) * 4; }
+constexpr int kWaves = 4;
+constexpr int kMinRange4 = 4;     // chunks of a range, at least: one for each wave
+constexpr int kMaxRanges4 = 128;  // ranges of a sequence
 
-// A workgroup takes 16 rows of one kv head (paged_attention.hip) over a range of chunks, chunk w, w + NW, ... by wave w.
-// Both products have the row as the matrix cores' column, so that a lane's scores, weights, sums and outputs are
-// one row's.
-template <typename E, int HD, int NG, int NW>
-__global__ __launch_bounds__(NW * 64) void paged_split4_kernel(PagedArgs a) {
+// Over the 64 lanes.
+template <int N>
+__device__ __forceinline__ int row_ror_i(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, 0x120 + N, 0xf, 0xf, false);
+}
+__device__ __forceinline__ int wave_sum(int v) {
+  v += row_ror_i<1>(v), v += row_ror_i<2>(v), v += row_ror_i<4>(v), v += row_ror_i<8>(v);
+  auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = p[0] + p[1];
+  p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return p[0] + p[1];
+}
+__device__ __forceinline__ int wave_max(int v) {
+  v = max(v, row_ror_i<1>(v)), v = max(v, row_ror_i<2>(v)), v = max(v, row_ror_i<4>(v)), v = max(v, row_ror_i<8>(v));
+  auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max((int)p[0], (int)p[1]);
+  p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return max((int)p[0], (int)p[1]);
+}
+// Chunks of a range, of `sum` chunks (of up to 64 sequences: below 2^26) in sequences of at most `most`.
+__device__ __forceinline__ int range_chunks4(const PagedArgs& a, int sum, int most) {
+  const int per = min((sum + a.spare - 1) / a.spare, most);
+  return max(per, max(kMinRange4, (most + kMaxRanges4 - 1) / kMaxRanges4));
+}
+// The sequence and range of workgroup `slot` of up to 64 sequences, one per lane. Whole ranges come first and each
+// sequence's last, shorter one after them, so that the short ones fill what the whole ones leave of the CUs.
+__device__ __forceinline__ Slot find_slot4(const PagedArgs& a, int slot, int lane) {
+  if (a.map) {
+    const int b = a.map[1 + slot];
+    if (b < 0) return Slot{-1, 0, 1, 0, 0};
+    const int first = a.plan[2 * b];
+    return Slot{b, slot - first, a.plan[2 * b + 1], first, a.map[0]};
+  }
+  const int n = lane < a.B ? seq_span(a, lane).n : 0;
+  const int per = range_chunks4(a, wave_sum(n), wave_max(n));
+  const int whole = n / per, rest = lane < a.B && (n % per || !n) ? 1 : 0;  // whole < 2^9: both in one word
+  int end = whole << 16 | rest;  // inclusive scan over the lanes
+  for (int off = 1; off < a.B; off *= 2) {
+    const int v = __shfl_up(end, off);
+    if (lane >= off) end += v;
+  }
+  const int wholes = __builtin_amdgcn_readlane(end, a.B - 1) >> 16;
+  const int w1 = end >> 16, r1 = end & 0xffff;
+  const bool mine = slot < wholes ? slot >= w1 - whole && slot < w1 : rest && slot - wholes == r1 - 1;
+  const uint64_t has = __ballot(mine);
+  if (!has) return Slot{-1, 0, 1, 0, per};
+  const int src = __builtin_ctzll(has);
+  return Slot{src, slot < wholes ? slot - __builtin_amdgcn_readlane(w1 - whole, src) : __builtin_amdgcn_readlane(whole, src),
+              __builtin_amdgcn_readlane(whole + rest, src), __builtin_amdgcn_readlane(w1 - whole + r1 - rest, src), per};
+}
+
+// LDS: q's operands and 16 bytes of zeros, the row's sums and scale; then the waves' results.
+constexpr int q4_bytes(int hd, int ng) { return 32 * hd + 64 + 16 * 4 * (ng + 3) + 64; }
+constexpr int split4_lds(int hd, int ng, int nw) { return q4_bytes(hd, ng) + nw * kRows * (2 + hd + kPad) * 4; }
+
+template <typename E, int HD, int NG, int NW, int C>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(kSplitOcc<HD, NG, C>))) void paged_split4_kernel(PagedArgs a) {
   typedef typename E::T T;
+  typedef T T4 __attribute__((ext_vector_type(4)));
   typedef Int4Block<HD, NG> L;
   constexpr int NS = HD / 32, NB = HD / 16, NP = HD / 64;  // K dim steps, V dim blocks, pairs of steps
   constexpr int NL = HD / 64;                              // 16-byte loads per lane of K's codes, and of V's
-  __shared__ __align__(16) unsigned char lds[split4_lds(HD, NW)];
-  float(*const mw)[kRows] = reinterpret_cast<float(*)[kRows]>(lds);
+  __shared__ __align__(16) unsigned char lds[split4_lds(HD, NG, NW)];
+  unsigned char* const q_at = lds;                         // [NS][64 lanes] 16 bytes, then zeros
+  float(*const us_at)[kRows] = reinterpret_cast<float(*)[kRows]>(lds + 32 * HD + 64);  // [NG + 1]: sums; then qs
+  float(*const ml)[kRows] = us_at + NG + 1;                // [2]: the rows' maxima and sums
+  int* const found = reinterpret_cast<int*>(ml + 2);
+  float(*const mw)[kRows] = reinterpret_cast<float(*)[kRows]>(lds + q4_bytes(HD, NG));
   float(*const lw)[kRows] = mw + NW;
-  float(*const ow)[kRows][HD + kPad] = reinterpret_cast<float(*)[kRows][HD + kPad]>(lds + NW * kRows * 8);
+  float(*const ow)[kRows][HD + kPad] = reinterpret_cast<float(*)[kRows][HD + kPad]>(lds + q4_bytes(HD, NG) + NW * kRows * 8);
   const int tid = threadIdx.x, lane = tid & 63, wg = (int)blockIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c16 = lane & 15, kb = lane >> 4;
   const int xy = a.nkv * a.nt, bxy = wg % xy;
   const int kvh = bxy % a.nkv, tile = bxy / a.nkv;
+  constexpr int R = 16 / C;
+  const int r16 = c16 % R, col = c16 / R;  // this lane's row and chunk of a group
+
+  // ---- one wave finds the range for all
   Slot sl{wg / xy, 0, 1, wg / xy, kAll};  // without a plan every sequence is one range
-  if (a.plan) {                           // found by one wave for all
-    int* const found = reinterpret_cast<int*>(lds);
+  if (a.plan) {
     if (wave == 0) {
-      sl = find_slot(a, wg / xy, lane);
+      sl = find_slot4(a, wg / xy, lane);
       if (lane == 0) found[0] = sl.b, found[1] = sl.split, found[2] = sl.ranges, found[3] = sl.first, found[4] = sl.per;
     }
     lds_barrier();
     auto uniform = [&](int i) { return __builtin_amdgcn_readfirstlane(found[i]); };
     sl = Slot{uniform(0), uniform(1), uniform(2), uniform(3), uniform(4)};
-    lds_barrier();  // read before the waves' results go there
-    if (sl.b < 0) return;
   }
+  if (sl.b < 0) return;
   Span sp = seq_span(a, sl.b);  // one sequence's for the whole workgroup: scalars, and with them what is formed of them
   sp.s.row0 = __builtin_amdgcn_readfirstlane(sp.s.row0);
   sp.s.n = __builtin_amdgcn_readfirstlane(sp.s.n);
@@ -167,93 +241,156 @@ __global__ __launch_bounds__(NW * 64) void paged_split4_kernel(PagedArgs a) {
   const int rows = min(kRows, sp.s.n * a.gq - tile * kRows);  // this tile's
   if (rows <= 0) return;
   // this lane's row and the positions that it sees: lo..hi and below sinks
-  const int row = tile * kRows + c16, tok = row / a.gq;
-  const int p = sp.s.pos0 + tok;
-  const int hi = c16 < rows ? min(p, a.cap - 1) : -1;
+  const int p = sp.s.pos0 + (tile * kRows + r16) / a.gq;
+  const int hi = r16 < rows ? min(p, a.cap - 1) : -1;
   const int lo = a.window > 0 ? max(0, p - a.window + 1) : 0;
   // of the tile's rows: the last position and the first that one of them sees past the sinks, and that all see
   const int pt0 = sp.s.pos0 + tile * kRows / a.gq, pt1 = sp.s.pos0 + (tile * kRows + rows - 1) / a.gq;
   const int thi = min(pt1, a.cap - 1), tlo = a.window > 0 ? max(0, pt0 - a.window + 1) : 0;
   const int alo = a.window > 0 ? max(0, pt1 - a.window + 1) : 0;
 
-  const T* qrow = (const T*)a.q + (int64_t)(sp.s.row0 + tok) * a.ldq + (int64_t)(kvh * a.gq + row % a.gq) * HD;
-  u32x4 qb[NS];
-  float us[NG];
-#pragma unroll
-  for (int s = 0; s < NS; ++s)
-    qb[s] = c16 < rows ? *reinterpret_cast<const u32x4*>(qrow + 32 * s + 8 * kb) : u32x4{0, 0, 0, 0};
-  const int qs = scale_q<E, NS, NG>(qb, us);
-  const float f1 = score_factor(a.scale, qs);
-
   // The maximum that is subtracted may lag the largest score by kLag4; it and the unit of the weights move where a lane
   // finds more, and with them what is summed so far. Scores start from -m (0 while m is -inf), so that differences
   // are formed before they are scaled: what m f1 rounds away would rescale a row at every chunk.
   float m_run = -__builtin_inff(), less = 0.0f, limit = -__builtin_inff(), l = 0.0f;
-  int ve = -100;                 // 2^ve: the row's largest step's power of two
+  int ve = -100;                 // 2^ve: the column's largest step's power of two
   float ms[NG];                  // sum of w z
-  float4_t o[NB];                // O^T[dim 16b + 4kb + r][row c16]; l, ms and o in units of 2^(kUnit4 - ve)
+  float4_t o[NB];                // O^T[dim 16b + 4kb + r][column c16]; l, ms and o in units of 2^(kUnit4 - ve)
 #pragma unroll
   for (int g = 0; g < NG; ++g) ms[g] = 0.0f;
 #pragma unroll
   for (int b = 0; b < NB; ++b) o[b] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
   const Unpack unpacked;
-  const ScalarInts trow = (ScalarInts)(uintptr_t)(a.table + (int64_t)sl.b * a.ldt);
-  const int jend = (int)min((sl.split + (int64_t)1) * sl.per, (int64_t)sp.n);
-  for (int j = sl.split * sl.per + wave; j < jend; j += NW) {
-    const int c = j < sp.cs ? j : j - sp.cs + sp.lo;
+  const int32_t* const trow = a.table + (int64_t)sl.b * a.ldt;
+  const char* const pool = (const char*)a.k + (int64_t)kvh * a.cpp.n * L::kBytes;
+  const uint32_t pstride = (uint32_t)a.kps * 2;  // bytes: below 2^32
+  const int jbegin = (int)min(sl.split * (int64_t)sl.per, (int64_t)sp.n), jend = (int)min((sl.split + (int64_t)1) * sl.per, (int64_t)sp.n);
+  const int group = min(C, max(1, (jend - jbegin + NW - 1) / NW));  // chunks that a wave takes at once
+  // The chunk j of the range and, where its page is in the pool and a row of the tile sees some of it, its block; else null
+  auto chunk_at = [&](int j) __attribute__((always_inline)) { return j < sp.cs ? j : j - sp.cs + sp.lo; };
+  auto block_of = [&](int j, int c, int page_id, int sub) __attribute__((always_inline)) {
     const int cb = c * kChunkPos;
-    if (cb > thi || (cb + kChunkPos <= tlo && cb >= a.sinks)) continue;
-    int at, sub;
+    const bool live = j < jend && cb <= thi && (cb + kChunkPos > tlo || cb < a.sinks) && (uint32_t)page_id < (uint32_t)a.pages;
+    return live ? pool + (uint64_t)(uint32_t)page_id * pstride + (uint32_t)sub * (uint32_t)L::kBytes : nullptr;
+  };
+  // Of the group from chunk j0 on: each lane's chunk c, its page id, and then its block and the block's steps and offsets (of
+  // no block: any, they are masked)
+  auto page_of = [&](int j0, int& c, int& sub) __attribute__((always_inline)) {
+    c = chunk_at(min(j0 + col, jend - 1));
+    int at;
     chunk_page(a.cpp, c, at, sub);
-    const int page = trow[at];
-    if (page < 0 || page >= a.pages) continue;
-    const auto rs = buffer_rsrc((const T*)a.k + page * a.kps + ((int64_t)kvh * a.cpp.n + sub) * L::kWords, L::kBytes);
-    u32x4 kc[NL], vc[NL], kp[NG][2], vp[NG][2];
+    return trow[at];
+  };
+  struct Loaded {
+    u32x4 w[NL];
+  };
+  // codes of chunk i of a group, its block from a lane that has it; zeros where there is none
+  auto load = [&](const char* mine, int i, int from) __attribute__((always_inline)) {
+    const uint64_t m = (uint64_t)mine;
+    const uint64_t u = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)m, i * R) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(m >> 32), i * R) << 32;
+    const auto rs = buffer_rsrc(u ? (const char*)u + from : pool, u ? 16 * HD : 0);
+    Loaded r;
 #pragma unroll
-    for (int t = 0; t < NL; ++t) kc[t] = buffer_load16(rs, (uint32_t)(t * 1024 + lane * 16));
+    for (int t = 0; t < NL; ++t) r.w[t] = buffer_load16(rs, (uint32_t)(t * 1024 + lane * 16));
+    return r;
+  };
+  u32x4 kp[NG][2], vp[NG][2];
+  auto params = [&](const char* mine) __attribute__((always_inline)) {
+    const char* const at = (mine ? mine : pool) + kb * 32;
 #pragma unroll
     for (int g = 0; g < NG; ++g)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) kp[g][i] = buffer_load16(rs, (uint32_t)(L::kParams + g * 128 + kb * 32 + i * 16));
+      for (int i = 0; i < 2; ++i) {
+        kp[g][i] = *reinterpret_cast<const u32x4*>(at + L::kParams + g * 128 + i * 16);
+        vp[g][i] = *reinterpret_cast<const u32x4*>(at + L::kVParams + g * 128 + i * 16);
+      }
+  };
+  const int step = NW * group;
+  int j0 = jbegin + wave * group, c, cn, subn;
+  const char *mine = nullptr, *next = nullptr;
+  Loaded x[C], y[C];
+  if (j0 < jend) {
+    int sub;
+    const int id = page_of(j0, c, sub), idn = page_of(j0 + step, cn, subn);
+    mine = block_of(col < group ? j0 + col : kAll, c, id, sub);
 #pragma unroll
-    for (int g = 0; g < NG; ++g)
+    for (int i = 0; i < C; ++i) x[i] = load(mine, i, 0);
+    params(mine);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) vp[g][i] = buffer_load16(rs, (uint32_t)(L::kVParams + g * 128 + kb * 32 + i * 16));
+    for (int i = 0; i < C; ++i) y[i] = load(mine, i, L::kV);
+    next = block_of(col < group ? j0 + step + col : kAll, cn, idn, subn);
+  }
+  // ---- with the first codes on their way, one wave prepares q for all
+  if (wave == 0) {
+    const int row = tile * kRows + r16;
+    const T* qrow = (const T*)a.q + (int64_t)(sp.s.row0 + row / a.gq) * a.ldq + (int64_t)(kvh * a.gq + row % a.gq) * HD;
+    u32x4 qb[NS];
+    float us[NG];
 #pragma unroll
-    for (int t = 0; t < NL; ++t) vc[t] = buffer_load16(rs, (uint32_t)(L::kV + t * 1024 + lane * 16));
-
-    // ---- scores of positions 8kb + e, less the row's maximum so far
-    float sv[8];
-    {
-      float4_t acc[2][NG];
+    for (int t = 0; t < NS; ++t)
+      qb[t] = r16 < rows ? *reinterpret_cast<const u32x4*>(qrow + 32 * t + 8 * kb) : u32x4{0, 0, 0, 0};
+    const int qs = scale_q<E, NS, NG>(qb, us);
+#pragma unroll
+    for (int t = 0; t < NS; ++t) *reinterpret_cast<u32x4*>(q_at + (t * 64 + lane) * 16) = qb[t];
+    if (lane < 4) reinterpret_cast<uint32_t*>(q_at + 32 * HD)[lane] = 0;
+    if (kb == 0) {
+#pragma unroll
+      for (int g = 0; g < NG; ++g) us_at[g][c16] = us[g];
+      us_at[NG][c16] = __builtin_bit_cast(float, qs);
+    }
+  }
+  lds_barrier();
+  float us[NG];
+#pragma unroll
+  for (int g = 0; g < NG; ++g) us[g] = us_at[g][c16];
+  const int qs = __builtin_bit_cast(int, us_at[NG][c16]);
+  const float f1 = score_factor(a.scale, qs);
+  for (; j0 < jend; j0 += step) {
+    int c2, sub2;
+    const int id2 = page_of(j0 + 2 * step, c2, sub2);
+    // ---- scores of positions 8kb + e of this lane's chunk
+    float4_t acc[2][NG];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int g = 0; g < NG; ++g) acc[h][g] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      // q in this chunk's columns; elsewhere zeros
+      int at_q = lane * 16;
+      asm volatile("" : "+v"(at_q));  // read each time: registers do not hold C copies of q beside the rest
+      const unsigned char* const src = q_at + (C == 1 || col == i ? at_q : 32 * HD);
+      const int stride = C == 1 || col == i ? 1024 : 0;
+      u32x4 qb[NS];
+#pragma unroll
+      for (int s = 0; s < NS; ++s) qb[s] = *reinterpret_cast<const u32x4*>(src + s * stride);
 #pragma unroll
       for (int n = 0; n < NP; ++n)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const Codes c = HD == 128 ? unpacked(kc[h % NL][2 * n], kc[h % NL][2 * n + 1]) : unpacked(kc[0][2 * h], kc[0][2 * h + 1]);
-#pragma unroll
-          for (int odd = 0; odd < 2; ++odd) {
-            const int s = 2 * n + odd, g = s * NG / NS;
-            const float4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
-            acc[h][g] = F16::mfma(odd ? c.high : c.low, qb[s], s % (NS / NG) ? acc[h][g] : zero);
-          }
+          const Codes k = HD == 128 ? unpacked(x[i].w[h % NL][2 * n], x[i].w[h % NL][2 * n + 1]) : unpacked(x[i].w[0][2 * h], x[i].w[0][2 * h + 1]);
+          acc[h][2 * n * NG / NS] = F16::mfma(k.low, qb[2 * n], acc[h][2 * n * NG / NS]);
+          acc[h][(2 * n + 1) * NG / NS] = F16::mfma(k.high, qb[2 * n + 1], acc[h][(2 * n + 1) * NG / NS]);
         }
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        float st[8], z[8];
-        params8<E>(kp[g][0], st);
-        params8<E>(kp[g][1], z);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sv[e] = __builtin_fmaf(st[e], acc[e >> 2][g][e & 3], __builtin_fmaf(z[e], us[g], g ? sv[e] : less));
-      }
+      x[i] = load(next, i, 0);
     }
-    // a chunk that not every row sees whole: what a row does not see has no score, and steps and offsets of 0 (they may
-    // be anything, and 0 x NaN is NaN)
-    if (cb + kChunkPos - 1 > pt0 || (cb < alo && cb + kChunkPos > a.sinks)) {
+    float sv[8];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      float st[8], z[8];
+      params8<E>(kp[g][0], st);
+      params8<E>(kp[g][1], z);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sv[e] = __builtin_fmaf(st[e], acc[e >> 2][g][e & 3], __builtin_fmaf(z[e], us[g], g ? sv[e] : less));
+    }
+    // chunks that not every row sees whole, or that are not there: what a row does not see has no score, and steps and
+    // offsets of 0 (they may be anything, and 0 x NaN is NaN)
+    const int cb = c * kChunkPos;
+    if (__any(!mine || cb + kChunkPos - 1 > pt0 || (cb < alo && cb + kChunkPos > a.sinks))) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int p0 = cb + 8 * kb + 2 * i;
-        const bool on0 = p0 <= hi && (p0 >= lo || p0 < a.sinks), on1 = p0 + 1 <= hi && (p0 + 1 >= lo || p0 + 1 < a.sinks);
+        const bool on0 = mine && p0 <= hi && (p0 >= lo || p0 < a.sinks), on1 = mine && p0 + 1 <= hi && (p0 + 1 >= lo || p0 + 1 < a.sinks);
         sv[2 * i] = on0 ? sv[2 * i] : -__builtin_inff();
         sv[2 * i + 1] = on1 ? sv[2 * i + 1] : -__builtin_inff();
         const uint32_t mk = (on0 ? 0x0000FFFFu : 0u) | (on1 ? 0xFFFF0000u : 0u);
@@ -301,61 +438,85 @@ __global__ __launch_bounds__(NW * 64) void paged_split4_kernel(PagedArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) pw[g][e] = pack2<F16>(w[2 * e] * st[2 * e], w[2 * e + 1] * st[2 * e + 1]);
     }
+    params(next);
+    // ---- the weights of each chunk's columns times its V
 #pragma unroll
-    for (int t = 0; t < NB / 2; ++t) {  // pairs of blocks
-      const Codes c = unpacked(vc[t / 2][2 * (t % 2)], vc[t / 2][2 * (t % 2) + 1]);
-      o[2 * t] = F16::mfma(c.low, pw[2 * t * NG / NB], o[2 * t]);
-      o[2 * t + 1] = F16::mfma(c.high, pw[2 * t * NG / NB], o[2 * t + 1]);
+    for (int i = 0; i < C; ++i) {
+      const uint32_t mk = C == 1 || col == i ? 0xFFFFFFFFu : 0u;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const u32x4 pi = {pw[g][0] & mk, pw[g][1] & mk, pw[g][2] & mk, pw[g][3] & mk};
+#pragma unroll
+        for (int t = g * NB / 2 / NG; t < (g + 1) * NB / 2 / NG; ++t) {  // the group's pairs of blocks
+          const Codes v = unpacked(y[i].w[t / 2][2 * (t % 2)], y[i].w[t / 2][2 * (t % 2) + 1]);
+          o[2 * t] = F16::mfma(v.low, pi, o[2 * t]);
+          o[2 * t + 1] = F16::mfma(v.high, pi, o[2 * t + 1]);
+        }
+      }
+      y[i] = load(next, i, L::kV);
     }
+    mine = next, c = cn, cn = c2;
+    next = block_of(col < group ? j0 + 2 * step + col : kAll, c2, id2, sub2);
   }
 
-  // ---- the waves meet, maxima in q.k's own units
-  l = add_xor32(add_xor16(l));
+  // ---- what the columns have, in q.k's and v's own units; then a row's columns and the waves meet
+  const float one = pow2i(ve - kUnit4), sc = a.scale * 1.44269504088896341f;
+  l = add_xor32(add_xor16(l)) * one;
 #pragma unroll
-  for (int g = 0; g < NG; ++g) ms[g] = add_xor32(add_xor16(ms[g]));
-  const float one = pow2i(ve - kUnit4);
+  for (int g = 0; g < NG; ++g) ms[g] = add_xor32(add_xor16(ms[g])) * one;
   if (kb == 0) {
     mw[wave][c16] = m_run * pow2i(-qs);
-    lw[wave][c16] = l * one;
+    lw[wave][c16] = l;
   }
-  if (c16 < rows) {
+  if (r16 < rows) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       float4_t v;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = (o[b][r] + ms[b * NG / NB]) * one;
+      for (int r = 0; r < 4; ++r) v[r] = __builtin_fmaf(o[b][r], one, ms[b * NG / NB]);
       *reinterpret_cast<float4_t*>(&ow[wave][c16][16 * b + 4 * kb]) = v;
     }
   }
   lds_barrier();
-  const float sc = a.scale * 1.44269504088896341f;
-  float* part = a.part + (int64_t)wg * part_floats(HD);
-  for (int e = tid; e < rows * HD; e += NW * 64) {
-    const int j = e / HD, d = e % HD;
-    float mv[NW], lv[NW], ov[NW], M = -__builtin_inff();
+  if (tid < rows) {  // a row's maximum and sum, and the columns' factors in the place of their maxima
+    float mv[NW * C], M = -__builtin_inff(), ls = 0.0f;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      mv[w] = mw[w][j];
-      lv[w] = lw[w][j];
-      ov[w] = ow[w][j][d];
+    for (int i = 0; i < NW * C; ++i) {
+      mv[i] = mw[i / C][i % C * R + tid];
+      M = fmaxf(M, mv[i]);
     }
 #pragma unroll
-    for (int w = 0; w < NW; ++w) M = fmaxf(M, mv[w]);
-    float ls = 0.0f, v = 0.0f;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float f = mv[w] != -__builtin_inff() ? __builtin_amdgcn_exp2f((mv[w] - M) * sc) : 0.0f;
-      ls = __builtin_fmaf(lv[w], f, ls);
-      v = __builtin_fmaf(ov[w], f, v);
+    for (int i = 0; i < NW * C; ++i) {
+      const float f = mv[i] != -__builtin_inff() ? __builtin_amdgcn_exp2f((mv[i] - M) * sc) : 0.0f;
+      ls = __builtin_fmaf(lw[i / C][i % C * R + tid], f, ls);
+      mw[i / C][i % C * R + tid] = f;
     }
+    ml[0][tid] = M, ml[1][tid] = ls;
+  }
+  lds_barrier();
+  float* part = a.part + ((int64_t)(sl.first + sl.split) * xy + bxy) * part_floats(HD);
+  for (int e = tid; e < rows * (HD / 4); e += NW * 64) {
+    const int j = e / (HD / 4), d = e % (HD / 4) * 4;
+    float4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < NW * C; ++i) {
+      const float f = mw[i / C][i % C * R + j];
+      const float4_t x = *reinterpret_cast<const float4_t*>(&ow[i / C][i % C * R + j][d]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = __builtin_fmaf(x[r], f, v[r]);
+    }
+    const float ls = ml[1][j];
     if (sl.ranges == 1) {
       const int g = tile * kRows + j;
-      T* dst = (T*)a.out + (int64_t)(sp.s.row0 + g / a.gq) * a.ldo + (int64_t)(kvh * a.gq + g % a.gq) * HD;
-      dst[d] = (T)(ls != 0.0f ? v / ls : 0.0f);
+      T* dst = (T*)a.out + (int64_t)(sp.s.row0 + g / a.gq) * a.ldo + (int64_t)(kvh * a.gq + g % a.gq) * HD + d;
+      T4 y;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) y[r] = (T)(ls != 0.0f ? v[r] / ls : 0.0f);
+      *reinterpret_cast<T4*>(dst) = y;
     } else {
-      part[2 * kRows + e] = v;
+      *reinterpret_cast<float4_t*>(part + 2 * kRows + j * HD + d) = v;
       if (d == 0) {
-        part[2 * j] = M;
+        part[2 * j] = ml[0][j];
         part[2 * j + 1] = ls;
       }
     }
@@ -755,7 +916,6 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
   }
 }
 
-constexpr int kWaves = 8;       // of a workgroup
 constexpr int kSingle4 = 20;    // chunks up to which a sequence is one range
 constexpr int kPlanSeqs4 = 64;  // more sequences have their ranges found in a launch before
 
@@ -776,13 +936,25 @@ Plan make_plan4(int64_t T, int64_t B, int64_t max_q, int64_t max_len, int64_t wi
     p.slots = B;
     return p;
   }
-  const int64_t w = nkv * p.nt, round = (hd == 128 ? 256 : 512) / w;
-  p.spare = 2 * round >= 3 * B ? 0 : std::max<int64_t>(1, 384 / w);
-  p.slots = p.spare ? B + p.spare : round;
-  p.mapped = p.spare && B > kPlanSeqs4;
+  const int64_t w = nkv * p.nt;
+  p.spare = std::max<int64_t>(1, 512 / w);
+  p.slots = B + p.spare;
+  p.mapped = B > kPlanSeqs4;
   p.part_bytes = p.slots * w * part_floats(hd) * 4;
   p.bytes = workspace_bytes(p, B);
   return p;
+}
+
+template <typename E, int HD, int NG>
+void launch_split(const PagedArgs& a, unsigned grid, hipStream_t s) {
+  const int rows = a.max_q * a.gq;  // of a sequence, at most: its one tile's, or 16
+  if constexpr (HD == 64) {
+    if (rows <= 4) return paged_split4_kernel<E, HD, NG, kWaves, 4><<<grid, kWaves * 64, 0, s>>>(a);
+  }
+  if (rows <= 8)
+    paged_split4_kernel<E, HD, NG, kWaves, 2><<<grid, kWaves * 64, 0, s>>>(a);
+  else
+    paged_split4_kernel<E, HD, NG, kWaves, 1><<<grid, kWaves * 64, 0, s>>>(a);
 }
 
 template <typename E, int HD, int NG>
@@ -796,7 +968,7 @@ int launch(const PagedArgs& a, const Plan& p, int dtype, hipStream_t s) {
   else if (p.bt)
     paged_block4_kernel<E, HD, NG, 64><<<blocks, kBlockThreads<64>, 0, s>>>(a);
   else
-    paged_split4_kernel<E, HD, NG, kWaves><<<(unsigned)(p.slots * a.nkv * p.nt), kWaves * 64, 0, s>>>(a);
+    launch_split<E, HD, NG>(a, (unsigned)(p.slots * a.nkv * p.nt), s);
   if ((st = ldk::check_launch("paged_attention_int4")) || !p.bytes) return st;
   return ldk::paged_join(a, dtype, HD, p.bt, s);
 }
