@@ -10,8 +10,8 @@
 // only the weight w_j step_jg, to fp16, for bf16 too: its 11 bits are the closer, and the units below keep its range.
 //
 // Units. A row of bf16 q is scaled by the power of two that brings its largest element below 2^14: fp16 keeps its bits down
-// to 2^-30 of the largest, and elements below 2^-38 are lost. Weights are held times 2^11 over a power of two that
-// follows the row's largest step so far (kept like the maximum): fp16 keeps weights down to 2^-35 of it, whatever the
+// to 2^-30 of the largest, and elements below 2^-38 are lost. Weights are held times 2^8 over a power of two that
+// follows the row's largest step so far (kept like the maximum): fp16 keeps weights down to 2^-32 of it, whatever the
 // size of V is.
 #include "paged_attention.h"
 #include "paged_int4.h"
@@ -70,46 +70,42 @@ struct Unpack {
   }
 };
 
-constexpr float kLag4 = 3.0f;  // powers of two that a row's maximum may lag
-constexpr int kUnit4 = 11;     // weights times 2^kUnit4: 2^(kLag4 + kUnit4 + 1) is inside fp16
+constexpr float kLag4 = 6.0f;  // powers of two that a row's maximum may lag (3: prompts 6% slower, a fifth of the chunks rescale)
+constexpr int kUnit4 = 8;      // weights times 2^kUnit4: 2^(kLag4 + kUnit4 + 1) is inside fp16
 
 // A row of q as the matrix cores' operands, 2^qs q in fp16: lane c16 + 16 kb has row c16's dims 8kb + 32s .. + 7, raw in
-// qb; us: the row's sums over the groups in the same units. Returns qs.
+// qb; us: the row's sums over the groups in the same units (of the elements as they came: what fp16 loses of the
+// smallest is below a sum's own rounding). Returns qs; fp16 q stays as it is.
 template <typename E, int NS, int NG>
 __device__ __forceinline__ int scale_q(u32x4* qb, float* us) {
+  constexpr bool kScaled = E::kOnes == BF16::kOnes;
   int qs = 0;
-  if constexpr (E::kOnes == BF16::kOnes) {
+  if constexpr (kScaled) {
     float amax = 0.0f;
 #pragma unroll
     for (int s = 0; s < NS; ++s)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float2_t f = unpack2<E>(qb[s][i]);
-        amax = fmaxf(amax, fmaxf(__builtin_fabsf(f[0]), __builtin_fabsf(f[1])));
+        amax = max3(amax, __builtin_fabsf(f[0]), __builtin_fabsf(f[1]));
       }
     amax = max_xor32(max_xor16(amax));
     qs = 13 - max(-100, min(127, (int)(f2u(amax) >> 23) - 127));  // amax < 2^(14 - qs)
-    const float by = pow2i(qs);
-#pragma unroll
-    for (int s = 0; s < NS; ++s)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2_t f = unpack2<E>(qb[s][i]);
-        qb[s][i] = pack2<F16>(f[0] * by, f[1] * by);
-      }
   }
+  const float by = pow2i(qs);
 #pragma unroll
   for (int g = 0; g < NG; ++g) us[g] = 0.0f;
 #pragma unroll
   for (int s = 0; s < NS; ++s)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2_t h = unpack2<F16>(qb[s][i]);
-      us[s * NG / NS] += h[0] + h[1];
+      const float2_t f = unpack2<E>(qb[s][i]);
+      us[s * NG / NS] += f[0] + f[1];
+      if constexpr (kScaled) qb[s][i] = pack2<F16>(f[0] * by, f[1] * by);
     }
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
-    us[g] = add_xor32(add_xor16(us[g]));
+    us[g] = add_xor32(add_xor16(us[g])) * by;
     if (!(__builtin_fabsf(us[g]) < __builtin_inff())) us[g] = __builtin_nanf("");  // a row with an infinity: no score
   }
   return qs;
@@ -505,13 +501,13 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(kSplitO
 #pragma unroll
       for (int r = 0; r < 4; ++r) v[r] = __builtin_fmaf(x[r], f, v[r]);
     }
-    const float ls = ml[1][j];
+    const float ls = ml[1][j], over = ls != 0.0f ? 1.0f / ls : 0.0f;
     if (sl.ranges == 1) {
       const int g = tile * kRows + j;
       T* dst = (T*)a.out + (int64_t)(sp.s.row0 + g / a.gq) * a.ldo + (int64_t)(kvh * a.gq + g % a.gq) * HD + d;
       T4 y;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) y[r] = (T)(ls != 0.0f ? v[r] / ls : 0.0f);
+      for (int r = 0; r < 4; ++r) y[r] = (T)(v[r] * over);
       *reinterpret_cast<T4*>(dst) = y;
     } else {
       *reinterpret_cast<float4_t*>(part + 2 * kRows + j * HD + d) = v;
@@ -527,13 +523,18 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(kSplitO
 //
 // As paged_attention.hip's: CG x KG waves take 32 CG rows of one kv head, wave (kg, cg) 32 rows (two column tiles) over the
 // chunks kg, kg + KG, ... of the block's range. The waves of a K group unpack each chunk once for all of its
-// rows, a step ahead of its use: each wave its part of the codes, into whole tiles of c - 8 in one of two LDS slots, and of
-// the steps and offsets, as fp32. What a wave unpacks it has loaded two steps before. One barrier per chunk: behind it
-// the chunk's slot is written, and the other slot, whose readers are done, is free for the next one.
+// rows, ahead of its use: each wave its part of the codes, into whole tiles of c - 8 in an LDS slot, and of the steps and
+// offsets, as fp32. What a wave unpacks it has loaded two steps before. One barrier per chunk. With one K group (128 rows)
+// there are three slots and a chunk's scores are formed a step ahead: their products run beside the exponentials of
+// the chunk before. (Not with four groups of dims, whose products 256 registers do not hold beside the rest.)
+template <int BT, int NG>
+constexpr bool kAhead4 = kBlockKG<BT> == 1 && NG < 4;
 
-// LDS bytes: of a K group two slots of tiles, steps and offsets; the K groups' m and l per column tile and lane.
-constexpr int slot4_bytes(int hd, int ng) { return hd / 8 * 1024 + 512 * ng; }
-constexpr int block4_lds(int hd, int ng, int cg, int kg) { return kg * 2 * slot4_bytes(hd, ng) + (kg > 1 ? cg * kg * 4 * 64 * 4 : 0); }
+// LDS bytes: of a slot its tiles, steps and offsets (as much as the K group's threads write); of a K group its slots; the
+// K groups' m and l per column tile and lane.
+constexpr int param4_words(int ng, int cg) { return (64 * ng + cg * 64 - 1) / (cg * 64); }  // per thread
+constexpr int slot4_bytes(int hd, int ng, int cg) { return hd / 8 * 1024 + param4_words(ng, cg) * cg * 64 * 8; }
+constexpr int block4_lds(int hd, int ng, int cg, int kg, int s) { return kg * s * slot4_bytes(hd, ng, cg) + (kg > 1 ? cg * kg * 4 * 64 * 4 : 0); }
 
 template <typename E, int HD, int NG, int BT>
 __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_eu(2))) void paged_block4_kernel(PagedArgs a) {
@@ -543,10 +544,11 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
   constexpr int CG = BT / 32, KG = kBlockKG<BT>, NS = HD / 32, NB = HD / 16, NP = HD / 64;
   constexpr int NU = 4 / CG;                                  // of a chunk's four quarters of codes, a wave's
   constexpr int NT = 2 * NP;                                  // tiles of a quarter
-  constexpr int PW = (64 * NG + CG * 64 - 1) / (CG * 64);     // words of steps and offsets per thread
-  constexpr int kSlot = slot4_bytes(HD, NG);
-  static_assert(KG == 1 || KG * 2 * kSlot >= (KG - 1) * CG * 2 * NB * 64 * 16, "the K groups meet in the slots");
-  __shared__ __align__(16) unsigned char lds[block4_lds(HD, NG, CG, KG)];
+  constexpr int PW = param4_words(NG, CG);                    // words of steps and offsets per thread
+  constexpr bool AHEAD = kAhead4<BT, NG>;
+  constexpr int S = AHEAD ? 3 : 2, kSlot = slot4_bytes(HD, NG, CG);
+  static_assert(KG == 1 || KG * S * kSlot >= (KG - 1) * CG * 2 * NB * 64 * 16, "the K groups meet in the slots");
+  __shared__ __align__(16) unsigned char lds[block4_lds(HD, NG, CG, KG, S)];
   const int tid = threadIdx.x, lane = tid & 63, wg = (int)blockIdx.x, split = (int)blockIdx.y;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kg = wave / CG, cg = wave % CG;
@@ -612,11 +614,14 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
     u32x4 codes[NU];
     uint32_t params[PW];
   };
+  Raw raw1;
   const int gt = cg * 64 + lane;  // of the K group's threads
   // A chunk's bytes that this thread unpacks; no page (an id outside the pool, a step past the range): zeros
+  const char* const pool = (const char*)a.k + (int64_t)kvh * a.cpp.n * L::kBytes;
+  const uint32_t pstride = (uint32_t)a.kps * 2;  // bytes: below 2^32
   auto load = [&](int j) __attribute__((always_inline)) {
-    const bool ok = j * KG + kg < nsteps && (uint32_t)page < (uint32_t)a.pages;
-    const auto rs = buffer_rsrc((const T*)a.k + (ok ? page * a.kps : 0) + ((int64_t)kvh * a.cpp.n + (ok ? sub : 0)) * L::kWords, ok ? L::kBytes : 0);
+    const bool ok = (j * KG + kg < nsteps) & ((uint32_t)page < (uint32_t)a.pages);
+    const auto rs = buffer_rsrc(pool + (uint64_t)(ok ? (uint32_t)page : 0u) * pstride + (uint32_t)sub * (uint32_t)L::kBytes, ok ? L::kBytes : 0);
     Raw r;
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
@@ -638,10 +643,11 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
     next_page(j + 1);
     return r;
   };
-  unsigned char* const slots = lds + kg * 2 * kSlot;
+  unsigned char* const slots = lds + kg * S * kSlot;
+  auto slot_of = [&](int j) __attribute__((always_inline)) { return slots + (S == 2 ? j & 1 : j % 3) * kSlot; };
   const Unpack unpacked;
   auto unpack = [&](const Raw& r, int j) __attribute__((always_inline)) {
-    unsigned char* const to = slots + (j & 1) * kSlot;
+    unsigned char* const to = slot_of(j);
 #pragma unroll
     for (int i = 0; i < NU; ++i)
 #pragma unroll
@@ -661,17 +667,22 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
       const int pos = (w >> 3 & 3) * 8 + (w & 3) * 2, kind = (w >> 2 & 1) + (w >= 32 * NG ? 2 : 0), g = w / 32 % NG;
       float2_t f = unpack2<E>(r.params[i]);
       const int p0 = cb + pos;
-      if (!(p0 <= bk.last && (p0 >= any_lo || p0 < a.sinks))) f[0] = 0.0f;
-      if (!(p0 + 1 <= bk.last && (p0 + 1 >= any_lo || p0 + 1 < a.sinks))) f[1] = 0.0f;
-      if (w < 64 * NG) *reinterpret_cast<float2_t*>(par + (kind * NG + g) * 32 + pos) = f;
+      f[0] = (p0 <= bk.last) & ((p0 >= any_lo) | (p0 < a.sinks)) ? f[0] : 0.0f;
+      f[1] = (p0 + 1 <= bk.last) & ((p0 + 1 >= any_lo) | (p0 + 1 < a.sinks)) ? f[1] : 0.0f;
+      // (threads past the last word write behind them)
+      *reinterpret_cast<float2_t*>(par + (w < 64 * NG ? (kind * NG + g) * 32 + pos : 2 * w)) = f;
     }
   };
+  constexpr int D = AHEAD ? 2 : 1;  // steps ahead that are unpacked
   next_page(0);
   {
-    const Raw r0 = load(0);
+    const Raw r0 = load(0), r1 = load(1);
     unpack(r0, 0);
+    if (AHEAD) unpack(r1, 1);
+    if (!AHEAD) raw1 = r1;
   }
-  Raw r1 = load(1), r2 = load(2);
+  if (AHEAD) raw1 = load(2);
+  Raw raw2 = load(D + 1);
 
   // this wave's q operands
   u32x4 q[2][NS];
@@ -700,140 +711,156 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
     for (int b = 0; b < NB; ++b) o[ct][b] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
+  auto param = [&](const unsigned char* slot, int kind, int g, float* f) __attribute__((always_inline)) {
+    const float* const par = reinterpret_cast<const float*>(slot + HD / 8 * 1024) + (kind * NG + g) * 32 + 8 * kb;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float4_t v = *reinterpret_cast<const float4_t*>(par + 4 * i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[4 * i + e] = v[e];
+    }
+  };
+  float4_t acc[AHEAD ? NG : 1][2][2];  // [half][column tile]: a chunk's products by group of dims
+  float sv[2][8];                      // its scores less the row's maximum, then its weights
+  auto products = [&](const unsigned char* from, int g, float4_t (&x)[2][2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = g * NS / NG; s < (g + 1) * NS / NG; ++s)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const u32x4 k = *reinterpret_cast<const u32x4*>(from + (h * NS + s) * 1024 + lane * 16);
+#pragma unroll
+        for (int ct = 0; ct < 2; ++ct) {
+          const float4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
+          x[h][ct] = F16::mfma(k, q[ct][s], s % (NS / NG) ? x[h][ct] : zero);
+        }
+      }
+  };
+  auto fold = [&](const unsigned char* from, int g, const float4_t (&x)[2][2]) __attribute__((always_inline)) {
+    float st[8], z[8];
+    param(from, 0, g, st);
+    param(from, 1, g, z);
+#pragma unroll
+    for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        sv[ct][e] = __builtin_fmaf(st[e], x[e >> 2][ct][e & 3], __builtin_fmaf(z[e], us[ct][g], g ? sv[ct][e] : less[ct]));
+  };
+  auto products_ahead = [&](int j) __attribute__((always_inline)) {
+    if constexpr (AHEAD)
+#pragma unroll
+      for (int g = 0; g < NG; ++g) products(slot_of(j), g, acc[g]);
+  };
+  auto fold_ahead = [&](int j) __attribute__((always_inline)) {
+    if constexpr (AHEAD)
+#pragma unroll
+      for (int g = 0; g < NG; ++g) fold(slot_of(j), g, acc[g]);
+  };
   auto step = [&](auto maskedc, int j) __attribute__((always_inline)) {
     constexpr bool kMasked = decltype(maskedc)::value;
     lds_barrier();
-    const unsigned char* const from = slots + (j & 1) * kSlot;
-    const float* const par = reinterpret_cast<const float*>(from + HD / 8 * 1024);
+    const unsigned char* const from = slot_of(j);
     const int cb = chunk_of(j) * kChunkPos;
-    const bool live = !kMasked || ((have >> 2 & 1) && cb <= whi && (cb + kChunkPos > wlo || cb < a.sinks));
-    float sv[2][8];
-    auto params = [&](int kind, int g, float* f) __attribute__((always_inline)) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float4_t v = *reinterpret_cast<const float4_t*>(par + (kind * NG + g) * 32 + 8 * kb + 4 * i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f[4 * i + e] = v[e];
-      }
-    };
-    if (live) {
+    const bool there = !kMasked || (have >> (D + 1) & 1);
+    if constexpr (!AHEAD) {
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        float4_t acc[2][2];
-#pragma unroll
-        for (int s = g * NS / NG; s < (g + 1) * NS / NG; ++s)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const u32x4 k = *reinterpret_cast<const u32x4*>(from + (h * NS + s) * 1024 + lane * 16);
-#pragma unroll
-            for (int ct = 0; ct < 2; ++ct) {
-              const float4_t zero = {0.0f, 0.0f, 0.0f, 0.0f};
-              acc[h][ct] = F16::mfma(k, q[ct][s], s % (NS / NG) ? acc[h][ct] : zero);
-            }
-          }
-        float st[8], z[8];
-        params(0, g, st);
-        params(1, g, z);
-#pragma unroll
-        for (int ct = 0; ct < 2; ++ct)
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            sv[ct][e] = __builtin_fmaf(st[e], acc[e >> 2][ct][e & 3], __builtin_fmaf(z[e], us[ct][g], g ? sv[ct][e] : less[ct]));
-        if constexpr (NG == 4) __builtin_amdgcn_sched_barrier(0);  // one group's reads at a time: 256 registers hold no more
+        products(from, g, acc[0]);
+        fold(from, g, acc[0]);
+        if constexpr (NG == 4) __builtin_amdgcn_sched_barrier(0);  // one group at a time: 256 registers hold no more
       }
     }
-    unpack(r1, j + 1);
-    r1 = r2;
-    r2 = load(j + 3);
-    if (live) {
-      float sm = 0.0f;
+    float sm = 0.0f;
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        float st[8];
-        params(2, g, st);
+    for (int g = 0; g < NG; ++g) {
+      float st[8];
+      param(from, 2, g, st);
+      sm = max3(max3(max3(sm, st[0], st[1]), st[2], st[3]), max3(st[4], st[5], st[6]), st[7]);
+    }
+    bool more_any = sm >= pow2i(ve + 1);
+    bool seen[2][8];
+    float mc[2];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sm = fmaxf(sm, st[e]);
+    for (int ct = 0; ct < 2; ++ct) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (kMasked) {
+          const int p = cb + 8 * kb + e;
+          seen[ct][e] = there && p <= hi[ct] && (p > hi[ct] - window || p < a.sinks);
+          sv[ct][e] = seen[ct][e] ? sv[ct][e] : -__builtin_inff();
+        }
       }
-      if constexpr (NG == 4) asm volatile("" : : : "memory");  // read again below rather than kept
-      bool more_any = sm >= pow2i(ve + 1);
-      bool seen[2][8];
+      mc[ct] = max3(max3(max3(sv[ct][0], sv[ct][1], sv[ct][2]), sv[ct][3], sv[ct][4]), max3(sv[ct][5], sv[ct][6], sv[ct][7]), sv[ct][7]);
+      more_any = more_any | (mc[ct] > limit[ct]);
+    }
+    if (__any(more_any)) {
+      sm = max_xor32(max_xor16(sm));
+      const int vn = min(126, max(ve, (int)(f2u(sm) >> 23) - 127));
+      const float by = pow2i(max(ve - vn, -126));
+      ve = vn;
 #pragma unroll
       for (int ct = 0; ct < 2; ++ct) {
-        float mc = -__builtin_inff();
+        const float mx = max_xor32(max_xor16(mc[ct]));
+        const float old = less[ct], m_new = fmaxf(m_run[ct], mx - old);
+        const float now = m_new == -__builtin_inff() ? 0.0f : -m_new, more = old - now;
+        const float al = (m_run[ct] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(-more * f1[ct])) * by;
+        l[ct] *= al;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if constexpr (kMasked) {
-            const int p = cb + 8 * kb + e;
-            seen[ct][e] = p <= hi[ct] && (p > hi[ct] - window || p < a.sinks);
-            sv[ct][e] = seen[ct][e] ? sv[ct][e] : -__builtin_inff();
-          }
-          mc = fmaxf(mc, sv[ct][e]);
-        }
-        more_any = more_any || mc > limit[ct];
-      }
-      if (__any(more_any)) {
-        sm = max_xor32(max_xor16(sm));
-        const int vn = min(126, max(ve, (int)(f2u(sm) >> 23) - 127));
-        const float by = pow2i(max(ve - vn, -126));
-        ve = vn;
+        for (int g = 0; g < NG; ++g) ms[ct][g] *= al;
 #pragma unroll
-        for (int ct = 0; ct < 2; ++ct) {
-          float mc = sv[ct][0];
+        for (int b = 0; b < NB; ++b) o[ct][b] *= al;
 #pragma unroll
-          for (int e = 1; e < 8; ++e) mc = fmaxf(mc, sv[ct][e]);
-          mc = max_xor32(max_xor16(mc));
-          const float old = less[ct], m_new = fmaxf(m_run[ct], mc - old);
-          const float now = m_new == -__builtin_inff() ? 0.0f : -m_new, more = old - now;
-          const float al = (m_run[ct] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(-more * f1[ct])) * by;
-          l[ct] *= al;
-#pragma unroll
-          for (int g = 0; g < NG; ++g) ms[ct][g] *= al;
-#pragma unroll
-          for (int b = 0; b < NB; ++b) o[ct][b] *= al;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) sv[ct][e] -= more;
-          m_run[ct] = m_new;
-          less[ct] = now;
-          limit[ct] = m_new == -__builtin_inff() ? m_new : kLag4 / f1[ct];
-        }
-      }
-      const float unit = (float)(kUnit4 - ve);
-#pragma unroll
-      for (int ct = 0; ct < 2; ++ct)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          sv[ct][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[ct][e], f1[ct], unit));
-          l[ct] += sv[ct][e];
-        }
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        float st[8], z[8];
-        params(2, g, st);
-        params(3, g, z);
-        u32x4 pw[2];
-#pragma unroll
-        for (int ct = 0; ct < 2; ++ct) {
-          float x[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            // what this row does not see and another does may be NaN
-            const bool on = !kMasked || seen[ct][e];
-            ms[ct][g] = __builtin_fmaf(sv[ct][e], on ? z[e] : 0.0f, ms[ct][g]);
-            x[e] = sv[ct][e] * (on ? st[e] : 0.0f);
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) pw[ct][e] = pack2<F16>(x[2 * e], x[2 * e + 1]);
-        }
-#pragma unroll
-        for (int b = g * NB / NG; b < (g + 1) * NB / NG; ++b) {
-          const u32x4 v = *reinterpret_cast<const u32x4*>(from + (2 * NS + b) * 1024 + lane * 16);
-#pragma unroll
-          for (int ct = 0; ct < 2; ++ct) o[ct][b] = F16::mfma(v, pw[ct], o[ct][b]);
-        }
-        if constexpr (NG == 4) __builtin_amdgcn_sched_barrier(0);
+        for (int e = 0; e < 8; ++e) sv[ct][e] -= more;
+        m_run[ct] = m_new;
+        less[ct] = now;
+        limit[ct] = m_new == -__builtin_inff() ? m_new : kLag4 / f1[ct];
       }
     }
+    products_ahead(j + 1);
+    const float unit = (float)(kUnit4 - ve);
+#pragma unroll
+    for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        sv[ct][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[ct][e], f1[ct], unit));
+        l[ct] += sv[ct][e];
+      }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      float st[8], z[8];
+      param(from, 2, g, st);
+      param(from, 3, g, z);
+      u32x4 pw[2];
+#pragma unroll
+      for (int ct = 0; ct < 2; ++ct) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          // what this row does not see and another does may be NaN
+          const bool on = !kMasked || seen[ct][e];
+          ms[ct][g] = __builtin_fmaf(sv[ct][e], on ? z[e] : 0.0f, ms[ct][g]);
+          x[e] = sv[ct][e] * (on ? st[e] : 0.0f);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pw[ct][e] = pack2<F16>(x[2 * e], x[2 * e + 1]);
+      }
+#pragma unroll
+      for (int b = g * NB / NG; b < (g + 1) * NB / NG; ++b) {
+        const u32x4 v = *reinterpret_cast<const u32x4*>(from + (2 * NS + b) * 1024 + lane * 16);
+#pragma unroll
+        for (int ct = 0; ct < 2; ++ct) o[ct][b] = F16::mfma(v, pw[ct], o[ct][b]);
+      }
+      if constexpr (NG == 4) __builtin_amdgcn_sched_barrier(0);
+    }
+    unpack(raw1, j + D);
+    raw1 = raw2;
+    raw2 = load(j + D + 2);
+    fold_ahead(j + 1);
   };
+  if (AHEAD) {
+    lds_barrier();
+    products_ahead(0);
+    fold_ahead(0);
+  }
   int j = 0;
   for (; j < nfull; ++j) step(IntC<0>(), j);
   for (; j < n; ++j) step(IntC<1>(), j);
@@ -852,7 +879,7 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
       for (int r = 0; r < 4; ++r) o[ct][b][r] = (o[ct][b][r] + ms[ct][b * NG / NB]) * one;
   }
   float4_t* const red = reinterpret_cast<float4_t*>(lds);  // [wave - CG][2 NB][64]
-  float(*const mls)[4][64] = reinterpret_cast<float(*)[4][64]>(lds + KG * 2 * kSlot);
+  float(*const mls)[4][64] = reinterpret_cast<float(*)[4][64]>(lds + KG * S * kSlot);
   if constexpr (KG > 1) {
     lds_barrier();  // the slots have been read
     if (kg > 0) {
@@ -884,6 +911,7 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
       f[g] = mv[g] != -__builtin_inff() ? __builtin_amdgcn_exp2f((mv[g] - M) * sc) : 0.0f;
       ls = __builtin_fmaf(g ? mls[cg + g * CG][2 * ct + 1][lane] : l[ct], f[g], ls);
     }
+    const float over = ls != 0.0f ? 1.0f / ls : 0.0f;
     const int col = 32 * cg + 16 * ct + c16;
     int t, h;
     row_of(ct, lane, t, h);
@@ -902,7 +930,7 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
         if (direct) {
           T4 y;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) y[r] = (T)(ls != 0.0f ? v[r] / ls : 0.0f);
+          for (int r = 0; r < 4; ++r) y[r] = (T)(v[r] * over);
           *reinterpret_cast<T4*>(dst + 16 * b) = y;
         } else {
           *reinterpret_cast<float4_t*>(pdst + 16 * b) = v;

@@ -148,10 +148,10 @@ def attention64(q, kq, vq, scale, positions, window=0, sinks=0, present=None):
             ds = scale * (x.abs() @ (2 * kz + 31 * ks).T * (hd + 16) * 2.0 ** -24 + x.abs().max(1).values[:, None] * (kz + 8 * ks).sum(1) * 2.0 ** -34)
             ds = torch.where(seen, ds, 0.0)
             dw = ds + ds.max(1).values[:, None] + torch.where(seen, m - s + 4, 0.0) * 2.0 ** -22
-            # a weight times its step: half a step of fp16, or 2^-36 of the largest step; fp32 products and sums of the uncentred codes
+            # a weight times its step: half a step of fp16, or 2^-33 of the largest step; fp32 products and sums of the uncentred codes
             vsz, vzz, ofz = (torch.where(seen.any(0)[:, None], t, 0.0) for t in (vs, vz, off))
             e = (w * dw) @ torch.where(seen.any(0)[:, None], v.abs(), 0.0) + (w * dw).sum(1)[:, None] * o.abs()
-            e = e + w @ (vsz * ofz) * 2.0 ** -12 * 1.01 + 8 * 2.0 ** -36 * vsz.max() * seen.sum(1)[:, None] / tot
+            e = e + w @ (vsz * ofz) * 2.0 ** -12 * 1.01 + 8 * 2.0 ** -33 * vsz.max() * seen.sum(1)[:, None] / tot
             e = e + w @ (23 * vsz + vzz) * (seen.sum(1)[:, None] + 64) * 2.0 ** -24
             e = e + half * o.abs() * 1.01 + (2.0 ** -25 if q.dtype == torch.float16 else 0.0)
             out[:, i], bound[:, i] = torch.where(some[:, None], o, 0.0), e
