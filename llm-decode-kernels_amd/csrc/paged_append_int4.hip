@@ -171,7 +171,8 @@ __global__ __launch_bounds__(kTokThreads) void append4_token_kernel(Append4Args 
   typedef Int4Block<HD, NG> L;
   constexpr int LH = HD / 16;  // lanes per q or k head
   constexpr int LV = HD / 8;   // lanes per v head
-  __shared__ __align__(16) double cs[2][HD / 2];
+  __shared__ __align__(16) double cs[2][HD / 2];  // k's
+  __shared__ __align__(16) float cq[2][HD / 2];   // q's, by another wave at the same time
   const int t = blockIdx.x, tid = threadIdx.x, i = tid + (int)blockIdx.y * kTokThreads;
   const int pairs = (a.nq + a.nkv) * LH, j = i - (pairs + 63) / 64 * 64;
   const bool rot = i < pairs, val = j >= 0 && j < a.nkv * LV;
@@ -188,7 +189,11 @@ __global__ __launch_bounds__(kTokThreads) void append4_token_kernel(Append4Args 
   int64_t page = -1;
   if (p >= 0 && p < a.cap) page = a.table[(int64_t)t * a.ldt + p / (kChunkPos * a.cpp)];
   if (a.inv_freq) {  // uniform
-    if (tid < HD / 2) angle64(a.rope_pos ? a.rope_pos[t] : (int64_t)p, a.inv_freq[tid], &cs[0][tid], &cs[1][tid]);
+    const int64_t at = a.rope_pos ? a.rope_pos[t] : (int64_t)p;
+    if (tid < HD / 2)
+      angle64(at, a.inv_freq[tid], &cs[0][tid], &cs[1][tid]);
+    else if (tid >= 64 && tid < 64 + HD / 2)
+      angle(at, a.inv_freq[tid - 64], &cq[0][tid - 64], &cq[1][tid - 64]);
     __syncthreads();
   }
   const bool wr = page >= 0 && page < a.pages;
@@ -196,12 +201,7 @@ __global__ __launch_bounds__(kTokThreads) void append4_token_kernel(Append4Args 
   // block of kv head g: where wr
   auto block = [&](int g) { return (unsigned char*)a.pool + (page * a.stride + ((int64_t)g * a.cpp + c) * L::kWords) * 2; };
   if (rot && h < a.nq) {
-    if (a.inv_freq) {
-      float cf[8], sf[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) cf[e] = (float)cs[0][d + e], sf[e] = (float)cs[1][d + e];
-      rotate8<E>(x0, x1, cf, sf);
-    }
+    if (a.inv_freq) rotate8<E>(x0, x1, &cq[0][d], &cq[1][d]);
     T* q = (T*)a.q + (int64_t)t * a.ldq + (int64_t)h * HD;
     *reinterpret_cast<u32x4*>(q + d) = x0;
     *reinterpret_cast<u32x4*>(q + HD / 2 + d) = x1;
@@ -223,13 +223,15 @@ constexpr int kChunkThreads = 256;
 
 // Workgroup x: of the sequences' chunks, sequence b's begin at index cu[b] / 32 + 2b (at most
 // (n + 62) / 32 chunks hold its n new tokens, which is at most floor((cu + n) / 32) - floor(cu / 32)
-// + 2). Each workgroup finds its sequence with a binary search.
+// + 2). Each workgroup finds its sequence with a binary search. The workgroups y of a chunk share the heads, k's first and q's
+// last: what takes longest starts first. A thread has one position and 8 dims of every q and k head that
+// it meets, so its 8 angles stay in registers.
 template <typename E, int HD, int NG>
 __global__ __launch_bounds__(kChunkThreads) void append4_chunk_kernel(Append4Args a) {
   typedef typename E::T T;
   typedef Int4Block<HD, NG> L;
   constexpr int LH = HD / 16, LV = HD / 8;
-  __shared__ __align__(16) double cs[2][kChunkPos][HD / 2];
+  constexpr int HP = kChunkThreads / (kChunkPos * LH);  // q or k heads at once
   __shared__ __align__(16) unsigned char vs[16 * HD];  // a head's codes of v
   const int tid = threadIdx.x, x = blockIdx.x;
   int b = 0;
@@ -255,67 +257,92 @@ __global__ __launch_bounds__(kChunkThreads) void append4_chunk_kernel(Append4Arg
   if (c0 >= 0 && base < a.cap) page = a.table[(int64_t)b * a.ldt + c0 / a.cpp];
   const bool wr = page >= 0 && page < a.pages;
   const int c = c0 >= 0 ? c0 % a.cpp : 0;
-  if (a.inv_freq) {
-    for (int i = tid; i < kChunkPos * (HD / 2); i += kChunkThreads) {
-      const int r = i / (HD / 2), j = i % (HD / 2);
-      if (r >= first && r < last)
-        angle64(a.rope_pos ? a.rope_pos[t0 + r] : base + r, a.inv_freq[j], &cs[0][r][j], &cs[1][r][j]);
-    }
-  }
-  __syncthreads();
   const T* rows = (const T*)a.qkv;
   auto block = [&](int g) { return (unsigned char*)a.pool + (page * a.stride + ((int64_t)g * a.cpp + c) * L::kWords) * 2; };
-  for (int h = (int)blockIdx.y; h < a.nq + 2 * a.nkv; h += (int)gridDim.y) {
-    if (h >= a.nq && !wr) continue;
-    if (h < a.nq + a.nkv) {
-      for (int i = tid; i < kChunkPos * LH; i += kChunkThreads) {
-        const int r = i / LH, d = i % LH * 8;
-        if (r < first || r >= last) continue;
-        const T* src = rows + (int64_t)(t0 + r) * a.ldqkv + (int64_t)h * HD;
-        u32x4 x0 = *reinterpret_cast<const u32x4*>(src + d), x1 = *reinterpret_cast<const u32x4*>(src + HD / 2 + d);
-        if (h < a.nq) {
-          if (a.inv_freq) {
-            float cf[8], sf[8];
+  const int heads = a.nq + 2 * a.nkv, y = blockIdx.y;
+  const int h0 = y * heads / (int)gridDim.y, h1 = (y + 1) * heads / (int)gridDim.y;  // of k's, then v's, then q's heads
+  // ---- k and q: this thread's position, dims and first head
+  const int d = tid % LH * 8, r = tid / LH % kChunkPos, hp = tid / (kChunkPos * LH);
+  const bool mine = r >= first && r < last;
+  const int64_t row = mine ? t0 + r : 0, at = !mine ? 0 : a.rope_pos ? a.rope_pos[row] : base + r;
+  const int ke = wr ? min(h1, a.nkv) : 0;
+  if (h0 + hp < ke && mine) {
+    const T* src = rows + row * a.ldqkv + (int64_t)(a.nq + h0 + hp) * HD + d;
+    u32x4 x0 = *reinterpret_cast<const u32x4*>(src), x1 = *reinterpret_cast<const u32x4*>(src + HD / 2);
+    double ck[8], sk[8];
+    if (a.inv_freq) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) cf[e] = (float)cs[0][r][d + e], sf[e] = (float)cs[1][r][d + e];
-            rotate8<E>(x0, x1, cf, sf);
-          }
-          T* q = (T*)a.q + (int64_t)(t0 + r) * a.ldq + (int64_t)h * HD;
-          *reinterpret_cast<u32x4*>(q + d) = x0;
-          *reinterpret_cast<u32x4*>(q + HD / 2 + d) = x1;
-        } else {
-          float y0[8], y1[8];
-          if (a.inv_freq)
-            turn8<E>(x0, x1, &cs[0][r][d], &cs[1][r][d], y0, y1);
-          else
-            values8<E>(x0, y0), values8<E>(x1, y1);
-          store_k<E, HD, NG>(block(h - a.nq), r, d / 8, y0, y1);
+      for (int e = 0; e < 8; ++e) angle64(at, a.inv_freq[d + e], &ck[e], &sk[e]);
+    }
+    for (int h = h0 + hp; h < ke; h += HP) {
+      float y0[8], y1[8];
+      if (a.inv_freq)
+        turn8<E>(x0, x1, ck, sk, y0, y1);
+      else
+        values8<E>(x0, y0), values8<E>(x1, y1);
+      if (h + HP < ke) {  // the next head's are on their way meanwhile
+        src += HP * HD;
+        x0 = *reinterpret_cast<const u32x4*>(src), x1 = *reinterpret_cast<const u32x4*>(src + HD / 2);
+      }
+      store_k<E, HD, NG>(block(h), r, d / 8, y0, y1);
+    }
+  }
+  // ---- v
+  constexpr int VI = kChunkPos * LV / kChunkThreads;  // items of a thread
+  auto load_v = [&](int h, u32x4* xv) {
+#pragma unroll
+    for (int n = 0; n < VI; ++n) {
+      const int r = (tid + n * kChunkThreads) / LV, d = tid % LV * 8;
+      if (r >= first && r < last)
+        xv[n] = *reinterpret_cast<const u32x4*>(rows + (int64_t)(t0 + r) * a.ldqkv + (int64_t)(a.nq + a.nkv + h) * HD + d);
+    }
+  };
+  const int v0 = max(h0 - a.nkv, 0), ve = wr ? min(h1 - a.nkv, a.nkv) : 0;
+  u32x4 xv[VI];
+  if (v0 < ve) load_v(v0, xv);
+  for (int h = v0; h < ve; ++h) {
+    unsigned char* const blk = block(h);
+    float y[VI][8];
+#pragma unroll
+    for (int n = 0; n < VI; ++n) values8<E>(xv[n], y[n]);
+    if (h + 1 < ve) load_v(h + 1, xv);
+    __syncthreads();  // the v head before has been copied
+#pragma unroll
+    for (int n = 0; n < VI; ++n) {
+      const int r = (tid + n * kChunkThreads) / LV;
+      if (r >= first && r < last) store_v<E, HD, NG>(vs, blk, r, tid % LV, y[n]);
+    }
+    __syncthreads();
+    // item u: the 16 bytes of positions 8 (u / 16 % 4) .. + 7
+    for (int u = tid; u < HD; u += kChunkThreads) {
+      const int r0 = 8 * (u / 16 % 4);
+      if (r0 >= first && r0 + 8 <= last) {
+        *reinterpret_cast<u32x4*>(blk + L::kV + u * 16) = *reinterpret_cast<const u32x4*>(vs + u * 16);
+      } else {
+        for (int r = max(r0, first); r < min(r0 + 8, last); ++r) {
+          const int at = u * 16 + ((r >> 2) & 1) * 4 + int4_byte(r & 3);
+          blk[L::kV + at] = vs[at];
+          blk[L::kV + at + 8] = vs[at + 8];
         }
       }
-    } else {
-      unsigned char* const blk = block(h - a.nq - a.nkv);
-      __syncthreads();  // the v head before has been copied
-      for (int i = tid; i < kChunkPos * LV; i += kChunkThreads) {
-        const int r = i / LV, d = i % LV * 8;
-        if (r < first || r >= last) continue;
-        float y[8];
-        values8<E>(*reinterpret_cast<const u32x4*>(rows + (int64_t)(t0 + r) * a.ldqkv + (int64_t)h * HD + d), y);
-        store_v<E, HD, NG>(vs, blk, r, d / 8, y);
-      }
-      __syncthreads();
-      // item u: the 16 bytes of positions 8 (u / 16 % 4) .. + 7
-      for (int u = tid; u < HD; u += kChunkThreads) {
-        const int r0 = 8 * (u / 16 % 4);
-        if (r0 >= first && r0 + 8 <= last) {
-          *reinterpret_cast<u32x4*>(blk + L::kV + u * 16) = *reinterpret_cast<const u32x4*>(vs + u * 16);
-        } else {
-          for (int r = max(r0, first); r < min(r0 + 8, last); ++r) {
-            const int at = u * 16 + ((r >> 2) & 1) * 4 + int4_byte(r & 3);
-            blk[L::kV + at] = vs[at];
-            blk[L::kV + at + 8] = vs[at + 8];
-          }
-        }
-      }
+    }
+  }
+  // ---- q
+  const int hq = max(h0 - 2 * a.nkv, 0) + hp, qe = h1 - 2 * a.nkv;
+  if (hq - hp < qe && mine) {
+    float cq[8], sq[8];
+    if (a.inv_freq) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) angle(at, a.inv_freq[d + e], &cq[e], &sq[e]);
+    }
+#pragma unroll 2
+    for (int h = hq; h < qe; h += HP) {
+      const T* src = rows + row * a.ldqkv + (int64_t)h * HD + d;
+      u32x4 x0 = *reinterpret_cast<const u32x4*>(src), x1 = *reinterpret_cast<const u32x4*>(src + HD / 2);
+      if (a.inv_freq) rotate8<E>(x0, x1, cq, sq);
+      T* q = (T*)a.q + row * a.ldq + (int64_t)h * HD + d;
+      *reinterpret_cast<u32x4*>(q) = x0;
+      *reinterpret_cast<u32x4*>(q + HD / 2) = x1;
     }
   }
 }
@@ -328,7 +355,8 @@ int launch(const Append4Args& a, hipStream_t s) {
     append4_token_kernel<E, HD, NG><<<dim3((unsigned)a.T, (unsigned)((items + kTokThreads - 1) / kTokThreads)), kTokThreads, 0, s>>>(a);
   } else {
     const unsigned gx = (unsigned)(a.T / kChunkPos + 2 * a.B);
-    const int hb = std::min(a.nq + 2 * a.nkv, std::max(1, 1024 / (int)(a.T / kChunkPos + a.B)));
+    // workgroups y: us of 6100 new tokens of 28/4 heads with 1024, 2048 and 4096 workgroups in all 22.3, 21.2, 24.6
+    const int hb = std::min(a.nq + 2 * a.nkv, std::max(1, 2048 / (int)(a.T / kChunkPos + a.B)));
     append4_chunk_kernel<E, HD, NG><<<dim3(gx, (unsigned)hb), kChunkThreads, 0, s>>>(a);
   }
   return ldk::check_launch("paged_append_int4");

@@ -112,6 +112,12 @@ def test_append_ragged(dtype, hd, group, nq, nkv, page, lens, news):
     check_append(lens, news, nq, nkv, hd, group, page, dtype)
 
 
+@pytest.mark.parametrize("hd,group,nq,nkv,B", [(64, 32, 4, 2, 1100), (128, 64, 3, 3, 700), (128, 128, 2, 1, 300), (64, 64, 7, 1, 500)])
+def test_append_many_sequences(hd, group, nq, nkv, B):
+    """So many chunks that a workgroup takes several or all of a token's heads."""
+    check_append([33 + b % 3 for b in range(B)], [b % 3 for b in range(B)], nq, nkv, hd, group, 32, F16)
+
+
 @pytest.mark.parametrize("cu", [False, True])
 def test_append_positions_apart_from_the_cache(cu):
     """rope_pos far away, and beyond 32 bits."""
@@ -285,6 +291,27 @@ def test_attention_one_token(dtype, hd, group, nq, nkv, page, lens):
                                        ([64, 0, 5, 97, 33, 12], [32, 0, 5, 97, 2, 0]), ([400], [3]), ([260, 900], [130, 140])])
 def test_attention_ragged(dtype, hd, group, nq, nkv, page, lens, news):
     check_attention(lens, news, nq, nkv, hd, group, page, dtype)
+
+
+@pytest.mark.parametrize("dtype,hd,group,nq,nkv,page", [
+    (F16, 64, 32, 4, 2, 32), (BF16, 64, 64, 3, 1, 64), (F16, 64, 64, 2, 2, 96), (BF16, 64, 32, 16, 2, 32), (F16, 64, 64, 5, 1, 32),
+    (BF16, 128, 32, 12, 2, 64), (F16, 128, 64, 1, 1, 32), (F16, 128, 128, 8, 1, 32), (BF16, 128, 128, 24, 2, 32)])
+def test_attention_few_query_heads(dtype, hd, group, nq, nkv, page):
+    """Heads and tokens whose rows fill a quarter of a tile, a half, or more, with the numbers of sequences that find their
+    ranges in either way; ranges of one chunk, of a group's and of others between."""
+    for lens in ([700, 32, 31, 65, 7, 2000, 90], [5000], [3, 641, 0, 673], [1281 + 32 * i for i in range(9)]):
+        check_attention(lens, [1] * len(lens), nq, nkv, hd, group, page, dtype, cu=False)
+    check_attention([700, 2000, 90, 4, 1700], [2, 1, 2, 0, 2], nq, nkv, hd, group, page, dtype)
+    check_attention([700, 2000, 90, 33], [2, 1, 2, 2], nq, nkv, hd, group, page, dtype, window=900, sinks=3)
+    check_attention([1 + (97 * i) % 700 for i in range(70)], [1] * 70, nq, nkv, hd, group, page, dtype, cu=False)
+
+
+@pytest.mark.parametrize("dtype,hd,group", [(F16, 128, 128), (BF16, 128, 64), (F16, 128, 32), (BF16, 64, 64), (F16, 64, 32)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (70, 2)])
+def test_attention_blocks_of_whole_sequences(dtype, hd, group, window, sinks):
+    """So many blocks that none is cut along its positions, of 128 rows and of 64."""
+    check_attention([900, 33], [880, 20], 32, 16, hd, group, 32, dtype, window, sinks)
+    check_attention([40 + 11 * i for i in range(10)], [40 - i for i in range(10)], 16, 16, hd, group, 32, dtype, window, sinks)
 
 
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (31, 0), (32, 4), (33, 33), (100, 70), (5000, 9), (64, 1000), (0, 5)])
@@ -562,6 +589,37 @@ def test_on_another_stream():
         again = paged_read_int4(kv, pg.table, pg.pool)
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(want, g) for g in got) and all(torch.equal(a, b) for a, b in zip(back, again))
+
+
+def test_append_and_read_on_another_stream_and_in_a_graph():
+    """Both forms, captured and replayed on a side stream at new lengths, with eager calls between."""
+    nq, nkv, hd, group, page = 6, 2, 128, 32, 32
+    for news in ([1, 1, 1], [40, 1, 70]):
+        T, lens = sum(news), [200, 40, 130]
+        cu = None if max(news) == 1 else i32(rows_of(news))
+        pg = Pages4([250] * 3, nkv, hd, group, page, F16)
+        other = pg.pool.clone()
+        qkv, kv, inv = torch.randn(T, (nq + 2 * nkv) * hd, device="cuda").half(), i32(lens), freqs(hd).cuda()
+
+        def call(pool):
+            q = paged_append_int4(qkv, kv, pg.table, pool, inv, nq, cu_seqlens=cu)
+            return (q,) + tuple(paged_read_int4(kv, pg.table, pool, T, cu_seqlens=cu))
+
+        call(other)
+        torch.cuda.synchronize()
+        graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(graph):
+            outs = call(pg.pool)
+        call(pg.pool)
+        for step in range(4):
+            kv.copy_(i32([n + 13 * step for n in lens]))
+            qkv.copy_(torch.randn(qkv.shape, device="cuda"))
+            want = call(other)
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                graph.replay()
+            torch.cuda.current_stream().wait_stream(side)
+            assert all(same_bits(a, b) for a, b in zip(outs, want)) and same_bits(pg.pool, other), step
 
 
 def test_two_graphs_at_new_lengths():
