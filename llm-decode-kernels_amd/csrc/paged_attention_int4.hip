@@ -954,7 +954,7 @@ Plan make_plan4(int64_t T, int64_t B, int64_t max_q, int64_t max_len, int64_t wi
     p.bt = rows >= 96 * B ? 128 : 64;
     p.btiles = rows / p.bt + B;
     const int64_t fill = p.bt == 64 ? 320 : hd == 128 ? 512 : 768, whole = nkv * p.btiles;
-    p.bsplits = 3 * whole >= fill ? 1 : std::max<int64_t>(1, std::min<int64_t>(32, fill / whole));
+    p.bsplits = (hd == 128 ? 2 : 3) * whole >= fill ? 1 : std::max<int64_t>(1, std::min<int64_t>(32, fill / whole));
     if (p.bsplits > 1) p.bpart_bytes = p.btiles * nkv * p.bsplits * p.bt * (2 + hd) * 4;
     p.bytes = workspace_bytes(p, B);
     return p;
@@ -965,7 +965,10 @@ Plan make_plan4(int64_t T, int64_t B, int64_t max_q, int64_t max_len, int64_t wi
     return p;
   }
   const int64_t w = nkv * p.nt;
-  p.spare = std::max<int64_t>(1, 512 / w);
+  // Whole ranges for two workgroups a CU, and more for the sequences' last, shorter ones, whose number is not known here:
+  // us with 512 / w, this and 512 / w + B / 2: 64 sequences of 28/4 heads 33.8, 32.4, 35.7; 40 of 20/20 heads of 64 43.8,
+  // 42.3, 42.9; half and twice the 512: 37 to 39 and 33 to 38.
+  p.spare = std::max<int64_t>(1, 512 / w + B / 4);
   p.slots = B + p.spare;
   p.mapped = B > kPlanSeqs4;
   p.part_bytes = p.slots * w * part_floats(hd) * 4;
