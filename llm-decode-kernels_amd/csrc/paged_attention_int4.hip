@@ -524,7 +524,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(kSplitO
 // As paged_attention.hip's: CG x KG waves take 32 CG rows of one kv head, wave (kg, cg) 32 rows (two column tiles) over the
 // chunks kg, kg + KG, ... of the block's range. The waves of a K group unpack each chunk once for all of its
 // rows, ahead of its use: each wave its part of the codes, into whole tiles of c - 8 in an LDS slot, and of the steps and
-// offsets, as fp32. What a wave unpacks it has loaded two steps before. One barrier per chunk. With one K group (128 rows)
+// offsets, as fp32. What a wave unpacks it has loaded a step before. One barrier per chunk. With one K group (128 rows)
 // there are three slots and a chunk's scores are formed a step ahead: their products run beside the exponentials of
 // the chunk before. (Not with four groups of dims, whose products 256 registers do not hold beside the rest.)
 template <int BT, int NG>
@@ -599,30 +599,33 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
     d = i < nf + bk.cs ? -nf : d;
     return i + (i < nf ? fl : d);
   };
-  // the page of a step that is to be loaded next, its id read through the scalar cache a step ahead
-  const ScalarInts table = (ScalarInts)(uintptr_t)(a.table + (int64_t)bk.b * a.ldt);
-  int page, sub;
+  // the page of a step that is to be loaded next. Its id comes as the codes do: read through the scalar cache, its way back
+  // would be waited for with the next read of LDS
+  const auto table = buffer_rsrc(a.table + (int64_t)bk.b * a.ldt, (uint32_t)kAll);
+  int page, sub, c_page;
   auto next_page = [&](int j) __attribute__((always_inline)) {
-    const int c = j * KG + kg < nsteps ? chunk_of(j) : 0;
+    c_page = j * KG + kg < nsteps ? chunk_of(j) : 0;
     int at;
-    chunk_page(a.cpp, c, at, sub);
-    page = table[at];
+    chunk_page(a.cpp, c_page, at, sub);
+    page = (int)__builtin_amdgcn_raw_buffer_load_b32(table, at * 4, 0, 0);
   };
   uint32_t have = 0;  // bit i: whether the step i before the last one loaded has a page
   int nfull = min(n, max(0, nf - j0 - kg + KG - 1) / KG);  // unmasked steps: to the first without a page
   struct Raw {
     u32x4 codes[NU];
     uint32_t params[PW];
+    int c;
   };
-  Raw raw1;
   const int gt = cg * 64 + lane;  // of the K group's threads
   // A chunk's bytes that this thread unpacks; no page (an id outside the pool, a step past the range): zeros
   const char* const pool = (const char*)a.k + (int64_t)kvh * a.cpp.n * L::kBytes;
   const uint32_t pstride = (uint32_t)a.kps * 2;  // bytes: below 2^32
   auto load = [&](int j) __attribute__((always_inline)) {
-    const bool ok = (j * KG + kg < nsteps) & ((uint32_t)page < (uint32_t)a.pages);
-    const auto rs = buffer_rsrc(pool + (uint64_t)(ok ? (uint32_t)page : 0u) * pstride + (uint32_t)sub * (uint32_t)L::kBytes, ok ? L::kBytes : 0);
+    const uint32_t id = (uint32_t)__builtin_amdgcn_readfirstlane(page);
+    const bool ok = (j * KG + kg < nsteps) & (id < (uint32_t)a.pages);
+    const auto rs = buffer_rsrc(pool + (uint64_t)(ok ? id : 0u) * pstride + (uint32_t)sub * (uint32_t)L::kBytes, ok ? L::kBytes : 0);
     Raw r;
+    r.c = c_page;
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
       const int u = cg + CG * i;
@@ -660,15 +663,18 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
     // word w of the params: of k or v, group, position / 8, step or offset, a pair of positions. What no row of the block
     // sees may be anything: zero
     float* const par = reinterpret_cast<float*>(to + HD / 8 * 1024);
-    const int cb = chunk_of(j) * kChunkPos;
+    const int cb = r.c * kChunkPos;
+    const bool edge = (cb + kChunkPos - 1 > bk.last) | ((cb < any_lo) & (cb + kChunkPos > a.sinks));  // for the whole workgroup
 #pragma unroll
     for (int i = 0; i < PW; ++i) {
       const int w = gt + i * CG * 64;
       const int pos = (w >> 3 & 3) * 8 + (w & 3) * 2, kind = (w >> 2 & 1) + (w >= 32 * NG ? 2 : 0), g = w / 32 % NG;
       float2_t f = unpack2<E>(r.params[i]);
-      const int p0 = cb + pos;
-      f[0] = (p0 <= bk.last) & ((p0 >= any_lo) | (p0 < a.sinks)) ? f[0] : 0.0f;
-      f[1] = (p0 + 1 <= bk.last) & ((p0 + 1 >= any_lo) | (p0 + 1 < a.sinks)) ? f[1] : 0.0f;
+      if (edge) {
+        const int p0 = cb + pos;
+        f[0] = (p0 <= bk.last) & ((p0 >= any_lo) | (p0 < a.sinks)) ? f[0] : 0.0f;
+        f[1] = (p0 + 1 <= bk.last) & ((p0 + 1 >= any_lo) | (p0 + 1 < a.sinks)) ? f[1] : 0.0f;
+      }
       // (threads past the last word write behind them)
       *reinterpret_cast<float2_t*>(par + (w < 64 * NG ? (kind * NG + g) * 32 + pos : 2 * w)) = f;
     }
@@ -676,13 +682,13 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
   constexpr int D = AHEAD ? 2 : 1;  // steps ahead that are unpacked
   next_page(0);
   {
-    const Raw r0 = load(0), r1 = load(1);
-    unpack(r0, 0);
-    if (AHEAD) unpack(r1, 1);
-    if (!AHEAD) raw1 = r1;
+    Raw r[D];
+#pragma unroll
+    for (int i = 0; i < D; ++i) r[i] = load(i);
+#pragma unroll
+    for (int i = 0; i < D; ++i) unpack(r[i], i);
   }
-  if (AHEAD) raw1 = load(2);
-  Raw raw2 = load(D + 1);
+  Raw raw = load(D);  // (one step's: a copy of registers that a load is to fill would wait for it)
 
   // this wave's q operands
   u32x4 q[2][NS];
@@ -759,8 +765,8 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
     constexpr bool kMasked = decltype(maskedc)::value;
     lds_barrier();
     const unsigned char* const from = slot_of(j);
-    const int cb = chunk_of(j) * kChunkPos;
-    const bool there = !kMasked || (have >> (D + 1) & 1);
+    const int cb = kMasked ? chunk_of(j) * kChunkPos : 0;
+    const bool there = !kMasked || (have >> D & 1);
     if constexpr (!AHEAD) {
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
@@ -851,9 +857,8 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
       }
       if constexpr (NG == 4) __builtin_amdgcn_sched_barrier(0);
     }
-    unpack(raw1, j + D);
-    raw1 = raw2;
-    raw2 = load(j + D + 2);
+    unpack(raw, j + D);
+    raw = load(j + D + 1);
     fold_ahead(j + 1);
   };
   if (AHEAD) {
