@@ -70,7 +70,7 @@ struct Unpack {
   }
 };
 
-constexpr float kLag4 = 6.0f;  // powers of two that a row's maximum may lag (3: prompts 6% slower, a fifth of the chunks rescale)
+constexpr float kLag4 = 6.0f;  // powers of two that a row's maximum may lag (3: prompts of 8755 tokens 239 us instead of 226)
 constexpr int kUnit4 = 8;      // weights times 2^kUnit4: 2^(kLag4 + kUnit4 + 1) is inside fp16
 
 // A row of q as the matrix cores' operands, 2^qs q in fp16: lane c16 + 16 kb has row c16's dims 8kb + 32s .. + 7, raw in
@@ -124,14 +124,22 @@ __device__ __forceinline__ float score_factor(float scale, int qs) {
 // columns when its V is. What is done per score is then done once for C chunks on full lanes, and each column
 // is a partial result over positions of its own; they meet at the end. A wave's loads are a group of chunks ahead.
 //
-// The vector unit bounds it next to memory: 9 instructions per word of 8 codes, some 110 per group of columns.
-// Waves of a SIMD that the registers are to leave room for.
-template <int HD, int NG, int C>
-constexpr int kSplitOcc = HD == 64 ? (NG == 1 && C < 4 ? 4 : 3) : NG == 4 ? 2 : 3;
+// Long contexts are bound by what a CU has in flight: 64 tokens of 28/4 heads (95 MB) 28 us and 4.5 for the merge, 3.4 TB/s where
+// a 2 GiB copy reaches 4.9; the CUs are busy for 20 us of it, the rest is the last ranges' unequal ends. Next to it stands the vector
+// unit, 62% of the busy cycles (9 instructions per word of 8 codes, some 110 per group of columns), the matrix cores 12%.
+// 40 tokens of 20/20 heads of 64 in groups of 32 (131 MB) 38 us. Short contexts are bound by the latency of finding the range,
+// the page, its codes and of two launches: one token behind a window of 1024, 9.8 us.
+// Waves of a SIMD that the registers are to leave room for: as many as need no spilling (two groups of dims of 128 with 2, 3
+// waves: two contexts of 100000 positions 20.1, 21.7 us; four groups: 64 sequences 46, 118 us).
+template <int HD, int NG>
+constexpr int kSplitOcc = HD == 64 || NG == 1 ? 3 : 2;
 constexpr int kPad = 4;  // floats after a row of outputs in LDS: 16 rows' float4 in different banks
 constexpr int kWaves = 4;
-constexpr int kMinRange4 = 4;     // chunks of a range, at least: one for each wave
-constexpr int kMaxRanges4 = 128;  // ranges of a sequence
+// Chunks of a range, at least: two for each wave (with 4, 8, 12: one token of 28/4 heads after 4000 positions 10.7, 10.2, 11.3 us,
+// after 16000 16.3, 12.1, 12.8).
+constexpr int kMinRange4 = 8;
+// Ranges of a sequence, at most (64, 128, 256: two contexts of 100000 positions 26.4, 21.9, 24.6 us, with the merge).
+constexpr int kMaxRanges4 = 128;
 
 // Over the 64 lanes.
 template <int N>
@@ -189,7 +197,7 @@ constexpr int q4_bytes(int hd, int ng) { return 32 * hd + 64 + 16 * 4 * (ng + 3)
 constexpr int split4_lds(int hd, int ng, int nw) { return q4_bytes(hd, ng) + nw * kRows * (2 + hd + kPad) * 4; }
 
 template <typename E, int HD, int NG, int NW, int C>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(kSplitOcc<HD, NG, C>))) void paged_split4_kernel(PagedArgs a) {
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(kSplitOcc<HD, NG>))) void paged_split4_kernel(PagedArgs a) {
   typedef typename E::T T;
   typedef T T4 __attribute__((ext_vector_type(4)));
   typedef Int4Block<HD, NG> L;
@@ -527,6 +535,12 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(kSplitO
 // offsets, as fp32. What a wave unpacks it has loaded a step before. One barrier per chunk. With one K group (128 rows)
 // there are three slots and a chunk's scores are formed a step ahead: their products run beside the exponentials of
 // the chunk before. (Not with four groups of dims, whose products 256 registers do not hold beside the rest.)
+//
+// The vector unit bounds it, 62% (heads of 64: 72%) of the cycles with two or three waves a SIMD, the matrix cores 26% (20%):
+// per score 2 instructions to form it, 2 for its exponential, 4 for its sums and weight, and unpacking a quarter of 9 per 8
+// codes. 8755 tokens of 32/8 heads behind a window of 1000 (bf16) 222 us, 560 TFLOP/s; 509 of 14/2 heads of 64 after
+// 20000 95 us, 390 TFLOP/s; with groups of 64 and 32 dims the former take 256 and 355 us. Tried to no gain: the products in
+// the compiler's scheduling groups, V's tiles read ahead of their products, wave priorities.
 template <int BT, int NG>
 constexpr bool kAhead4 = kBlockKG<BT> == 1 && NG < 4;
 
@@ -949,8 +963,12 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
   }
 }
 
-constexpr int kSingle4 = 20;    // chunks up to which a sequence is one range
-constexpr int kPlanSeqs4 = 64;  // more sequences have their ranges found in a launch before
+// Chunks up to which a sequence is one range, without a merge (19 chunks 8.8 us, in ranges 9.9; 24 chunks 8.9 and 10.0; 34
+// chunks 11.5 and 9.7).
+constexpr int kSingle4 = 28;
+// More sequences have their ranges found in a launch before (256 sequences of 20/20 heads of 64, to 1500 positions: 77 us; found
+// by every workgroup, four sequences a lane, 104; 200 of 28/4 heads 36 and 38).
+constexpr int kPlanSeqs4 = 64;
 
 Plan make_plan4(int64_t T, int64_t B, int64_t max_q, int64_t max_len, int64_t window, int64_t sinks, int nq, int nkv, int hd) {
   Plan p;
@@ -958,11 +976,23 @@ Plan make_plan4(int64_t T, int64_t B, int64_t max_q, int64_t max_len, int64_t wi
   if (max_q * gq > 2 * kRows) {  // blocks of rows
     p.bt = rows >= 96 * B ? 128 : 64;
     p.btiles = rows / p.bt + B;
+    // Blocks are cut along the positions while they do not fill the card: this many workgroups (two a CU with heads of 128,
+    // three with 64), unless a half or a third of it is there uncut. us with half, this and twice as many: 300 tokens of 32/8
+    // heads 43.8, 34.4, 33.4, 200 of 28/4 after 10000 87, 68, 76; blocks of 64 rows, 4 x 10 tokens of 32/8 after 5000 33.5, 29.6,
+    // 39.8; heads of 64, 509 tokens of 14/2 after 20000 138, 98. Uncut from a half and from a third: 2000 tokens of 12/2 heads of
+    // 128 65.7 and 73.7, 2 x 1500 of 14/2 of 64 73.4 and 48.9.
     const int64_t fill = p.bt == 64 ? 320 : hd == 128 ? 512 : 768, whole = nkv * p.btiles;
-    p.bsplits = (hd == 128 ? 2 : 3) * whole >= fill ? 1 : std::max<int64_t>(1, std::min<int64_t>(32, fill / whole));
-    if (p.bsplits > 1) p.bpart_bytes = p.btiles * nkv * p.bsplits * p.bt * (2 + hd) * 4;
-    p.bytes = workspace_bytes(p, B);
-    return p;
+    const bool uncut = (hd == 128 ? 2 : 3) * whole >= fill;
+    // Tiles of 16 rows that each unpack what they read are the faster up to some 20 a sequence, but against whole blocks of 128
+    // rows. us in blocks and in tiles: 16 x 9 tokens of 28/4 heads after 4000 44.7, 33.0; 40 x 11 of 32/8 174, 99; 4 x 60 of 32/8
+    // alone 15.4, 7.3; 50 of 12/2 after 8000 30.2, 22.3; 60 beside 200 that decode 123, 72; but 40 x 30 of 32/8 after 3000 146, 166.
+    if (max_q * gq > 20 * kRows || (p.bt == 128 && uncut)) {
+      p.bsplits = uncut ? 1 : std::max<int64_t>(1, std::min<int64_t>(32, fill / whole));
+      if (p.bsplits > 1) p.bpart_bytes = p.btiles * nkv * p.bsplits * p.bt * (2 + hd) * 4;
+      p.bytes = workspace_bytes(p, B);
+      return p;
+    }
+    p.bt = p.btiles = 0;
   }
   p.nt = (max_q * gq + kRows - 1) / kRows;
   if (most_chunks(max_len, max_q, window, sinks) <= kSingle4) {

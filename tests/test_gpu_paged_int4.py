@@ -299,7 +299,7 @@ def test_attention_ragged(dtype, hd, group, nq, nkv, page, lens, news):
 def test_attention_few_query_heads(dtype, hd, group, nq, nkv, page):
     """Heads and tokens whose rows fill a quarter of a tile, a half, or more, with the numbers of sequences that find their
     ranges in either way; ranges of one chunk, of a group's and of others between."""
-    for lens in ([700, 32, 31, 65, 7, 2000, 90], [5000], [3, 641, 0, 673], [1281 + 32 * i for i in range(9)]):
+    for lens in ([700, 32, 31, 65, 7, 2000, 90], [5000], [3, 641, 0, 673], [833 + 32 * i for i in range(4)], [1281 + 32 * i for i in range(9)]):
         check_attention(lens, [1] * len(lens), nq, nkv, hd, group, page, dtype, cu=False)
     check_attention([700, 2000, 90, 4, 1700], [2, 1, 2, 0, 2], nq, nkv, hd, group, page, dtype)
     check_attention([700, 2000, 90, 33], [2, 1, 2, 2], nq, nkv, hd, group, page, dtype, window=900, sinks=3)
@@ -311,7 +311,16 @@ def test_attention_few_query_heads(dtype, hd, group, nq, nkv, page):
 def test_attention_blocks_of_whole_sequences(dtype, hd, group, window, sinks):
     """So many blocks that none is cut along its positions, of 128 rows and of 64."""
     check_attention([900, 33], [880, 20], 32, 16, hd, group, 32, dtype, window, sinks)
-    check_attention([40 + 11 * i for i in range(10)], [40 - i for i in range(10)], 16, 16, hd, group, 32, dtype, window, sinks)
+    check_attention([40 + 31 * i for i in range(21)] + [400], [1] * 20 + [30, 340], 16, 16, hd, group, 32, dtype, window, sinks)
+
+
+@pytest.mark.parametrize("dtype,hd,group", [(F16, 128, 128), (BF16, 128, 64), (F16, 128, 32), (BF16, 64, 64), (F16, 64, 32)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (70, 2)])
+def test_attention_long_prompts_beside_tokens(dtype, hd, group, window, sinks):
+    """Blocks of 64 rows that are cut along their positions; and tiles of 16 rows, up to 20 a sequence."""
+    check_attention([900] + [40 + 131 * i for i in range(12)], [180] + [1] * 12, 2, 1, hd, group, 32, dtype, window, sinks)
+    check_attention([1900] + [40 + 131 * i for i in range(12)], [80] + [1, 3] * 6, 4, 1, hd, group, 32, dtype, window, sinks)
+    check_attention([60, 59, 3], [60, 40, 3], 10, 2, hd, group, 32, dtype, window, sinks)
 
 
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (31, 0), (32, 4), (33, 33), (100, 70), (5000, 9), (64, 1000), (0, 5)])
