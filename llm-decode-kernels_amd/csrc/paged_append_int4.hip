@@ -177,6 +177,8 @@ __device__ __forceinline__ void store_v(unsigned char* bytes, unsigned char* blo
 
 constexpr int kTokThreads = 256;
 
+// Latency bounds it: the length, the page's id, the angles, one after the other. One token of 12/2 heads 3.8 us, 96 of 32/8
+// 5.1.
 // Thread i of a token's workgroups (y) takes 8 dims of a q or k head and their partners, or (from a wave's first lane
 // on, so that a head's lanes stay in one wave) 8 of a v head; its loads go out before the angles.
 template <typename E, int HD, int NG>
@@ -239,7 +241,11 @@ constexpr int kChunkThreads = 256;
 // (n + 62) / 32 chunks hold its n new tokens, which is at most floor((cu + n) / 32) - floor(cu / 32)
 // + 2). Each workgroup finds its sequence with a binary search. The workgroups y of a chunk share the heads, k's first and q's
 // last: what takes longest starts first. A thread has one position and 8 dims of every q and k head that
-// it meets, so its 8 angles stay in registers.
+// it meets, so its 8 angles stay in registers; the next head's values come in while one is quantised. (With the
+// angles in LDS for every head, which holds a CU to 4 workgroups: 26.7 us where this takes 20.4.)
+//
+// 5279 new tokens of 28/4 heads, 90 MB: 19 to 20 us, 4.5 TB/s. The vector unit is next to memory (67% of the busy cycles):
+// its part for k, angles and rotation in 64 bits, is 4 to 6 us, v's 4, q's 4.
 template <typename E, int HD, int NG>
 __global__ __launch_bounds__(kChunkThreads) void append4_chunk_kernel(Append4Args a) {
   typedef typename E::T T;

@@ -974,19 +974,21 @@ Plan make_plan4(int64_t T, int64_t B, int64_t max_q, int64_t max_len, int64_t wi
   Plan p;
   const int64_t gq = nq / nkv, rows = T * gq;
   if (max_q * gq > 2 * kRows) {  // blocks of rows
+    // blocks of 128 rows where a sequence has 96 on average (from 48 on: 400 tokens of 32/8 heads beside 30 that decode 114 us, not 75)
     p.bt = rows >= 96 * B ? 128 : 64;
     p.btiles = rows / p.bt + B;
     // Blocks are cut along the positions while they do not fill the card: this many workgroups (two a CU with heads of 128,
     // three with 64), unless a half or a third of it is there uncut. us with half, this and twice as many: 300 tokens of 32/8
-    // heads 43.8, 34.4, 33.4, 200 of 28/4 after 10000 87, 68, 76; blocks of 64 rows, 4 x 10 tokens of 32/8 after 5000 33.5, 29.6,
-    // 39.8; heads of 64, 509 tokens of 14/2 after 20000 138, 98. Uncut from a half and from a third: 2000 tokens of 12/2 heads of
+    // heads 43.8, 34.4, 33.4, 200 of 28/4 after 10000 87, 68, 76; blocks of 64 rows, 150 tokens of 28/4 beside 12 that decode 86, 57,
+    // 65; heads of 64, 509 tokens of 14/2 after 20000 138, 98. Uncut from a half and from a third: 2000 tokens of 12/2 heads of
     // 128 65.7 and 73.7, 2 x 1500 of 14/2 of 64 73.4 and 48.9.
     const int64_t fill = p.bt == 64 ? 320 : hd == 128 ? 512 : 768, whole = nkv * p.btiles;
     const bool uncut = (hd == 128 ? 2 : 3) * whole >= fill;
     // Tiles of 16 rows that each unpack what they read are the faster up to some 20 a sequence, but against whole blocks of 128
     // rows. us in blocks and in tiles: 16 x 9 tokens of 28/4 heads after 4000 44.7, 33.0; 40 x 11 of 32/8 174, 99; 4 x 60 of 32/8
     // alone 15.4, 7.3; 50 of 12/2 after 8000 30.2, 22.3; 60 beside 200 that decode 123, 72; but 40 x 30 of 32/8 after 3000 146, 166.
-    if (max_q * gq > 20 * kRows || (p.bt == 128 && uncut)) {
+    // (And not where there would be a million of them, most of them of sequences of fewer rows.)
+    if (max_q * gq > 20 * kRows || (p.bt == 128 && uncut) || B * nkv * (max_q * gq / kRows) > (1 << 20)) {
       p.bsplits = uncut ? 1 : std::max<int64_t>(1, std::min<int64_t>(32, fill / whole));
       if (p.bsplits > 1) p.bpart_bytes = p.btiles * nkv * p.bsplits * p.bt * (2 + hd) * 4;
       p.bytes = workspace_bytes(p, B);

@@ -346,6 +346,7 @@ def test_attention_ranges_of_many_sequences(window, sinks):
     lens[3], lens[50], lens[99] = 5000, 3300, 2500
     check_attention([max(n, 1) for n in lens], [1] * 150, 4, 2, 128, 128, 32, F16, window, sinks, cu=False)
     check_attention(lens, [min(n, i % 3) for i, n in enumerate(lens)], 8, 2, 64, 32, 32, BF16, window, sinks)
+    check_attention(lens, [min(n, 55 if i % 40 == 10 else 1) for i, n in enumerate(lens)], 4, 1, 64, 64, 32, F16, window, sinks)
 
 
 @pytest.mark.parametrize("new", [200, 600])
