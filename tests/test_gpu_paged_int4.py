@@ -364,6 +364,40 @@ def test_attention_long_contexts_beside_prompts():
     check_attention([9000, 300, 17000, 40], [1, 300, 2, 1], 4, 1, 128, 128, 32, BF16)
 
 
+def test_attention_past_four_gibibytes():
+    """Pages whose offsets pass 32 bits give what the same pages in a small pool give, in every form."""
+    nq, nkv, hd, page, group = 4, 2, 128, 512, 32
+    pages = 60000
+    pg = Pages4([1000, 1500], nkv, hd, group, page, F16)
+    big = torch.empty(kv_int4_shape(pages, nkv, page, hd, group), dtype=F16, device="cuda")
+    ids = torch.linspace(pages - 1, 2, pg.pool.shape[0]).to(torch.int32).cuda()  # of the small pool's pages
+    big[ids.long()] = pg.pool
+    table = torch.where(pg.table >= 0, ids[pg.table.clamp(min=0).long()], -1).to(torch.int32)
+    for news in ([1, 1], [60, 3], [300, 200]):
+        q, cu = q_of(sum(news), nq, hd, F16).cuda(), None if max(news) == 1 else i32(rows_of(news))
+        want, got = (paged_attention_int4(q, i32([1000, 1500]), t, pool, 0.09, cu_seqlens=cu, max_q=max(news))
+                     for t, pool in ((pg.table, pg.pool), (table, big)))
+        assert same_bits(want, got), news
+
+
+def test_attention_of_thousands_of_sequences_beside_a_prompt():
+    """So many that tiles of 16 rows for the longest would be a million and more: in blocks, and without the prompt in tiles.
+    All sequences read the same pages."""
+    B, nkv, hd, page = 9000, 8, 64, 32
+    pg = Pages4([400], nkv, hd, 64, page, F16)
+    lens = torch.arange(B, dtype=torch.int32) % 400 + 1
+    table = pg.table.expand(B, -1).contiguous()
+    for first in (320, 1):
+        lens[0] = 400
+        cu = torch.cat([torch.zeros(1), torch.arange(B) + first]).to(torch.int32)
+        q = q_of(B - 1 + first, nkv, hd, F16)
+        got = paged_attention_int4(q.cuda(), lens.cuda(), table, pg.pool, 0.125, cu_seqlens=cu.cuda(), max_q=first).cpu()
+        for b in (0, 1, 31, 32, 399, 4567, B - 1):
+            n, r = int(lens[b]), slice(int(cu[b]), int(cu[b + 1]))
+            ref, bound = attention64(q[r], *(tuple(t[:n] for t in x[0]) for x in (pg.kq, pg.vq)), 0.125, list(range(n - (r.stop - r.start), n)))
+            assert_within(got[r], ref, bound, f"sequence {b}")
+
+
 @pytest.mark.parametrize("v_scale", [2.0 ** -12, 3000.0])
 @pytest.mark.parametrize("dtype,hd,group", [(F16, 128, 128), (BF16, 64, 32)])
 def test_attention_of_small_and_large_values(v_scale, dtype, hd, group):
