@@ -10,9 +10,11 @@
 // only the weight w_j step_jg, to fp16, for bf16 too: its 11 bits are the closer, and the units below keep its range.
 //
 // Units. A row of bf16 q is scaled by the power of two that brings its largest element below 2^14: fp16 keeps its bits down
-// to 2^-30 of the largest, and elements below 2^-38 are lost. Weights are held times 2^8 over a power of two that
-// follows the row's largest step so far (kept like the maximum): fp16 keeps weights down to 2^-32 of it, whatever the
-// size of V is.
+// to 2^-30 of the largest, and elements below 2^-38 are lost. Weights are held times 2^8 over a power of two, 2^ve, that
+// follows the row's largest step so far (kept like the maximum): fp16 keeps weights down to 2^-32 of it. Sums in these
+// units, of weights (up to 2^(14 - ve)) and of weights times offsets, have to stay inside fp32 where steps are 0 too (a group of one value):
+// ve begins at fp16's least step, whose offsets are below 2^16; with bf16, where it begins at 2^-80, it follows
+// 2^-40 of the largest offset too, which is below any step of the same group but 0. So 2^25 positions sum to at most 2^119.
 #include "paged_attention.h"
 #include "paged_int4.h"
 
@@ -72,15 +74,45 @@ struct Unpack {
 
 constexpr float kLag4 = 6.0f;  // powers of two that a row's maximum may lag (3: prompts of 8755 tokens 239 us instead of 226)
 constexpr int kUnit4 = 8;      // weights times 2^kUnit4: 2^(kLag4 + kUnit4 + 1) is inside fp16
+template <typename E>
+constexpr bool kWide4 = E::kOnes == BF16::kOnes;  // of fp32's range: q is scaled, and the unit follows offsets
+template <typename E>
+constexpr int kLeast4 = kWide4<E> ? -80 : -24;  // of the weights' unit
+// What the unit of the weights follows, of steps up to sm and 8 offsets (NaN aside: what it weights is NaN).
+template <typename E>
+__device__ __forceinline__ float follow8(float sm, const float* z) {
+  if constexpr (kWide4<E>) {
+    float m;
+    asm("v_max3_f32 %0, |%1|, |%2|, |%3|" : "=v"(m) : "v"(z[0]), "v"(z[1]), "v"(z[2]));
+    asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(m) : "v"(m), "v"(z[3]), "v"(z[4]));
+    asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(m) : "v"(m), "v"(z[5]), "v"(z[6]));
+    sm = fmaxf(sm, fmaxf(m, __builtin_fabsf(z[7])) * 0x1p-40f);
+  }
+  return sm;
+}
+// In words of two bf16 steps, whose offsets are the word four lanes on, puts 2^-40 of an offset in the place of a step that is
+// smaller, which is 0 (times a code less 8, that is at most 2^-37 of the offset beside it); words of offsets stay. As
+// numbers of 16 bits: infinities and NaN, 0x7F80 on, wrap to negative ones, and 40 less in the exponent.
+struct Follow {
+  uint32_t mask, wrap, less;  // in registers of each lane: scalar ones are short
+  __device__ __forceinline__ Follow(bool offsets) : mask(offsets ? 0u : 0x7FFF7FFFu), wrap(offsets ? 0x80008000u : 0x00800080u), less(vgpr_const<0x14801480u>()) {
+    asm volatile("" : "+v"(mask), "+v"(wrap));
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t word) const {
+    typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+    auto two = [](uint32_t v) { return __builtin_bit_cast(i16x2, v); };
+    const i16x2 z = two(__builtin_amdgcn_update_dpp(0, word, 0x104, 0xf, 0xf, true) & mask) + two(wrap);
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(two(word), __builtin_elementwise_sub_sat(z, two(less))));
+  }
+};
 
 // A row of q as the matrix cores' operands, 2^qs q in fp16: lane c16 + 16 kb has row c16's dims 8kb + 32s .. + 7, raw in
 // qb; us: the row's sums over the groups in the same units (of the elements as they came: what fp16 loses of the
 // smallest is below a sum's own rounding). Returns qs; fp16 q stays as it is.
 template <typename E, int NS, int NG>
 __device__ __forceinline__ int scale_q(u32x4* qb, float* us) {
-  constexpr bool kScaled = E::kOnes == BF16::kOnes;
   int qs = 0;
-  if constexpr (kScaled) {
+  if constexpr (kWide4<E>) {
     float amax = 0.0f;
 #pragma unroll
     for (int s = 0; s < NS; ++s)
@@ -101,7 +133,7 @@ __device__ __forceinline__ int scale_q(u32x4* qb, float* us) {
     for (int i = 0; i < 4; ++i) {
       const float2_t f = unpack2<E>(qb[s][i]);
       us[s * NG / NS] += f[0] + f[1];
-      if constexpr (kScaled) qb[s][i] = pack2<F16>(f[0] * by, f[1] * by);
+      if constexpr (kWide4<E>) qb[s][i] = pack2<F16>(f[0] * by, f[1] * by);
     }
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
@@ -257,7 +289,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(kSplitO
   // finds more, and with them what is summed so far. Scores start from -m (0 while m is -inf), so that differences
   // are formed before they are scaled: what m f1 rounds away would rescale a row at every chunk.
   float m_run = -__builtin_inff(), less = 0.0f, limit = -__builtin_inff(), l = 0.0f;
-  int ve = -100;                 // 2^ve: the column's largest step's power of two
+  int ve = kLeast4<E>;           // 2^ve: the column's largest step's power of two
   float ms[NG];                  // sum of w z
   float4_t o[NB];                // O^T[dim 16b + 4kb + r][column c16]; l, ms and o in units of 2^(kUnit4 - ve)
 #pragma unroll
@@ -405,6 +437,14 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(kSplitO
     float sm = largest8<E>(vp[0][0]);
 #pragma unroll
     for (int g = 1; g < NG; ++g) sm = fmaxf(sm, largest8<E>(vp[g][0]));
+    if constexpr (kWide4<E>) {
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        float z[8];
+        params8<E>(vp[g][1], z);
+        sm = follow8<E>(sm, z);
+      }
+    }
     float mc = max3(max3(max3(sv[0], sv[1], sv[2]), sv[3], sv[4]), max3(sv[5], sv[6], sv[7]), sv[7]);
     if (__any(mc > limit || sm >= pow2i(ve + 1))) {
       mc = max_xor32(max_xor16(mc));
@@ -663,6 +703,7 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
   unsigned char* const slots = lds + kg * S * kSlot;
   auto slot_of = [&](int j) __attribute__((always_inline)) { return slots + (S == 2 ? j & 1 : j % 3) * kSlot; };
   const Unpack unpacked;
+  const Follow follow(gt & 4);
   auto unpack = [&](const Raw& r, int j) __attribute__((always_inline)) {
     unsigned char* const to = slot_of(j);
 #pragma unroll
@@ -683,7 +724,7 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
     for (int i = 0; i < PW; ++i) {
       const int w = gt + i * CG * 64;
       const int pos = (w >> 3 & 3) * 8 + (w & 3) * 2, kind = (w >> 2 & 1) + (w >= 32 * NG ? 2 : 0), g = w / 32 % NG;
-      float2_t f = unpack2<E>(r.params[i]);
+      float2_t f = unpack2<E>(kWide4<E> ? follow(r.params[i]) : r.params[i]);
       if (edge) {
         const int p0 = cb + pos;
         f[0] = (p0 <= bk.last) & ((p0 >= any_lo) | (p0 < a.sinks)) ? f[0] : 0.0f;
@@ -719,7 +760,7 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
     f1[ct] = score_factor(a.scale, qs[ct]);
   }
   float m_run[2], less[2], limit[2], l[2], ms[2][NG];
-  int ve = -100;      // 2^ve: the power of two of the largest step of v that a row of the block has seen
+  int ve = kLeast4<E>;  // 2^ve: the power of two of the largest step of v that a row of the block has seen
   float4_t o[2][NB];  // O^T[dim 16b + 4kb + r][row c16], unnormalised; l, ms and o in units of 2^(kUnit4 - ve)
 #pragma unroll
   for (int ct = 0; ct < 2; ++ct) {

@@ -620,6 +620,103 @@ def test_attention_of_nan(news, dtype, hd, group):
         assert_within(torch.where(bad, 0, mine), torch.where(bad, 0, ref), torch.where(bad, 1, bound))
 
 
+# ------------------------------------------------------- attention of values at the format's edges
+# forms of the call by (new tokens of the first sequence, of the others, sequences): its heads are one kv head's
+FORMS = {"one token": (1, 1, 2), "tiles": (40, 7, 3), "cut blocks": (400, 400, 2), "whole blocks": (340, 340, 80), "blocks of 64": (340, 1, 13)}
+EDGES = [(F16, 128, 128), (F16, 64, 32), (BF16, 128, 32), (BF16, 128, 64), (BF16, 64, 64)]
+
+
+def flat(values, hd, group, first=False):
+    """(code, step, z) of one kv head whose groups (first: the first alone, the others 0) are constant, values[p] at position p."""
+    z = values[:, None, None].expand(-1, 1, hd // group).clone()
+    if first:
+        z[..., 1:] = 0
+    return torch.full((len(values), 1, hd), 8, dtype=torch.uint8), torch.zeros_like(z), z
+
+
+def attend_one_pool(form, kq, vq, hd, dtype, q1, scale, nq=1):
+    """Attention in one of the FORMS, every sequence over the same pages of one kv head, every head's row q1 [hd]: [(rows, first
+    position)] of each sequence's results, as float64."""
+    first, others, B = FORMS[form]
+    L, page = kq[0].shape[0], 64
+    pool, table = one_pool(kq, vq, hd, page, dtype)
+    news = [first] + [others] * (B - 1)
+    T = sum(news)
+    q = q1.to(dtype).expand(T, nq, hd).contiguous().cuda()
+    got = paged_attention_int4(q, i32([L] * B), table.expand(B, -1).contiguous(), pool, scale,
+                               cu_seqlens=None if T == B else i32(rows_of(news)), max_q=first).cpu().double()
+    return [(got[lo:hi], L - (hi - lo)) for lo, hi in zip(rows_of(news), rows_of(news)[1:])]
+
+
+@pytest.mark.parametrize("scores", ["equal", "just below the lag"])
+@pytest.mark.parametrize("dtype,hd,group", EDGES)
+@pytest.mark.parametrize("form", FORMS)
+def test_attention_of_constant_groups(form, dtype, hd, group, scores):
+    """V whose groups have no step at any position, and scores that are equal or rise by 5.95 powers of two after the first
+    positions, which is less than a maximum may lag. The answer is a weighted mean of the offsets: fp32 sums of n
+    weights and products (n + 64) 2^-23, and 2^-16 for exponents up to 2^7 in size."""
+    first, _, B = FORMS[form]
+    half = torch.finfo(dtype).eps / 2
+    for L in (832, 8192) if first == 1 else (8192,):
+        p = torch.arange(L).double()
+        s = torch.where(p < 512, 0.0, 4.125) if scores != "equal" else torch.full((L,), 1.0)
+        kq = flat(s.to(dtype), hd, group, first=True)
+        w = torch.exp(s.double() - s.max())
+        q1 = torch.zeros(hd)
+        q1[0] = 1.0
+        kinds = {"zero": 0 * p, "one": 0 * p + 1, "a thousand": 0 * p + 1000, "the largest": 0 * p + (65504.0 if dtype == F16 else 2.0 ** 80),
+                 "by position": p % 256, "of both signs": 30000 * (1 - 2 * (p % 2)), "once": torch.where(p == 700, 2.0 ** 15, 0.0)}
+        for name, v in kinds.items():
+            vq = flat(v.to(dtype), hd, group)
+            v = vq[2][:, 0, 0].double()
+            n = torch.cumsum(w, 0)
+            ref, around = torch.cumsum(w * v, 0) / n, torch.cumsum(w * v.abs(), 0) / n
+            bound = around * ((L + 64) * 2.0 ** -23 + 2.0 ** -16) + half * ref.abs() * 1.01 + 2.0 ** -25
+            for rows, at in attend_one_pool(form, kq, vq, hd, dtype, q1, 1.0):
+                r = slice(at, at + rows.shape[0])
+                assert_within(rows[:, 0], ref[r, None].expand(-1, hd), bound[r, None].expand(-1, hd), f"{name}, {L} positions")
+
+
+EDGE_VALUES = {
+    "zeros": lambda x, f: torch.zeros_like(x),
+    "zeros, then values": lambda x, f: torch.where(torch.arange(len(x))[:, None, None] < 130, 0, x),
+    "values, then one value": lambda x, f: torch.where(torch.arange(len(x))[:, None, None] < 130, x, 3.0),
+    "one value, then small ones": lambda x, f: torch.where(torch.arange(len(x))[:, None, None] < 130, 3.0, x * 2.0 ** -10),
+    "two values a step of the type apart": lambda x, f: torch.where(x > 0, 1.0 + f.eps, 1.0),
+    "far from zero": lambda x, f: x.float() * 0.05 + 900,
+    "one dim of many times the others": lambda x, f: torch.where(torch.arange(x.shape[-1]) == 37, 200 * x, x),
+    "the smallest": lambda x, f: torch.randint(-20, 21, x.shape) * (2.0 ** -24 if f.bits == 16 and f.eps < 2 ** -8 else 2.0 ** -70),
+    "zeros, then large ones": lambda x, f: torch.where(torch.arange(len(x))[:, None, None] < 130, 0, x.double() * (10000.0 if f.eps < 2 ** -8 else 2.0 ** 30)),
+}
+
+
+@pytest.mark.parametrize("what", EDGE_VALUES)
+@pytest.mark.parametrize("dtype,hd,group", EDGES)
+@pytest.mark.parametrize("lens,news", [([300, 1200], [1, 1]), ([300, 1200], [40, 9]), ([450, 1200], [400, 330])])
+def test_attention_of_edge_values(lens, news, dtype, hd, group, what):
+    """v of the quantiser's edges, and steps that appear only after positions without one."""
+    check_edge(lens, news, dtype, hd, group, EDGE_VALUES[what])
+
+
+def check_edge(lens, news, dtype, hd, group, make):
+    nq, nkv, page = 2, 1, 64
+    pg = Pages4(lens, nkv, hd, group, page, dtype, seed=11)
+    for b, n in enumerate(lens):
+        x = torch.randn(n, nkv, hd, generator=torch.Generator().manual_seed(b)).to(dtype)
+        pg.vq[b] = quantise(make(x, torch.finfo(dtype)).to(dtype), group)
+        for p in range(n):
+            block = pg.pool[int(pg.table[b, p // page]), :, p % page // 32]
+            held = block.cpu()
+            put(held, p % 32, hd, tuple(t[p] for t in pg.kq[b]), tuple(t[p] for t in pg.vq[b]))
+            block.copy_(held)
+    cu = rows_of(news)
+    q = q_of(cu[-1], nq, hd, dtype)
+    got = paged_attention_int4(q.cuda(), i32(lens), pg.table, pg.pool, hd ** -0.5, cu_seqlens=None if max(news) == 1 else i32(cu), max_q=max(news))
+    for b, n in enumerate(lens):
+        ref, bound = attention64(q[cu[b]:cu[b + 1]], pg.kq[b], pg.vq[b], hd ** -0.5, list(range(n - news[b], n)))
+        assert_within(got[cu[b]:cu[b + 1]], ref, bound, f"sequence {b}")
+
+
 # ------------------------------------------------------------------------- streams, graphs, together
 def test_on_another_stream():
     pg = Pages4([900, 40], 2, 128, 32, 32, F16, seed=3)
