@@ -698,6 +698,15 @@ def test_attention_of_edge_values(lens, news, dtype, hd, group, what):
     check_edge(lens, news, dtype, hd, group, EDGE_VALUES[what])
 
 
+@pytest.mark.parametrize("lens,news", [([300, 1200], [1, 1]), ([300, 1200], [40, 9]), ([450, 1200], [400, 330])])
+@pytest.mark.parametrize("hd,group", [(128, 32), (128, 128), (64, 64)])
+@pytest.mark.parametrize("power", [45, 60, 80])
+def test_attention_of_zeros_before_large_values(lens, news, hd, group, power):
+    """bf16 v: zeros, then values of 2^power, more than fp32's range of exponents above the least step that the weights' unit
+    tells apart."""
+    check_edge(lens, news, BF16, hd, group, lambda x, f: torch.where(torch.arange(len(x))[:, None, None] < 130, 0, x.double() * 2.0 ** power))
+
+
 def check_edge(lens, news, dtype, hd, group, make):
     nq, nkv, page = 2, 1, 64
     pg = Pages4(lens, nkv, hd, group, page, dtype, seed=11)
