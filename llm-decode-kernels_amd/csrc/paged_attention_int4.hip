@@ -767,18 +767,21 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
     f1[ct] = score_factor(a.scale, qs[ct]);
   }
   float m_run[2], less[2], limit[2], l[2], ms[2][NG];
-  int ve = kLeast4<E>;  // 2^ve: the power of two of the largest step of v that a row of the block has seen
-  float4_t o[2][NB];  // O^T[dim 16b + 4kb + r][row c16], unnormalised; l, ms and o in units of 2^(kUnit4 - ve)
+  float unit[2];      // kUnit4 - ve, 2^ve the row's largest step's power of two: the units of l, ms and o
+  float top = pow2i(kLeast4<E> + 1);  // 2^(ve + 1) of the rows' smaller one
+  float4_t o[2][NB];  // O^T[dim 16b + 4kb + r][row c16], unnormalised
 #pragma unroll
   for (int ct = 0; ct < 2; ++ct) {
     m_run[ct] = limit[ct] = -__builtin_inff();
     less[ct] = l[ct] = 0.0f;
+    unit[ct] = (float)(kUnit4 - kLeast4<E>);
 #pragma unroll
     for (int g = 0; g < NG; ++g) ms[ct][g] = 0.0f;
 #pragma unroll
     for (int b = 0; b < NB; ++b) o[ct][b] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
+  auto unit_exponent = [](float u) { return kUnit4 - (int)u; };
   auto param = [&](const unsigned char* slot, int kind, int g, float* f) __attribute__((always_inline)) {
     const float* const par = reinterpret_cast<const float*>(slot + HD / 8 * 1024) + (kind * NG + g) * 32 + 8 * kb;
 #pragma unroll
@@ -837,16 +840,8 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
         if constexpr (NG == 4) __builtin_amdgcn_sched_barrier(0);  // one group at a time: 256 registers hold no more
       }
     }
-    float sm = 0.0f;
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      float st[8];
-      param(from, 2, g, st);
-      sm = max3(max3(max3(sm, st[0], st[1]), st[2], st[3]), max3(st[4], st[5], st[6]), st[7]);
-    }
-    bool more_any = sm >= pow2i(ve + 1);
     bool seen[2][8];
-    float mc[2];
+    float mc[2], sm[2] = {0.0f, 0.0f};  // the largest score, and the largest step of what the row sees
 #pragma unroll
     for (int ct = 0; ct < 2; ++ct) {
 #pragma unroll
@@ -858,19 +853,30 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
         }
       }
       mc[ct] = max3(max3(max3(sv[ct][0], sv[ct][1], sv[ct][2]), sv[ct][3], sv[ct][4]), max3(sv[ct][5], sv[ct][6], sv[ct][7]), sv[ct][7]);
-      more_any = more_any | (mc[ct] > limit[ct]);
     }
-    if (__any(more_any)) {
-      sm = max_xor32(max_xor16(sm));
-      const int vn = min(126, max(ve, (int)(f2u(sm) >> 23) - 127));
-      const float by = pow2i(max(ve - vn, -126)), rest = rest4<E>(ve - vn);
-      ve = vn;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      float st[8];
+      param(from, 2, g, st);
+      if constexpr (kMasked) {
+#pragma unroll
+        for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sm[ct] = fmaxf(sm[ct], seen[ct][e] ? st[e] : 0.0f);
+      } else {
+        sm[0] = max3(max3(max3(sm[0], st[0], st[1]), st[2], st[3]), max3(st[4], st[5], st[6]), st[7]);
+      }
+    }
+    if constexpr (!kMasked) sm[1] = sm[0];
+    if (__any(mc[0] > limit[0] || mc[1] > limit[1] || sm[0] >= top || (kMasked && sm[1] >= top))) {
 #pragma unroll
       for (int ct = 0; ct < 2; ++ct) {
+        const int ve = unit_exponent(unit[ct]), vn = min(126, max(ve, (int)(f2u(max_xor32(max_xor16(sm[ct]))) >> 23) - 127)), by = ve - vn;
+        unit[ct] = (float)(kUnit4 - vn);
         const float mx = max_xor32(max_xor16(mc[ct]));
         const float old = less[ct], m_new = fmaxf(m_run[ct], mx - old);
         const float now = m_new == -__builtin_inff() ? 0.0f : -m_new, more = old - now;
-        const float al = (m_run[ct] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(-more * f1[ct])) * by;
+        const float al = (m_run[ct] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(-more * f1[ct])) * pow2i(max(by, -126)), rest = rest4<E>(by);
         l[ct] = l[ct] * al * rest;
 #pragma unroll
         for (int g = 0; g < NG; ++g) ms[ct][g] = ms[ct][g] * al * rest;
@@ -882,16 +888,17 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
         less[ct] = now;
         limit[ct] = m_new == -__builtin_inff() ? m_new : kLag4 / f1[ct];
       }
+      top = pow2i(unit_exponent(fmaxf(unit[0], unit[1])) + 1);
     }
     products_ahead(j + 1);
-    const float unit = (float)(kUnit4 - ve);
 #pragma unroll
-    for (int ct = 0; ct < 2; ++ct)
+    for (int ct = 0; ct < 2; ++ct) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        sv[ct][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[ct][e], f1[ct], unit));
+        sv[ct][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[ct][e], f1[ct], unit[ct]));
         l[ct] += sv[ct][e];
       }
+    }
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       float st[8], z[8];
@@ -935,7 +942,7 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
   // ---- what the rows have, in q.k's and v's own units; groups past the first leave it to the first, lane for lane
 #pragma unroll
   for (int ct = 0; ct < 2; ++ct) {
-    const float one = pow2i(ve - kUnit4);
+    const float one = pow2i(-(int)unit[ct]);
     l[ct] = add_xor32(add_xor16(l[ct])) * one;
     m_run[ct] *= pow2i(-qs[ct]);
 #pragma unroll

@@ -726,6 +726,25 @@ def check_edge(lens, news, dtype, hd, group, make):
         assert_within(got[cu[b]:cu[b + 1]], ref, bound, f"sequence {b}")
 
 
+@pytest.mark.parametrize("dtype,hd,group", EDGES)
+@pytest.mark.parametrize("form", ["tiles", "cut blocks", "whole blocks", "blocks of 64"])
+def test_attention_of_a_later_large_value(form, dtype, hd, group):
+    """The step of a position that a row does not see has no part in how its weights are held: a v of far more than the others'
+    size at a late position, small ones before, each row against a bound of what it sees alone."""
+    L = 512
+    g = torch.Generator().manual_seed(3)
+    kq = quantise((1.3 * torch.randn(L, 1, hd, generator=g)).to(dtype), group)
+    v = torch.randn(L, 1, hd, generator=g) * (2.0 ** -11 if dtype == F16 else 1.0)
+    v[-12] = (60000.0 if dtype == F16 else 2.0 ** 40) * (1 - 2 * (torch.arange(hd) % 2))
+    vq = quantise(v.to(dtype), group)
+    q1 = torch.randn(hd, generator=g)
+    for rows, at in attend_one_pool(form, kq, vq, hd, dtype, q1, hd ** -0.5)[:2]:
+        for i in range(0, rows.shape[0], 1 if rows.shape[0] < 50 else 13):
+            n = at + i + 1
+            ref, bound = attention64(q1.to(dtype).expand(1, 1, hd), *(tuple(t[:n] for t in x) for x in (kq, vq)), hd ** -0.5, [n - 1])
+            assert_within(rows[i:i + 1], ref, bound, f"row at {n - 1}")
+
+
 # ------------------------------------------------------------------------- streams, graphs, together
 def test_on_another_stream():
     pg = Pages4([900, 40], 2, 128, 32, 32, F16, seed=3)
