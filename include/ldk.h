@@ -483,7 +483,8 @@ int ldk_shared_prefix_attention(const void* q, int64_t ldq, int dtype, const int
  *  - Position by position, kv head by kv head and group by group, value = z + (code - 8) step, code 0..15. Of the
  *    group's values x, which have dtype: step = rnd((max/2 - min/2) / 7.5), z = rnd((min/2 + max/2) + step/2), code =
  *    clamp(rint((x - z) / step) + 8, 0, 15), in fp32, rnd to dtype; step 0: code 8. A group with a NaN or an
- *    infinity gets step 0 and z NaN. */
+ *    infinity gets step 0 and z NaN. The values of the outermost codes may lie past the type's largest number by the step's and
+ *    the offset's rounding: they are read as that number, and attention's results do not pass it. */
 
 /* ldk_paged_append into 4-bit pages. q is rotated as there; k in 64 bits, angles included, then rounded to fp32, to
  * dtype, and quantised; v is quantised as it comes. Two new tokens of one call may not share a slot. */

@@ -21,6 +21,7 @@ namespace ldk {
 struct F16 {
   typedef half_t T;
   static constexpr uint32_t kOnes = 0x3C003C00u;  // (1, 1)
+  static constexpr float kMost = 65504.0f;        // the largest finite number
   // softmax numerators are held times 2^kShift: a weight of 2^-25 of the largest, where fp16 alone ends,
   // would be lost, and with it a long context's many small ones beside a large one
   static constexpr float kShift = 7.0f;
@@ -32,6 +33,7 @@ struct F16 {
 struct BF16 {
   typedef __bf16 T;
   static constexpr uint32_t kOnes = 0x3F803F80u;
+  static constexpr float kMost = 0x1.FEp127f;
   static constexpr float kShift = 0.0f;
   typedef __bf16 T2 __attribute__((ext_vector_type(2)));
   typedef __bf16 T8 __attribute__((ext_vector_type(8)));
@@ -48,6 +50,11 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 template <typename E>
 __device__ __forceinline__ float2_t unpack2(uint32_t u) {
   return __builtin_convertvector(__builtin_bit_cast(typename E::T2, u), float2_t);
+}
+// x, or the type's largest number in the place of a finite one that would round to an infinity.
+template <typename E>
+__device__ __forceinline__ float bounded(float x) {
+  return __builtin_fabsf(x) < __builtin_inff() ? __builtin_amdgcn_fmed3f(x, -E::kMost, E::kMost) : x;
 }
 
 constexpr int kChunkPos = 32;          // positions of a chunk

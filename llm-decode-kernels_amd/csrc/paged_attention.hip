@@ -767,7 +767,7 @@ __global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_kernel(PagedArgs
   if (lane >= LR) return;
   out_t y;
 #pragma unroll
-  for (int i = 0; i < VL; ++i) y[i] = (T)(l != 0.0f ? o[i] / l : 0.0f);
+  for (int i = 0; i < VL; ++i) y[i] = (T)bounded<E>(l != 0.0f ? o[i] / l : 0.0f);
   *reinterpret_cast<out_t*>((T*)a.out + (int64_t)t * a.ldo + (int64_t)h * HD + VL * ld) = y;
 }
 

@@ -562,7 +562,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(kSplitO
       T* dst = (T*)a.out + (int64_t)(sp.s.row0 + g / a.gq) * a.ldo + (int64_t)(kvh * a.gq + g % a.gq) * HD + d;
       T4 y;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) y[r] = (T)(v[r] * over);
+      for (int r = 0; r < 4; ++r) y[r] = (T)bounded<E>(v[r] * over);
       *reinterpret_cast<T4*>(dst) = y;
     } else {
       *reinterpret_cast<float4_t*>(part + 2 * kRows + j * HD + d) = v;
@@ -1004,7 +1004,7 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
         if (direct) {
           T4 y;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) y[r] = (T)(v[r] * over);
+          for (int r = 0; r < 4; ++r) y[r] = (T)bounded<E>(v[r] * over);
           *reinterpret_cast<T4*>(dst + 16 * b) = y;
         } else {
           *reinterpret_cast<float4_t*>(pdst + 16 * b) = v;

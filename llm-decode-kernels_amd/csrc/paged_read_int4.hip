@@ -1,5 +1,5 @@
 // Reading the values of a paged cache held in 4 bits (paged_int4.h) back as rows [token, kv head, hd] of the cache's type:
-// z + (code - 8) step in fp32 (the product is exact), rounded once.
+// z + (code - 8) step in fp32 (the product is exact), rounded once, at most the type's largest number.
 //
 // A workgroup takes the rows of one 32-position chunk of one sequence and some of its kv heads. k's codes are rows
 // already (a lane's 16 bytes are 8 dims of each step of one position); v's, whose bytes run along the positions, are turned
@@ -24,6 +24,17 @@ struct Read4Args {
   int64_t ldk, ldv;  // row strides, elements
   int T, B, nkv, pages, cpp, cap;
 };
+
+// The outermost codes of a group near the type's largest number may stand for a value past it, by the step's and the offset's
+// rounding: it is read as the largest. most4: that number, or NaN for a group that is (as med3 of three NaN is).
+template <typename E>
+__device__ __forceinline__ float most4(float z) {
+  return __builtin_fmaf(z, 0.0f, E::kMost);
+}
+template <typename E>
+__device__ __forceinline__ float value4(uint32_t code, float step, float z, float most) {
+  return __builtin_amdgcn_fmed3f(__builtin_fmaf((float)(int)code - 8.0f, step, z), -most, most);
+}
 
 constexpr int kThreads = 256;
 
@@ -67,7 +78,7 @@ __global__ __launch_bounds__(kThreads) void read4_kernel(Read4Args a) {
       if (r >= first && r < last) {
         T* dst = (T*)a.k + (int64_t)(t0 + r) * a.ldk + (int64_t)h * HD + 8 * kb;
         uint32_t w[2 * NP] = {};
-        float step[NG] = {}, z[NG] = {};
+        float step[NG] = {}, z[NG] = {}, most[NG] = {};
         if (held) {
 #pragma unroll
           for (int n = 0; n < NP; ++n) {
@@ -77,7 +88,7 @@ __global__ __launch_bounds__(kThreads) void read4_kernel(Read4Args a) {
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
             const T* p = reinterpret_cast<const T*>(blk + L::kParams + int4_param_at(g, r));
-            step[g] = (float)p[0], z[g] = (float)p[8];
+            step[g] = (float)p[0], z[g] = (float)p[8], most[g] = most4<E>(z[g]);
           }
         }
 #pragma unroll
@@ -91,7 +102,7 @@ __global__ __launch_bounds__(kThreads) void read4_kernel(Read4Args a) {
             for (int n = 0; n < 2; ++n) {
               const int el = 2 * e + n;
               const uint32_t code = (w[2 * (s / 2) + (el >> 2)] >> (8 * int4_byte(el & 3) + 4 * (s & 1))) & 15u;
-              f[n] = __builtin_fmaf((float)(int)code - 8.0f, step[g], z[g]);
+              f[n] = value4<E>(code, step[g], z[g], most[g]);
             }
             y[e] = pack2<E>(f[0], f[1]);
           }
@@ -124,9 +135,10 @@ __global__ __launch_bounds__(kThreads) void read4_kernel(Read4Args a) {
           for (int n = 0; n < 2; ++n) {
             const int el = 2 * e + n;
             const uint32_t byte = w[2 * t + (el >> 2)] >> (8 * int4_byte(el & 3));
+            const float most = most4<E>(z2[n]);
             T* dst = &vs[8 * kb + el][(2 * quad + t) * 32 + col];
-            dst[0] = (T)__builtin_fmaf((float)(int)(byte & 15u) - 8.0f, s2[n], z2[n]);
-            dst[16] = (T)__builtin_fmaf((float)(int)(byte >> 4 & 15u) - 8.0f, s2[n], z2[n]);
+            dst[0] = (T)value4<E>(byte & 15u, s2[n], z2[n], most);
+            dst[16] = (T)value4<E>(byte >> 4 & 15u, s2[n], z2[n], most);
           }
         }
     }

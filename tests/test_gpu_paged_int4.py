@@ -745,6 +745,39 @@ def test_attention_of_a_later_large_value(form, dtype, hd, group):
             assert_within(rows[i:i + 1], ref, bound, f"row at {n - 1}")
 
 
+@pytest.mark.parametrize("dtype,hd,group", EDGES)
+@pytest.mark.parametrize("cu", [False, True])
+def test_values_near_the_largest_are_finite(cu, dtype, hd, group):
+    """Groups from the type's lowest to its largest value: their outermost codes are by up to the step's rounding beyond, and
+    are read as the largest."""
+    big = torch.finfo(dtype).max
+    x = torch.randn(3, 2 + 2 * 2, hd)
+    x = torch.stack([torch.where(x[0] > 0, big, -big), torch.where(x[1] > 0, big, big / 2), torch.where(x[2] > 0, -big, big / 4)]).to(dtype)
+    pg = check_append([5, 40, 64], [1, 1, 1], 2, 2, hd, group, 32, dtype, rotate=False, cu=cu, x=x)
+    for i, y in enumerate(paged_read_int4(i32([5, 40, 64]), pg.table, pg.pool, 3, cu_seqlens=i32([0, 1, 2, 3]) if cu else None)):
+        want = values(*quantise(x[:, 2 + 2 * i:4 + 2 * i], group)).clamp(-big, big).to(dtype)
+        assert torch.isfinite(y).all() and torch.equal(y.cpu(), want)
+
+
+@pytest.mark.parametrize("hd,group", [(128, 128), (128, 32), (64, 64)])
+@pytest.mark.parametrize("L", [64, 4096])
+@pytest.mark.parametrize("form", FORMS)
+def test_attention_near_the_largest_value_is_finite(form, L, hd, group):
+    """fp16 v of -65504 and 65504 in every group, the same at every position: the answer is what is read, half a step of fp16
+    more for the weights times their steps, of values of 8 steps and an offset of half a step."""
+    if FORMS[form][0] > L:
+        L = 512
+    v = torch.where(torch.arange(hd) % 3 == 0, -65504.0, 65504.0).half()
+    vq = quantise(v.expand(L, 1, hd), group)
+    want = values(*(t[:1] for t in vq))[0, 0].clamp(-65504, 65504)
+    kq = flat(torch.ones(L).half(), hd, group, first=True)
+    q1 = torch.zeros(hd)
+    q1[0] = 1.0
+    for rows, _ in attend_one_pool(form, kq, vq, hd, F16, q1, 1.0, nq=2):
+        off = (rows - want).abs()
+        assert torch.isfinite(rows).all() and (off <= 65504 * (2.0 ** -11 + 2.0 ** -12 + (L + 64) * 2.0 ** -23)).all(), off.max()
+
+
 # ------------------------------------------------------------------------- streams, graphs, together
 def test_on_another_stream():
     pg = Pages4([900, 40], 2, 128, 32, 32, F16, seed=3)
