@@ -18,11 +18,12 @@ struct PagedArgs {
   int64_t kps, vps;  // page strides, elements
   void* out;
   int64_t ldo;
-  float* part;    // paged_split_kernel's partials, per (slot, tile, kv head): [16 rows]{m, l} and [16 rows][hd]
+  float* part;    // paged_split_kernel's partials, per (slot, tile, kv head): [16 rows]{m, l} and [16 rows][hd] (part_at)
   float* bpart;   // paged_block_kernel's, per (tile, kv head, split): [rows]{m, l} and [rows][hd]
   int32_t* plan;  // [B][2]: first slot and ranges of every sequence
   int32_t* map;   // of many sequences: [0] chunks of a range, [1 + slot] its sequence; else null
   int T, B, max_q, nq, nkv, gq, nt;  // nt: 16-row tiles of a sequence
+  int tiles;                         // partials of a sequence's own tiles alone: the call's tiles; else 0
   int pages, cap;                    // cap: positions a sequence can hold
   PageDiv cpp;                       // chunks per page
   int pchunks, skip;                 // chunks of the shared prefix; of them, those that its own blocks take
@@ -170,6 +171,15 @@ __device__ __forceinline__ float max_xor32(float v) {
 // Floats of one partial: 16 rows of {m, l} and of hd outputs.
 constexpr int part_floats(int hd) { return kRows * (2 + hd); }
 
+// Place among the partials, in kv heads, of the range `split` of the 16 rows `tile` of sequence b, whose first row is row0 and first slot
+// `first`. Slot by slot, nt tiles each; or, where sequences have far fewer tiles than nt, the tiles of every sequence's first
+// range as the call's rows have them (sequence b's begin at row0 gq / 16 + b, rounded down: as many as ceil(n gq / 16) fit before the
+// next one's), then nt for each of the ranges past the first, of which there are `spare` at most (first - b before b's).
+__device__ __forceinline__ int64_t part_at(const PagedArgs& a, int b, int row0, int first, int split, int tile) {
+  if (!a.tiles) return (int64_t)(first + split) * a.nt + tile;
+  return split ? a.tiles + (int64_t)(first - b + split - 1) * a.nt + tile : row0 * (int64_t)a.gq / kRows + b + tile;
+}
+
 // ---- blocks of rows (the kernels' own words on them stand there)
 
 struct Block {
@@ -245,7 +255,7 @@ __device__ __forceinline__ int row_position(const PagedArgs& a, int t) {
 // What a call launches, from its sizes alone.
 struct Plan {
   bool apart = false;                               // the shared prefix in blocks of its own
-  int64_t nt = 0, slots = 0, spare = 0;             // paged_split_kernel, slots == 0: not launched
+  int64_t nt = 0, slots = 0, spare = 0, tiles = 0;  // paged_split_kernel, slots == 0: not launched
   int64_t bt = 0, btiles = 0, bsplits = 0;          // paged_block_kernel, bt == 0: not launched
   bool mapped = false;                              // paged_plan_kernel
   int64_t part_bytes = 0, bpart_bytes = 0, bytes = 0;
@@ -262,6 +272,7 @@ inline int64_t workspace_bytes(const Plan& p, int64_t B) {
 }
 inline void lay_out(PagedArgs& a, const Plan& p, void* ws, int64_t B) {
   a.part = (float*)ws;
+  a.tiles = (int)p.tiles;
   a.bpart = (float*)((char*)ws + p.part_bytes);
   a.plan = p.part_bytes ? (int32_t*)((char*)ws + p.part_bytes + p.bpart_bytes) : nullptr;
   a.map = p.mapped ? a.plan + 2 * B : nullptr;

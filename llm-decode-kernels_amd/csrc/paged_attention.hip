@@ -689,9 +689,10 @@ __global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_kernel(PagedArgs
   if (WR == 1 && !run) return;
   const float sc = a.scale * 1.44269504088896341f;
   const int kvh = h / a.gq, row = tok * a.gq + h % a.gq;
-  // the two lists: {m, l} and outputs of range i at p + i * step
+  // the two lists: {m, l} and outputs of range i at p + i * step (the tiles' first range at p0)
   const int64_t sa = (int64_t)a.nkv * a.nt * part_floats(HD);
-  const float* pa = a.part + ((int64_t)first * a.nkv * a.nt + row / kRows * a.nkv + kvh) * part_floats(HD);
+  auto part = [&](int split) { return a.part + (part_at(a, b, s.row0, first, split, row / kRows) * a.nkv + kvh) * part_floats(HD); };
+  const float *p0 = part(0), *pa = part(1) - sa;
   const float* pb = nullptr;
   int nb = 0, jb = 0;
   if (run && a.bsplits && !nothing) {
@@ -722,7 +723,7 @@ __global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_kernel(PagedArgs
 #pragma unroll 4
     for (int r = w * G + lane / LR; r < na + nb; r += WR * G) {
       const bool split = r < na;
-      const float* p = split ? pa + r * sa : pb + (int64_t)(r - na) * BT * (2 + HD);
+      const float* p = split ? (r ? pa + r * sa : p0) : pb + (int64_t)(r - na) * BT * (2 + HD);
       const int j = split ? row % kRows : jb, rows = split ? kRows : BT;
       const float m = p[2 * j], lr = p[2 * j + 1];
       const vec_t v = *reinterpret_cast<const vec_t*>(p + 2 * rows + j * HD + VL * ld);

@@ -545,7 +545,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(kSplitO
     ml[0][tid] = M, ml[1][tid] = ls;
   }
   lds_barrier();
-  float* part = a.part + ((int64_t)(sl.first + sl.split) * xy + bxy) * part_floats(HD);
+  float* part = a.part + (part_at(a, sl.b, sp.s.row0, sl.first, sl.split, tile) * a.nkv + kvh) * part_floats(HD);
   for (int e = tid; e < rows * (HD / 4); e += NW * 64) {
     const int j = e / (HD / 4), d = e % (HD / 4) * 4;
     float4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -1056,14 +1056,16 @@ Plan make_plan4(int64_t T, int64_t B, int64_t max_q, int64_t max_len, int64_t wi
     p.slots = B;
     return p;
   }
-  const int64_t w = nkv * p.nt;
+  const int64_t w = nkv * p.nt, most = rows / kRows + B;  // the batch has most tiles or fewer
   // Whole ranges for two workgroups a CU, and more for the sequences' last, shorter ones, whose number is not known here:
   // us with 512 / w, this and 512 / w + B / 2: 64 sequences of 28/4 heads 33.8, 32.4, 35.7; 40 of 20/20 heads of 64 43.8,
   // 42.3, 42.9; half and twice the 512: 37 to 39 and 33 to 38.
-  p.spare = std::max<int64_t>(1, 512 / w + B / 4);
+  p.spare = std::max<int64_t>(1, 512 / w + std::min(most, B * p.nt) / (4 * p.nt));
   p.slots = B + p.spare;
   p.mapped = B > kPlanSeqs4;
-  p.part_bytes = p.slots * w * part_floats(hd) * 4;
+  // (of nt tiles a sequence: one prompt of 80 tokens of 32/8 heads beside 1000 that decode, 1.7 GB and not 0.1)
+  if (p.nt > 1) p.tiles = most;
+  p.part_bytes = (p.nt > 1 ? p.tiles + p.spare * p.nt : p.slots) * nkv * part_floats(hd) * 4;
   p.bytes = workspace_bytes(p, B);
   return p;
 }

@@ -96,6 +96,19 @@ def test_workspace_queries():
         assert query(*ok[:at], bad, *ok[at + 1:]) == -_lib.ERR_INVALID
 
 
+@pytest.mark.parametrize("B,new,gq,nkv,hd", [(201, 80, 4, 8, 128), (1001, 80, 4, 8, 128), (64, 45, 7, 4, 128), (9, 300, 1, 2, 64), (3000, 20, 8, 2, 128),
+                                             (12, 2, 100, 1, 64)])
+def test_workspace_follows_the_rows(B, new, gq, nkv, hd):
+    """One prompt beside many tokens: partials of 16 rows of fp32 for the rows that there are (a sequence's last 16 not full) and for
+    ranges past each sequence's first, not for as many as the longest has of every sequence."""
+    lib = _lib.load()
+    T, tile = B - 1 + new, 16 * (2 + hd) * 4
+    need = lib.ldk_paged_attention_int4_workspace_bytes(T, B, new, 65536, 0, 0, gq * nkv, nkv, hd)
+    tiles, longest = T * gq // 16 + B, -(-new * gq // 16)
+    plan = 4 * (2 * B + 1 + B + 512 + B // 4)
+    assert 0 < need <= (1.25 * tiles + 512 // nkv + longest) * nkv * tile + plan
+
+
 # ------------------------------------------------------------------------------- the Python wrappers
 @pytest.mark.parametrize("hd,group", [(128, None), (128, 128), (128, 64), (128, 32), (64, None), (64, 32)])
 def test_shape(hd, group):
