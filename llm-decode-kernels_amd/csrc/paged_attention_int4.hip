@@ -78,12 +78,6 @@ template <typename E>
 constexpr bool kWide4 = E::kOnes == BF16::kOnes;  // of fp32's range: q is scaled, and the unit follows offsets
 template <typename E>
 constexpr int kLeast4 = kWide4<E> ? -80 : -24;  // of the weights' unit
-// Where the unit moves by 2^d, d <= 0 and with bf16 down to -206: what a factor of 2^max(d, -126) leaves of 2^d, for the sums of weights
-// and of weights times offsets. (The codes' sums, below 2^43, are far below the unit's least weight after such a move.)
-template <typename E>
-__device__ __forceinline__ float rest4(int d) {
-  return kWide4<E> ? pow2i(min(0, d + 126)) : 1.0f;
-}
 // What the unit of the weights follows, of steps up to sm and 8 offsets (NaN aside: what it weights is NaN).
 template <typename E>
 __device__ __forceinline__ float follow8(float sm, const float* z) {
@@ -458,11 +452,10 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(kSplitO
       const float old = less, m_new = fmaxf(m_run, mc - old);
       const float now = m_new == -__builtin_inff() ? 0.0f : -m_new, more = old - now;
       const int vn = min(126, max(ve, (int)(f2u(sm) >> 23) - 127));
-      const float al = (m_run == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(-more * f1)) * pow2i(max(ve - vn, -126));
-      const float rest = rest4<E>(ve - vn);
-      l = l * al * rest;
+      const float was = m_run == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(-more * f1), al = __builtin_ldexpf(was, ve - vn);
+      l = __builtin_ldexpf(l * was, ve - vn);
 #pragma unroll
-      for (int g = 0; g < NG; ++g) ms[g] = ms[g] * al * rest;
+      for (int g = 0; g < NG; ++g) ms[g] = __builtin_ldexpf(ms[g] * was, ve - vn);
 #pragma unroll
       for (int b = 0; b < NB; ++b) o[b] *= al;
 #pragma unroll
@@ -876,10 +869,10 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
         const float mx = max_xor32(max_xor16(mc[ct]));
         const float old = less[ct], m_new = fmaxf(m_run[ct], mx - old);
         const float now = m_new == -__builtin_inff() ? 0.0f : -m_new, more = old - now;
-        const float al = (m_run[ct] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(-more * f1[ct])) * pow2i(max(by, -126)), rest = rest4<E>(by);
-        l[ct] = l[ct] * al * rest;
+        const float was = m_run[ct] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(-more * f1[ct]), al = __builtin_ldexpf(was, by);
+        l[ct] = __builtin_ldexpf(l[ct] * was, by);
 #pragma unroll
-        for (int g = 0; g < NG; ++g) ms[ct][g] = ms[ct][g] * al * rest;
+        for (int g = 0; g < NG; ++g) ms[ct][g] = __builtin_ldexpf(ms[ct][g] * was, by);
 #pragma unroll
         for (int b = 0; b < NB; ++b) o[ct][b] *= al;
 #pragma unroll
