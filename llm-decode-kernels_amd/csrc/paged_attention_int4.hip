@@ -617,29 +617,20 @@ __global__ __launch_bounds__(kBlockThreads<BT>) __attribute__((amdgpu_waves_per_
   const int n = (nsteps + KG - 1) / KG;  // steps of a K group (the last ones may be dead)
 
   // this lane's two rows see the positions above hi - window up to hi, and those below sinks; rows past
-  // the block's are not stored. whi, wlo: the last and the first past the sinks that a row of the wave sees
+  // the block's are not stored
   const int window = a.window > 0 ? a.window : kAll;
   auto row_of = [&](int ct, int ln, int& tok, int& head) __attribute__((always_inline)) {
     const int r = bk.r0 + min(32 * cg + 16 * ct + (ln & 15), bk.rows - 1);
     tok = r / a.gq;
     head = kvh * a.gq + r % a.gq;
   };
-  int hi[2], whi = -1, wlo = kAll;
+  int hi[2];
 #pragma unroll
   for (int ct = 0; ct < 2; ++ct) {
     int t, h;
     row_of(ct, lane, t, h);
     hi[ct] = max(-1, bk.pos0 + t);
-    whi = max(whi, hi[ct]);
-    wlo = min(wlo, max(0, hi[ct] - window + 1));
   }
-#pragma unroll
-  for (int off = 1; off < 16; off *= 2) {
-    whi = max(whi, __shfl_xor(whi, off));
-    wlo = min(wlo, __shfl_xor(wlo, off));
-  }
-  whi = __builtin_amdgcn_readfirstlane(whi);
-  wlo = __builtin_amdgcn_readfirstlane(wlo);
   // of the block: positions that every row sees, all_lo .. first, and that one sees, any_lo .. last
   const int all_lo = a.window > 0 ? max(0, bk.last - a.window + 1) : 0;
   const int any_lo = a.window > 0 ? max(0, bk.first - a.window + 1) : 0;
