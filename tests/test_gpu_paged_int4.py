@@ -778,6 +778,29 @@ def test_attention_near_the_largest_value_is_finite(form, L, hd, group):
         assert torch.isfinite(rows).all() and (off <= 65504 * (2.0 ** -11 + 2.0 ** -12 + (L + 64) * 2.0 ** -23)).all(), off.max()
 
 
+def test_what_is_read_back_attended_to_in_16_bits():
+    """Sequences moved to 16-bit pages through what is read back, whose attention is within its own bound of 64 bits over those
+    values."""
+    import _paged
+    from kernels import paged
+
+    lens, nq, nkv, hd, page = [300, 41, 700], 8, 2, 128, 32
+    pg = Pages4(lens, nkv, hd, 64, page, F16)
+    cu = i32(rows_of(lens))
+    k, v = paged_read_int4(i32(lens), pg.table, pg.pool, sum(lens), cu_seqlens=cu)
+    pages = pg.pool.shape[0]
+    k16 = torch.zeros(paged.k_pages_shape(pages, nkv, page, hd), dtype=F16, device="cuda")
+    v16 = torch.zeros(paged.vt_pages_shape(pages, nkv, page, hd), dtype=F16, device="cuda")
+    qkv = torch.cat([torch.zeros(sum(lens), nq, hd, dtype=F16, device="cuda"), k, v], 1).reshape(sum(lens), -1)
+    paged.paged_append(qkv, i32(lens), pg.table, k16, v16, None, nq, cu_seqlens=cu)
+    q = q_of(3, nq, hd, F16)
+    got = paged.paged_attention(q.cuda(), i32(lens), pg.table, k16, v16, 0.09)
+    for b, n in enumerate(lens):
+        r = slice(rows_of(lens)[b], rows_of(lens)[b + 1])
+        ref, bound = _paged.attention64(q[b:b + 1], k[r].cpu(), v[r].cpu(), 0.09, [n - 1])
+        assert_within(got[b:b + 1], ref, bound, f"sequence {b}")
+
+
 # ------------------------------------------------------------------------- streams, graphs, together
 def test_on_another_stream():
     pg = Pages4([900, 40], 2, 128, 32, 32, F16, seed=3)
