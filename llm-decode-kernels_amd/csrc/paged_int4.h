@@ -5,8 +5,11 @@
 // cache's type, as codes 0..15:  value = z + (code - 8) step. Of a group's values x, which have the type (k after
 // its rotation is rounded to it):
 //   step = rnd((max/2 - min/2) / 7.5)   z = rnd((min/2 + max/2) + step/2)   code = clamp(rint((x - z) / step) + 8)
-// in fp32, rnd to the type, so that codes 0 and 15 lie at the minimum and the maximum. step = 0: code 8. A group with a NaN
-// or an infinity gets step 0 and z NaN; a value that the roundings put past the type's largest number is read as that. One pair per position (not per channel): a token is quantised as it
+// in fp32, rnd to the type, so that codes 0 and 15 lie at the minimum and the maximum but for the roundings of step and z: with
+// u half a step of the type at 1 (2^-11, bf16 2^-8) a value is off by at most step/2 + u (|z| + 7.5 step), which the
+// offset rules where a group lies far from 0 (bf16 900 .. 904: z 904, and 900 is held as 901.9). step = 0: code 8. A group with
+// a NaN or an infinity gets step 0 and z NaN; a value that the roundings put past the type's largest number is read as that.
+// One pair per position (not per channel): a token is quantised as it
 // comes, whatever its neighbours are, and a group's range is that of one head's dims; the finer groups keep a
 // dim that is far larger than the others (as some of k's are) from coarsening all of them.
 //

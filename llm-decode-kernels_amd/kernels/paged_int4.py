@@ -13,7 +13,8 @@ A step of ragged sequences, as with kernels.paged:
   group, 3.8 (group 128) to 3.2 (32) times less than 16-bit pages.
 - Each position's k and v are quantised for themselves, per kv head and group of 32, 64 or 128 dims, to value = z + (code - 8)
   step with codes 0..15 over the group's range. Smaller groups follow dims of unlike sizes, as k's often are, at 0.25
-  bits per value for each halving from 128 to 64, 0.5 to 32. A group with a NaN or an infinity reads as NaN.
+  bits per value for each halving from 128 to 64, 0.5 to 32. step and z are rounded to the dtype, so that a group far from 0
+  is held to its offset's rounding. A group with a NaN or an infinity reads as NaN.
 - block_table, kv_lens and cu_seqlens are kernels.paged's, absent pages and padded batches too. Two sequences of a call may
   append to one page, as each byte is one position's alone, but not at one position.
 
@@ -102,9 +103,9 @@ def paged_read_int4(kv_lens: torch.Tensor, block_table: torch.Tensor, kv_pages: 
                     out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The values that the pages hold, (k, v), each [rows, n_kv, hd] of the pages' dtype: the rows cu_seqlens[b]:
     cu_seqlens[b + 1] are the last of sequence b's kv_lens[b] positions (None: its last position, row b), z + (code - 8)
-    step rounded once. rows: as many as cu_seqlens ends with, or more (a host number; without cu_seqlens or with `out` it
-    need not be given). Rows at positions without a page, or below 0, are zeros; rows behind the last sequence's are
-    left as they were (of outputs that are not given: undefined)."""
+    step rounded once, at most the dtype's largest number. rows: as many as cu_seqlens ends with, or more (a host number;
+    without cu_seqlens or with `out` it need not be given). Rows at positions without a page, or below 0, are zeros; rows
+    behind the last sequence's are left as they were (of outputs that are not given: undefined)."""
     what = "paged_read_int4"
     pages, nkv, page, hd, group, stride = _pool(kv_pages, what)
     dtype = kv_pages.dtype
@@ -135,8 +136,8 @@ def paged_attention_int4(q: torch.Tensor, kv_lens: torch.Tensor, block_table: to
     tokens that a sequence has (a host number that chooses the launch; rows past it are not computed; None: as many as
     there are rows). Returns [tokens, n_heads, hd]; a token that sees nothing gives zeros. scale > 0.
 
-    A NaN in a position's k or v reaches the tokens that see it and no other. max_q chooses one kernel for the
-    call: a batch that decodes over long contexts beside prompts runs faster as two calls."""
+    A NaN in a position's k or v reaches the tokens that see it and no other. bf16 k and v are taken up to 2^90 in size.
+    max_q chooses one kernel for the call: a batch that decodes over long contexts beside prompts runs faster as two calls."""
     what = "paged_attention_int4"
     pages, nkv, page, hd, group, stride = _pool(kv_pages, what)
     dtype = kv_pages.dtype

@@ -707,19 +707,27 @@ def test_attention_of_zeros_before_large_values(lens, news, hd, group, power):
     check_edge(lens, news, BF16, hd, group, lambda x, f: torch.where(torch.arange(len(x))[:, None, None] < 130, 0, x.double() * 2.0 ** power))
 
 
-def check_edge(lens, news, dtype, hd, group, make):
+@pytest.mark.parametrize("lens,news", [([300, 1200], [1, 1]), ([300, 1200], [40, 9]), ([450, 1200], [400, 330])])
+@pytest.mark.parametrize("hd,group", [(128, 32), (128, 128), (64, 64)])
+def test_attention_near_the_limit_of_bf16(lens, news, hd, group):
+    """k and v of up to 2^90 in size, q as much smaller."""
+    check_edge(lens, news, BF16, hd, group, lambda x, f: x.double() * 2.0 ** 87, k_size=2.0 ** 85)
+
+
+def check_edge(lens, news, dtype, hd, group, make, k_size=None):
     nq, nkv, page = 2, 1, 64
     pg = Pages4(lens, nkv, hd, group, page, dtype, seed=11)
+    pool, table = pg.pool.cpu(), pg.table.cpu()
     for b, n in enumerate(lens):
         x = torch.randn(n, nkv, hd, generator=torch.Generator().manual_seed(b)).to(dtype)
+        if k_size:
+            pg.kq[b] = quantise((x.flip(0).double() * k_size).to(dtype), group)
         pg.vq[b] = quantise(make(x, torch.finfo(dtype)).to(dtype), group)
         for p in range(n):
-            block = pg.pool[int(pg.table[b, p // page]), :, p % page // 32]
-            held = block.cpu()
-            put(held, p % 32, hd, tuple(t[p] for t in pg.kq[b]), tuple(t[p] for t in pg.vq[b]))
-            block.copy_(held)
+            put(pool[int(table[b, p // page]), :, p % page // 32], p % 32, hd, tuple(t[p] for t in pg.kq[b]), tuple(t[p] for t in pg.vq[b]))
+    pg.pool.copy_(pool)
     cu = rows_of(news)
-    q = q_of(cu[-1], nq, hd, dtype)
+    q = (q_of(cu[-1], nq, hd, dtype).double() / (k_size or 1)).to(dtype)
     got = paged_attention_int4(q.cuda(), i32(lens), pg.table, pg.pool, hd ** -0.5, cu_seqlens=None if max(news) == 1 else i32(cu), max_q=max(news))
     for b, n in enumerate(lens):
         ref, bound = attention64(q[cu[b]:cu[b + 1]], pg.kq[b], pg.vq[b], hd ** -0.5, list(range(n - news[b], n)))
