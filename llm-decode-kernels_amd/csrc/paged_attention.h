@@ -171,10 +171,11 @@ __device__ __forceinline__ float max_xor32(float v) {
 // Floats of one partial: 16 rows of {m, l} and of hd outputs.
 constexpr int part_floats(int hd) { return kRows * (2 + hd); }
 
-// Place among the partials, in kv heads, of the range `split` of the 16 rows `tile` of sequence b, whose first row is row0 and first slot
-// `first`. Slot by slot, nt tiles each; or, where sequences have far fewer tiles than nt, the tiles of every sequence's first
-// range as the call's rows have them (sequence b's begin at row0 gq / 16 + b, rounded down: as many as ceil(n gq / 16) fit before the
-// next one's), then nt for each of the ranges past the first, of which there are `spare` at most (first - b before b's).
+// Place among the partials, in kv heads, of the range `split` of the 16 rows `tile` of sequence b, whose first row is row0
+// and first slot `first`. Slot by slot, nt tiles each; or, where the call's tiles are counted, first the tiles of every
+// sequence's first range as the call's rows have them (sequence b's from row0 gq / 16 + b on, rounded down: its
+// ceil(n gq / 16) end before the next one's begin), then nt for each of the ranges past the first, of which there are
+// `spare` at most, first - b of them before b's.
 __device__ __forceinline__ int64_t part_at(const PagedArgs& a, int b, int row0, int first, int split, int tile) {
   if (!a.tiles) return (int64_t)(first + split) * a.nt + tile;
   return split ? a.tiles + (int64_t)(first - b + split - 1) * a.nt + tile : row0 * (int64_t)a.gq / kRows + b + tile;

@@ -12,9 +12,10 @@
 // Units. A row of bf16 q is scaled by the power of two that brings its largest element below 2^14: fp16 keeps its bits down
 // to 2^-30 of the largest, and elements below 2^-38 are lost. Weights are held times 2^8 over a power of two, 2^ve, that
 // follows the row's largest step so far (kept like the maximum): fp16 keeps weights down to 2^-32 of it. Sums in these
-// units, of weights (up to 2^(14 - ve)) and of weights times offsets, have to stay inside fp32 where steps are 0 too (a group of one value):
-// ve begins at fp16's least step, whose offsets are below 2^16; with bf16, where it begins at 2^-80, it follows
-// 2^-40 of the largest offset too, which is below any step of the same group but 0. So 2^25 positions sum to at most 2^119.
+// units, of weights (up to 2^(14 - ve)) and of weights times offsets, have to stay inside fp32 where steps are 0 too (a
+// group of one value): 2^ve begins at fp16's least step, whose offsets are below 2^16; with bf16, where it begins at
+// 2^-80, it follows 2^-40 of the largest offset too, which is below any step of the same group but 0. So 2^25
+// positions sum to at most 2^119.
 #include "paged_attention.h"
 #include "paged_int4.h"
 
@@ -72,7 +73,7 @@ struct Unpack {
   }
 };
 
-constexpr float kLag4 = 6.0f;  // powers of two that a row's maximum may lag (3: prompts of 8755 tokens 239 us instead of 226)
+constexpr float kLag4 = 6.0f;  // powers of two that a row's maximum may lag (3: prompts of 8755 tokens 246 us instead of 231)
 constexpr int kUnit4 = 8;      // weights times 2^kUnit4: 2^(kLag4 + kUnit4 + 1) is inside fp16
 template <typename E>
 constexpr bool kWide4 = E::kOnes == BF16::kOnes;  // of fp32's range: q is scaled, and the unit follows offsets
@@ -95,7 +96,8 @@ __device__ __forceinline__ float follow8(float sm, const float* z) {
 // numbers of 16 bits: infinities and NaN, 0x7F80 on, wrap to negative ones, and 40 less in the exponent.
 struct Follow {
   uint32_t mask, wrap, less;  // in registers of each lane: scalar ones are short
-  __device__ __forceinline__ Follow(bool offsets) : mask(offsets ? 0u : 0x7FFF7FFFu), wrap(offsets ? 0x80008000u : 0x00800080u), less(vgpr_const<0x14801480u>()) {
+  __device__ __forceinline__ Follow(bool offsets)
+      : mask(offsets ? 0u : 0x7FFF7FFFu), wrap(offsets ? 0x80008000u : 0x00800080u), less(vgpr_const<0x14801480u>()) {
     asm volatile("" : "+v"(mask), "+v"(wrap));
   }
   __device__ __forceinline__ uint32_t operator()(uint32_t word) const {
@@ -156,11 +158,11 @@ __device__ __forceinline__ float score_factor(float scale, int qs) {
 // columns when its V is. What is done per score is then done once for C chunks on full lanes, and each column
 // is a partial result over positions of its own; they meet at the end. A wave's loads are a group of chunks ahead.
 //
-// Long contexts are bound by what a CU has in flight: 64 tokens of 28/4 heads (95 MB) 28 us and 4.5 for the merge, 3.4 TB/s where
+// Long contexts are bound by what a CU has in flight: 64 tokens of 28/4 heads (95 MB) 27 us and 4.9 for the merge, 3.4 TB/s where
 // a 2 GiB copy reaches 4.9; the CUs are busy for 20 us of it, the rest is the last ranges' unequal ends. Next to it stands the vector
-// unit, 62% of the busy cycles (9 instructions per word of 8 codes, some 110 per group of columns), the matrix cores 12%.
+// unit, 59% of the busy cycles (9 instructions per word of 8 codes, some 110 per group of columns), the matrix cores 11%.
 // 40 tokens of 20/20 heads of 64 in groups of 32 (131 MB) 38 us. Short contexts are bound by the latency of finding the range,
-// the page, its codes and of two launches: one token behind a window of 1024, 9.8 us.
+// the page, its codes and of two launches: one token behind a window of 1024, 9.9 us.
 // Waves of a SIMD that the registers are to leave room for: as many as need no spilling (two groups of dims of 128 with 2, 3
 // waves: two contexts of 100000 positions 20.1, 21.7 us; four groups: 64 sequences 46, 118 us).
 template <int HD, int NG>
@@ -576,11 +578,12 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(kSplitO
 // there are three slots and a chunk's scores are formed a step ahead: their products run beside the exponentials of
 // the chunk before. (Not with four groups of dims, whose products 256 registers do not hold beside the rest.)
 //
-// The vector unit bounds it, 62% (heads of 64: 72%) of the cycles with two or three waves a SIMD, the matrix cores 26% (20%):
+// The vector unit bounds it, 63% (heads of 64: 72%) of the cycles with two or three waves a SIMD, the matrix cores 25% (20%):
 // per score 2 instructions to form it, 2 for its exponential, 4 for its sums and weight, and unpacking a quarter of 9 per 8
-// codes. 8755 tokens of 32/8 heads behind a window of 1000 (bf16) 222 us, 560 TFLOP/s; 509 of 14/2 heads of 64 after
-// 20000 95 us, 390 TFLOP/s; with groups of 64 and 32 dims the former take 256 and 355 us. Tried to no gain: the products in
-// the compiler's scheduling groups, V's tiles read ahead of their products, wave priorities.
+// codes. 8755 tokens of 32/8 heads behind a window of 1000 (bf16) 231 us, 540 TFLOP/s; 509 of 14/2 heads of 64 after
+// 20000 96 us with the merge, 385 TFLOP/s; with groups of 64 and 32 dims the former take 257 (fp16) and 362 us (bf16). Of the
+// bf16 figures 2% are the unit's following offsets (Follow; as maxima beside the steps' 4 to 6%), 1% its being each row's own. Tried to
+// no gain: the products in the compiler's scheduling groups, V's tiles read ahead of their products, wave priorities.
 template <int BT, int NG>
 constexpr bool kAhead4 = kBlockKG<BT> == 1 && NG < 4;
 
@@ -1024,8 +1027,10 @@ Plan make_plan4(int64_t T, int64_t B, int64_t max_q, int64_t max_len, int64_t wi
     const int64_t fill = p.bt == 64 ? 320 : hd == 128 ? 512 : 768, whole = nkv * p.btiles;
     const bool uncut = (hd == 128 ? 2 : 3) * whole >= fill;
     // Tiles of 16 rows that each unpack what they read are the faster up to some 20 a sequence, but against whole blocks of 128
-    // rows. us in blocks and in tiles: 16 x 9 tokens of 28/4 heads after 4000 44.7, 33.0; 40 x 11 of 32/8 174, 99; 4 x 60 of 32/8
-    // alone 15.4, 7.3; 50 of 12/2 after 8000 30.2, 22.3; 60 beside 200 that decode 123, 72; but 40 x 30 of 32/8 after 3000 146, 166.
+    // rows. us in blocks and in tiles: 16 x 9 tokens of 28/4 heads after 4000 46.0, 34.3; 40 x 11 of 32/8 175, 104; 4 x 60 of 32/8
+    // alone 16.2, 7.4; 50 of 12/2 after 8000 30.2, 22.7; 60 of 32/8 beside 200 that decode 127, 72; 32 x 1 to 40 108, 76.
+    // They are even with 8 x 40 of 28/4 (46, 47) and 20 x 64 of 32/8 after 500 (41, 42), and slower with several prompts
+    // beside tokens: 8 x 64 beside 32 that decode 60, 69. Where whole blocks are left alone: 40 x 30 of 32/8 after 3000 146, 166.
     // (And not where there would be a million of them, most of them of sequences of fewer rows.)
     if (max_q * gq > 20 * kRows || (p.bt == 128 && uncut) || B * nkv * (max_q * gq / kRows) > (1 << 20)) {
       p.bsplits = uncut ? 1 : std::max<int64_t>(1, std::min<int64_t>(32, fill / whole));

@@ -5,7 +5,7 @@
 // already (a lane's 16 bytes are 8 dims of each step of one position); v's, whose bytes run along the positions, are turned
 // in LDS.
 //
-// The stores bound it: 39439 positions of 8 heads of 128 in groups of 32, 50 MB of codes to 162 MB of values, 47 us, 4.5 TB/s (a
+// The stores bound it: 39439 positions of 8 heads of 128 in groups of 32, 50 MB of codes to 162 MB of values, 48 us, 4.4 TB/s (a
 // 2 GiB copy: 4.9). 700 positions of 2 heads 4.6 us, the latency of the length, the page's id, the codes and the stores.
 #include <algorithm>
 
