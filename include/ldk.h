@@ -508,7 +508,7 @@ int64_t ldk_paged_attention_int4_workspace_bytes(int64_t T, int64_t B, int64_t m
 
 /* ldk_paged_attention over the values that 4-bit pages hold: masks, max_q, workspace and limits as there. Scores,
  * softmax and sums in fp32 from the codes as they are; the weights times v's steps are rounded to fp16 (with 11
- * bits down to 2^-22 of the row's largest weight times the largest step that it sees, with fewer to 2^-32), one
+ * bits down to 2^-22 of the row's largest weight times the largest step that it sees, of any group, with fewer to 2^-32), one
  * rounding at the end. An element of bf16 q below 2^-38 of its head's largest counts as 0. A head of q with an infinity or a NaN
  * gives NaN. fp16 k and v may have any finite values; bf16 ones up to 2^90 in size (and scores inside fp32's range), and
  * bf16 steps of v below 2^-80 lose bits. What a token does not see may hold anything. */
